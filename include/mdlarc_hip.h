@@ -13,7 +13,8 @@
  *   - Nothing allocates, frees or synchronises; all work is ordered on `stream`.
  *   - Return 0 on success, a negative MDL_ERR_* for arguments rejected on the host before any
  *     launch, or a positive hipError_t reported by the launch.
- *   - Head dimension is 64 (all reference model sizes, src/transformer.py:728-745).
+ *   - Head dimension is 64 (all reference model sizes, src/transformer.py:728-745); the entries for
+ *     grouped key / value heads (K7, K8) take 64 and 128.
  *   - GEMM inputs ("split activations") are written as hi|lo bf16 pairs: a row of K values is 2K
  *     bf16, hi = bf16(v) in columns [0, K), lo = bf16(v - hi) in [K, 2K).  Multiplied with a
  *     weight packed as [W | W] ([N, 2K] bf16) a bf16 GEMM with fp32 accumulation returns
@@ -52,7 +53,7 @@ extern "C" {
 #define MDL_ERR_NULL (-1)          /* a required pointer is NULL */
 #define MDL_ERR_ALIGN (-2)         /* a pointer or leading dimension breaks 16-byte alignment */
 #define MDL_ERR_SHAPE (-3)         /* a dimension is out of the supported range */
-#define MDL_ERR_HEAD_DIM (-4)      /* head_dim != 64 or d_model != n_heads * 64 */
+#define MDL_ERR_HEAD_DIM (-4)      /* head_dim the entry does not take, or d_model != n_heads * 64 */
 #define MDL_ERR_CACHE (-5)         /* slot range outside the cache */
 #define MDL_ERR_WORKSPACE (-6)     /* workspace too small */
 #define MDL_ERR_DTYPE (-7)         /* unsupported dtype code */
@@ -63,6 +64,12 @@ extern "C" {
 
 #define MDL_DTYPE_F32 0
 #define MDL_DTYPE_BF16 1
+
+/* How mdl_attn_grouped / mdl_attn_decode_shared write their output (their out_form argument): in the
+ * type of q, row-major [rows, n_heads * head_dim], or as the split input of a projection. */
+#define MDL_OUT_PLAIN 0
+#define MDL_OUT_SPLIT_ROWS 1       /* split bf16 [rows, 2 * n_heads * head_dim], row-major */
+#define MDL_OUT_SPLIT_TILES 2      /* the same in MFMA tiles */
 
 /* Layout of a split activation written by a producer entry point (its *_layout argument). */
 #define MDL_LAYOUT_ROWS 0          /* row-major [rows, 2K]: hi in columns [0, K), lo in [K, 2K) */
@@ -643,6 +650,89 @@ int mdl_attn_decode_f32(const float* q, const float* k_cache, const float* v_cac
                         int prompt_len, const int32_t* kv_start, int seq_pos,
                         const int32_t* seq_dev, float* workspace, int64_t workspace_bytes,
                         int split_len, uint16_t* out, int out_layout, void* stream);
+
+/*
+ * K7 -- RMS norms of each query and key head, RoPE and the cache write in one pass over the qkv
+ * projection of a layer with grouped key / value heads (n_heads query heads, n_kv_heads key and value
+ * heads, n_heads a multiple of n_kv_heads).  No counterpart in the reference, whose heads have
+ * neither norm nor groups; without them this is mdl_qkv_rope_cache_packed.
+ * qkv: [rows, (n_heads + 2 n_kv_heads) * head_dim] of in_dtype (MDL_DTYPE_F32, the projection's
+ * output, or MDL_DTYPE_BF16), query heads, key heads, value heads; row stride ld in elements, a
+ * multiple of 16 bytes.  For head x of token m, y = rstd[m] * x (rstd may be NULL: 1):
+ *   query, key   n = y / sqrt(mean(y^2) + eps) * gamma   (q_gamma or k_gamma, fp32 [head_dim])
+ *                pair j of n rotated by the token's position (the table and clamping of
+ *                mdl_qkv_rope_cache; px + py + pz == head_dim / 2)
+ *                query: times q_scale -> q_out [rows, n_heads, head_dim];  key -> k_cache
+ *   value        y -> v_cache
+ * Everything between the load and the store is fp32.  Token m goes to slot token_slot[m] of cache
+ * row token_row[m] of [batch, n_kv_heads, cache_slots, head_dim]; a slot or row outside the cache
+ * writes nothing there.  No two tokens may name the same slot of a row (which of their values
+ * remain is not defined).  q_out and the caches are of out_dtype and must not overlap qkv.
+ */
+int mdl_qk_norm_rope_cache(const void* qkv, int in_dtype, int64_t ld, const float* rstd,
+                           const int64_t* pos, const float* rope_tab, int64_t rows,
+                           const int32_t* token_row, const int32_t* token_slot, int batch,
+                           int n_heads, int n_kv_heads, int head_dim, int max_x, int max_y,
+                           int max_z, int px, int py, int pz, const float* q_gamma,
+                           const float* k_gamma, float eps, float q_scale, void* q_out,
+                           void* k_cache, void* v_cache, int out_dtype, int cache_slots,
+                           void* stream);
+
+/*
+ * K8 -- attention of packed sequences of different lengths with grouped key / value heads: whole
+ * prompts, prompts that continue a cached context, single tokens.  No counterpart in the reference
+ * (its heads have no groups); F.scaled_dot_product_attention of src/inference.py:409, :452 is the
+ * case n_kv_heads == n_heads.
+ * q: [tokens, n_heads, head_dim] of dtype (MDL_DTYPE_BF16 or MDL_DTYPE_F32), pre-scaled by the
+ * softmax scale times log2(e); k_cache / v_cache: [n_seq, n_kv_heads, cache_slots, head_dim], same
+ * dtype.  Query head h reads key / value head h / (n_heads / n_kv_heads).  head_dim is 64 or 128.
+ * Sequence s has the queries q_offset[s] .. q_offset[s + 1] - 1 (q_offset int32 [n_seq + 1], not
+ * decreasing) and the keys in slots [0, kv_len[s]) of cache row s (kv_len int32 [n_seq], counting
+ * the keys of its own queries).  Its query i of n sees slot j iff j < kv_len[s] and, if causal,
+ * j <= kv_len[s] - n + i:
+ *   out = sum_j 2^(q . k_j) v_j / sum_j 2^(q . k_j),   0 where a query sees no slot.
+ * A value that is not finite in a slot that a query does not see does not reach it.  Softmax
+ * statistics and sums are fp32; bf16: the weights are rounded to bf16 for the product with V.
+ * max_q: at least the most queries of a sequence; queries past it, and rows of q behind the last
+ * sequence, are not computed and their rows of out stay as they were.  Lengths and offsets outside
+ * their ranges are clamped.
+ * workspace (16-byte aligned) lets launches with few rows cut their keys into parts that a second
+ * launch joins; mdl_attn_grouped_workspace_bytes of the same sizes (0: not used).  NULL: never
+ * cut.  Smaller than that: MDL_ERR_WORKSPACE.  Calls that may overlap in time need workspaces of
+ * their own.  The sums of a row are split by n_seq, max_q and cache_slots, so their order, and
+ * with it the last bits, may change with those; equal calls give equal bits.
+ */
+int mdl_attn_grouped(const void* q, const void* k_cache, const void* v_cache, int dtype, int n_seq,
+                     int tokens, int max_q, int n_heads, int n_kv_heads, int head_dim,
+                     int cache_slots, const int32_t* q_offset, const int32_t* kv_len, int causal,
+                     void* out, int out_form, float* workspace, int64_t workspace_bytes,
+                     void* stream);
+int64_t mdl_attn_grouped_workspace_bytes(int n_seq, int tokens, int max_q, int n_heads,
+                                         int n_kv_heads, int head_dim, int dtype,
+                                         int cache_slots);
+
+/*
+ * K8 for a decode step whose rows share prefixes: row b (one query) of group g sees the slots
+ * [0, prefix_len[g]) of prefix g, of which the whole group has one copy, and the slots
+ * [0, kv_len[b]) of its own cache row.  Several samples of one prompt, which
+ * predict_with_augmentations(num_samples) decodes as rows with a cache each
+ * (src/inference.py:700-760), read the prompt's keys once.
+ * q, out: [batch, n_heads, head_dim]; prefix_k / prefix_v: [n_prefix, n_kv_heads, prefix_slots,
+ * head_dim]; k_cache / v_cache: [batch, n_kv_heads, cache_slots, head_dim].  Group g has the rows
+ * row_offset[g] .. row_offset[g + 1] - 1 (int32 [n_prefix + 1], not decreasing), at most max_rows
+ * (the rows past max_rows of a group, and rows in no group, have no prefix).  workspace:
+ * mdl_attn_decode_shared_workspace_bytes of the same sizes, required.  Otherwise as
+ * mdl_attn_grouped.
+ */
+int mdl_attn_decode_shared(const void* q, const void* prefix_k, const void* prefix_v,
+                           const int32_t* row_offset, const int32_t* prefix_len, int n_prefix,
+                           int prefix_slots, int max_rows, const void* k_cache,
+                           const void* v_cache, const int32_t* kv_len, int batch, int cache_slots,
+                           int dtype, int n_heads, int n_kv_heads, int head_dim, void* out,
+                           int out_form, float* workspace, int64_t workspace_bytes, void* stream);
+int64_t mdl_attn_decode_shared_workspace_bytes(int batch, int n_prefix, int max_rows, int n_heads,
+                                               int n_kv_heads, int head_dim, int dtype,
+                                               int prefix_slots, int cache_slots);
 
 /*
  * Every layer of a prompt or decode step from one call (host code over the entries above, which

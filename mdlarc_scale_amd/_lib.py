@@ -137,6 +137,15 @@ SIGNATURES: dict[str, tuple[object, list]] = {
                                      P, c_int, P]),
     "mdl_attn_decode_f32": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P, c_int, P, c_int, P, P,
                                     c_int64, c_int, P, c_int, P]),
+    "mdl_qk_norm_rope_cache": (c_int, [P, c_int, c_int64, P, P, P, c_int64, P, P, c_int, c_int, c_int,
+                                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P,
+                                       c_float, c_float, P, P, P, c_int, c_int, P]),
+    "mdl_attn_grouped": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                 P, P, c_int, P, c_int, P, c_int64, P]),
+    "mdl_attn_grouped_workspace_bytes": (c_int64, [c_int] * 8),
+    "mdl_attn_decode_shared": (c_int, [P, P, P, P, P, c_int, c_int, c_int, P, P, P, c_int, c_int,
+                                       c_int, c_int, c_int, c_int, P, c_int, P, c_int64, P]),
+    "mdl_attn_decode_shared_workspace_bytes": (c_int64, [c_int] * 9),
     "mdl_lm_head": (c_int, [P, P, c_int, c_int, P, c_float, P, c_int, P, P, CONS, c_int, P]),
     "mdl_decode_head": (c_int, [P, c_int, c_int, P, c_float, P, c_int, P, P, P, c_int64, c_int,
                                 P, P, c_int, c_int, CONS, c_int, P]),

@@ -31,6 +31,8 @@ SOURCES = [
     "attn_decode.hip",
     "attn_prefill.hip",
     "attn_f32.hip",
+    "attn_grouped.hip",
+    "qk_norm.hip",
     "head_state.hip",
     "prompt_build.hip",
     "split_gemm.hip",

@@ -1,0 +1,822 @@
+// K8 -- attention with grouped key / value heads, over packed sequences and over shared prefixes.
+//
+// Query head h reads key / value head h / G (G = n_heads / n_kv_heads).  The G heads of a query
+// are G neighbouring rows of q, so a sequence of n queries is, for one key / value head, a matrix
+// of n G rows (row i G + g: query i, head kv G + g) against one key list; a work item is a tile of
+// those rows.  Row i G + g sees the keys j <= lim, lim = kv_len - n + i (causal) or kv_len - 1:
+//   out = sum_j 2^(q . k_j) v_j / sum_j 2^(q . k_j)      (q carries softmax scale * log2(e))
+// and is zero where it sees no key.
+//
+// A wave owns 32 rows and works on 32 keys at a time with the 32 x 32 MFMAs (bf16: k = 16, fp32:
+// k = 2).  S^T = K Q^T leaves row c = lane % 32 of the tile in the lane's column: accumulator
+// element r of lane half h = lane / 32 is key (r % 4) + 8 (r / 4) + 4 h, so the softmax runs inside
+// a lane but for one exchange of the halves, and O^T = V^T P^T takes the probabilities as its B
+// operand from the registers they are in.  bf16: k-step s (16 keys) takes elements 8 s .. 8 s + 7,
+// i.e. keys 16 s + 4 h + {0..3, 8..11}, and the V^T operand in that key order comes from the
+// row-major V tile by two transposing LDS reads.  fp32: k-step r pairs key(r, 0) and key(r, 1); dim
+// block i of the output holds dims (D / 32) m + i, so a lane's V values of all blocks are one read.
+//
+// Softmax: online, base 2, fp32; a row's reference maximum moves only when a score passes it by
+// more than 2^8 (its first visible key always sets it), which keeps the rescale out of most tiles
+// and depends on the row alone.  The scores' accumulators start at minus the reference.
+//
+// A value that is not finite reaches the rows that see it and no others: keys past every row's
+// limit enter as zeros, and where a step holds keys that some rows of the wave see and others do
+// not, a value there that is not finite is worked on apart (masked_step).
+//
+// Staging: key tiles of KT keys go through a ring of two LDS stages filled by direct global -> LDS
+// copies, the next tile's under this one's work.  16-byte chunks are XOR-swizzled by row (swz).
+// WR waves share a ring and split the rows; WK groups of WR waves take the tiles in turn, each with
+// a ring of its own, and merge at the end.  A launch may also cut each tile's keys in n_split parts
+// whose states (fp32 m, l, o) go to the workspace; merge_kernel joins them.
+#include <type_traits>
+
+#include "lds_dma.h"
+#include "mfma.h"
+
+namespace mdl {
+
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr float kGap = 8.f;   // log2 of the largest p between moves of the reference maximum
+
+// how outputs leave: the type of q in rows, or the split (hi|lo bf16) input of K5 / K6
+enum OutForm { kOutPlain = MDL_OUT_PLAIN, kOutSplitRows = MDL_OUT_SPLIT_ROWS,
+               kOutSplitTiles = MDL_OUT_SPLIT_TILES };
+
+struct GroupedArgs {
+  const void* q;               // [tokens, heads, D]
+  const void* k;               // [n_seq, kv_heads, slots, D]
+  const void* v;
+  const int32_t* q_offset;     // [n_seq + 1] first row of each sequence; NULL: row s is sequence s
+  const int32_t* kv_len;       // [n_seq]
+  void* out;
+  float* ws_o;                 // [parts][tokens * heads][D], NULL: outputs leave directly
+  float* ws_ml;                // [parts][tokens * heads][2]
+  int n_seq, tokens, heads, kv_heads, group, slots, max_q, causal, n_tiles, n_split, part0;
+  int out_form;
+};
+
+// Chunk swizzle of a tile row (16-byte chunks), by its low 4 bits r3..r0.  Both reads are then free
+// of bank conflicts whether 16-byte reads go 8 lanes a cycle and transposing ones 16 (32 banks) or
+// 16 and 32 (64 banks): 8 and 16 rows of one chunk, and 4 rows of a 32-byte or 64-byte run.
+template <typename T, int D>
+__device__ __forceinline__ constexpr int swz(int r) {
+  if (sizeof(T) == 4) return r & 15;
+  const int r0 = r & 1, r1 = (r >> 1) & 1, r2 = (r >> 2) & 1, r3 = (r >> 3) & 1;
+  return D == 128 ? r2 | (r0 << 1) | (r1 << 2) | ((r0 ^ r3) << 3)
+                  : r2 | ((r0 ^ r3) << 1) | (r1 << 2);
+}
+
+__device__ __forceinline__ float other_half(float v) {   // the value of lane ^ 32
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float((threadIdx.x & 32) ? a[0] : a[1]);
+}
+
+__device__ __forceinline__ float max_halves(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+__device__ __forceinline__ f32x16_t splat16(float v) {
+  return f32x16_t{v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v};
+}
+
+// Four consecutive channels `col` .. + 3 of output row `row` (width `d` = heads * D).
+template <typename T>
+__device__ __forceinline__ void store_out4(void* out, int form, int64_t row, int col, int d,
+                                           float a, float b, float c, float e) {
+  if (form == kOutPlain) {
+    T* p = static_cast<T*>(out) + row * d + col;
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(p) = make_float4(a, b, c, e);
+    else
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf2(a, b), pack_bf2(c, e));
+    return;
+  }
+  const float t[4] = {a, b, c, e};
+  uint2 hi, lo;
+  split4(t, hi, lo);
+  uint16_t* o = static_cast<uint16_t*>(out);
+  if (form == kOutSplitTiles) {
+    *reinterpret_cast<uint2*>(o + tile_off(row, col, 2 * d)) = hi;
+    *reinterpret_cast<uint2*>(o + tile_off(row, d + col, 2 * d)) = lo;
+  } else {
+    *reinterpret_cast<uint2*>(o + row * 2 * d + col) = hi;
+    *reinterpret_cast<uint2*>(o + row * 2 * d + d + col) = lo;
+  }
+}
+
+template <typename T, int D, int WR, int WK, int KT>
+struct GroupedShape {
+  static constexpr int kRowBytes = D * static_cast<int>(sizeof(T));
+  static constexpr int kTile = KT * kRowBytes;            // bytes of a K or V tile
+  static constexpr int kLds = WK * 4 * kTile;             // two stages of K and V per group
+  static constexpr int kRows = 32 * WR;                   // rows of a block
+  static constexpr int kCopies = kTile / 1024 / WR;       // 1 KB copies of a wave, K or V
+  static constexpr int kRowsPerCopy = 1024 / kRowBytes;
+  // fp32 with 128 dims: q and the output alone are 128 registers
+  static constexpr int kWavesPerSimd = kLds > 80 * 1024 || kRowBytes == 512 ? 1 : 2;
+  static_assert(kTile % (1024 * WR) == 0, "whole copies per wave");
+  static_assert(KT % 32 == 0 && (D == 64 || D == 128), "whole MFMA blocks");
+  // the merge of the groups goes through the ring's memory
+  static_assert((WK - 1) * WR * (2 + D / 2) * 256 <= kLds, "states of the other groups fit");
+};
+
+template <typename T, int D, int WR, int WK, int KT>
+__device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, uint8_t* lds) {
+  using S = GroupedShape<T, D, WR, WK, KT>;
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int NB = KT / 32, DB = D / 32;
+  const int pairs = p.n_seq * p.kv_heads;
+  const int rest = block / pairs, pair = block - rest * pairs;
+  const int seq = pair / p.kv_heads, kvh = pair - seq * p.kv_heads;
+  const int rank = rest / p.n_split, split = rest - rank * p.n_split;
+  const int tile = p.n_tiles - 1 - rank;   // the latest rows, with the most keys, first
+  int lo = seq, hi = seq + 1;
+  if (p.q_offset) {
+    lo = min(max(p.q_offset[seq], 0), p.tokens);
+    hi = min(max(p.q_offset[seq + 1], lo), p.tokens);
+  }
+  const int n = hi - lo;
+  const int G = p.group;
+  const int rows = min(n, p.max_q) * G;
+  const int r0 = tile * S::kRows;
+  if (r0 >= rows) return;
+  const int len = min(max(p.kv_len[seq], 0), p.slots);
+
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave % WR, wk = wave / WR;
+  // the limits of the block's last row, this lane's row, and the wave's first and last
+  auto limit = [&](int r) { return p.causal ? len - n + r / G : len - 1; };
+  const int kend = max(limit(min(r0 + S::kRows, rows) - 1) + 1, 0);
+  const int w0 = r0 + 32 * wr;
+  const int row = w0 + c;
+  const bool real = row < rows;
+  const int qi = min(row, rows - 1) / G, hg = min(row, rows - 1) - qi * G;
+  const int lim = real ? limit(row) : -1;
+  const int lim_lo = w0 < rows ? limit(w0) : -1;
+  const int lim_hi = w0 < rows ? limit(min(w0 + 32, rows) - 1) : -1;
+  // keys of this part, in whole turns of the groups
+  constexpr int kTurn = KT * WK;
+  const int per = ((kend + p.n_split - 1) / p.n_split + kTurn - 1) / kTurn * kTurn;
+  const int k0 = min(split * per, kend), k1 = min(k0 + per, kend);
+
+  const int64_t qrow = static_cast<int64_t>(lo + qi) * p.heads + kvh * G + hg;   // head row
+  using QFrag = typename std::conditional<kF32, float4, bf16x8_t>::type;
+  constexpr int NQ = kF32 ? D / 8 : D / 16;
+  QFrag qf[NQ];
+  {
+    const T* qp = static_cast<const T*>(p.q) + qrow * D;
+#pragma unroll
+    for (int s = 0; s < NQ; ++s) {
+      // bf16: dims 16 s + 8 h .. + 7; fp32: dims h D / 2 + 4 s .. + 3
+      if constexpr (kF32)
+        qf[s] = *reinterpret_cast<const float4*>(qp + h * (D / 2) + 4 * s);
+      else
+        qf[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qp + 16 * s + 8 * h));
+    }
+  }
+
+  const int64_t head = (static_cast<int64_t>(seq) * p.kv_heads + kvh) * p.slots * D;
+  const T* Kg = static_cast<const T*>(p.k) + head;
+  const T* Vg = static_cast<const T*>(p.v) + head;
+  uint8_t* ring = lds + wk * 4 * S::kTile;
+  const uint32_t ring0 = lds_addr(ring);
+  // Copy j of a tile: rows (1024 / row bytes) j .. of K and of V, one kilobyte each; a lane takes
+  // physical chunk lane % chunks of its row.  Rows past the last key copy that key.
+  constexpr int kChunks = S::kRowBytes / 16;
+  auto issue = [&](int kt, int st) {
+    const T* kb = scalar_ptr(Kg + static_cast<int64_t>(kt) * D);
+    const T* vb = scalar_ptr(Vg + static_cast<int64_t>(kt) * D);
+#pragma unroll
+    for (int jj = 0; jj < S::kCopies; ++jj) {
+      const int j = wr + WR * jj;
+      const int r = S::kRowsPerCopy * j + lane / kChunks;
+      const uint32_t off = min(r, kend - 1 - kt) * S::kRowBytes +
+                           16 * ((lane % kChunks) ^ swz<T, D>(r & 15));
+      const uint32_t dst = ring0 + st * 2 * S::kTile + 1024 * j;
+      dma16_sbase(kb, off, __builtin_amdgcn_readfirstlane(dst));
+      dma16_sbase(vb, off, __builtin_amdgcn_readfirstlane(dst + S::kTile));
+    }
+  };
+
+  // Lane parts of the swizzled read addresses.  K operand: row c, bf16 chunk 2 s + h, fp32 chunk
+  // h D / 8 + s.  V^T operand, bf16: rows 4 h + lane / 4 % 4 (and + 8) of a 16-key step, dims
+  // 32 db + 16 (lane / 16 % 2) + 4 (lane % 4) .. + 3.
+  const uint32_t krow = c * S::kRowBytes;
+  const int kswz = swz<T, D>(c & 15);
+  const int vr = 4 * h + ((lane >> 2) & 3);
+  const int vchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  uint32_t vofs[DB][2];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      vofs[db][e] = (vr + 8 * e) * S::kRowBytes +
+                    16 * ((vchunk + 4 * db) ^ swz<T, D>(vr + 8 * e)) + 8 * (lane & 1);
+
+  float negm = 0.f, thr = -INFINITY, l = 0.f;   // l: this lane half's part of the sum
+  f32x16_t o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = splat16(0.f);
+
+  auto vt_frag = [&](const uint8_t* Vt, int key, int db) -> bf16x8_t {
+    const uint8_t* base = Vt + key * S::kRowBytes;
+    const s16x4_t a = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + vofs[db][0]));
+    const s16x4_t b = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + vofs[db][1]));
+    return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  // V operands `va` of the 16 keys from kk on, of which not every row sees all: keys past lim_hi
+  // become zeros; if a value that is left is not finite, each set of rows with one limit gets a
+  // product over its own keys here and the operands become zeros.
+  auto masked_step = [&](uint4 (&va)[DB], int kk, const bf16x8_t& pb) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = kk + 4 * h + 8 * (i >> 1) + 2 * (i & 1);
+      const uint32_t keep = (k <= lim_hi ? 0xffffu : 0u) | (k + 1 <= lim_hi ? 0xffff0000u : 0u);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        uint32_t& x = i == 0 ? va[db].x : i == 1 ? va[db].y : i == 2 ? va[db].z : va[db].w;
+        x &= keep;
+        odd |= (x & 0x7fff7fffu) + 0x00800080u;   // an exponent of all ones carries into the sign
+      }
+    }
+    if (__ballot((odd & 0x80008000u) != 0) == 0) return;
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e) {   // the rows that see keys up to kk + e of this step
+      const bool mine = e == 15 ? lim >= kk + 15 : lim == kk + e;
+      if (__ballot(mine) == 0) continue;
+      uint32_t see[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 4 * h + 8 * (i >> 1) + 2 * (i & 1);
+        see[i] = (k <= e ? 0xffffu : 0u) | (k + 1 <= e ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint4 a = make_uint4(va[db].x & see[0], va[db].y & see[1], va[db].z & see[2],
+                                   va[db].w & see[3]);
+        const f32x16_t t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), pb, splat16(0.f),
+                                                                   0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] += mine ? t[i] : 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db) va[db] = make_uint4(0, 0, 0, 0);
+  };
+
+  // fp32: the V values of lane half h for step r, key kr of the tile (absolute kt + kr), zero past
+  // key `last`.  kr = 8 (r / 4) + r % 4 + 4 h.
+  auto v_pair = [&](const uint8_t* Vt, int kt, int kr, int last, float (&v)[DB]) {
+    const uint8_t* base = Vt + kr * S::kRowBytes;
+    if constexpr (D == 128) {
+      const float4 t = *reinterpret_cast<const float4*>(base + 16 * (c ^ swz<T, D>(kr & 15)));
+      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    } else {
+      const float2 t = *reinterpret_cast<const float2*>(
+          base + 16 * ((c >> 1) ^ swz<T, D>(kr & 15)) + 8 * (c & 1));
+      v[0] = t.x; v[1] = t.y;
+    }
+    const bool seen = kt + kr <= last;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) v[db] = seen ? v[db] : 0.f;
+  };
+
+  // The fp32 form of masked_step, for a whole tile: true if it holds values that are not finite in
+  // slots that some row sees; its product is then added here, each row over its own keys.
+  auto masked_tile = [&](const uint8_t* Vt, int kt, const f32x16_t& pr) -> bool {
+    bool odd = false;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float v[DB];
+      v_pair(Vt, kt, (r & 3) + 8 * (r >> 2) + 4 * h, lim_hi, v);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) odd |= !(fabsf(v[db]) < INFINITY);
+      if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (__ballot(odd) == 0) return false;
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r) {   // keys ka and ka + 4: a row sees both, the first, or none
+      const int ka = kt + (r & 3) + 8 * (r >> 2);
+      float v[DB], x = pr[0];
+      v_pair(Vt, kt, ka - kt + 4 * h, lim_hi, v);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) x = r == i ? pr[i] : x;
+      const bool two = lim >= ka + 4, one = lim >= ka && !two;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const f32x16_t t2 = __builtin_amdgcn_mfma_f32_32x32x2f32(v[db], x, splat16(0.f), 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] += two ? t2[i] : 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x16_t t1 = __builtin_amdgcn_mfma_f32_32x32x2f32(h ? 0.f : v[db], x, splat16(0.f),
+                                                                 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] += one ? t1[i] : 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    return true;
+  };
+
+  auto compute = [&](const uint8_t* Kt, const uint8_t* Vt, int kt) {
+    const bool masked = kt + KT - 1 > lim_lo;   // some row does not see the whole tile
+    f32x16_t sc[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      sc[nb] = splat16(negm);
+#pragma unroll
+      for (int s = 0; s < NQ; ++s) {
+        const int chunk = kF32 ? h * (D / 8) + s : 2 * s + h;
+        const uint4 a = *reinterpret_cast<const uint4*>(Kt + krow + 32 * nb * S::kRowBytes +
+                                                        16 * (chunk ^ kswz));
+        if constexpr (kF32) {
+          const float4 b = qf[s];
+          sc[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), b.x, sc[nb], 0, 0, 0);
+          sc[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), b.y, sc[nb], 0, 0, 0);
+          sc[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), b.z, sc[nb], 0, 0, 0);
+          sc[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), b.w, sc[nb], 0, 0, 0);
+          if ((s & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+        } else {
+          sc[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), qf[s], sc[nb], 0, 0, 0);
+        }
+      }
+    }
+    if (masked) {
+      const int x = lim - kt - 4 * h;   // the last visible key, from this lane half's first
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * nb + (r & 3) + 8 * (r >> 2) > x) sc[nb][r] = -INFINITY;
+    }
+    float lmax = sc[0][0];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) lmax = fmaxf(lmax, sc[nb][r]);
+    if (__ballot(lmax > thr) != 0) {
+      const float tmax = max_halves(lmax);
+      if (tmax > thr) {   // the same in both lanes of a row
+        const bool fresh = thr == -INFINITY;
+        const float alpha = fresh ? 0.f : __builtin_amdgcn_exp2f(-tmax);
+        negm = fresh ? -tmax : negm - tmax;
+        thr = kGap;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) sc[nb] -= tmax;
+        l *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[nb][r] = __builtin_amdgcn_exp2f(sc[nb][r]);
+    if constexpr (kF32) {
+      static_assert(!kF32 || NB == 1, "fp32 tiles are 32 keys");
+#pragma unroll
+      for (int r = 0; r < 16; ++r) l += sc[0][r];
+      // worked on there: zeros here
+      const int last = masked && masked_tile(Vt, kt, sc[0]) ? -1 : lim_hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float v[DB];
+        v_pair(Vt, kt, (r & 3) + 8 * (r >> 2) + 4 * h, last, v);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[db], sc[0][r], o[db], 0, 0, 0);
+        if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int key = 32 * nb + 16 * s;
+          const f32x16_t& t = sc[nb];
+          const bf16x8_t pb = {(__bf16)t[8 * s], (__bf16)t[8 * s + 1], (__bf16)t[8 * s + 2],
+                               (__bf16)t[8 * s + 3], (__bf16)t[8 * s + 4], (__bf16)t[8 * s + 5],
+                               (__bf16)t[8 * s + 6], (__bf16)t[8 * s + 7]};
+          // the sum of the rounded weights that the product below takes
+#pragma unroll
+          for (int i = 0; i < 8; ++i) l += (float)pb[i];
+          uint4 va[DB];
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            va[db] = __builtin_bit_cast(uint4, vt_frag(Vt, key, db));
+          __builtin_amdgcn_sched_barrier(0);
+          if (kt + key + 15 > lim_lo) masked_step(va, kt + key, pb);
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(va[db]), pb, o[db], 0, 0, 0);
+        }
+    }
+  };
+
+  // Turns: group wk's tile of a turn is k0 + KT wk past it.  Every wave of the block makes the same
+  // number of them, so the barriers match.
+  const int first = k0 + KT * wk;
+  if (first < k1) issue(first, 0);
+  auto turn = [&](int kt, auto stc) {
+    constexpr int ST = decltype(stc)::value;
+    // tile kt has landed for every wave of the group, which are done with the other stage; a group
+    // of one wave needs no barrier.  The builtin wait also covers the loads the compiler knows of.
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    if constexpr (WR > 1)
+      asm volatile("s_barrier" ::: "memory");
+    else
+      asm volatile("" ::: "memory");   // no read of the tile moves above the wait
+    if (kt + kTurn < k1) issue(kt + kTurn, ST ^ 1);
+    if (kt >= k1 || kt > lim_hi) return;   // past the part, or no row of the wave sees a key
+    const uint8_t* Kt = ring + ST * 2 * S::kTile;
+    compute(Kt, Kt + S::kTile, kt);
+  };
+  for (int t = k0; t < k1; t += 2 * kTurn) {
+    turn(t + KT * wk, std::integral_constant<int, 0>{});
+    if (t + kTurn < k1) turn(t + kTurn + KT * wk, std::integral_constant<int, 1>{});
+  }
+
+  l += other_half(l);
+  // -inf marks a state without keys (scores that are all NaN make one with keys)
+  float m = thr == -INFINITY && l == 0.f ? -INFINITY : -negm;
+  if constexpr (WK > 1) {
+    // the other groups' states through the ring's memory, in the lanes' own order
+    __syncthreads();   // every wave is done with its tiles
+    float* st = reinterpret_cast<float*>(lds);
+    if (wk > 0) {
+      float* w = st + ((wk - 1) * WR + wr) * (2 + 16 * DB) * kWave + lane;
+      w[0] = m;
+      w[kWave] = l;
+#pragma unroll
+      for (int i = 0; i < 16 * DB; ++i) w[(2 + i) * kWave] = o[i >> 4][i & 15];
+    }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll 1
+    for (int j = 0; j < WK - 1; ++j) {
+      const float* w = st + (j * WR + wr) * (2 + 16 * DB) * kWave + lane;
+      const float mj = w[0], top = fmaxf(m, mj), base = top == -INFINITY ? 0.f : top;
+      const float a = __builtin_amdgcn_exp2f(m - base), aj = __builtin_amdgcn_exp2f(mj - base);
+      m = top;
+      l = l * a + w[kWave] * aj;
+#pragma unroll
+      for (int i = 0; i < 16 * DB; ++i)
+        o[i >> 4][i & 15] = fmaf(w[(2 + i) * kWave], aj, o[i >> 4][i & 15] * a);
+    }
+  }
+  if (!real) return;
+  // elements 4 j .. 4 j + 3: bf16, dims 32 db + 8 j + 4 h .. + 3 of block db; fp32, dims
+  // DB (8 j + 4 h + e) + db, e = 0..3: 4 DB neighbours
+  auto at = [&](int j, int u, int e) -> float {   // e-th of the 4 channels of store u
+    if constexpr (kF32) {
+      const int x = 4 * u + e;
+      return o[x % DB][4 * j + x / DB];
+    } else {
+      return o[u][4 * j + e];
+    }
+  };
+  auto dim = [&](int j, int u) { return kF32 ? DB * (8 * j + 4 * h) + 4 * u : 32 * u + 8 * j + 4 * h; };
+  if (p.ws_o) {
+    const int64_t all = static_cast<int64_t>(p.tokens) * p.heads;
+    const int64_t at_row = (p.part0 + split) * all + qrow;
+    if (h == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * at_row) = make_float2(m, l);
+    if (m == -INFINITY) return;   // the merge takes no value of such a state
+    float* w = p.ws_o + at_row * D;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int u = 0; u < DB; ++u)
+        *reinterpret_cast<float4*>(w + dim(j, u)) =
+            make_float4(at(j, u, 0), at(j, u, 1), at(j, u, 2), at(j, u, 3));
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // no visible key: 0; NaN stays
+  const int d = p.heads * D, col0 = (kvh * G + hg) * D;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int u = 0; u < DB; ++u)
+      store_out4<T>(p.out, p.out_form, lo + qi, col0 + dim(j, u), d, at(j, u, 0) * inv,
+                    at(j, u, 1) * inv, at(j, u, 2) * inv, at(j, u, 3) * inv);
+}
+
+template <typename T, int D, int WR, int WK, int KT>
+__global__ __launch_bounds__(64 * WR * WK, (GroupedShape<T, D, WR, WK, KT>::kWavesPerSimd)) void
+attn_grouped_kernel(const GroupedArgs p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[GroupedShape<T, D, WR, WK, KT>::kLds];
+  grouped_block<T, D, WR, WK, KT>(p, blockIdx.x, lds);
+}
+
+struct MergeArgs {
+  const float* ws_o;
+  const float* ws_ml;
+  const int32_t* q_offset;   // of parts [0, n0)
+  void* out;
+  int n_seq, tokens, heads, max_q, n0, n1, out_form;
+};
+
+// Joins the parts of one output row (token, head) per wave: parts [0, n0) hold it if the token is
+// one of a sequence's first max_q, parts [n0, n0 + n1) always do.  Lane s reads the m and l of part
+// s (at most 64 parts); the values come eight parts at a time, in the parts' order.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
+  constexpr int C = D / 64;
+  const int64_t all = static_cast<int64_t>(p.tokens) * p.heads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 +
+                      __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= all) return;
+  const int lane = threadIdx.x & 63;
+  const int t = static_cast<int>(row / p.heads), head = static_cast<int>(row - static_cast<int64_t>(t) * p.heads);
+  // the last sequence that starts at or before the token
+  int a = 0, b = p.n_seq;
+  while (a < b) {
+    const int mid = (a + b) >> 1;
+    if (p.q_offset[mid] <= t) a = mid + 1; else b = mid;
+  }
+  bool held = a > 0;
+  if (held) {
+    const int first = max(p.q_offset[a - 1], 0);
+    held = t < p.q_offset[a] && t - first < p.max_q;
+  }
+  const int s0 = held ? 0 : p.n0, n = p.n0 + p.n1;
+  if (s0 >= n) return;   // the token is in no sequence: its row stays as it was
+  const int s = s0 + min(lane, n - s0 - 1);
+  const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + 2 * (s * all + row));
+  const bool live = lane < n - s0 && ml.x != -INFINITY;
+  const float top = wave_max(live ? ml.x : -INFINITY);
+  const float w = live ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
+  const uint64_t mask = __ballot(live);
+  const float L = wave_sum(live ? ml.y * w : 0.f);
+  float O[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) O[i] = 0.f;
+  for (int q0 = 0; q0 < n - s0; q0 += 8) {
+    float v[8][C];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float* src = p.ws_o + (min(s0 + q0 + q, n - 1) * all + row) * D + C * lane;
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[q][i] = src[i];
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (!((mask >> (q0 + q)) & 1u)) continue;   // a state without keys wrote no values
+      const float wq = from_lane(w, q0 + q);
+#pragma unroll
+      for (int i = 0; i < C; ++i) O[i] = fmaf(v[q][i], wq, O[i]);
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  const int d = p.heads * D, col = head * D + C * lane;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const float x = O[i] * inv;
+    if (p.out_form == kOutPlain) {
+      T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(t) * d + col + i;
+      if constexpr (sizeof(T) == 4)
+        *dst = x;
+      else
+        *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(f2bf(x));
+      continue;
+    }
+    const uint32_t hi = f2bf(x);
+    const uint16_t lo = static_cast<uint16_t>(f2bf(x - bf2f(hi)));
+    uint16_t* dst = static_cast<uint16_t*>(p.out);
+    if (p.out_form == kOutSplitTiles) {
+      dst[tile_off(t, col + i, 2 * d)] = static_cast<uint16_t>(hi);
+      dst[tile_off(t, d + col + i, 2 * d)] = lo;
+    } else {
+      dst[static_cast<int64_t>(t) * 2 * d + col + i] = static_cast<uint16_t>(hi);
+      dst[static_cast<int64_t>(t) * 2 * d + d + col + i] = lo;
+    }
+  }
+}
+
+constexpr int kMaxParts = 32;     // parts of one list of keys (a merge wave holds 64 states)
+constexpr int kFillBlocks = 512;  // two blocks on each of 256 CUs
+
+// How one list of tiles runs: tall blocks (4 waves, 128 rows) where they fill the GPU, otherwise
+// flat ones (32 rows, the waves share out the keys) and as many parts as fill it.
+struct Plan {
+  bool tall;
+  int n_tiles, n_split;
+};
+
+Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, bool may_split) {
+  Plan r;
+  r.tall = max_rows > 32 && pairs * ((max_rows + 127) / 128) >= kFillBlocks / 2;
+  r.n_tiles = static_cast<int>(r.tall ? (max_rows + 127) / 128 : (max_rows + 31) / 32);
+  const int64_t blocks = pairs * r.n_tiles;
+  const int64_t want = r.tall || !may_split ? 1 : (kFillBlocks + blocks - 1) / blocks;
+  const int64_t most = (slots + 255) / 256;   // a part of less than 256 keys is mostly its start
+  const int64_t ns = want < most ? want : most;
+  r.n_split = static_cast<int>(ns < 1 ? 1 : ns > kMaxParts ? kMaxParts : ns);
+  return r;
+}
+
+template <typename T, int D>
+int launch_tiles(const GroupedArgs& a, bool tall, hipStream_t st) {
+  const int64_t blocks = static_cast<int64_t>(a.n_seq) * a.kv_heads * a.n_tiles * a.n_split;
+  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  const unsigned n = static_cast<unsigned>(blocks);
+  constexpr bool f32 = sizeof(T) == 4;
+  constexpr int kTallKeys = f32 ? 32 : 64, kFlatGroups = f32 && D == 128 ? 2 : 4;
+  if (tall)
+    attn_grouped_kernel<T, D, 4, 1, kTallKeys><<<n, 256, 0, st>>>(a);
+  else
+    attn_grouped_kernel<T, D, 1, kFlatGroups, 32><<<n, 64 * kFlatGroups, 0, st>>>(a);
+  return launch_status();
+}
+
+int run_tiles(const GroupedArgs& a, bool tall, int dtype, int head_dim, hipStream_t st) {
+  if (dtype == MDL_DTYPE_F32)
+    return head_dim == 64 ? launch_tiles<float, 64>(a, tall, st)
+                          : launch_tiles<float, 128>(a, tall, st);
+  return head_dim == 64 ? launch_tiles<uint16_t, 64>(a, tall, st)
+                        : launch_tiles<uint16_t, 128>(a, tall, st);
+}
+
+int run_merge(const MergeArgs& m, int dtype, int head_dim, hipStream_t st) {
+  const int64_t blocks = (static_cast<int64_t>(m.tokens) * m.heads + 3) / 4;
+  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  const unsigned n = static_cast<unsigned>(blocks);
+  if (dtype == MDL_DTYPE_F32) {
+    if (head_dim == 64) attn_merge_kernel<float, 64><<<n, 256, 0, st>>>(m);
+    else attn_merge_kernel<float, 128><<<n, 256, 0, st>>>(m);
+  } else {
+    if (head_dim == 64) attn_merge_kernel<uint16_t, 64><<<n, 256, 0, st>>>(m);
+    else attn_merge_kernel<uint16_t, 128><<<n, 256, 0, st>>>(m);
+  }
+  return launch_status();
+}
+
+// sizes that both entries take
+int check_sizes(int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, int head_dim,
+                int dtype, int slots) {
+  if (head_dim != 64 && head_dim != 128) return MDL_ERR_HEAD_DIM;
+  if (dtype != MDL_DTYPE_F32 && dtype != MDL_DTYPE_BF16) return MDL_ERR_DTYPE;
+  if (n_seq < 0 || tokens < 0 || max_q < 0 || n_heads <= 0 || n_kv_heads <= 0 ||
+      n_heads % n_kv_heads != 0 || n_heads > 65536 || slots < 0 || slots > (1 << 30))
+    return MDL_ERR_SHAPE;
+  // row and pair numbers of a launch, and column numbers of a split row, are ints
+  const int64_t lim = 0x7fffffff;
+  if (static_cast<int64_t>(max_q) * (n_heads / n_kv_heads) + 128 > lim ||
+      static_cast<int64_t>(n_seq) * n_kv_heads > lim)
+    return MDL_ERR_SHAPE;
+  return MDL_OK;
+}
+
+int64_t state_bytes(int parts, int64_t rows, int head_dim) {
+  return parts * rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+}  // namespace
+
+}  // namespace mdl
+
+using namespace mdl;
+
+extern "C" int64_t mdl_attn_grouped_workspace_bytes(int n_seq, int tokens, int max_q, int n_heads,
+                                                    int n_kv_heads, int head_dim, int dtype,
+                                                    int cache_slots) {
+  if (check_sizes(n_seq, tokens, max_q, n_heads, n_kv_heads, head_dim, dtype, cache_slots) !=
+          MDL_OK || n_seq == 0 || max_q == 0)
+    return 0;
+  const Plan pl = plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
+                             static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), cache_slots,
+                             true);
+  return pl.n_split > 1 ? state_bytes(pl.n_split, static_cast<int64_t>(tokens) * n_heads, head_dim)
+                        : 0;
+}
+
+extern "C" int mdl_attn_grouped(const void* q, const void* k_cache, const void* v_cache, int dtype,
+                                int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads,
+                                int head_dim, int cache_slots, const int32_t* q_offset,
+                                const int32_t* kv_len, int causal, void* out, int out_form,
+                                float* workspace, int64_t workspace_bytes, void* stream) {
+  if (!q || !k_cache || !v_cache || !q_offset || !kv_len || !out) return MDL_ERR_NULL;
+  const int bad = check_sizes(n_seq, tokens, max_q, n_heads, n_kv_heads, head_dim, dtype,
+                              cache_slots);
+  if (bad != MDL_OK) return bad;
+  if (out_form < MDL_OUT_PLAIN || out_form > MDL_OUT_SPLIT_TILES) return MDL_ERR_SHAPE;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) ||
+      !aligned16(workspace) || !aligned4(q_offset) || !aligned4(kv_len))
+    return MDL_ERR_ALIGN;
+  if (n_seq == 0 || tokens == 0 || max_q == 0) return MDL_OK;
+  const Plan pl = plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
+                             static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), cache_slots,
+                             workspace != nullptr);
+  const int64_t rows = static_cast<int64_t>(tokens) * n_heads;
+  if (pl.n_split > 1 && workspace_bytes < state_bytes(pl.n_split, rows, head_dim))
+    return MDL_ERR_WORKSPACE;
+  GroupedArgs a{};
+  a.q = q; a.k = k_cache; a.v = v_cache; a.q_offset = q_offset; a.kv_len = kv_len; a.out = out;
+  a.n_seq = n_seq; a.tokens = tokens; a.heads = n_heads; a.kv_heads = n_kv_heads;
+  a.group = n_heads / n_kv_heads; a.slots = cache_slots; a.max_q = max_q; a.causal = causal ? 1 : 0;
+  a.n_tiles = pl.n_tiles; a.n_split = pl.n_split; a.out_form = out_form;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (pl.n_split > 1) {
+    a.ws_o = workspace;
+    a.ws_ml = workspace + pl.n_split * rows * head_dim;
+  }
+  const int rc = run_tiles(a, pl.tall, dtype, head_dim, st);
+  if (rc != MDL_OK || pl.n_split == 1) return rc;
+  MergeArgs m{a.ws_o, a.ws_ml, q_offset, out, n_seq, tokens, n_heads, max_q, pl.n_split, 0,
+              out_form};
+  return run_merge(m, dtype, head_dim, st);
+}
+
+namespace mdl {
+namespace {
+
+struct SharedPlan {
+  Plan prefix, own;
+};
+
+SharedPlan plan_shared(int batch, int n_prefix, int max_rows, int n_heads, int n_kv_heads,
+                       int prefix_slots, int cache_slots) {
+  const int64_t g = n_heads / n_kv_heads;
+  SharedPlan r;
+  r.prefix = plan_tiles(static_cast<int64_t>(n_prefix) * n_kv_heads, max_rows * g, prefix_slots,
+                        true);
+  r.own = plan_tiles(static_cast<int64_t>(batch) * n_kv_heads, g, cache_slots, true);
+  return r;
+}
+
+}  // namespace
+}  // namespace mdl
+
+extern "C" int64_t mdl_attn_decode_shared_workspace_bytes(int batch, int n_prefix, int max_rows,
+                                                          int n_heads, int n_kv_heads,
+                                                          int head_dim, int dtype,
+                                                          int prefix_slots, int cache_slots) {
+  if (check_sizes(n_prefix, batch, max_rows, n_heads, n_kv_heads, head_dim, dtype, prefix_slots) !=
+          MDL_OK ||
+      check_sizes(batch, batch, 1, n_heads, n_kv_heads, head_dim, dtype, cache_slots) != MDL_OK ||
+      batch == 0 || n_prefix == 0 || max_rows == 0)
+    return 0;
+  const SharedPlan pl = plan_shared(batch, n_prefix, max_rows, n_heads, n_kv_heads, prefix_slots,
+                                    cache_slots);
+  return state_bytes(pl.prefix.n_split + pl.own.n_split, static_cast<int64_t>(batch) * n_heads,
+                     head_dim);
+}
+
+extern "C" int mdl_attn_decode_shared(const void* q, const void* prefix_k, const void* prefix_v,
+                                      const int32_t* row_offset, const int32_t* prefix_len,
+                                      int n_prefix, int prefix_slots, int max_rows,
+                                      const void* k_cache, const void* v_cache,
+                                      const int32_t* kv_len, int batch, int cache_slots, int dtype,
+                                      int n_heads, int n_kv_heads, int head_dim, void* out,
+                                      int out_form, float* workspace, int64_t workspace_bytes,
+                                      void* stream) {
+  if (!q || !prefix_k || !prefix_v || !row_offset || !prefix_len || !k_cache || !v_cache ||
+      !kv_len || !out || !workspace)
+    return MDL_ERR_NULL;
+  int bad = check_sizes(n_prefix, batch, max_rows, n_heads, n_kv_heads, head_dim, dtype,
+                        prefix_slots);
+  if (bad == MDL_OK)
+    bad = check_sizes(batch, batch, 1, n_heads, n_kv_heads, head_dim, dtype, cache_slots);
+  if (bad != MDL_OK) return bad;
+  if (n_prefix == 0 || max_rows == 0 || out_form < MDL_OUT_PLAIN || out_form > MDL_OUT_SPLIT_TILES)
+    return MDL_ERR_SHAPE;
+  if (!aligned16(q) || !aligned16(prefix_k) || !aligned16(prefix_v) || !aligned16(k_cache) ||
+      !aligned16(v_cache) || !aligned16(out) || !aligned16(workspace) || !aligned4(row_offset) ||
+      !aligned4(prefix_len) || !aligned4(kv_len))
+    return MDL_ERR_ALIGN;
+  if (batch == 0) return MDL_OK;
+  const SharedPlan pl = plan_shared(batch, n_prefix, max_rows, n_heads, n_kv_heads, prefix_slots,
+                                    cache_slots);
+  const int64_t rows = static_cast<int64_t>(batch) * n_heads;
+  const int parts = pl.prefix.n_split + pl.own.n_split;
+  if (workspace_bytes < state_bytes(parts, rows, head_dim)) return MDL_ERR_WORKSPACE;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  GroupedArgs a{};
+  a.q = q; a.k = prefix_k; a.v = prefix_v; a.q_offset = row_offset; a.kv_len = prefix_len;
+  a.ws_o = workspace;
+  a.ws_ml = workspace + parts * rows * head_dim;
+  a.n_seq = n_prefix; a.tokens = batch; a.heads = n_heads; a.kv_heads = n_kv_heads;
+  a.group = n_heads / n_kv_heads; a.slots = prefix_slots; a.max_q = max_rows;
+  a.n_tiles = pl.prefix.n_tiles; a.n_split = pl.prefix.n_split;
+  int rc = run_tiles(a, pl.prefix.tall, dtype, head_dim, st);
+  if (rc != MDL_OK) return rc;
+  a.k = k_cache; a.v = v_cache; a.q_offset = nullptr; a.kv_len = kv_len;
+  a.n_seq = batch; a.slots = cache_slots; a.max_q = 1;
+  a.n_tiles = pl.own.n_tiles; a.n_split = pl.own.n_split; a.part0 = pl.prefix.n_split;
+  rc = run_tiles(a, pl.own.tall, dtype, head_dim, st);
+  if (rc != MDL_OK) return rc;
+  MergeArgs m{a.ws_o, a.ws_ml, row_offset, out, n_prefix, batch, n_heads, max_rows,
+              pl.prefix.n_split, pl.own.n_split, out_form};
+  return run_merge(m, dtype, head_dim, st);
+}

@@ -9,6 +9,7 @@ non-zero library status raises ``RuntimeError`` / ``ValueError``.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 
 import torch
 
@@ -1099,6 +1100,200 @@ def attn_decode_rope_noalloc(qkv: torch.Tensor, rstd: torch.Tensor, pos: torch.T
         prompt_len, _p(row_holes), _p(kv_start), _p(row_order), seq_pos, _p(seq_dev),
         split_len, _p(out), _layout(tiled), _stream()),
         "mdl_attn_decode_rope_noalloc")
+
+
+# --- grouped key / value heads (K7, K8) ----------------------------------------------------------
+
+GROUPED_HEAD_DIMS = (64, 128)
+
+
+def _one_device(first: torch.Tensor, *rest: torch.Tensor | None):
+    """A context in which the device of ``first`` is the current one, so that a launch goes to its
+    device and that device's current stream; every other tensor has to be there too."""
+    dev = first.device
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: one call runs on one device")
+    if dev.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _grouped_cache(k: torch.Tensor, v: torch.Tensor, name: str, rows: int, kv_heads: int | None,
+                   head_dim: int, dtype: torch.dtype) -> None:
+    """K and V caches [rows, kv_heads, slots, head_dim] of one shape and type."""
+    _need(k, f"{name}k", dtype)
+    _need(v, f"{name}v", dtype)
+    if (k.dim() != 4 or k.shape != v.shape or k.shape[0] != rows or k.shape[3] != head_dim or
+            (kv_heads is not None and k.shape[1] != kv_heads)):
+        raise ValueError(f"{name}k and {name}v must both be [{rows}, "
+                         f"{'n_kv_heads' if kv_heads is None else kv_heads}, slots, {head_dim}] "
+                         f"(got {tuple(k.shape)} and {tuple(v.shape)})")
+    if rows and k.numel() == 0:
+        raise ValueError(f"{name}k has no slots (got {tuple(k.shape)})")
+
+
+def _grouped_q(q: torch.Tensor) -> tuple[int, int, int]:
+    if q.dim() != 3 or q.shape[2] not in GROUPED_HEAD_DIMS:
+        raise ValueError(f"q must be [rows, n_heads, 64 or 128] (got {tuple(q.shape)})")
+    _need(q, "q", q.dtype)
+    cache_dtype_code(q)
+    return q.shape
+
+
+def _out_form(out: torch.Tensor, q: torch.Tensor, split: bool, tiled: bool) -> int:
+    rows, width = q.shape[0], q.shape[1] * q.shape[2]
+    if not split:
+        if tiled:
+            raise ValueError("the tile layout is a layout of the split output")
+        _need(out, "out", q.dtype)
+        if out.numel() != rows * width:
+            raise ValueError(f"out has {out.numel()} elements, needs {rows * width}")
+        return 0
+    _need(out, "out", BF16, split_numel(rows, width, tiled))
+    return 2 if tiled else 1
+
+
+def _ws(workspace: torch.Tensor | None) -> int:
+    _need(workspace, "workspace", F32, optional=True)
+    return 0 if workspace is None else workspace.numel() * 4
+
+
+def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.Tensor,
+                       rope_tab: torch.Tensor, rope_geom: tuple[int, int, int, int, int, int],
+                       q_gamma: torch.Tensor, k_gamma: torch.Tensor, eps: float,
+                       token_row: torch.Tensor, token_slot: torch.Tensor, q_scale: float,
+                       q_out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    """RMS norm of each query and key head of ``qkv`` [rows, (n_heads + 2 n_kv_heads) * D] (fp32 or
+    bf16; rows may be strided), times its gain, rotated by the token's position; q (times
+    ``q_scale``) to q_out [rows, n_heads, D], K and V (as it is) to slot token_slot[m] of cache row
+    token_row[m] of [batch, n_kv_heads, slots, D]; a slot or row outside the cache is not written.
+    q_out and the caches are bf16 or fp32.  ``rstd`` [rows]: a factor of each row before all else
+    (the ln1 scale).  With ``qkv_rope_cache_packed``'s table, positions and cache rules."""
+    if k_cache.dim() != 4 or k_cache.shape[3] not in GROUPED_HEAD_DIMS:
+        raise ValueError("k_cache must be [batch, n_kv_heads, slots, 64 or 128]")
+    batch, kv, slots, d = k_cache.shape
+    if qkv.dim() != 2:
+        raise ValueError("qkv must be [rows, (n_heads + 2 * n_kv_heads) * head_dim]")
+    rows, width = qkv.shape
+    heads = width // d - 2 * kv
+    if width % d or heads <= 0 or heads % kv:
+        raise ValueError(f"qkv rows of {width} do not hold a multiple of {kv} query heads, {kv} key "
+                         f"heads and {kv} value heads of {d}")
+    if not qkv.is_cuda or (width > 1 and qkv.stride(1) != 1):
+        raise ValueError("qkv must be a GPU tensor with contiguous rows")
+    ld = qkv.stride(0) if rows > 1 else width
+    _need(q_gamma, "q_gamma", F32, d)
+    _need(k_gamma, "k_gamma", F32, d)
+    _need(rstd, "rstd", F32, rows, optional=True)
+    _need(pos, "pos", I64, rows * 3)
+    mx, my, mz, px, py, pz = rope_geom
+    _need(rope_tab, "rope_tab", F32, 2 * (mx * px + my * py + mz * pz))
+    _need(token_row, "token_row", I32, rows)
+    _need(token_slot, "token_slot", I32, rows)
+    _grouped_cache(k_cache, v_cache, "cache ", batch, kv, d, k_cache.dtype)
+    _need(q_out, "q_out", k_cache.dtype, rows * heads * d)
+    in_dt, out_dt = cache_dtype_code(qkv), cache_dtype_code(k_cache)
+    if rows == 0:
+        return
+    with _one_device(qkv, rstd, pos, rope_tab, q_gamma, k_gamma, token_row, token_slot, q_out,
+                     k_cache, v_cache):
+        _lib.check(_lib.lib().mdl_qk_norm_rope_cache(
+            _p(qkv), in_dt, ld, _p(rstd), _p(pos), _p(rope_tab), rows, _p(token_row),
+            _p(token_slot), batch, heads, kv, d, mx, my, mz, px, py, pz, _p(q_gamma), _p(k_gamma),
+            eps, q_scale, _p(q_out), _p(k_cache), _p(v_cache), out_dt, slots, _stream()),
+            "mdl_qk_norm_rope_cache")
+
+
+def attn_grouped_workspace_bytes(q: torch.Tensor, k_cache: torch.Tensor, max_q: int) -> int:
+    """Bytes of ``attn_grouped``'s workspace for tensors of these shapes (0: none is used)."""
+    tokens, heads, d = _grouped_q(q)
+    return _lib.lib().mdl_attn_grouped_workspace_bytes(
+        k_cache.shape[0], tokens, max_q, heads, k_cache.shape[1], d, cache_dtype_code(q),
+        k_cache.shape[2])
+
+
+def attn_grouped(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 q_offset: torch.Tensor, kv_len: torch.Tensor, max_q: int, out: torch.Tensor,
+                 causal: bool = True, workspace: torch.Tensor | None = None, split: bool = False,
+                 tiled: bool = False) -> None:
+    """Attention of packed sequences over their cache rows, several query heads to a key / value
+    head.  q [tokens, n_heads, D] (bf16 or fp32, pre-scaled as for attn_prefill; D 64 or 128);
+    caches [n_seq, n_kv_heads, slots, D]; sequence s has the rows q_offset[s] .. q_offset[s + 1] - 1
+    (int32 [n_seq + 1], at most ``max_q``) and the keys in slots [0, kv_len[s]); with ``causal`` its
+    query i of n sees slots up to kv_len[s] - n + i.  A query that sees none gives 0; rows of no
+    sequence stay as they were.  out: q's type, [tokens, n_heads * D], or ``split`` (hi|lo bf16,
+    row-major or ``tiled``: a projection's input).  ``workspace`` (fp32,
+    attn_grouped_workspace_bytes; calls that overlap need one each) lets a call with few rows split
+    its keys."""
+    tokens, heads, d = _grouped_q(q)
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be [n_seq, n_kv_heads, slots, head_dim]")
+    n_seq, kv, slots = k_cache.shape[:3]
+    _grouped_cache(k_cache, v_cache, "cache ", n_seq, kv, d, q.dtype)
+    if kv == 0 or heads % kv:
+        raise ValueError(f"{heads} query heads do not divide over {kv} key / value heads")
+    if q_offset.numel() != n_seq + 1 or kv_len.numel() != n_seq:
+        raise ValueError(f"q_offset and kv_len must have {n_seq + 1} and {n_seq} elements")
+    _need(q_offset, "q_offset", I32)
+    _need(kv_len, "kv_len", I32)
+    form, ws_bytes = _out_form(out, q, split, tiled), _ws(workspace)
+    if tokens == 0 or n_seq == 0:
+        return
+    with _one_device(q, k_cache, v_cache, q_offset, kv_len, out, workspace):
+        _lib.check(_lib.lib().mdl_attn_grouped(
+            _p(q), _p(k_cache), _p(v_cache), cache_dtype_code(q), n_seq, tokens, max_q, heads, kv,
+            d, slots, _p(q_offset), _p(kv_len), int(causal), _p(out), form, _p(workspace),
+            ws_bytes, _stream()), "mdl_attn_grouped")
+
+
+def attn_decode_shared_workspace_bytes(q: torch.Tensor, prefix_k: torch.Tensor,
+                                       k_cache: torch.Tensor, max_rows: int) -> int:
+    """Bytes of ``attn_decode_shared``'s workspace for tensors of these shapes."""
+    batch, heads, d = _grouped_q(q)
+    return _lib.lib().mdl_attn_decode_shared_workspace_bytes(
+        batch, prefix_k.shape[0], max_rows, heads, k_cache.shape[1], d, cache_dtype_code(q),
+        prefix_k.shape[2], k_cache.shape[2])
+
+
+def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
+                       row_offset: torch.Tensor, prefix_len: torch.Tensor, max_rows: int,
+                       k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
+                       out: torch.Tensor, workspace: torch.Tensor, split: bool = False,
+                       tiled: bool = False) -> None:
+    """Decode attention (one query a row) of rows that share prefixes: row b of group g sees slots
+    [0, prefix_len[g]) of prefix g and slots [0, kv_len[b]) of its own cache row.  q [batch,
+    n_heads, D]; prefixes [n_prefix, n_kv_heads, prefix_slots, D]; caches [batch, n_kv_heads, slots,
+    D]; group g has the rows row_offset[g] .. row_offset[g + 1] - 1 (int32 [n_prefix + 1], at most
+    ``max_rows``).  ``workspace``: fp32, attn_decode_shared_workspace_bytes.  Otherwise as
+    attn_grouped."""
+    batch, heads, d = _grouped_q(q)
+    if prefix_k.dim() != 4 or prefix_k.shape[0] == 0 or prefix_k.shape[1] == 0:
+        raise ValueError("prefix_k must be [n_prefix, n_kv_heads, prefix_slots, head_dim]")
+    n_prefix, kv, p_slots = prefix_k.shape[:3]
+    _grouped_cache(prefix_k, prefix_v, "prefix_", n_prefix, kv, d, q.dtype)
+    _grouped_cache(k_cache, v_cache, "cache ", batch, kv, d, q.dtype)
+    if heads % kv:
+        raise ValueError(f"{heads} query heads do not divide over {kv} key / value heads")
+    if row_offset.numel() != n_prefix + 1 or prefix_len.numel() != n_prefix:
+        raise ValueError(f"row_offset and prefix_len must have {n_prefix + 1} and {n_prefix} "
+                         "elements")
+    if kv_len.numel() != batch:
+        raise ValueError(f"kv_len must have {batch} elements")
+    _need(row_offset, "row_offset", I32)
+    _need(prefix_len, "prefix_len", I32)
+    _need(kv_len, "kv_len", I32)
+    _need(workspace, "workspace", F32)
+    form, ws_bytes = _out_form(out, q, split, tiled), _ws(workspace)
+    if batch == 0:
+        return
+    with _one_device(q, prefix_k, prefix_v, row_offset, prefix_len, k_cache, v_cache, kv_len, out,
+                     workspace):
+        _lib.check(_lib.lib().mdl_attn_decode_shared(
+            _p(q), _p(prefix_k), _p(prefix_v), _p(row_offset), _p(prefix_len), n_prefix, p_slots,
+            max_rows, _p(k_cache), _p(v_cache), _p(kv_len), batch, k_cache.shape[2],
+            cache_dtype_code(q), heads, kv, d, _p(out), form, _p(workspace), ws_bytes, _stream()),
+            "mdl_attn_decode_shared")
 
 
 class HeadConstraints:
