@@ -63,12 +63,13 @@ struct GroupedArgs {
 // Chunk swizzle of a tile row (16-byte chunks), by its low 4 bits r3..r0.  Both reads are then free
 // of bank conflicts whether 16-byte reads go 8 lanes a cycle and transposing ones 16 (32 banks) or
 // 16 and 32 (64 banks): 8 and 16 rows of one chunk, and 4 rows of a 32-byte or 64-byte run.
+// bf16, D = 128: bits r2, r0, r1, r0 ^ r3 of the chunk (lowest first); D = 64: r2, r0 ^ r3, r1.
 template <typename T, int D>
 __device__ __forceinline__ constexpr int swz(int r) {
   if (sizeof(T) == 4) return r & 15;
-  const int r0 = r & 1, r1 = (r >> 1) & 1, r2 = (r >> 2) & 1, r3 = (r >> 3) & 1;
-  return D == 128 ? r2 | (r0 << 1) | (r1 << 2) | ((r0 ^ r3) << 3)
-                  : r2 | ((r0 ^ r3) << 1) | (r1 << 2);
+  // the value of row r in bits 4 r .. 4 r + 3
+  constexpr uint64_t kTable = D == 128 ? 0x7d396c28f5b1e4a0ull : 0x5713460275316420ull;
+  return static_cast<int>(kTable >> (4 * r)) & 15;
 }
 
 __device__ __forceinline__ float other_half(float v) {   // the value of lane ^ 32
@@ -85,6 +86,21 @@ __device__ __forceinline__ float max_halves(float v) {
 
 __device__ __forceinline__ f32x16_t splat16(float v) {
   return f32x16_t{v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v};
+}
+
+// At most N of the wave's copies (and other vector memory operations) are outstanding.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// The wave's LDS reads have returned.
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// l + the two bf16 of w
+__device__ __forceinline__ float add_pair(float l, uint32_t w) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w),
+                                         __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
 }
 
 // Four consecutive channels `col` .. + 3 of output row `row` (width `d` = heads * D).
@@ -120,8 +136,13 @@ struct GroupedShape {
   static constexpr int kRows = 32 * WR;                   // rows of a block
   static constexpr int kCopies = kTile / 1024 / WR;       // 1 KB copies of a wave, K or V
   static constexpr int kRowsPerCopy = 1024 / kRowBytes;
+  // registers for as many waves as LDS lets reside (four per CU are one per SIMD), at most three;
   // fp32 with 128 dims: q and the output alone are 128 registers
-  static constexpr int kWavesPerSimd = kLds > 80 * 1024 || kRowBytes == 512 ? 1 : 2;
+  static constexpr int kResident = 160 * 1024 / kLds * WR * WK / 4;
+  static constexpr int kWavesPerSimd = kRowBytes == 512 || kResident < 2 ? 1
+                                       : kRowBytes == 128 && WR > 1      ? 3
+                                                                         : 2;
+  static_assert(WR > 1 || 3 * kCopies < 63, "copies in flight fit the counter");
   static_assert(kTile % (1024 * WR) == 0, "whole copies per wave");
   static_assert(KT % 32 == 0 && (D == 64 || D == 128), "whole MFMA blocks");
   // the merge of the groups goes through the ring's memory
@@ -133,11 +154,17 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   using S = GroupedShape<T, D, WR, WK, KT>;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int NB = KT / 32, DB = D / 32;
+  // Blocks go to the XCDs in turn.  A pair (sequence, key / value head) keeps to one XCD, whose L2
+  // then serves its row tiles, for a sixteenth of the tiles (at least four) and moves on to the next:
+  // sequences differ in length, and pairs that stayed would leave some XCDs with the long ones.  Four
+  // prompts of 3,900 to 6,000 tokens, 16 heads of 64: 294 us staying, 261 so; two of up to 8,192, 32
+  // heads of 128 (eight pairs each, nothing to balance): 901, and 980 moving at every tile.
   const int pairs = p.n_seq * p.kv_heads;
-  const int rest = block / pairs, pair = block - rest * pairs;
-  const int seq = pair / p.kv_heads, kvh = pair - seq * p.kv_heads;
+  const int rest = block / pairs, idx = block - rest * pairs;
   const int rank = rest / p.n_split, split = rest - rank * p.n_split;
   const int tile = p.n_tiles - 1 - rank;   // the latest rows, with the most keys, first
+  const int pair = (idx + ((block - idx) & 7) + rank / max(4, p.n_tiles / 16)) % pairs;
+  const int seq = pair / p.kv_heads, kvh = pair - seq * p.kv_heads;
   int lo = seq, hi = seq + 1;
   if (p.q_offset) {
     lo = min(max(p.q_offset[seq], 0), p.tokens);
@@ -154,15 +181,23 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave % WR, wk = wave / WR;
   // the limits of the block's last row, this lane's row, and the wave's first and last
-  auto limit = [&](int r) { return p.causal ? len - n + r / G : len - 1; };
-  const int kend = max(limit(min(r0 + S::kRows, rows) - 1) + 1, 0);
+  // (row r's query is r / G: q0 + (r - G q0) / G with q0 = r0 / G, the small quotient in fp32, exact
+  // below 2^20: (x + 1/2) / G is at least 1 / (2 G) away from a whole number)
+  const int q0 = r0 / G;
+  const float inv_g = 1.f / G;
+  auto query = [&](int r) {
+    return q0 + static_cast<int>((static_cast<float>(r - G * q0) + 0.5f) * inv_g);
+  };
+  auto limit = [&](int q) { return p.causal ? len - n + q : len - 1; };
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int kend = uniform(max(limit(query(min(r0 + S::kRows, rows) - 1)) + 1, 0));
   const int w0 = r0 + 32 * wr;
   const int row = w0 + c;
   const bool real = row < rows;
-  const int qi = min(row, rows - 1) / G, hg = min(row, rows - 1) - qi * G;
-  const int lim = real ? limit(row) : -1;
-  const int lim_lo = w0 < rows ? limit(w0) : -1;
-  const int lim_hi = w0 < rows ? limit(min(w0 + 32, rows) - 1) : -1;
+  const int qi = query(min(row, rows - 1)), hg = min(row, rows - 1) - qi * G;
+  const int lim = real ? limit(qi) : -1;
+  const int lim_lo = uniform(w0 < rows ? limit(query(w0)) : -1);
+  const int lim_hi = uniform(w0 < rows ? limit(query(min(w0 + 32, rows) - 1)) : -1);
   // keys of this part, in whole turns of the groups
   constexpr int kTurn = KT * WK;
   const int per = ((kend + p.n_split - 1) / p.n_split + kTurn - 1) / kTurn * kTurn;
@@ -192,20 +227,24 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   // Copy j of a tile: rows (1024 / row bytes) j .. of K and of V, one kilobyte each; a lane takes
   // physical chunk lane % chunks of its row.  Rows past the last key copy that key.
   constexpr int kChunks = S::kRowBytes / 16;
-  auto issue = [&](int kt, int st) {
-    const T* kb = scalar_ptr(Kg + static_cast<int64_t>(kt) * D);
-    const T* vb = scalar_ptr(Vg + static_cast<int64_t>(kt) * D);
+  auto issue = [&](const T* src, int kt, uint32_t at) {
+    const T* from = scalar_ptr(src + static_cast<int64_t>(kt) * D);
 #pragma unroll
     for (int jj = 0; jj < S::kCopies; ++jj) {
       const int j = wr + WR * jj;
       const int r = S::kRowsPerCopy * j + lane / kChunks;
       const uint32_t off = min(r, kend - 1 - kt) * S::kRowBytes +
                            16 * ((lane % kChunks) ^ swz<T, D>(r & 15));
-      const uint32_t dst = ring0 + st * 2 * S::kTile + 1024 * j;
-      dma16_sbase(kb, off, __builtin_amdgcn_readfirstlane(dst));
-      dma16_sbase(vb, off, __builtin_amdgcn_readfirstlane(dst + S::kTile));
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + at + 1024 * j);
+      if constexpr (WR == 1)
+        dma16_stream(from, off, dst);
+      else
+        dma16_sbase(from, off, dst);
     }
   };
+  // slots of a ring: K of stage 0 and 1, V of stage 0 and 1
+  auto k_slot = [](int st) { return st * S::kTile; };
+  auto v_slot = [](int st) { return (2 + st) * S::kTile; };
 
   // Lane parts of the swizzled read addresses.  K operand: row c, bf16 chunk 2 s + h, fp32 chunk
   // h D / 8 + s.  V^T operand, bf16: rows 4 h + lane / 4 % 4 (and + 8) of a 16-key step, dims
@@ -223,6 +262,10 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
                     16 * ((vchunk + 4 * db) ^ swz<T, D>(vr + 8 * e)) + 8 * (lane & 1);
 
   float negm = 0.f, thr = -INFINITY, l = 0.f;   // l: this lane half's part of the sum
+  // minus the reference in every element, kept where registers allow (2 x 12 moves a tile less: 941 ->
+  // 908 us on two prompts of up to 8,192 tokens, 32 heads of 128; nothing with 64 dims)
+  constexpr bool kKeepStart = !kF32 && D == 128 && WR > 1;
+  f32x16_t start = splat16(0.f);
   f32x16_t o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = splat16(0.f);
@@ -234,10 +277,42 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  // V operands `va` of the 16 keys from kk on, of which not every row sees all: keys past lim_hi
-  // become zeros; if a value that is left is not finite, each set of rows with one limit gets a
-  // product over its own keys here and the operands become zeros.
-  auto masked_step = [&](uint4 (&va)[DB], int kk, const bf16x8_t& pb) {
+  // o += w V of the key at row `kr` of a V tile, for the rows that see it (`sees`); w is the row's
+  // weight, in lane half `half` of its lane.  Key by key and channel by channel: for keys with a
+  // value that is not finite, which a product over several keys would give to every row.
+  auto add_key = [&](const uint8_t* Vt, int kr, int half, float w, bool sees) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(w), __float_as_uint(w),
+                                                       false, false);
+    const float x = __uint_as_float(half ? both[1] : both[0]);
+    const uint8_t* base = Vt + kr * S::kRowBytes;
+    const int sw = swz<T, D>(kr & 15);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int u = 0; u < DB; ++u) {
+        float v[4];   // channels of elements 4 j .. + 3 of block u (bf16), of all blocks (fp32)
+        if constexpr (kF32) {
+          const float4 t = *reinterpret_cast<const float4*>(
+              base + 16 * ((DB * (2 * j + h) + u) ^ sw));
+          v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+        } else {
+          const uint2 t = *reinterpret_cast<const uint2*>(base + 16 * ((4 * u + j) ^ sw) + 8 * h);
+          v[0] = bf2f(t.x & 0xffffu); v[1] = bf2f(t.x >> 16);
+          v[2] = bf2f(t.y & 0xffffu); v[3] = bf2f(t.y >> 16);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int q = 4 * u + e;
+          const int block = kF32 ? q % DB : u, i = 4 * j + (kF32 ? q / DB : e);
+          o[block][i] = sees ? fmaf(x, v[e], o[block][i]) : o[block][i];
+        }
+      }
+  };
+
+  // V operands `va` of the 16 keys from kk on (tile rows from `key` on), of which not every row sees
+  // all: keys past lim_hi become zeros; if a value that is left is not finite, the step is worked on
+  // here and the operands become zeros.
+  auto masked_step = [&](uint4 (&va)[DB], const uint8_t* Vt, int kk, int key, uint32_t p0, uint32_t p1, uint32_t p2, uint32_t p3) {
     uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -252,25 +327,9 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     }
     if (__ballot((odd & 0x80008000u) != 0) == 0) return;
 #pragma unroll 1
-    for (int e = 0; e < 16; ++e) {   // the rows that see keys up to kk + e of this step
-      const bool mine = e == 15 ? lim >= kk + 15 : lim == kk + e;
-      if (__ballot(mine) == 0) continue;
-      uint32_t see[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = 4 * h + 8 * (i >> 1) + 2 * (i & 1);
-        see[i] = (k <= e ? 0xffffu : 0u) | (k + 1 <= e ? 0xffff0000u : 0u);
-      }
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const uint4 a = make_uint4(va[db].x & see[0], va[db].y & see[1], va[db].z & see[2],
-                                   va[db].w & see[3]);
-        const f32x16_t t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), pb, splat16(0.f),
-                                                                   0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[db][i] += mine ? t[i] : 0.f;
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int e = 0; e < 16 && kk + e <= lim_hi; ++e) {
+      const uint32_t w = (e & 8) != 0 ? ((e & 2) != 0 ? p3 : p2) : ((e & 2) != 0 ? p1 : p0);
+      add_key(Vt, key + e, (e >> 2) & 1, bf2f(e & 1 ? w >> 16 : w & 0xffffu), lim >= kk + e);
     }
 #pragma unroll
     for (int db = 0; db < DB; ++db) va[db] = make_uint4(0, 0, 0, 0);
@@ -294,7 +353,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   };
 
   // The fp32 form of masked_step, for a whole tile: true if it holds values that are not finite in
-  // slots that some row sees; its product is then added here, each row over its own keys.
+  // slots that some row sees; its product is then added here.
   auto masked_tile = [&](const uint8_t* Vt, int kt, const f32x16_t& pr) -> bool {
     bool odd = false;
 #pragma unroll
@@ -307,35 +366,23 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     }
     if (__ballot(odd) == 0) return false;
 #pragma unroll 1
-    for (int r = 0; r < 16; ++r) {   // keys ka and ka + 4: a row sees both, the first, or none
-      const int ka = kt + (r & 3) + 8 * (r >> 2);
-      float v[DB], x = pr[0];
-      v_pair(Vt, kt, ka - kt + 4 * h, lim_hi, v);
+    for (int e = 0; e < 32 && kt + e <= lim_hi; ++e) {
+      const int r = (e & 3) + 4 * (e >> 3);   // element of key e, in lane half e / 4 % 2
+      float w = pr[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) x = r == i ? pr[i] : x;
-      const bool two = lim >= ka + 4, one = lim >= ka && !two;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const f32x16_t t2 = __builtin_amdgcn_mfma_f32_32x32x2f32(v[db], x, splat16(0.f), 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[db][i] += two ? t2[i] : 0.f;
-        __builtin_amdgcn_sched_barrier(0);
-        const f32x16_t t1 = __builtin_amdgcn_mfma_f32_32x32x2f32(h ? 0.f : v[db], x, splat16(0.f),
-                                                                 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[db][i] += one ? t1[i] : 0.f;
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      for (int i = 1; i < 16; ++i) w = r == i ? pr[i] : w;
+      add_key(Vt, e, (e >> 2) & 1, w, lim >= kt + e);
     }
     return true;
   };
 
-  auto compute = [&](const uint8_t* Kt, const uint8_t* Vt, int kt) {
-    const bool masked = kt + KT - 1 > lim_lo;   // some row does not see the whole tile
+  auto compute = [&](const uint8_t* Kt, const uint8_t* Vt, int kt, auto fullc, auto after_qk) {
+    // some row does not see the whole tile
+    const bool masked = !decltype(fullc)::value && kt + KT - 1 > lim_lo;
     f32x16_t sc[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      sc[nb] = splat16(negm);
+      sc[nb] = kKeepStart ? start : splat16(negm);
 #pragma unroll
       for (int s = 0; s < NQ; ++s) {
         const int chunk = kF32 ? h * (D / 8) + s : 2 * s + h;
@@ -353,8 +400,11 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
         }
       }
     }
+    after_qk();
     if (masked) {
-      const int x = lim - kt - 4 * h;   // the last visible key, from this lane half's first
+      int x = lim - kt - 4 * h;   // the last visible key, from this lane half's first
+      // a value made here keeps this a branch: as selects it would cost every tile 60 instructions
+      asm volatile("" : "+v"(x));
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -372,6 +422,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
         const bool fresh = thr == -INFINITY;
         const float alpha = fresh ? 0.f : __builtin_amdgcn_exp2f(-tmax);
         negm = fresh ? -tmax : negm - tmax;
+        if constexpr (kKeepStart) start = splat16(negm);
         thr = kGap;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) sc[nb] -= tmax;
@@ -409,15 +460,15 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
           const bf16x8_t pb = {(__bf16)t[8 * s], (__bf16)t[8 * s + 1], (__bf16)t[8 * s + 2],
                                (__bf16)t[8 * s + 3], (__bf16)t[8 * s + 4], (__bf16)t[8 * s + 5],
                                (__bf16)t[8 * s + 6], (__bf16)t[8 * s + 7]};
-          // the sum of the rounded weights that the product below takes
-#pragma unroll
-          for (int i = 0; i < 8; ++i) l += (float)pb[i];
+          // the sum of the rounded weights that the product below takes, a pair at a time
+          const uint4 pw = __builtin_bit_cast(uint4, pb);
+          l = add_pair(add_pair(add_pair(add_pair(l, pw.x), pw.y), pw.z), pw.w);
           uint4 va[DB];
 #pragma unroll
           for (int db = 0; db < DB; ++db)
             va[db] = __builtin_bit_cast(uint4, vt_frag(Vt, key, db));
           __builtin_amdgcn_sched_barrier(0);
-          if (kt + key + 15 > lim_lo) masked_step(va, kt + key, pb);
+          if (masked && kt + key + 15 > lim_lo) masked_step(va, Vt, kt + key, key, pw.x, pw.y, pw.z, pw.w);
 #pragma unroll
           for (int db = 0; db < DB; ++db)
             o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(va[db]), pb, o[db], 0, 0, 0);
@@ -425,27 +476,86 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     }
   };
 
-  // Turns: group wk's tile of a turn is k0 + KT wk past it.  Every wave of the block makes the same
-  // number of them, so the barriers match.
+  // Tiles first + i kTurn are this group's.  Tiles that every row of a wave sees whole come first, in
+  // a loop of their own: it is free of branches, and the output stays in the same registers, which a
+  // choice inside one loop costs.  Tiles go two at a time, so that their stage is a constant.
   const int first = k0 + KT * wk;
-  if (first < k1) issue(first, 0);
-  auto turn = [&](int kt, auto stc) {
-    constexpr int ST = decltype(stc)::value;
-    // tile kt has landed for every wave of the group, which are done with the other stage; a group
-    // of one wave needs no barrier.  The builtin wait also covers the loads the compiler knows of.
-    __builtin_amdgcn_s_waitcnt(kWaitAll);
-    if constexpr (WR > 1)
+  constexpr std::integral_constant<int, 0> kEven{};
+  constexpr std::integral_constant<int, 1> kOdd{};
+  if constexpr (WR > 1) {
+    if (first < k1) {
+      issue(Kg, first, k_slot(0));
+      issue(Vg, first, v_slot(0));
+    }
+    // every wave of the block makes the same number of turns, so the barriers match
+    auto turn = [&](int kt, auto stc, auto fullc) {
+      constexpr int ST = decltype(stc)::value;
+      // tile kt has landed for every wave, and every wave is done with the other stage.  The builtin
+      // wait also covers the loads that the compiler knows of.
+      __builtin_amdgcn_s_waitcnt(kWaitAll);
       asm volatile("s_barrier" ::: "memory");
-    else
-      asm volatile("" ::: "memory");   // no read of the tile moves above the wait
-    if (kt + kTurn < k1) issue(kt + kTurn, ST ^ 1);
-    if (kt >= k1 || kt > lim_hi) return;   // past the part, or no row of the wave sees a key
-    const uint8_t* Kt = ring + ST * 2 * S::kTile;
-    compute(Kt, Kt + S::kTile, kt);
-  };
-  for (int t = k0; t < k1; t += 2 * kTurn) {
-    turn(t + KT * wk, std::integral_constant<int, 0>{});
-    if (t + kTurn < k1) turn(t + kTurn + KT * wk, std::integral_constant<int, 1>{});
+      if (kt + kTurn < k1) {
+        issue(Kg, kt + kTurn, k_slot(ST ^ 1));
+        issue(Vg, kt + kTurn, v_slot(ST ^ 1));
+      }
+      // past the part, or no row of the wave sees a key
+      if (!decltype(fullc)::value && (kt >= k1 || kt > lim_hi)) return;
+      compute(ring + k_slot(ST), ring + v_slot(ST), kt, fullc, [] {});
+    };
+    int t = k0;
+    for (; t + 2 * kTurn <= k1 && t + kTurn + KT * (wk + 1) - 1 <= lim_lo; t += 2 * kTurn) {
+      turn(t + KT * wk, kEven, std::true_type{});
+      turn(t + kTurn + KT * wk, kOdd, std::true_type{});
+    }
+    for (; t < k1; t += 2 * kTurn) {
+      turn(t + KT * wk, kEven, std::false_type{});
+      if (t + kTurn < k1) turn(t + kTurn + KT * wk, kOdd, std::false_type{});
+    }
+  } else {
+    // A wave with a ring of its own needs no barrier, and refills K's slot as soon as its scores are
+    // there and V's after the product: three of the four slots are in flight.  Copies land in the
+    // order they were issued in, K V K V .., so a wait names how many may be outstanding.
+    constexpr int C = S::kCopies;
+    const int nt = first < k1 ? (k1 - first + kTurn - 1) / kTurn : 0;
+    for (int i = 0; i < 2 && i < nt; ++i) {
+      issue(Kg, first + i * kTurn, k_slot(i));
+      issue(Vg, first + i * kTurn, v_slot(i));
+    }
+    // a wait that the compiler sees, for q: it would wait for q inside the loop otherwise, and with
+    // it for every copy
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    auto step = [&](int i, auto stc, auto fullc) {
+      constexpr int ST = decltype(stc)::value;
+      const int kt = first + i * kTurn;
+      if (i + 1 < nt)
+        wait_copies<3 * C>();
+      else
+        wait_copies<C>();
+      compute(ring + k_slot(ST), ring + v_slot(ST), kt, fullc, [&] {
+        if (i + 2 < nt) {
+          wait_reads();   // of K's slot
+          issue(Kg, kt + 2 * kTurn, k_slot(ST));
+          wait_copies<3 * C>();
+        } else if (i + 1 < nt) {
+          wait_copies<2 * C>();
+        } else {
+          wait_copies<0>();
+        }
+      });
+      if (i + 2 < nt) {
+        wait_reads();     // of V's slot
+        issue(Vg, kt + 2 * kTurn, v_slot(ST));
+      }
+    };
+    int i = 0;
+    for (; i + 2 <= nt && first + (i + 1) * kTurn + KT - 1 <= lim_lo; i += 2) {
+      step(i, kEven, std::true_type{});
+      step(i + 1, kOdd, std::true_type{});
+    }
+    for (; i < nt; i += 2) {
+      step(i, kEven, std::false_type{});
+      if (i + 1 < nt) step(i + 1, kOdd, std::false_type{});
+    }
   }
 
   l += other_half(l);
@@ -605,21 +715,27 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
 }
 
 constexpr int kMaxParts = 32;     // parts of one list of keys (a merge wave holds 64 states)
-constexpr int kFillBlocks = 512;  // two blocks on each of 256 CUs
+constexpr int kFlatFill = 512;    // blocks that fill the GPU: flat ones of 128 threads
+constexpr int kTallFill = 256;    // and tall ones of 256
 
-// How one list of tiles runs: tall blocks (4 waves, 128 rows) where they fill the GPU, otherwise
-// flat ones (32 rows, the waves share out the keys) and as many parts as fill it.
+// How one list of tiles runs: tall blocks (4 waves, 128 rows) or flat ones (32 rows, two waves that
+// share out the keys), and in how many parts the keys are cut.  Tall blocks read a key a quarter as
+// often; flat ones are more, with fewer rows to wait for.  So: tall where they fill the GPU uncut, and
+// where flat ones would have to be cut too; flat in between.  us, flat / tall: 704 flat blocks of a
+// 700-token prompt 23 / 30 (in two parts); 72 of 17 tokens behind 4,099 keys 21 / 19; 64 of 64
+// samples behind 32,749 keys (with their own keys and the merge) 117 / 73.
 struct Plan {
   bool tall;
   int n_tiles, n_split;
 };
 
 Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, bool may_split) {
+  const int64_t tall = pairs * ((max_rows + 127) / 128), flat = pairs * ((max_rows + 31) / 32);
   Plan r;
-  r.tall = max_rows > 32 && pairs * ((max_rows + 127) / 128) >= kFillBlocks / 2;
+  r.tall = max_rows > 32 && (tall >= kTallFill || (may_split && flat < kFlatFill));
   r.n_tiles = static_cast<int>(r.tall ? (max_rows + 127) / 128 : (max_rows + 31) / 32);
-  const int64_t blocks = pairs * r.n_tiles;
-  const int64_t want = r.tall || !may_split ? 1 : (kFillBlocks + blocks - 1) / blocks;
+  const int64_t blocks = r.tall ? tall : flat, fill = r.tall ? kTallFill : kFlatFill;
+  const int64_t want = may_split ? (fill + blocks - 1) / blocks : 1;
   const int64_t most = (slots + 255) / 256;   // a part of less than 256 keys is mostly its start
   const int64_t ns = want < most ? want : most;
   r.n_split = static_cast<int>(ns < 1 ? 1 : ns > kMaxParts ? kMaxParts : ns);
@@ -632,7 +748,7 @@ int launch_tiles(const GroupedArgs& a, bool tall, hipStream_t st) {
   if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
   const unsigned n = static_cast<unsigned>(blocks);
   constexpr bool f32 = sizeof(T) == 4;
-  constexpr int kTallKeys = f32 ? 32 : 64, kFlatGroups = f32 && D == 128 ? 2 : 4;
+  constexpr int kTallKeys = f32 ? 32 : 64, kFlatGroups = sizeof(T) * D == 512 ? 1 : 2;
   if (tall)
     attn_grouped_kernel<T, D, 4, 1, kTallKeys><<<n, 256, 0, st>>>(a);
   else

@@ -47,6 +47,12 @@ __device__ __forceinline__ void dma16_sbase(const void* base, uint32_t off, uint
                :: "v"(off), "s"(base), "s"(lds) : "memory");
 }
 
+// dma16_sbase with the non-temporal hint, for data that a launch reads once (common.h, load_nt16).
+__device__ __forceinline__ void dma16_stream(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+               :: "v"(off), "s"(base), "s"(lds) : "memory");
+}
+
 // A wave-uniform pointer in scalar registers, also where the compiler computed it in vector ones.
 template <typename T>
 __device__ __forceinline__ const T* scalar_ptr(const T* p) {

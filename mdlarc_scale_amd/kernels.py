@@ -1107,56 +1107,56 @@ def attn_decode_rope_noalloc(qkv: torch.Tensor, rstd: torch.Tensor, pos: torch.T
 GROUPED_HEAD_DIMS = (64, 128)
 
 
-def _one_device(first: torch.Tensor, *rest: torch.Tensor | None):
-    """A context in which the device of ``first`` is the current one, so that a launch goes to its
-    device and that device's current stream; every other tensor has to be there too."""
-    dev = first.device
-    for t in rest:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}: one call runs on one device")
-    if dev.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(dev)
+def _need_all(dev: int, specs) -> None:
+    """``_need`` for (tensor, name, dtype, elements) specs, all on GPU ``dev``; None where a tensor
+    is optional.  One plain loop: these calls take tens of microseconds in all."""
+    if dev < 0:
+        raise ValueError("q must be a GPU tensor")
+    for t, name, dtype, numel in specs:
+        if t is None or (t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and
+                         t.numel() >= numel):
+            continue
+        _need(t, name, dtype, numel)
+        raise ValueError(f"{name} is on {t.device}, another tensor on GPU {dev}: one call runs on "
+                         "one device")
 
 
-def _grouped_cache(k: torch.Tensor, v: torch.Tensor, name: str, rows: int, kv_heads: int | None,
-                   head_dim: int, dtype: torch.dtype) -> None:
-    """K and V caches [rows, kv_heads, slots, head_dim] of one shape and type."""
-    _need(k, f"{name}k", dtype)
-    _need(v, f"{name}v", dtype)
-    if (k.dim() != 4 or k.shape != v.shape or k.shape[0] != rows or k.shape[3] != head_dim or
-            (kv_heads is not None and k.shape[1] != kv_heads)):
-        raise ValueError(f"{name}k and {name}v must both be [{rows}, "
-                         f"{'n_kv_heads' if kv_heads is None else kv_heads}, slots, {head_dim}] "
-                         f"(got {tuple(k.shape)} and {tuple(v.shape)})")
-    if rows and k.numel() == 0:
-        raise ValueError(f"{name}k has no slots (got {tuple(k.shape)})")
+def _on_device(dev: int):
+    """A context in which GPU ``dev`` is the current device, as a launch on its stream needs."""
+    return nullcontext() if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
-def _grouped_q(q: torch.Tensor) -> tuple[int, int, int]:
+def _cache_shapes(k: torch.Tensor, v: torch.Tensor, name: str, want: tuple) -> None:
+    """K and V caches [rows, kv_heads, slots, head_dim] of one shape; ``want`` without the slots."""
+    shape = k.shape
+    if shape != v.shape or len(shape) != 4 or (shape[0], shape[1], shape[3]) != want:
+        raise ValueError(f"{name}k and {name}v must both be [{want[0]}, {want[1]}, slots, "
+                         f"{want[2]}] (got {tuple(shape)} and {tuple(v.shape)})")
+    if shape[0] and not shape[2]:
+        raise ValueError(f"{name}k has no slots (got {tuple(shape)})")
+
+
+def _grouped_q(q: torch.Tensor, k: torch.Tensor) -> tuple[int, int, int, int]:
+    """rows, n_heads, head_dim of q and n_kv_heads of the cache k."""
     if q.dim() != 3 or q.shape[2] not in GROUPED_HEAD_DIMS:
         raise ValueError(f"q must be [rows, n_heads, 64 or 128] (got {tuple(q.shape)})")
-    _need(q, "q", q.dtype)
-    cache_dtype_code(q)
-    return q.shape
+    rows, heads, d = q.shape
+    kv = k.shape[1] if k.dim() == 4 else 0
+    if kv == 0 or heads == 0 or heads % kv:
+        raise ValueError(f"{heads} query heads do not divide over the key / value heads of "
+                         f"{tuple(k.shape)}")
+    return rows, heads, d, kv
 
 
-def _out_form(out: torch.Tensor, q: torch.Tensor, split: bool, tiled: bool) -> int:
-    rows, width = q.shape[0], q.shape[1] * q.shape[2]
-    if not split:
-        if tiled:
-            raise ValueError("the tile layout is a layout of the split output")
-        _need(out, "out", q.dtype)
-        if out.numel() != rows * width:
-            raise ValueError(f"out has {out.numel()} elements, needs {rows * width}")
-        return 0
-    _need(out, "out", BF16, split_numel(rows, width, tiled))
-    return 2 if tiled else 1
-
-
-def _ws(workspace: torch.Tensor | None) -> int:
-    _need(workspace, "workspace", F32, optional=True)
-    return 0 if workspace is None else workspace.numel() * 4
+def _out_spec(out: torch.Tensor, q: torch.Tensor, rows: int, width: int, split: bool,
+              tiled: bool) -> tuple:
+    if split:
+        return out, "out", BF16, split_numel(rows, width, tiled)
+    if tiled:
+        raise ValueError("the tile layout is a layout of the split output")
+    if out.numel() != rows * width:
+        raise ValueError(f"out has {out.numel()} elements, needs {rows * width}")
+    return out, "out", q.dtype, rows * width
 
 
 def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.Tensor,
@@ -1180,37 +1180,37 @@ def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.
     if width % d or heads <= 0 or heads % kv:
         raise ValueError(f"qkv rows of {width} do not hold a multiple of {kv} query heads, {kv} key "
                          f"heads and {kv} value heads of {d}")
-    if not qkv.is_cuda or (width > 1 and qkv.stride(1) != 1):
+    dev = qkv.get_device()
+    if dev < 0 or qkv.stride(1) != 1:
         raise ValueError("qkv must be a GPU tensor with contiguous rows")
     ld = qkv.stride(0) if rows > 1 else width
-    _need(q_gamma, "q_gamma", F32, d)
-    _need(k_gamma, "k_gamma", F32, d)
-    _need(rstd, "rstd", F32, rows, optional=True)
-    _need(pos, "pos", I64, rows * 3)
     mx, my, mz, px, py, pz = rope_geom
-    _need(rope_tab, "rope_tab", F32, 2 * (mx * px + my * py + mz * pz))
-    _need(token_row, "token_row", I32, rows)
-    _need(token_slot, "token_slot", I32, rows)
-    _grouped_cache(k_cache, v_cache, "cache ", batch, kv, d, k_cache.dtype)
-    _need(q_out, "q_out", k_cache.dtype, rows * heads * d)
+    out = k_cache.dtype
+    _cache_shapes(k_cache, v_cache, "cache ", (batch, kv, d))
     in_dt, out_dt = cache_dtype_code(qkv), cache_dtype_code(k_cache)
+    _need_all(dev, (
+        (rstd, "rstd", F32, rows), (pos, "pos", I64, rows * 3),
+        (rope_tab, "rope_tab", F32, 2 * (mx * px + my * py + mz * pz)),
+        (q_gamma, "q_gamma", F32, d), (k_gamma, "k_gamma", F32, d),
+        (token_row, "token_row", I32, rows), (token_slot, "token_slot", I32, rows),
+        (q_out, "q_out", out, rows * heads * d), (k_cache, "k_cache", out, 0),
+        (v_cache, "v_cache", out, 0)))
     if rows == 0:
         return
-    with _one_device(qkv, rstd, pos, rope_tab, q_gamma, k_gamma, token_row, token_slot, q_out,
-                     k_cache, v_cache):
+    with _on_device(dev):
         _lib.check(_lib.lib().mdl_qk_norm_rope_cache(
-            _p(qkv), in_dt, ld, _p(rstd), _p(pos), _p(rope_tab), rows, _p(token_row),
-            _p(token_slot), batch, heads, kv, d, mx, my, mz, px, py, pz, _p(q_gamma), _p(k_gamma),
-            eps, q_scale, _p(q_out), _p(k_cache), _p(v_cache), out_dt, slots, _stream()),
-            "mdl_qk_norm_rope_cache")
+            qkv.data_ptr(), in_dt, ld, None if rstd is None else rstd.data_ptr(), pos.data_ptr(),
+            rope_tab.data_ptr(), rows, token_row.data_ptr(), token_slot.data_ptr(), batch, heads,
+            kv, d, mx, my, mz, px, py, pz, q_gamma.data_ptr(), k_gamma.data_ptr(), eps, q_scale,
+            q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out_dt, slots,
+            torch._C._cuda_getCurrentRawStream(dev)), "mdl_qk_norm_rope_cache")
 
 
 def attn_grouped_workspace_bytes(q: torch.Tensor, k_cache: torch.Tensor, max_q: int) -> int:
     """Bytes of ``attn_grouped``'s workspace for tensors of these shapes (0: none is used)."""
-    tokens, heads, d = _grouped_q(q)
+    tokens, heads, d, kv = _grouped_q(q, k_cache)
     return _lib.lib().mdl_attn_grouped_workspace_bytes(
-        k_cache.shape[0], tokens, max_q, heads, k_cache.shape[1], d, cache_dtype_code(q),
-        k_cache.shape[2])
+        k_cache.shape[0], tokens, max_q, heads, kv, d, cache_dtype_code(q), k_cache.shape[2])
 
 
 def attn_grouped(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -1226,34 +1226,35 @@ def attn_grouped(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     row-major or ``tiled``: a projection's input).  ``workspace`` (fp32,
     attn_grouped_workspace_bytes; calls that overlap need one each) lets a call with few rows split
     its keys."""
-    tokens, heads, d = _grouped_q(q)
-    if k_cache.dim() != 4:
-        raise ValueError("k_cache must be [n_seq, n_kv_heads, slots, head_dim]")
-    n_seq, kv, slots = k_cache.shape[:3]
-    _grouped_cache(k_cache, v_cache, "cache ", n_seq, kv, d, q.dtype)
-    if kv == 0 or heads % kv:
-        raise ValueError(f"{heads} query heads do not divide over {kv} key / value heads")
+    tokens, heads, d, kv = _grouped_q(q, k_cache)
+    n_seq, slots = k_cache.shape[0], k_cache.shape[2]
+    _cache_shapes(k_cache, v_cache, "cache ", (n_seq, kv, d))
     if q_offset.numel() != n_seq + 1 or kv_len.numel() != n_seq:
         raise ValueError(f"q_offset and kv_len must have {n_seq + 1} and {n_seq} elements")
-    _need(q_offset, "q_offset", I32)
-    _need(kv_len, "kv_len", I32)
-    form, ws_bytes = _out_form(out, q, split, tiled), _ws(workspace)
+    dev, dt, code = q.get_device(), q.dtype, cache_dtype_code(q)
+    _need_all(dev, ((q, "q", dt, 0), (k_cache, "k_cache", dt, 0), (v_cache, "v_cache", dt, 0),
+                    (q_offset, "q_offset", I32, 0), (kv_len, "kv_len", I32, 0),
+                    _out_spec(out, q, tokens, heads * d, split, tiled),
+                    (workspace, "workspace", F32, 0)))
     if tokens == 0 or n_seq == 0:
         return
-    with _one_device(q, k_cache, v_cache, q_offset, kv_len, out, workspace):
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(),
+                                                        workspace.numel() * 4)
+    with _on_device(dev):
         _lib.check(_lib.lib().mdl_attn_grouped(
-            _p(q), _p(k_cache), _p(v_cache), cache_dtype_code(q), n_seq, tokens, max_q, heads, kv,
-            d, slots, _p(q_offset), _p(kv_len), int(causal), _p(out), form, _p(workspace),
-            ws_bytes, _stream()), "mdl_attn_grouped")
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), code, n_seq, tokens, max_q,
+            heads, kv, d, slots, q_offset.data_ptr(), kv_len.data_ptr(), int(causal),
+            out.data_ptr(), split + tiled, ws, ws_bytes,
+            torch._C._cuda_getCurrentRawStream(dev)), "mdl_attn_grouped")
 
 
 def attn_decode_shared_workspace_bytes(q: torch.Tensor, prefix_k: torch.Tensor,
                                        k_cache: torch.Tensor, max_rows: int) -> int:
     """Bytes of ``attn_decode_shared``'s workspace for tensors of these shapes."""
-    batch, heads, d = _grouped_q(q)
+    batch, heads, d, kv = _grouped_q(q, k_cache)
     return _lib.lib().mdl_attn_decode_shared_workspace_bytes(
-        batch, prefix_k.shape[0], max_rows, heads, k_cache.shape[1], d, cache_dtype_code(q),
-        prefix_k.shape[2], k_cache.shape[2])
+        batch, prefix_k.shape[0], max_rows, heads, kv, d, cache_dtype_code(q), prefix_k.shape[2],
+        k_cache.shape[2])
 
 
 def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
@@ -1267,33 +1268,35 @@ def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     D]; group g has the rows row_offset[g] .. row_offset[g + 1] - 1 (int32 [n_prefix + 1], at most
     ``max_rows``).  ``workspace``: fp32, attn_decode_shared_workspace_bytes.  Otherwise as
     attn_grouped."""
-    batch, heads, d = _grouped_q(q)
-    if prefix_k.dim() != 4 or prefix_k.shape[0] == 0 or prefix_k.shape[1] == 0:
-        raise ValueError("prefix_k must be [n_prefix, n_kv_heads, prefix_slots, head_dim]")
-    n_prefix, kv, p_slots = prefix_k.shape[:3]
-    _grouped_cache(prefix_k, prefix_v, "prefix_", n_prefix, kv, d, q.dtype)
-    _grouped_cache(k_cache, v_cache, "cache ", batch, kv, d, q.dtype)
-    if heads % kv:
-        raise ValueError(f"{heads} query heads do not divide over {kv} key / value heads")
-    if row_offset.numel() != n_prefix + 1 or prefix_len.numel() != n_prefix:
-        raise ValueError(f"row_offset and prefix_len must have {n_prefix + 1} and {n_prefix} "
-                         "elements")
-    if kv_len.numel() != batch:
-        raise ValueError(f"kv_len must have {batch} elements")
-    _need(row_offset, "row_offset", I32)
-    _need(prefix_len, "prefix_len", I32)
-    _need(kv_len, "kv_len", I32)
-    _need(workspace, "workspace", F32)
-    form, ws_bytes = _out_form(out, q, split, tiled), _ws(workspace)
+    batch, heads, d, kv = _grouped_q(q, k_cache)
+    n_prefix = prefix_k.shape[0]
+    if n_prefix == 0:
+        raise ValueError("prefix_k holds no prefix")
+    _cache_shapes(prefix_k, prefix_v, "prefix_", (n_prefix, kv, d))
+    _cache_shapes(k_cache, v_cache, "cache ", (batch, kv, d))
+    if (row_offset.numel() != n_prefix + 1 or prefix_len.numel() != n_prefix or
+            kv_len.numel() != batch):
+        raise ValueError(f"row_offset, prefix_len and kv_len must have {n_prefix + 1}, {n_prefix} "
+                         f"and {batch} elements")
+    dev, dt, code = q.get_device(), q.dtype, cache_dtype_code(q)
+    if workspace is None:
+        raise ValueError("workspace is required")
+    _need_all(dev, ((q, "q", dt, 0), (prefix_k, "prefix_k", dt, 0), (prefix_v, "prefix_v", dt, 0),
+                    (row_offset, "row_offset", I32, 0), (prefix_len, "prefix_len", I32, 0),
+                    (k_cache, "k_cache", dt, 0), (v_cache, "v_cache", dt, 0),
+                    (kv_len, "kv_len", I32, 0),
+                    _out_spec(out, q, batch, heads * d, split, tiled),
+                    (workspace, "workspace", F32, 0)))
     if batch == 0:
         return
-    with _one_device(q, prefix_k, prefix_v, row_offset, prefix_len, k_cache, v_cache, kv_len, out,
-                     workspace):
+    with _on_device(dev):
         _lib.check(_lib.lib().mdl_attn_decode_shared(
-            _p(q), _p(prefix_k), _p(prefix_v), _p(row_offset), _p(prefix_len), n_prefix, p_slots,
-            max_rows, _p(k_cache), _p(v_cache), _p(kv_len), batch, k_cache.shape[2],
-            cache_dtype_code(q), heads, kv, d, _p(out), form, _p(workspace), ws_bytes, _stream()),
-            "mdl_attn_decode_shared")
+            q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), row_offset.data_ptr(),
+            prefix_len.data_ptr(), n_prefix, prefix_k.shape[2], max_rows, k_cache.data_ptr(),
+            v_cache.data_ptr(), kv_len.data_ptr(), batch, k_cache.shape[2], code, heads, kv, d,
+            out.data_ptr(), split + tiled, workspace.data_ptr(), workspace.numel() * 4,
+            torch._C._cuda_getCurrentRawStream(dev)), "mdl_attn_decode_shared")
+
 
 
 class HeadConstraints:
