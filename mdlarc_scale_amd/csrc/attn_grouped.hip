@@ -629,6 +629,20 @@ attn_grouped_kernel(const GroupedArgs p) {
   grouped_block<T, D, WR, WK, KT>(p, blockIdx.x, lds);
 }
 
+// Two lists of flat tiles in one launch: the first n_first blocks work on list 0.
+struct GroupedPair {
+  GroupedArgs list[2];
+  int n_first;
+};
+
+template <typename T, int D, int WK>
+__global__ __launch_bounds__(64 * WK, (GroupedShape<T, D, 1, WK, 32>::kWavesPerSimd)) void
+attn_flat_kernel(const GroupedPair p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[GroupedShape<T, D, 1, WK, 32>::kLds];
+  const int second = static_cast<int>(blockIdx.x) >= p.n_first;
+  grouped_block<T, D, 1, WK, 32>(p.list[second], blockIdx.x - (second ? p.n_first : 0), lds);
+}
+
 struct MergeArgs {
   const float* ws_o;
   const float* ws_ml;
@@ -714,7 +728,8 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
   }
 }
 
-constexpr int kMaxParts = 32;     // parts of one list of keys (a merge wave holds 64 states)
+constexpr int kMaxParts = 64;     // states that a wave of the merge holds
+constexpr int kMaxOwn = 16;       // of them for a row's own keys behind a prefix
 constexpr int kFlatFill = 512;    // blocks that fill the GPU: flat ones of 128 threads
 constexpr int kTallFill = 256;    // and tall ones of 256
 
@@ -729,39 +744,56 @@ struct Plan {
   int n_tiles, n_split;
 };
 
-Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, bool may_split) {
+Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts) {
   const int64_t tall = pairs * ((max_rows + 127) / 128), flat = pairs * ((max_rows + 31) / 32);
   Plan r;
-  r.tall = max_rows > 32 && (tall >= kTallFill || (may_split && flat < kFlatFill));
+  r.tall = max_rows > 32 && (tall >= kTallFill || (max_parts > 1 && flat < kFlatFill));
   r.n_tiles = static_cast<int>(r.tall ? (max_rows + 127) / 128 : (max_rows + 31) / 32);
   const int64_t blocks = r.tall ? tall : flat, fill = r.tall ? kTallFill : kFlatFill;
-  const int64_t want = may_split ? (fill + blocks - 1) / blocks : 1;
-  const int64_t most = (slots + 255) / 256;   // a part of less than 256 keys is mostly its start
+  const int64_t want = (fill + blocks - 1) / blocks;
+  const int64_t most = (slots + 63) / 64;   // a turn of a block
   const int64_t ns = want < most ? want : most;
-  r.n_split = static_cast<int>(ns < 1 ? 1 : ns > kMaxParts ? kMaxParts : ns);
+  r.n_split = static_cast<int>(ns < 1 ? 1 : ns > max_parts ? max_parts : ns);
   return r;
 }
 
 template <typename T, int D>
-int launch_tiles(const GroupedArgs& a, bool tall, hipStream_t st) {
-  const int64_t blocks = static_cast<int64_t>(a.n_seq) * a.kv_heads * a.n_tiles * a.n_split;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
-  const unsigned n = static_cast<unsigned>(blocks);
+int launch_tiles(const GroupedArgs* a, const bool* tall, int lists, hipStream_t st) {
   constexpr bool f32 = sizeof(T) == 4;
-  constexpr int kTallKeys = f32 ? 32 : 64, kFlatGroups = sizeof(T) * D == 512 ? 1 : 2;
-  if (tall)
-    attn_grouped_kernel<T, D, 4, 1, kTallKeys><<<n, 256, 0, st>>>(a);
-  else
-    attn_grouped_kernel<T, D, 1, kFlatGroups, 32><<<n, 64 * kFlatGroups, 0, st>>>(a);
+  // waves of a flat block: two, but one where a ring is 64 KB.  Four (half as many blocks on a CU, one
+  // with 128 dims) were 1-40% slower.
+  constexpr int kFlatGroups = f32 && D == 128 ? 1 : 2;
+  GroupedPair flat{};
+  int64_t n_flat = 0;
+  for (int i = 0; i < lists; ++i) {
+    const int64_t blocks =
+        static_cast<int64_t>(a[i].n_seq) * a[i].kv_heads * a[i].n_tiles * a[i].n_split;
+    if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+    if (tall[i]) {
+      attn_grouped_kernel<T, D, 4, 1, f32 ? 32 : 64>
+          <<<static_cast<unsigned>(blocks), 256, 0, st>>>(a[i]);
+      const int rc = launch_status();
+      if (rc != MDL_OK) return rc;
+    } else {
+      flat.list[n_flat == 0 ? 0 : 1] = a[i];
+      if (n_flat == 0) flat.n_first = static_cast<int>(blocks);
+      n_flat += blocks;
+    }
+  }
+  if (n_flat > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (n_flat == 0) return MDL_OK;
+  attn_flat_kernel<T, D, kFlatGroups>
+      <<<static_cast<unsigned>(n_flat), 64 * kFlatGroups, 0, st>>>(flat);
   return launch_status();
 }
 
-int run_tiles(const GroupedArgs& a, bool tall, int dtype, int head_dim, hipStream_t st) {
+int run_tiles(const GroupedArgs* a, const bool* tall, int lists, int dtype, int head_dim,
+              hipStream_t st) {
   if (dtype == MDL_DTYPE_F32)
-    return head_dim == 64 ? launch_tiles<float, 64>(a, tall, st)
-                          : launch_tiles<float, 128>(a, tall, st);
-  return head_dim == 64 ? launch_tiles<uint16_t, 64>(a, tall, st)
-                        : launch_tiles<uint16_t, 128>(a, tall, st);
+    return head_dim == 64 ? launch_tiles<float, 64>(a, tall, lists, st)
+                          : launch_tiles<float, 128>(a, tall, lists, st);
+  return head_dim == 64 ? launch_tiles<uint16_t, 64>(a, tall, lists, st)
+                        : launch_tiles<uint16_t, 128>(a, tall, lists, st);
 }
 
 int run_merge(const MergeArgs& m, int dtype, int head_dim, hipStream_t st) {
@@ -812,7 +844,7 @@ extern "C" int64_t mdl_attn_grouped_workspace_bytes(int n_seq, int tokens, int m
     return 0;
   const Plan pl = plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
                              static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), cache_slots,
-                             true);
+                             kMaxParts);
   return pl.n_split > 1 ? state_bytes(pl.n_split, static_cast<int64_t>(tokens) * n_heads, head_dim)
                         : 0;
 }
@@ -833,7 +865,7 @@ extern "C" int mdl_attn_grouped(const void* q, const void* k_cache, const void* 
   if (n_seq == 0 || tokens == 0 || max_q == 0) return MDL_OK;
   const Plan pl = plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
                              static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), cache_slots,
-                             workspace != nullptr);
+                             workspace ? kMaxParts : 1);
   const int64_t rows = static_cast<int64_t>(tokens) * n_heads;
   if (pl.n_split > 1 && workspace_bytes < state_bytes(pl.n_split, rows, head_dim))
     return MDL_ERR_WORKSPACE;
@@ -847,7 +879,7 @@ extern "C" int mdl_attn_grouped(const void* q, const void* k_cache, const void* 
     a.ws_o = workspace;
     a.ws_ml = workspace + pl.n_split * rows * head_dim;
   }
-  const int rc = run_tiles(a, pl.tall, dtype, head_dim, st);
+  const int rc = run_tiles(&a, &pl.tall, 1, dtype, head_dim, st);
   if (rc != MDL_OK || pl.n_split == 1) return rc;
   MergeArgs m{a.ws_o, a.ws_ml, q_offset, out, n_seq, tokens, n_heads, max_q, pl.n_split, 0,
               out_form};
@@ -866,8 +898,8 @@ SharedPlan plan_shared(int batch, int n_prefix, int max_rows, int n_heads, int n
   const int64_t g = n_heads / n_kv_heads;
   SharedPlan r;
   r.prefix = plan_tiles(static_cast<int64_t>(n_prefix) * n_kv_heads, max_rows * g, prefix_slots,
-                        true);
-  r.own = plan_tiles(static_cast<int64_t>(batch) * n_kv_heads, g, cache_slots, true);
+                        kMaxParts - kMaxOwn);
+  r.own = plan_tiles(static_cast<int64_t>(batch) * n_kv_heads, g, cache_slots, kMaxOwn);
   return r;
 }
 
@@ -918,21 +950,22 @@ extern "C" int mdl_attn_decode_shared(const void* q, const void* prefix_k, const
   const int parts = pl.prefix.n_split + pl.own.n_split;
   if (workspace_bytes < state_bytes(parts, rows, head_dim)) return MDL_ERR_WORKSPACE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  GroupedArgs a{};
-  a.q = q; a.k = prefix_k; a.v = prefix_v; a.q_offset = row_offset; a.kv_len = prefix_len;
-  a.ws_o = workspace;
-  a.ws_ml = workspace + parts * rows * head_dim;
-  a.n_seq = n_prefix; a.tokens = batch; a.heads = n_heads; a.kv_heads = n_kv_heads;
-  a.group = n_heads / n_kv_heads; a.slots = prefix_slots; a.max_q = max_rows;
-  a.n_tiles = pl.prefix.n_tiles; a.n_split = pl.prefix.n_split;
-  int rc = run_tiles(a, pl.prefix.tall, dtype, head_dim, st);
+  GroupedArgs a[2]{};
+  a[0].q = q; a[0].k = prefix_k; a[0].v = prefix_v; a[0].q_offset = row_offset;
+  a[0].kv_len = prefix_len;
+  a[0].ws_o = workspace;
+  a[0].ws_ml = workspace + parts * rows * head_dim;
+  a[0].n_seq = n_prefix; a[0].tokens = batch; a[0].heads = n_heads; a[0].kv_heads = n_kv_heads;
+  a[0].group = n_heads / n_kv_heads; a[0].slots = prefix_slots; a[0].max_q = max_rows;
+  a[0].n_tiles = pl.prefix.n_tiles; a[0].n_split = pl.prefix.n_split;
+  a[1] = a[0];
+  a[1].k = k_cache; a[1].v = v_cache; a[1].q_offset = nullptr; a[1].kv_len = kv_len;
+  a[1].n_seq = batch; a[1].slots = cache_slots; a[1].max_q = 1;
+  a[1].n_tiles = pl.own.n_tiles; a[1].n_split = pl.own.n_split; a[1].part0 = pl.prefix.n_split;
+  const bool tall[2] = {pl.prefix.tall, pl.own.tall};
+  const int rc = run_tiles(a, tall, 2, dtype, head_dim, st);
   if (rc != MDL_OK) return rc;
-  a.k = k_cache; a.v = v_cache; a.q_offset = nullptr; a.kv_len = kv_len;
-  a.n_seq = batch; a.slots = cache_slots; a.max_q = 1;
-  a.n_tiles = pl.own.n_tiles; a.n_split = pl.own.n_split; a.part0 = pl.prefix.n_split;
-  rc = run_tiles(a, pl.own.tall, dtype, head_dim, st);
-  if (rc != MDL_OK) return rc;
-  MergeArgs m{a.ws_o, a.ws_ml, row_offset, out, n_prefix, batch, n_heads, max_rows,
+  MergeArgs m{a[0].ws_o, a[0].ws_ml, row_offset, out, n_prefix, batch, n_heads, max_rows,
               pl.prefix.n_split, pl.own.n_split, out_form};
   return run_merge(m, dtype, head_dim, st);
 }
