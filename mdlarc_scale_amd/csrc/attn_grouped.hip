@@ -136,12 +136,9 @@ struct GroupedShape {
   static constexpr int kRows = 32 * WR;                   // rows of a block
   static constexpr int kCopies = kTile / 1024 / WR;       // 1 KB copies of a wave, K or V
   static constexpr int kRowsPerCopy = 1024 / kRowBytes;
-  // registers for as many waves as LDS lets reside (four per CU are one per SIMD), at most three;
-  // fp32 with 128 dims: q and the output alone are 128 registers
+  // registers for as many waves as LDS lets reside (four on a CU are one on each SIMD), at most three
   static constexpr int kResident = 160 * 1024 / kLds * WR * WK / 4;
-  static constexpr int kWavesPerSimd = kRowBytes == 512 || kResident < 2 ? 1
-                                       : kRowBytes == 128 && WR > 1      ? 3
-                                                                         : 2;
+  static constexpr int kWavesPerSimd = kResident < 2 ? 1 : D == 64 && WR > 1 ? 3 : 2;
   static_assert(WR > 1 || 3 * kCopies < 63, "copies in flight fit the counter");
   static_assert(kTile % (1024 * WR) == 0, "whole copies per wave");
   static_assert(KT % 32 == 0 && (D == 64 || D == 128), "whole MFMA blocks");
@@ -227,14 +224,16 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   // Copy j of a tile: rows (1024 / row bytes) j .. of K and of V, one kilobyte each; a lane takes
   // physical chunk lane % chunks of its row.  Rows past the last key copy that key.
   constexpr int kChunks = S::kRowBytes / 16;
+  // (fp32 reads V by whole rows, which need no swizzle: their addresses are one lane offset then.)
   auto issue = [&](const T* src, int kt, uint32_t at) {
+    const bool plain = kF32 && src == Vg;
     const T* from = scalar_ptr(src + static_cast<int64_t>(kt) * D);
 #pragma unroll
     for (int jj = 0; jj < S::kCopies; ++jj) {
       const int j = wr + WR * jj;
       const int r = S::kRowsPerCopy * j + lane / kChunks;
       const uint32_t off = min(r, kend - 1 - kt) * S::kRowBytes +
-                           16 * ((lane % kChunks) ^ swz<T, D>(r & 15));
+                           16 * ((lane % kChunks) ^ (plain ? 0 : swz<T, D>(r & 15)));
       const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + at + 1024 * j);
       if constexpr (WR == 1)
         dma16_stream(from, off, dst);
@@ -253,11 +252,13 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   const int kswz = swz<T, D>(c & 15);
   const int vr = 4 * h + ((lane >> 2) & 3);
   const int vchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  uint32_t vofs[DB][2];
+  // Eight rows on, the swizzle differs in chunk bit 3 (D = 128) or 1 (D = 64); bit 3 is that of dim
+  // block db ^ 2, so 128 dims need no second set of addresses.
+  uint32_t vofs[DB][D == 128 ? 1 : 2];
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < (D == 128 ? 1 : 2); ++e)
       vofs[db][e] = (vr + 8 * e) * S::kRowBytes +
                     16 * ((vchunk + 4 * db) ^ swz<T, D>(vr + 8 * e)) + 8 * (lane & 1);
 
@@ -273,46 +274,23 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   auto vt_frag = [&](const uint8_t* Vt, int key, int db) -> bf16x8_t {
     const uint8_t* base = Vt + key * S::kRowBytes;
     const s16x4_t a = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + vofs[db][0]));
-    const s16x4_t b = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + vofs[db][1]));
+    const uint32_t next = D == 128 ? vofs[(db ^ 2) % DB][0] + 8 * S::kRowBytes : vofs[db][D == 64];
+    const s16x4_t b = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + next));
     return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  // o += w V of the key at row `kr` of a V tile, for the rows that see it (`sees`); w is the row's
-  // weight, in lane half `half` of its lane.  Key by key and channel by channel: for keys with a
-  // value that is not finite, which a product over several keys would give to every row.
-  auto add_key = [&](const uint8_t* Vt, int kr, int half, float w, bool sees) {
-    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(w), __float_as_uint(w),
-                                                       false, false);
-    const float x = __uint_as_float(half ? both[1] : both[0]);
-    const uint8_t* base = Vt + kr * S::kRowBytes;
-    const int sw = swz<T, D>(kr & 15);
+  // o[db] += A B for the rows `mine` alone
+  auto add_product = [&](int db, auto product, bool mine) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int u = 0; u < DB; ++u) {
-        float v[4];   // channels of elements 4 j .. + 3 of block u (bf16), of all blocks (fp32)
-        if constexpr (kF32) {
-          const float4 t = *reinterpret_cast<const float4*>(
-              base + 16 * ((DB * (2 * j + h) + u) ^ sw));
-          v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-        } else {
-          const uint2 t = *reinterpret_cast<const uint2*>(base + 16 * ((4 * u + j) ^ sw) + 8 * h);
-          v[0] = bf2f(t.x & 0xffffu); v[1] = bf2f(t.x >> 16);
-          v[2] = bf2f(t.y & 0xffffu); v[3] = bf2f(t.y >> 16);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int q = 4 * u + e;
-          const int block = kF32 ? q % DB : u, i = 4 * j + (kF32 ? q / DB : e);
-          o[block][i] = sees ? fmaf(x, v[e], o[block][i]) : o[block][i];
-        }
-      }
+    for (int i = 0; i < 16; ++i) product[i] = mine ? product[i] : 0.f;
+    o[db] += product;
+    __builtin_amdgcn_sched_barrier(0);   // rare code: one product's registers at a time
   };
 
-  // V operands `va` of the 16 keys from kk on (tile rows from `key` on), of which not every row sees
-  // all: keys past lim_hi become zeros; if a value that is left is not finite, the step is worked on
-  // here and the operands become zeros.
-  auto masked_step = [&](uint4 (&va)[DB], const uint8_t* Vt, int kk, int key, uint32_t p0, uint32_t p1, uint32_t p2, uint32_t p3) {
+  // V operands `va` of the 16 keys from kk on, of which not every row sees all: keys past lim_hi
+  // become zeros; if a value that is left is not finite, each set of rows with one limit gets a
+  // product over its own keys here and the operands become zeros.
+  auto masked_step = [&](uint4 (&va)[DB], int kk, const bf16x8_t& pb) {
     uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -327,53 +305,56 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     }
     if (__ballot((odd & 0x80008000u) != 0) == 0) return;
 #pragma unroll 1
-    for (int e = 0; e < 16 && kk + e <= lim_hi; ++e) {
-      const uint32_t w = (e & 8) != 0 ? ((e & 2) != 0 ? p3 : p2) : ((e & 2) != 0 ? p1 : p0);
-      add_key(Vt, key + e, (e >> 2) & 1, bf2f(e & 1 ? w >> 16 : w & 0xffffu), lim >= kk + e);
+    for (int e = 0; e < 16; ++e) {   // the rows that see keys up to kk + e of this step
+      const bool mine = e == 15 ? lim >= kk + 15 : lim == kk + e;
+      if (__ballot(mine) == 0) continue;
+      uint32_t see[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 4 * h + 8 * (i >> 1) + 2 * (i & 1);
+        see[i] = (k <= e ? 0xffffu : 0u) | (k + 1 <= e ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint4 a = make_uint4(va[db].x & see[0], va[db].y & see[1], va[db].z & see[2],
+                                   va[db].w & see[3]);
+        add_product(db, __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), pb, splat16(0.f), 0,
+                                                                0, 0), mine);
+      }
     }
 #pragma unroll
     for (int db = 0; db < DB; ++db) va[db] = make_uint4(0, 0, 0, 0);
   };
 
-  // fp32: the V values of lane half h for step r, key kr of the tile (absolute kt + kr), zero past
-  // key `last`.  kr = 8 (r / 4) + r % 4 + 4 h.
-  auto v_pair = [&](const uint8_t* Vt, int kt, int kr, int last, float (&v)[DB]) {
-    const uint8_t* base = Vt + kr * S::kRowBytes;
+  // fp32: the V values of lane half h at row kr of the tile.
+  auto v_row = [&](const uint8_t* Vt, int kr, float (&v)[DB]) {
+    const uint8_t* at = Vt + kr * S::kRowBytes + 4 * DB * c;
     if constexpr (D == 128) {
-      const float4 t = *reinterpret_cast<const float4*>(base + 16 * (c ^ swz<T, D>(kr & 15)));
+      const float4 t = *reinterpret_cast<const float4*>(at);
       v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
     } else {
-      const float2 t = *reinterpret_cast<const float2*>(
-          base + 16 * ((c >> 1) ^ swz<T, D>(kr & 15)) + 8 * (c & 1));
+      const float2 t = *reinterpret_cast<const float2*>(at);
       v[0] = t.x; v[1] = t.y;
     }
-    const bool seen = kt + kr <= last;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) v[db] = seen ? v[db] : 0.f;
   };
 
-  // The fp32 form of masked_step, for a whole tile: true if it holds values that are not finite in
-  // slots that some row sees; its product is then added here.
-  auto masked_tile = [&](const uint8_t* Vt, int kt, const f32x16_t& pr) -> bool {
+  // The fp32 form of masked_step: the V values of keys ka and ka + 4 (lane half h's is ka + 4 h).
+  auto masked_pair = [&](float (&v)[DB], int ka, float pr) {
     bool odd = false;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float v[DB];
-      v_pair(Vt, kt, (r & 3) + 8 * (r >> 2) + 4 * h, lim_hi, v);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) odd |= !(fabsf(v[db]) < INFINITY);
-      if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+    for (int db = 0; db < DB; ++db) {
+      v[db] = ka + 4 * h <= lim_hi ? v[db] : 0.f;
+      odd |= !(fabsf(v[db]) < INFINITY);
     }
-    if (__ballot(odd) == 0) return false;
+    if (__ballot(odd) == 0) return;
 #pragma unroll 1
-    for (int e = 0; e < 32 && kt + e <= lim_hi; ++e) {
-      const int r = (e & 3) + 4 * (e >> 3);   // element of key e, in lane half e / 4 % 2
-      float w = pr[0];
+    for (int k = 0; k < 2; ++k)   // one key alone, for the rows that see it
 #pragma unroll
-      for (int i = 1; i < 16; ++i) w = r == i ? pr[i] : w;
-      add_key(Vt, e, (e >> 2) & 1, w, lim >= kt + e);
-    }
-    return true;
+      for (int db = 0; db < DB; ++db)
+        add_product(db, __builtin_amdgcn_mfma_f32_32x32x2f32(h == k ? v[db] : 0.f, pr, splat16(0.f),
+                                                             0, 0, 0), lim >= ka + 4 * k);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) v[db] = 0.f;
   };
 
   auto compute = [&](const uint8_t* Kt, const uint8_t* Vt, int kt, auto fullc, auto after_qk) {
@@ -439,12 +420,12 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       static_assert(!kF32 || NB == 1, "fp32 tiles are 32 keys");
 #pragma unroll
       for (int r = 0; r < 16; ++r) l += sc[0][r];
-      // worked on there: zeros here
-      const int last = masked && masked_tile(Vt, kt, sc[0]) ? -1 : lim_hi;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
+        const int ka = (r & 3) + 8 * (r >> 2);
         float v[DB];
-        v_pair(Vt, kt, (r & 3) + 8 * (r >> 2) + 4 * h, last, v);
+        v_row(Vt, ka + 4 * h, v);
+        if (masked && kt + ka + 4 > lim_lo) masked_pair(v, kt + ka, sc[0][r]);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
           o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[db], sc[0][r], o[db], 0, 0, 0);
@@ -468,7 +449,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
           for (int db = 0; db < DB; ++db)
             va[db] = __builtin_bit_cast(uint4, vt_frag(Vt, key, db));
           __builtin_amdgcn_sched_barrier(0);
-          if (masked && kt + key + 15 > lim_lo) masked_step(va, Vt, kt + key, key, pw.x, pw.y, pw.z, pw.w);
+          if (masked && kt + key + 15 > lim_lo) masked_step(va, kt + key, pb);
 #pragma unroll
           for (int db = 0; db < DB; ++db)
             o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(va[db]), pb, o[db], 0, 0, 0);
