@@ -58,6 +58,7 @@ struct GroupedArgs {
   float* ws_ml;                // [parts][tokens * heads][2]
   int n_seq, tokens, heads, kv_heads, group, slots, max_q, causal, n_tiles, n_split, part0;
   int out_form;
+  int n_serp;   // blocks of a tall launch, 0 otherwise
 };
 
 // Chunk swizzle of a tile row (16-byte chunks), by its low 4 bits r3..r0.  Both reads are then free
@@ -151,16 +152,22 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   using S = GroupedShape<T, D, WR, WK, KT>;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int NB = KT / 32, DB = D / 32;
-  // Blocks go to the XCDs in turn.  A pair (sequence, key / value head) keeps to one XCD, whose L2
-  // then serves its row tiles, for a sixteenth of the tiles (at least four) and moves on to the next:
-  // sequences differ in length, and pairs that stayed would leave some XCDs with the long ones.  Four
-  // prompts of 3,900 to 6,000 tokens, 16 heads of 64: 294 us staying, 261 so; two of up to 8,192, 32
-  // heads of 128 (eight pairs each, nothing to balance): 901, and 980 moving at every tile.
+  // Order of the work.  Blocks are placed in turn, the first 256 on a CU each and so on, and to the
+  // XCDs in turn; the longest tiles (the latest rows, with the most keys) go first.
+  // The second 256 run backwards, so that a CU with one of the longest gets one of the shortest of
+  // those: 2 prompts of 4,000 tokens (12 fp32 heads of 64, 768 blocks that all fit) 501 -> 427 us, 2 of
+  // up to 8,192 (32 heads of 128) 908 -> 877, 5 of up to 811 (16 heads of 64) 19.6 -> 18.1.
+  // A pair (sequence, key / value head) keeps to one XCD, whose L2 then serves its row tiles, for six
+  // ranks of tiles and then moves on by five: sequences differ in length, and pairs that stayed would
+  // leave some XCDs with the long ones.  4 prompts of 3,900 to 6,000 tokens (16 heads of 64) 295 us
+  // staying, 256 so; 2 of up to 3,000 (16 fp32 heads of 128) 592, 545; where nothing is to be balanced
+  // it costs 0-2% (the 8,192 above 875, 893).
+  if ((block >> 8) == 1 && (block | 255) < p.n_serp) block ^= 248;
   const int pairs = p.n_seq * p.kv_heads;
   const int rest = block / pairs, idx = block - rest * pairs;
   const int rank = rest / p.n_split, split = rest - rank * p.n_split;
-  const int tile = p.n_tiles - 1 - rank;   // the latest rows, with the most keys, first
-  const int pair = (idx + ((block - idx) & 7) + rank / max(4, p.n_tiles / 16)) % pairs;
+  const int tile = p.n_tiles - 1 - rank;
+  const int pair = (idx + ((block - idx) & 7) + 5 * (rank / 6)) % pairs;
   const int seq = pair / p.kv_heads, kvh = pair - seq * p.kv_heads;
   int lo = seq, hi = seq + 1;
   if (p.q_offset) {
@@ -751,8 +758,10 @@ int launch_tiles(const GroupedArgs* a, const bool* tall, int lists, hipStream_t 
         static_cast<int64_t>(a[i].n_seq) * a[i].kv_heads * a[i].n_tiles * a[i].n_split;
     if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
     if (tall[i]) {
+      GroupedArgs t = a[i];
+      t.n_serp = static_cast<int>(blocks);
       attn_grouped_kernel<T, D, 4, 1, f32 ? 32 : 64>
-          <<<static_cast<unsigned>(blocks), 256, 0, st>>>(a[i]);
+          <<<static_cast<unsigned>(blocks), 256, 0, st>>>(t);
       const int rc = launch_status();
       if (rc != MDL_OK) return rc;
     } else {
