@@ -29,6 +29,7 @@
 // WR waves share a ring and split the rows; WK groups of WR waves take the tiles in turn, each with
 // a ring of its own, and merge at the end.  A launch may also cut each tile's keys in n_split parts
 // whose states (fp32 m, l, o) go to the workspace; merge_kernel joins them.
+#include <climits>
 #include <type_traits>
 
 #include "lds_dma.h"
@@ -640,8 +641,10 @@ struct MergeArgs {
 };
 
 // Joins the parts of one output row (token, head) per wave: parts [0, n0) hold it if the token is
-// one of a sequence's first max_q, parts [n0, n0 + n1) always do.  Lane s reads the m and l of part
-// s (at most 64 parts); the values come eight parts at a time, in the parts' order.
+// one of a sequence's first max_q, parts [n0, n0 + n1) always do.  Lane s has the m and l of part s (at
+// most 64 parts); the values come eight parts at a time, in the parts' order.  The first values are
+// read with the states and with the search for the sequence, whose results decide what counts: one
+// wait on memory after another is all the time this takes.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
   constexpr int C = D / 64;
@@ -649,24 +652,39 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 +
                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= all) return;
-  const int lane = threadIdx.x & 63;
-  const int t = static_cast<int>(row / p.heads), head = static_cast<int>(row - static_cast<int64_t>(t) * p.heads);
-  // the last sequence that starts at or before the token
-  int a = 0, b = p.n_seq;
-  while (a < b) {
-    const int mid = (a + b) >> 1;
-    if (p.q_offset[mid] <= t) a = mid + 1; else b = mid;
+  const int lane = threadIdx.x & 63, n = p.n0 + p.n1;
+  const int t = static_cast<int>(row / p.heads);
+  const int head = static_cast<int>(row - static_cast<int64_t>(t) * p.heads);
+  const float2 ml =
+      *reinterpret_cast<const float2*>(p.ws_ml + 2 * (min(lane, n - 1) * all + row));
+  float v[8][C];
+  auto load = [&](int q0) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float* src = p.ws_o + (min(q0 + q, n - 1) * all + row) * D + C * lane;
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[q][i] = src[i];
+    }
+  };
+  load(0);
+  // sequences that start at or before the token, 64 at a time; a token of none is in no part
+  int first = 0, end = 0, before = 0;
+  for (int s0 = 0; s0 < p.n_seq; s0 += kWave) {
+    const int s = s0 + lane;
+    const int at = s < p.n_seq ? p.q_offset[s] : INT_MAX;
+    const int after = s < p.n_seq ? p.q_offset[s + 1] : INT_MAX;
+    const int k = __popcll(__ballot(at <= t));
+    if (k > 0) {
+      first = __builtin_amdgcn_readlane(at, k - 1);
+      end = __builtin_amdgcn_readlane(after, k - 1);
+    }
+    before += k;
+    if (k < kWave) break;
   }
-  bool held = a > 0;
-  if (held) {
-    const int first = max(p.q_offset[a - 1], 0);
-    held = t < p.q_offset[a] && t - first < p.max_q;
-  }
-  const int s0 = held ? 0 : p.n0, n = p.n0 + p.n1;
-  if (s0 >= n) return;   // the token is in no sequence: its row stays as it was
-  const int s = s0 + min(lane, n - s0 - 1);
-  const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + 2 * (s * all + row));
-  const bool live = lane < n - s0 && ml.x != -INFINITY;
+  const bool held = before > 0 && t < end && t - max(first, 0) < p.max_q;
+  const int part0 = held ? 0 : p.n0;
+  if (part0 >= n) return;   // the token is in no sequence: its row stays as it was
+  const bool live = lane >= part0 && lane < n && ml.x != -INFINITY;
   const float top = wave_max(live ? ml.x : -INFINITY);
   const float w = live ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
   const uint64_t mask = __ballot(live);
@@ -674,14 +692,8 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
   float O[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) O[i] = 0.f;
-  for (int q0 = 0; q0 < n - s0; q0 += 8) {
-    float v[8][C];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float* src = p.ws_o + (min(s0 + q0 + q, n - 1) * all + row) * D + C * lane;
-#pragma unroll
-      for (int i = 0; i < C; ++i) v[q][i] = src[i];
-    }
+  for (int q0 = 0; q0 < n; q0 += 8) {
+    if (q0 > 0) load(q0);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       if (!((mask >> (q0 + q)) & 1u)) continue;   // a state without keys wrote no values
@@ -720,13 +732,16 @@ constexpr int kMaxParts = 64;     // states that a wave of the merge holds
 constexpr int kMaxOwn = 16;       // of them for a row's own keys behind a prefix
 constexpr int kFlatFill = 512;    // blocks that fill the GPU: flat ones of 128 threads
 constexpr int kTallFill = 256;    // and tall ones of 256
+constexpr int kLongPart = 1280;   // keys of a part that make up for its state's way through memory
 
 // How one list of tiles runs: tall blocks (4 waves, 128 rows) or flat ones (32 rows, two waves that
 // share out the keys), and in how many parts the keys are cut.  Tall blocks read a key a quarter as
 // often; flat ones are more, with fewer rows to wait for.  So: tall where they fill the GPU uncut, and
 // where flat ones would have to be cut too; flat in between.  us, flat / tall: 704 flat blocks of a
 // 700-token prompt 23 / 30 (in two parts); 72 of 17 tokens behind 4,099 keys 21 / 19; 64 of 64
-// samples behind 32,749 keys (with their own keys and the merge) 117 / 73.
+// samples behind 32,749 keys (with their own keys and the merge) 117 / 73.  Tall blocks are cut to
+// one for each CU, and to two where the parts stay long: 4 continuations of 100 tokens behind 6,000
+// keys 64 / 53 us; the 64 samples above 73 / 75, 17 tokens behind 4,099 keys 19 / 21.
 struct Plan {
   bool tall;
   int n_tiles, n_split;
@@ -737,7 +752,9 @@ Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts) {
   Plan r;
   r.tall = max_rows > 32 && (tall >= kTallFill || (max_parts > 1 && flat < kFlatFill));
   r.n_tiles = static_cast<int>(r.tall ? (max_rows + 127) / 128 : (max_rows + 31) / 32);
-  const int64_t blocks = r.tall ? tall : flat, fill = r.tall ? kTallFill : kFlatFill;
+  const int64_t blocks = r.tall ? tall : flat;
+  int64_t fill = r.tall ? kTallFill : kFlatFill;
+  if (r.tall && (2 * fill + blocks - 1) / blocks * kLongPart <= slots) fill *= 2;
   const int64_t want = (fill + blocks - 1) / blocks;
   const int64_t most = (slots + 63) / 64;   // a turn of a block
   const int64_t ns = want < most ? want : most;
