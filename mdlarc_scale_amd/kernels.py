@@ -9,7 +9,6 @@ non-zero library status raises ``RuntimeError`` / ``ValueError``.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 
 import torch
 
@@ -1108,44 +1107,51 @@ GROUPED_HEAD_DIMS = (64, 128)
 
 
 def _need_all(dev: int, specs) -> None:
-    """``_need`` for (tensor, name, dtype, elements) specs, all on GPU ``dev``; None where a tensor
-    is optional.  One plain loop: these calls take tens of microseconds in all."""
+    """``_need`` for (tensor, name, dtype, elements) specs, all on GPU ``dev`` (elements 0: the caller
+    has compared the shape).  One plain loop: the host's part of these calls is most of a small one."""
     if dev < 0:
-        raise ValueError("q must be a GPU tensor")
+        raise ValueError("the tensors must be GPU tensors")
     for t, name, dtype, numel in specs:
-        if t is None or (t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and
-                         t.numel() >= numel):
+        if (t is not None and t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and
+                (numel == 0 or t.numel() >= numel)):
             continue
         _need(t, name, dtype, numel)
         raise ValueError(f"{name} is on {t.device}, another tensor on GPU {dev}: one call runs on "
                          "one device")
 
 
-def _on_device(dev: int):
-    """A context in which GPU ``dev`` is the current device, as a launch on its stream needs."""
-    return nullcontext() if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+def _launch(dev: int, name: str, *args) -> None:
+    """Call entry ``name`` with ``args`` and the current stream of GPU ``dev``, which is made the
+    current device as the launch needs."""
+    fn = getattr(_lib.lib(), name)
+    if dev == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if code:
+        _lib.check(code, name)
 
 
-def _cache_shapes(k: torch.Tensor, v: torch.Tensor, name: str, want: tuple) -> None:
-    """K and V caches [rows, kv_heads, slots, head_dim] of one shape; ``want`` without the slots."""
-    shape = k.shape
-    if shape != v.shape or len(shape) != 4 or (shape[0], shape[1], shape[3]) != want:
+def _same_shapes(k: torch.Tensor, v: torch.Tensor, name: str, shape: tuple, want: tuple) -> None:
+    """K (of ``shape``) and V caches [rows, kv_heads, slots, head_dim] of one shape; ``want`` without
+    the slots."""
+    if v.shape != shape or (shape[0], shape[1], shape[3]) != want:
         raise ValueError(f"{name}k and {name}v must both be [{want[0]}, {want[1]}, slots, "
                          f"{want[2]}] (got {tuple(shape)} and {tuple(v.shape)})")
     if shape[0] and not shape[2]:
         raise ValueError(f"{name}k has no slots (got {tuple(shape)})")
 
 
-def _grouped_q(q: torch.Tensor, k: torch.Tensor) -> tuple[int, int, int, int]:
-    """rows, n_heads, head_dim of q and n_kv_heads of the cache k."""
-    if q.dim() != 3 or q.shape[2] not in GROUPED_HEAD_DIMS:
-        raise ValueError(f"q must be [rows, n_heads, 64 or 128] (got {tuple(q.shape)})")
-    rows, heads, d = q.shape
-    kv = k.shape[1] if k.dim() == 4 else 0
-    if kv == 0 or heads == 0 or heads % kv:
-        raise ValueError(f"{heads} query heads do not divide over the key / value heads of "
-                         f"{tuple(k.shape)}")
-    return rows, heads, d, kv
+def _grouped_shapes(q: torch.Tensor, k: torch.Tensor) -> tuple[tuple, tuple]:
+    """The shapes of q [rows, n_heads, D] and of the cache k [.., n_kv_heads, slots, D]."""
+    shape, cache = q.shape, k.shape
+    if len(shape) != 3 or shape[2] not in GROUPED_HEAD_DIMS:
+        raise ValueError(f"q must be [rows, n_heads, 64 or 128] (got {tuple(shape)})")
+    if len(cache) != 4 or not cache[1] or not shape[1] or shape[1] % cache[1]:
+        raise ValueError(f"{shape[1]} query heads do not divide over the key / value heads of a "
+                         f"{tuple(cache)} cache")
+    return shape, cache
 
 
 def _out_spec(out: torch.Tensor, q: torch.Tensor, rows: int, width: int, split: bool,
@@ -1170,47 +1176,50 @@ def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.
     token_row[m] of [batch, n_kv_heads, slots, D]; a slot or row outside the cache is not written.
     q_out and the caches are bf16 or fp32.  ``rstd`` [rows]: a factor of each row before all else
     (the ln1 scale).  With ``qkv_rope_cache_packed``'s table, positions and cache rules."""
-    if k_cache.dim() != 4 or k_cache.shape[3] not in GROUPED_HEAD_DIMS:
+    cache, shape = k_cache.shape, qkv.shape
+    if len(cache) != 4 or cache[3] not in GROUPED_HEAD_DIMS:
         raise ValueError("k_cache must be [batch, n_kv_heads, slots, 64 or 128]")
-    batch, kv, slots, d = k_cache.shape
-    if qkv.dim() != 2:
+    batch, kv, slots, d = cache
+    if len(shape) != 2:
         raise ValueError("qkv must be [rows, (n_heads + 2 * n_kv_heads) * head_dim]")
-    rows, width = qkv.shape
+    rows, width = shape
     heads = width // d - 2 * kv
-    if width % d or heads <= 0 or heads % kv:
+    if not kv or width % d or heads <= 0 or heads % kv:
         raise ValueError(f"qkv rows of {width} do not hold a multiple of {kv} query heads, {kv} key "
                          f"heads and {kv} value heads of {d}")
+    _same_shapes(k_cache, v_cache, "cache ", cache, (batch, kv, d))
     dev = qkv.get_device()
-    if dev < 0 or qkv.stride(1) != 1:
-        raise ValueError("qkv must be a GPU tensor with contiguous rows")
-    ld = qkv.stride(0) if rows > 1 else width
+    ld, step = qkv.stride()
+    if step != 1:
+        raise ValueError("the rows of qkv must be contiguous")
+    if rows <= 1:
+        ld = width
     mx, my, mz, px, py, pz = rope_geom
     out = k_cache.dtype
-    _cache_shapes(k_cache, v_cache, "cache ", (batch, kv, d))
     in_dt, out_dt = cache_dtype_code(qkv), cache_dtype_code(k_cache)
+    if rstd is not None:
+        _need_all(dev, ((rstd, "rstd", F32, rows),))
     _need_all(dev, (
-        (rstd, "rstd", F32, rows), (pos, "pos", I64, rows * 3),
+        (pos, "pos", I64, rows * 3),
         (rope_tab, "rope_tab", F32, 2 * (mx * px + my * py + mz * pz)),
         (q_gamma, "q_gamma", F32, d), (k_gamma, "k_gamma", F32, d),
         (token_row, "token_row", I32, rows), (token_slot, "token_slot", I32, rows),
         (q_out, "q_out", out, rows * heads * d), (k_cache, "k_cache", out, 0),
         (v_cache, "v_cache", out, 0)))
-    if rows == 0:
+    if rows == 0 or batch == 0:
         return
-    with _on_device(dev):
-        _lib.check(_lib.lib().mdl_qk_norm_rope_cache(
-            qkv.data_ptr(), in_dt, ld, None if rstd is None else rstd.data_ptr(), pos.data_ptr(),
-            rope_tab.data_ptr(), rows, token_row.data_ptr(), token_slot.data_ptr(), batch, heads,
-            kv, d, mx, my, mz, px, py, pz, q_gamma.data_ptr(), k_gamma.data_ptr(), eps, q_scale,
-            q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out_dt, slots,
-            torch._C._cuda_getCurrentRawStream(dev)), "mdl_qk_norm_rope_cache")
+    _launch(dev, "mdl_qk_norm_rope_cache", qkv.data_ptr(), in_dt, ld,
+            None if rstd is None else rstd.data_ptr(), pos.data_ptr(), rope_tab.data_ptr(), rows,
+            token_row.data_ptr(), token_slot.data_ptr(), batch, heads, kv, d, mx, my, mz, px, py,
+            pz, q_gamma.data_ptr(), k_gamma.data_ptr(), eps, q_scale, q_out.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), out_dt, slots)
 
 
 def attn_grouped_workspace_bytes(q: torch.Tensor, k_cache: torch.Tensor, max_q: int) -> int:
     """Bytes of ``attn_grouped``'s workspace for tensors of these shapes (0: none is used)."""
-    tokens, heads, d, kv = _grouped_q(q, k_cache)
-    return _lib.lib().mdl_attn_grouped_workspace_bytes(
-        k_cache.shape[0], tokens, max_q, heads, kv, d, cache_dtype_code(q), k_cache.shape[2])
+    (tokens, heads, d), (n_seq, kv, slots, _) = _grouped_shapes(q, k_cache)
+    return _lib.lib().mdl_attn_grouped_workspace_bytes(n_seq, tokens, max_q, heads, kv, d,
+                                                       cache_dtype_code(q), slots)
 
 
 def attn_grouped(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -1226,35 +1235,33 @@ def attn_grouped(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     row-major or ``tiled``: a projection's input).  ``workspace`` (fp32,
     attn_grouped_workspace_bytes; calls that overlap need one each) lets a call with few rows split
     its keys."""
-    tokens, heads, d, kv = _grouped_q(q, k_cache)
-    n_seq, slots = k_cache.shape[0], k_cache.shape[2]
-    _cache_shapes(k_cache, v_cache, "cache ", (n_seq, kv, d))
+    (tokens, heads, d), cache = _grouped_shapes(q, k_cache)
+    n_seq, kv, slots = cache[:3]
+    _same_shapes(k_cache, v_cache, "cache ", cache, (n_seq, kv, d))
     if q_offset.numel() != n_seq + 1 or kv_len.numel() != n_seq:
         raise ValueError(f"q_offset and kv_len must have {n_seq + 1} and {n_seq} elements")
     dev, dt, code = q.get_device(), q.dtype, cache_dtype_code(q)
     _need_all(dev, ((q, "q", dt, 0), (k_cache, "k_cache", dt, 0), (v_cache, "v_cache", dt, 0),
                     (q_offset, "q_offset", I32, 0), (kv_len, "kv_len", I32, 0),
-                    _out_spec(out, q, tokens, heads * d, split, tiled),
-                    (workspace, "workspace", F32, 0)))
+                    _out_spec(out, q, tokens, heads * d, split, tiled)))
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        _need_all(dev, ((workspace, "workspace", F32, 0),))
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * 4
     if tokens == 0 or n_seq == 0:
         return
-    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(),
-                                                        workspace.numel() * 4)
-    with _on_device(dev):
-        _lib.check(_lib.lib().mdl_attn_grouped(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), code, n_seq, tokens, max_q,
-            heads, kv, d, slots, q_offset.data_ptr(), kv_len.data_ptr(), int(causal),
-            out.data_ptr(), split + tiled, ws, ws_bytes,
-            torch._C._cuda_getCurrentRawStream(dev)), "mdl_attn_grouped")
+    _launch(dev, "mdl_attn_grouped", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), code,
+            n_seq, tokens, max_q, heads, kv, d, slots, q_offset.data_ptr(), kv_len.data_ptr(),
+            int(causal), out.data_ptr(), split + tiled, ws, ws_bytes)
 
 
 def attn_decode_shared_workspace_bytes(q: torch.Tensor, prefix_k: torch.Tensor,
                                        k_cache: torch.Tensor, max_rows: int) -> int:
     """Bytes of ``attn_decode_shared``'s workspace for tensors of these shapes."""
-    batch, heads, d, kv = _grouped_q(q, k_cache)
+    (batch, heads, d), (_, kv, slots, _) = _grouped_shapes(q, k_cache)
     return _lib.lib().mdl_attn_decode_shared_workspace_bytes(
         batch, prefix_k.shape[0], max_rows, heads, kv, d, cache_dtype_code(q), prefix_k.shape[2],
-        k_cache.shape[2])
+        slots)
 
 
 def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
@@ -1268,19 +1275,21 @@ def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     D]; group g has the rows row_offset[g] .. row_offset[g + 1] - 1 (int32 [n_prefix + 1], at most
     ``max_rows``).  ``workspace``: fp32, attn_decode_shared_workspace_bytes.  Otherwise as
     attn_grouped."""
-    batch, heads, d, kv = _grouped_q(q, k_cache)
-    n_prefix = prefix_k.shape[0]
-    if n_prefix == 0:
-        raise ValueError("prefix_k holds no prefix")
-    _cache_shapes(prefix_k, prefix_v, "prefix_", (n_prefix, kv, d))
-    _cache_shapes(k_cache, v_cache, "cache ", (batch, kv, d))
+    (batch, heads, d), cache = _grouped_shapes(q, k_cache)
+    kv, prefix = cache[1], prefix_k.shape
+    if len(prefix) != 4 or not prefix[0]:
+        raise ValueError("prefix_k must be [n_prefix, n_kv_heads, prefix_slots, head_dim], with a "
+                         f"prefix at least (got {tuple(prefix)})")
+    n_prefix = prefix[0]
+    _same_shapes(prefix_k, prefix_v, "prefix_", prefix, (n_prefix, kv, d))
+    _same_shapes(k_cache, v_cache, "cache ", cache, (batch, kv, d))
     if (row_offset.numel() != n_prefix + 1 or prefix_len.numel() != n_prefix or
             kv_len.numel() != batch):
         raise ValueError(f"row_offset, prefix_len and kv_len must have {n_prefix + 1}, {n_prefix} "
                          f"and {batch} elements")
-    dev, dt, code = q.get_device(), q.dtype, cache_dtype_code(q)
     if workspace is None:
         raise ValueError("workspace is required")
+    dev, dt, code = q.get_device(), q.dtype, cache_dtype_code(q)
     _need_all(dev, ((q, "q", dt, 0), (prefix_k, "prefix_k", dt, 0), (prefix_v, "prefix_v", dt, 0),
                     (row_offset, "row_offset", I32, 0), (prefix_len, "prefix_len", I32, 0),
                     (k_cache, "k_cache", dt, 0), (v_cache, "v_cache", dt, 0),
@@ -1289,13 +1298,10 @@ def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
                     (workspace, "workspace", F32, 0)))
     if batch == 0:
         return
-    with _on_device(dev):
-        _lib.check(_lib.lib().mdl_attn_decode_shared(
-            q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), row_offset.data_ptr(),
-            prefix_len.data_ptr(), n_prefix, prefix_k.shape[2], max_rows, k_cache.data_ptr(),
-            v_cache.data_ptr(), kv_len.data_ptr(), batch, k_cache.shape[2], code, heads, kv, d,
-            out.data_ptr(), split + tiled, workspace.data_ptr(), workspace.numel() * 4,
-            torch._C._cuda_getCurrentRawStream(dev)), "mdl_attn_decode_shared")
+    _launch(dev, "mdl_attn_decode_shared", q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(),
+            row_offset.data_ptr(), prefix_len.data_ptr(), n_prefix, prefix[2], max_rows,
+            k_cache.data_ptr(), v_cache.data_ptr(), kv_len.data_ptr(), batch, cache[2], code, heads,
+            kv, d, out.data_ptr(), split + tiled, workspace.data_ptr(), workspace.numel() * 4)
 
 
 
