@@ -48,6 +48,23 @@ constexpr float kGap = 8.f;   // log2 of the largest p between moves of the refe
 enum OutForm { kOutPlain = MDL_OUT_PLAIN, kOutSplitRows = MDL_OUT_SPLIT_ROWS,
                kOutSplitTiles = MDL_OUT_SPLIT_TILES };
 
+// n / d for 0 <= n < 2^31 as (n m) >> s, m = ceil(2^s / d), s = 31 + ceil(log2 d): m d exceeds 2^s by
+// less than d <= 2^(s - 31), so n of them by less than 2^s.  A block's place takes four divisions by
+// numbers of the launch, some 200 cycles each the usual way.
+struct Divisor {
+  uint32_t m, s;
+};
+
+inline Divisor divisor(uint32_t d) {
+  uint32_t s = 31;
+  while ((uint64_t{1} << (s - 31)) < d) ++s;
+  return {static_cast<uint32_t>(((uint64_t{1} << s) + d - 1) / d), s};
+}
+
+__device__ __forceinline__ int quotient(int n, Divisor d) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * d.m) >> d.s);
+}
+
 struct GroupedArgs {
   const void* q;               // [tokens, heads, D]
   const void* k;               // [n_seq, kv_heads, slots, D]
@@ -60,6 +77,7 @@ struct GroupedArgs {
   int n_seq, tokens, heads, kv_heads, group, slots, max_q, causal, n_tiles, n_split, part0;
   int out_form;
   int n_serp;   // blocks of a tall launch, 0 otherwise
+  Divisor by_pairs, by_split, by_kv, by_group;
 };
 
 // Chunk swizzle of a tile row (16-byte chunks), by its low 4 bits r3..r0.  Both reads are then free
@@ -165,11 +183,12 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   // it costs 0-2% (the 8,192 above 875, 893).
   if ((block >> 8) == 1 && (block | 255) < p.n_serp) block ^= 248;
   const int pairs = p.n_seq * p.kv_heads;
-  const int rest = block / pairs, idx = block - rest * pairs;
-  const int rank = rest / p.n_split, split = rest - rank * p.n_split;
+  const int rest = quotient(block, p.by_pairs), idx = block - rest * pairs;
+  const int rank = quotient(rest, p.by_split), split = rest - rank * p.n_split;
   const int tile = p.n_tiles - 1 - rank;
-  const int pair = (idx + ((block - idx) & 7) + 5 * (rank / 6)) % pairs;
-  const int seq = pair / p.kv_heads, kvh = pair - seq * p.kv_heads;
+  const int turned = idx + ((block - idx) & 7) + 5 * (rank / 6);
+  const int pair = turned - pairs * quotient(turned, p.by_pairs);
+  const int seq = quotient(pair, p.by_kv), kvh = pair - seq * p.kv_heads;
   int lo = seq, hi = seq + 1;
   if (p.q_offset) {
     lo = min(max(p.q_offset[seq], 0), p.tokens);
@@ -188,7 +207,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   // the limits of the block's last row, this lane's row, and the wave's first and last
   // (row r's query is r / G: q0 + (r - G q0) / G with q0 = r0 / G, the small quotient in fp32, exact
   // below 2^20: (x + 1/2) / G is at least 1 / (2 G) away from a whole number)
-  const int q0 = r0 / G;
+  const int q0 = quotient(r0, p.by_group);
   const float inv_g = 1.f / G;
   auto query = [&](int r) {
     return q0 + static_cast<int>((static_cast<float>(r - G * q0) + 0.5f) * inv_g);
@@ -431,6 +450,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int ka = (r & 3) + 8 * (r >> 2);
+        if (masked && kt + 8 * (r >> 2) > lim_hi) continue;   // no row sees these steps
         float v[DB];
         v_row(Vt, ka + 4 * h, v);
         if (masked && kt + ka + 4 > lim_lo) masked_pair(v, kt + ka, sc[0][r]);
@@ -445,6 +465,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const int key = 32 * nb + 16 * s;
+          if (masked && kt + key > lim_hi) continue;   // no row sees the step: its weights are zero
           const f32x16_t& t = sc[nb];
           const bf16x8_t pb = {(__bf16)t[8 * s], (__bf16)t[8 * s + 1], (__bf16)t[8 * s + 2],
                                (__bf16)t[8 * s + 3], (__bf16)t[8 * s + 4], (__bf16)t[8 * s + 5],
@@ -774,15 +795,19 @@ int launch_tiles(const GroupedArgs* a, const bool* tall, int lists, hipStream_t 
     const int64_t blocks =
         static_cast<int64_t>(a[i].n_seq) * a[i].kv_heads * a[i].n_tiles * a[i].n_split;
     if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+    GroupedArgs t = a[i];
+    t.by_pairs = divisor(static_cast<uint32_t>(t.n_seq) * t.kv_heads);
+    t.by_split = divisor(t.n_split);
+    t.by_kv = divisor(t.kv_heads);
+    t.by_group = divisor(t.group);
     if (tall[i]) {
-      GroupedArgs t = a[i];
       t.n_serp = static_cast<int>(blocks);
       attn_grouped_kernel<T, D, 4, 1, f32 ? 32 : 64>
           <<<static_cast<unsigned>(blocks), 256, 0, st>>>(t);
       const int rc = launch_status();
       if (rc != MDL_OK) return rc;
     } else {
-      flat.list[n_flat == 0 ? 0 : 1] = a[i];
+      flat.list[n_flat == 0 ? 0 : 1] = t;
       if (n_flat == 0) flat.n_first = static_cast<int>(blocks);
       n_flat += blocks;
     }
