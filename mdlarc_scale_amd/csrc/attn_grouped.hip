@@ -48,9 +48,9 @@ constexpr float kGap = 8.f;   // log2 of the largest p between moves of the refe
 enum OutForm { kOutPlain = MDL_OUT_PLAIN, kOutSplitRows = MDL_OUT_SPLIT_ROWS,
                kOutSplitTiles = MDL_OUT_SPLIT_TILES };
 
-// n / d for 0 <= n < 2^31 as (n m) >> s, m = ceil(2^s / d), s = 31 + ceil(log2 d): m d exceeds 2^s by
-// less than d <= 2^(s - 31), so n of them by less than 2^s.  A block's place takes four divisions by
-// numbers of the launch, some 200 cycles each the usual way.
+// n / d for 0 <= n < 2^31 as (n m) >> s, m = ceil(2^s / d), s = 31 + ceil(log2 d): m d exceeds 2^s
+// by less than d <= 2^(s - 31), so n of them by less than 2^s.  A block's place takes four
+// divisions by numbers of the launch, some 200 cycles each the usual way.
 struct Divisor {
   uint32_t m, s;
 };
@@ -156,7 +156,8 @@ struct GroupedShape {
   static constexpr int kRows = 32 * WR;                   // rows of a block
   static constexpr int kCopies = kTile / 1024 / WR;       // 1 KB copies of a wave, K or V
   static constexpr int kRowsPerCopy = 1024 / kRowBytes;
-  // registers for as many waves as LDS lets reside (four on a CU are one on each SIMD), at most three
+  // registers for as many waves as LDS lets reside (four on a CU are one on each SIMD), at most
+  // three
   static constexpr int kResident = 160 * 1024 / kLds * WR * WK / 4;
   static constexpr int kWavesPerSimd = kResident < 2 ? 1 : D == 64 && WR > 1 ? 3 : 2;
   static_assert(WR > 1 || 3 * kCopies < 63, "copies in flight fit the counter");
@@ -172,15 +173,15 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int NB = KT / 32, DB = D / 32;
   // Order of the work.  Blocks are placed in turn, the first 256 on a CU each and so on, and to the
-  // XCDs in turn; the longest tiles (the latest rows, with the most keys) go first.
-  // The second 256 run backwards, so that a CU with one of the longest gets one of the shortest of
-  // those: 2 prompts of 4,000 tokens (12 fp32 heads of 64, 768 blocks that all fit) 501 -> 427 us, 2 of
-  // up to 8,192 (32 heads of 128) 908 -> 877, 5 of up to 811 (16 heads of 64) 19.6 -> 18.1.
-  // A pair (sequence, key / value head) keeps to one XCD, whose L2 then serves its row tiles, for six
-  // ranks of tiles and then moves on by five: sequences differ in length, and pairs that stayed would
-  // leave some XCDs with the long ones.  4 prompts of 3,900 to 6,000 tokens (16 heads of 64) 295 us
-  // staying, 256 so; 2 of up to 3,000 (16 fp32 heads of 128) 592, 545; where nothing is to be balanced
-  // it costs 0-2% (the 8,192 above 875, 893).
+  // XCDs in turn; the longest tiles (the latest rows, with the most keys) go first. The second 256
+  // run backwards, so that a CU with one of the longest gets one of the shortest of those: 2
+  // prompts of 4,000 tokens (12 fp32 heads of 64, 768 blocks that all fit) 501 -> 427 us, 2 of up
+  // to 8,192 (32 heads of 128) 908 -> 877, 5 of up to 811 (16 heads of 64) 19.6 -> 18.1. A pair
+  // (sequence, key / value head) keeps to one XCD, whose L2 then serves its row tiles, for six
+  // ranks of tiles and then moves on by five: sequences differ in length, and pairs that stayed
+  // would leave some XCDs with the long ones.  4 prompts of 3,900 to 6,000 tokens (16 heads of 64)
+  // 295 us staying, 256 so; 2 of up to 3,000 (16 fp32 heads of 128) 592, 545; where nothing is to
+  // be balanced it costs 0-2% (the 8,192 above 875, 893).
   if ((block >> 8) == 1 && (block | 255) < p.n_serp) block ^= 248;
   const int pairs = p.n_seq * p.kv_heads;
   const int rest = quotient(block, p.by_pairs), idx = block - rest * pairs;
@@ -204,9 +205,9 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave % WR, wk = wave / WR;
-  // the limits of the block's last row, this lane's row, and the wave's first and last
-  // (row r's query is r / G: q0 + (r - G q0) / G with q0 = r0 / G, the small quotient in fp32, exact
-  // below 2^20: (x + 1/2) / G is at least 1 / (2 G) away from a whole number)
+  // the limits of the block's last row, this lane's row, and the wave's first and last (row r's
+  // query is r / G: q0 + (r - G q0) / G with q0 = r0 / G, the small quotient in fp32, exact below
+  // 2^20: (x + 1/2) / G is at least 1 / (2 G) away from a whole number)
   const int q0 = quotient(r0, p.by_group);
   const float inv_g = 1.f / G;
   auto query = [&](int r) {
@@ -290,8 +291,8 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
                     16 * ((vchunk + 4 * db) ^ swz<T, D>(vr + 8 * e)) + 8 * (lane & 1);
 
   float negm = 0.f, thr = -INFINITY, l = 0.f;   // l: this lane half's part of the sum
-  // minus the reference in every element, kept where registers allow (2 x 12 moves a tile less: 941 ->
-  // 908 us on two prompts of up to 8,192 tokens, 32 heads of 128; nothing with 64 dims)
+  // minus the reference in every element, kept where registers allow (2 x 12 moves a tile less: 941
+  // -> 908 us on two prompts of up to 8,192 tokens, 32 heads of 128; nothing with 64 dims)
   constexpr bool kKeepStart = !kF32 && D == 128 && WR > 1;
   f32x16_t start = splat16(0.f);
   f32x16_t o[DB];
@@ -486,9 +487,10 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     }
   };
 
-  // Tiles first + i kTurn are this group's.  Tiles that every row of a wave sees whole come first, in
-  // a loop of their own: it is free of branches, and the output stays in the same registers, which a
-  // choice inside one loop costs.  Tiles go two at a time, so that their stage is a constant.
+  // Tiles first + i kTurn are this group's.  Tiles that every row of a wave sees whole come first,
+  // in a loop of their own: it is free of branches, and the output stays in the same registers,
+  // which a choice inside one loop costs.  Tiles go two at a time, so that their stage is a
+  // constant.
   const int first = k0 + KT * wk;
   constexpr std::integral_constant<int, 0> kEven{};
   constexpr std::integral_constant<int, 1> kOdd{};
@@ -500,8 +502,8 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     // every wave of the block makes the same number of turns, so the barriers match
     auto turn = [&](int kt, auto stc, auto fullc) {
       constexpr int ST = decltype(stc)::value;
-      // tile kt has landed for every wave, and every wave is done with the other stage.  The builtin
-      // wait also covers the loads that the compiler knows of.
+      // tile kt has landed for every wave, and every wave is done with the other stage.  The
+      // builtin wait also covers the loads that the compiler knows of.
       __builtin_amdgcn_s_waitcnt(kWaitAll);
       asm volatile("s_barrier" ::: "memory");
       if (kt + kTurn < k1) {
@@ -522,9 +524,9 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       if (t + kTurn < k1) turn(t + kTurn + KT * wk, kOdd, std::false_type{});
     }
   } else {
-    // A wave with a ring of its own needs no barrier, and refills K's slot as soon as its scores are
-    // there and V's after the product: three of the four slots are in flight.  Copies land in the
-    // order they were issued in, K V K V .., so a wait names how many may be outstanding.
+    // A wave with a ring of its own needs no barrier, and refills K's slot as soon as its scores
+    // are there and V's after the product: three of the four slots are in flight.  Copies land in
+    // the order they were issued in, K V K V .., so a wait names how many may be outstanding.
     constexpr int C = S::kCopies;
     const int nt = first < k1 ? (k1 - first + kTurn - 1) / kTurn : 0;
     for (int i = 0; i < 2 && i < nt; ++i) {
@@ -607,7 +609,9 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       return o[u][4 * j + e];
     }
   };
-  auto dim = [&](int j, int u) { return kF32 ? DB * (8 * j + 4 * h) + 4 * u : 32 * u + 8 * j + 4 * h; };
+  auto dim = [&](int j, int u) {
+    return kF32 ? DB * (8 * j + 4 * h) + 4 * u : 32 * u + 8 * j + 4 * h;
+  };
   if (p.ws_o) {
     const int64_t all = static_cast<int64_t>(p.tokens) * p.heads;
     const int64_t at_row = (p.part0 + split) * all + qrow;
@@ -662,10 +666,10 @@ struct MergeArgs {
 };
 
 // Joins the parts of one output row (token, head) per wave: parts [0, n0) hold it if the token is
-// one of a sequence's first max_q, parts [n0, n0 + n1) always do.  Lane s has the m and l of part s (at
-// most 64 parts); the values come eight parts at a time, in the parts' order.  The first values are
-// read with the states and with the search for the sequence, whose results decide what counts: one
-// wait on memory after another is all the time this takes.
+// one of a sequence's first max_q, parts [n0, n0 + n1) always do.  Lane s has the m and l of part s
+// (at most 64 parts); the values come eight parts at a time, in the parts' order.  The first values
+// are read with the states and with the search for the sequence, whose results decide what counts:
+// one wait on memory after another is all the time this takes.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
   constexpr int C = D / 64;
@@ -757,9 +761,9 @@ constexpr int kLongPart = 1280;   // keys of a part that make up for its state's
 
 // How one list of tiles runs: tall blocks (4 waves, 128 rows) or flat ones (32 rows, two waves that
 // share out the keys), and in how many parts the keys are cut.  Tall blocks read a key a quarter as
-// often; flat ones are more, with fewer rows to wait for.  So: tall where they fill the GPU uncut, and
-// where flat ones would have to be cut too; flat in between.  us, flat / tall: 704 flat blocks of a
-// 700-token prompt 23 / 30 (in two parts); 72 of 17 tokens behind 4,099 keys 21 / 19; 64 of 64
+// often; flat ones are more, with fewer rows to wait for.  So: tall where they fill the GPU uncut,
+// and where flat ones would have to be cut too; flat in between.  us, flat / tall: 704 flat blocks
+// of a 700-token prompt 23 / 30 (in two parts); 72 of 17 tokens behind 4,099 keys 21 / 19; 64 of 64
 // samples behind 32,749 keys (with their own keys and the merge) 117 / 73.  Tall blocks are cut to
 // one for each CU, and to two where the parts stay long: 4 continuations of 100 tokens behind 6,000
 // keys 64 / 53 us; the 64 samples above 73 / 75, 17 tokens behind 4,099 keys 19 / 21.
@@ -768,10 +772,11 @@ struct Plan {
   int n_tiles, n_split;
 };
 
-Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts) {
+Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts, bool stay_flat = false) {
   const int64_t tall = pairs * ((max_rows + 127) / 128), flat = pairs * ((max_rows + 31) / 32);
   Plan r;
-  r.tall = max_rows > 32 && (tall >= kTallFill || (max_parts > 1 && flat < kFlatFill));
+  r.tall = max_rows > 32 && !stay_flat &&
+           (tall >= kTallFill || (max_parts > 1 && flat < kFlatFill));
   r.n_tiles = static_cast<int>(r.tall ? (max_rows + 127) / 128 : (max_rows + 31) / 32);
   const int64_t blocks = r.tall ? tall : flat;
   int64_t fill = r.tall ? kTallFill : kFlatFill;
@@ -786,8 +791,8 @@ Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts) {
 template <typename T, int D>
 int launch_tiles(const GroupedArgs* a, const bool* tall, int lists, hipStream_t st) {
   constexpr bool f32 = sizeof(T) == 4;
-  // waves of a flat block: two, but one where a ring is 64 KB.  Four (half as many blocks on a CU, one
-  // with 128 dims) were 1-40% slower.
+  // waves of a flat block: two, but one where a ring is 64 KB.  Four (half as many blocks on a CU,
+  // one with 128 dims) were 1-40% slower.
   constexpr int kFlatGroups = f32 && D == 128 ? 1 : 2;
   GroupedPair flat{};
   int64_t n_flat = 0;
@@ -871,6 +876,7 @@ using namespace mdl;
 extern "C" int64_t mdl_attn_grouped_workspace_bytes(int n_seq, int tokens, int max_q, int n_heads,
                                                     int n_kv_heads, int head_dim, int dtype,
                                                     int cache_slots) {
+  max_q = max_q < tokens ? max_q : tokens;
   if (check_sizes(n_seq, tokens, max_q, n_heads, n_kv_heads, head_dim, dtype, cache_slots) !=
           MDL_OK || n_seq == 0 || max_q == 0)
     return 0;
@@ -887,6 +893,7 @@ extern "C" int mdl_attn_grouped(const void* q, const void* k_cache, const void* 
                                 const int32_t* kv_len, int causal, void* out, int out_form,
                                 float* workspace, int64_t workspace_bytes, void* stream) {
   if (!q || !k_cache || !v_cache || !q_offset || !kv_len || !out) return MDL_ERR_NULL;
+  max_q = max_q < tokens ? max_q : tokens;
   const int bad = check_sizes(n_seq, tokens, max_q, n_heads, n_kv_heads, head_dim, dtype,
                               cache_slots);
   if (bad != MDL_OK) return bad;
@@ -925,12 +932,22 @@ struct SharedPlan {
   Plan prefix, own;
 };
 
+// Where the rows' own keys are the larger part, the prefixes go in flat tiles, although those read
+// a key more often: in one launch with the own keys their work lies under that traffic.  us, tall /
+// flat: 64 samples of a 1,763-token prompt (16 heads on 4 of 64, up to 700 own keys) 23.1 / 17.5;
+// 128 of a 4,000-token one (16 heads of 64, up to 100) 29.3 / 25.0.  With 128 dims a flat block
+// leaves the products fewer waves, and only a quarter of the own keys' traffic hides them: 64 rows
+// of two 1,763-token prompts (32 heads on 8, up to 900) 54 / 58.
 SharedPlan plan_shared(int batch, int n_prefix, int max_rows, int n_heads, int n_kv_heads,
-                       int prefix_slots, int cache_slots) {
+                       int prefix_slots, int cache_slots, int head_dim) {
   const int64_t g = n_heads / n_kv_heads;
+  const double prefix_reads =
+      static_cast<double>((max_rows * g + 31) / 32) * n_prefix * prefix_slots;
+  const bool own_first = prefix_reads * (head_dim == 128 ? 4 : 1) <=
+                         static_cast<double>(batch) * cache_slots;
   SharedPlan r;
   r.prefix = plan_tiles(static_cast<int64_t>(n_prefix) * n_kv_heads, max_rows * g, prefix_slots,
-                        kMaxParts - kMaxOwn);
+                        kMaxParts - kMaxOwn, own_first);
   r.own = plan_tiles(static_cast<int64_t>(batch) * n_kv_heads, g, cache_slots, kMaxOwn);
   return r;
 }
@@ -942,13 +959,14 @@ extern "C" int64_t mdl_attn_decode_shared_workspace_bytes(int batch, int n_prefi
                                                           int n_heads, int n_kv_heads,
                                                           int head_dim, int dtype,
                                                           int prefix_slots, int cache_slots) {
+  max_rows = max_rows < batch ? max_rows : batch;
   if (check_sizes(n_prefix, batch, max_rows, n_heads, n_kv_heads, head_dim, dtype, prefix_slots) !=
           MDL_OK ||
       check_sizes(batch, batch, 1, n_heads, n_kv_heads, head_dim, dtype, cache_slots) != MDL_OK ||
       batch == 0 || n_prefix == 0 || max_rows == 0)
     return 0;
   const SharedPlan pl = plan_shared(batch, n_prefix, max_rows, n_heads, n_kv_heads, prefix_slots,
-                                    cache_slots);
+                                    cache_slots, head_dim);
   return state_bytes(pl.prefix.n_split + pl.own.n_split, static_cast<int64_t>(batch) * n_heads,
                      head_dim);
 }
@@ -976,8 +994,9 @@ extern "C" int mdl_attn_decode_shared(const void* q, const void* prefix_k, const
       !aligned4(prefix_len) || !aligned4(kv_len))
     return MDL_ERR_ALIGN;
   if (batch == 0) return MDL_OK;
+  max_rows = max_rows < batch ? max_rows : batch;
   const SharedPlan pl = plan_shared(batch, n_prefix, max_rows, n_heads, n_kv_heads, prefix_slots,
-                                    cache_slots);
+                                    cache_slots, head_dim);
   const int64_t rows = static_cast<int64_t>(batch) * n_heads;
   const int parts = pl.prefix.n_split + pl.own.n_split;
   if (workspace_bytes < state_bytes(parts, rows, head_dim)) return MDL_ERR_WORKSPACE;

@@ -1,5 +1,5 @@
-"""Arguments that K7 and K8 refuse before any launch (no GPU needed: the C entries check pointers and
-sizes on the host, the Python wrappers check tensors)."""
+"""Arguments that K7 and K8 refuse before any launch (no GPU needed: the C entries check pointers
+and sizes on the host, the Python wrappers check tensors)."""
 
 import pytest
 import torch
@@ -44,7 +44,8 @@ AG = dict(q=FAKE, k=FAKE, v=FAKE, dtype=1, n_seq=2, tokens=9, max_q=5, heads=6, 
     (dict(q=None), NULL), (dict(kv_len=None), NULL), (dict(q_offset=None), NULL),
     (dict(out=None), NULL), (dict(dim=80), HEAD), (dict(dtype=3), DTYPE), (dict(heads=7), SHAPE),
     (dict(kv=0), SHAPE), (dict(tokens=-1), SHAPE), (dict(max_q=-2), SHAPE), (dict(form=3), SHAPE),
-    (dict(slots=2 ** 31 - 1), SHAPE), (dict(max_q=2 ** 31 - 1), SHAPE), (dict(n_seq=2 ** 30 + 1), SHAPE),
+    (dict(slots=2 ** 31 - 1), SHAPE), (dict(n_seq=2 ** 30 + 1), SHAPE),
+    (dict(tokens=2 ** 31 - 1, max_q=2 ** 31 - 1), SHAPE),
     (dict(q=FAKE + 8), ALIGN), (dict(out=FAKE + 2), ALIGN), (dict(ws=FAKE + 4), ALIGN),
     (dict(kv_len=FAKE + 2), ALIGN), (dict(), WORKSPACE)])
 def test_grouped_refusals(L, change, code):
@@ -58,6 +59,9 @@ def test_grouped_workspace(L):
     assert L.mdl_attn_grouped_workspace_bytes(64, 6400, 100, 16, 16, 64, 1, 4096) == 0
     assert L.mdl_attn_grouped_workspace_bytes(2, 9, 5, 6, 2, 64, 1, 64) == 0
     assert L.mdl_attn_grouped_workspace_bytes(2, 9, 5, 6, 4, 64, 1, 4096) == 0
+    # a bound above the number of rows is that number
+    assert (L.mdl_attn_grouped_workspace_bytes(2, 9, 2 ** 31 - 1, 6, 2, 64, 1, 4096) ==
+            L.mdl_attn_grouped_workspace_bytes(2, 9, 9, 6, 2, 64, 1, 4096) > 0)
 
 
 SH = dict(q=FAKE, pk=FAKE, pv=FAKE, row_offset=FAKE, prefix_len=FAKE, n_prefix=1, prefix_slots=512,
