@@ -123,22 +123,11 @@ __device__ __forceinline__ float add_pair(float l, uint32_t w) {
                                          __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
 }
 
-// Four consecutive channels `col` .. + 3 of output row `row` (width `d` = heads * D).
-template <typename T>
-__device__ __forceinline__ void store_out4(void* out, int form, int64_t row, int col, int d,
-                                           float a, float b, float c, float e) {
-  if (form == kOutPlain) {
-    T* p = static_cast<T*>(out) + row * d + col;
-    if constexpr (sizeof(T) == 4)
-      *reinterpret_cast<float4*>(p) = make_float4(a, b, c, e);
-    else
-      *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf2(a, b), pack_bf2(c, e));
-    return;
-  }
-  const float t[4] = {a, b, c, e};
+// Four consecutive channels `col` .. + 3 of output row `row` (width `d`) as hi|lo bf16.
+__device__ __forceinline__ void store_split4(uint16_t* o, int form, int64_t row, int col, int d,
+                                             const float* t) {
   uint2 hi, lo;
   split4(t, hi, lo);
-  uint16_t* o = static_cast<uint16_t*>(out);
   if (form == kOutSplitTiles) {
     *reinterpret_cast<uint2*>(o + tile_off(row, col, 2 * d)) = hi;
     *reinterpret_cast<uint2*>(o + tile_off(row, d + col, 2 * d)) = lo;
@@ -152,7 +141,11 @@ template <typename T, int D, int WR, int WK, int KT>
 struct GroupedShape {
   static constexpr int kRowBytes = D * static_cast<int>(sizeof(T));
   static constexpr int kTile = KT * kRowBytes;            // bytes of a K or V tile
-  static constexpr int kLds = WK * 4 * kTile;             // two stages of K and V per group
+  // Two stages of K and V per group.  One for the flat fp32 blocks of 128 dims, where either product
+  // of a tile (4,096 cycles) outlasts a copy: twice the waves on a CU, 16 rows of 2,000 keys (16
+  // heads) 45 -> 33 us.  With 64 dims the copies are waited for: 2 prompts of up to 731 tokens 37 -> 42.
+  static constexpr int kStages = WR == 1 && kRowBytes == 512 ? 1 : 2;
+  static constexpr int kLds = WK * 2 * kStages * kTile;
   static constexpr int kRows = 32 * WR;                   // rows of a block
   static constexpr int kCopies = kTile / 1024 / WR;       // 1 KB copies of a wave, K or V
   static constexpr int kRowsPerCopy = 1024 / kRowBytes;
@@ -163,7 +156,8 @@ struct GroupedShape {
   static_assert(WR > 1 || 3 * kCopies < 63, "copies in flight fit the counter");
   static_assert(kTile % (1024 * WR) == 0, "whole copies per wave");
   static_assert(KT % 32 == 0 && (D == 64 || D == 128), "whole MFMA blocks");
-  // the merge of the groups goes through the ring's memory
+  // the results of the waves, and the merge of the groups, go through the ring's memory
+  static_assert(WR * 32 * D * 4 <= kLds, "rows of floats fit");
   static_assert((WK - 1) * WR * (2 + D / 2) * 256 <= kLds, "states of the other groups fit");
 };
 
@@ -220,6 +214,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   const int row = w0 + c;
   const bool real = row < rows;
   const int qi = query(min(row, rows - 1)), hg = min(row, rows - 1) - qi * G;
+  const int q_first = uniform(query(min(w0, rows - 1)));   // of the wave
   const int lim = real ? limit(qi) : -1;
   const int lim_lo = uniform(w0 < rows ? limit(query(w0)) : -1);
   const int lim_hi = uniform(w0 < rows ? limit(query(min(w0 + 32, rows) - 1)) : -1);
@@ -232,7 +227,9 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   using QFrag = typename std::conditional<kF32, float4, bf16x8_t>::type;
   constexpr int NQ = kF32 ? D / 8 : D / 16;
   QFrag qf[NQ];
-  {
+  // tall bf16 blocks take q through the ring (below)
+  constexpr bool kCopyQ = !kF32 && WR > 1;
+  if constexpr (!kCopyQ) {
     const T* qp = static_cast<const T*>(p.q) + qrow * D;
 #pragma unroll
     for (int s = 0; s < NQ; ++s) {
@@ -247,7 +244,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   const int64_t head = (static_cast<int64_t>(seq) * p.kv_heads + kvh) * p.slots * D;
   const T* Kg = static_cast<const T*>(p.k) + head;
   const T* Vg = static_cast<const T*>(p.v) + head;
-  uint8_t* ring = lds + wk * 4 * S::kTile;
+  uint8_t* ring = lds + wk * 2 * S::kStages * S::kTile;
   const uint32_t ring0 = lds_addr(ring);
   // Copy j of a tile: rows (1024 / row bytes) j .. of K and of V, one kilobyte each; a lane takes
   // physical chunk lane % chunks of its row.  Rows past the last key copy that key.
@@ -269,9 +266,9 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
         dma16_sbase(from, off, dst);
     }
   };
-  // slots of a ring: K of stage 0 and 1, V of stage 0 and 1
+  // slots of a ring: K of each stage, then V
   auto k_slot = [](int st) { return st * S::kTile; };
-  auto v_slot = [](int st) { return (2 + st) * S::kTile; };
+  auto v_slot = [](int st) { return (S::kStages + st) * S::kTile; };
 
   // Lane parts of the swizzled read addresses.  K operand: row c, bf16 chunk 2 s + h, fp32 chunk
   // h D / 8 + s.  V^T operand, bf16: rows 4 h + lane / 4 % 4 (and + 8) of a 16-key step, dims
@@ -499,6 +496,27 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       issue(Kg, first, k_slot(0));
       issue(Vg, first, v_slot(0));
     }
+    // q of the wave's 32 rows through the second stage (the first turn's barrier frees it), whole
+    // rows to a copy: read into registers directly, an instruction takes 16 bytes of 64 places.
+    if constexpr (kCopyQ) {
+      static_assert(!kCopyQ || (KT == 64 && WR == 4 && WK == 1), "two waves' rows to a slot");
+      const uint32_t at = (wr < 2 ? k_slot(1) : v_slot(1)) + (wr & 1) * 32 * S::kRowBytes;
+      const T* from = scalar_ptr(static_cast<const T*>(p.q) +
+                                 (static_cast<int64_t>(lo + q_first) * p.heads + kvh * G) * D);
+#pragma unroll
+      for (int j = 0; j < 32 / S::kRowsPerCopy; ++j) {
+        const int r = S::kRowsPerCopy * j + lane / kChunks;
+        const int g = min(w0 + r, rows - 1), gq = query(g);
+        const uint32_t off = ((gq - q_first) * p.heads + g - gq * G) * S::kRowBytes +
+                             16 * ((lane % kChunks) ^ swz<T, D>(r & 15));
+        dma16_sbase(from, off, __builtin_amdgcn_readfirstlane(ring0 + at + 1024 * j));
+      }
+      wait_copies<0>();
+#pragma unroll
+      for (int s = 0; s < NQ; ++s)
+        qf[s] = as_bf16x8(
+            *reinterpret_cast<const uint4*>(ring + at + krow + 16 * ((2 * s + h) ^ kswz)));
+    }
     // every wave of the block makes the same number of turns, so the barriers match
     auto turn = [&](int kt, auto stc, auto fullc) {
       constexpr int ST = decltype(stc)::value;
@@ -524,12 +542,12 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       if (t + kTurn < k1) turn(t + kTurn + KT * wk, kOdd, std::false_type{});
     }
   } else {
-    // A wave with a ring of its own needs no barrier, and refills K's slot as soon as its scores
-    // are there and V's after the product: three of the four slots are in flight.  Copies land in
-    // the order they were issued in, K V K V .., so a wait names how many may be outstanding.
-    constexpr int C = S::kCopies;
+    // A wave with a ring of its own needs no barrier, and refills K's slot as soon as its scores are
+    // there and V's after the product: all slots but one are in flight.  Copies land in the order
+    // they were issued in, K V K V .., so a wait names how many may be outstanding.
+    constexpr int C = S::kCopies, NS = S::kStages;
     const int nt = first < k1 ? (k1 - first + kTurn - 1) / kTurn : 0;
-    for (int i = 0; i < 2 && i < nt; ++i) {
+    for (int i = 0; i < NS && i < nt; ++i) {
       issue(Kg, first + i * kTurn, k_slot(i));
       issue(Vg, first + i * kTurn, v_slot(i));
     }
@@ -537,26 +555,26 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     // it for every copy
     __builtin_amdgcn_s_waitcnt(kWaitAll);
     auto step = [&](int i, auto stc, auto fullc) {
-      constexpr int ST = decltype(stc)::value;
+      constexpr int ST = NS == 1 ? 0 : decltype(stc)::value;
       const int kt = first + i * kTurn;
-      if (i + 1 < nt)
-        wait_copies<3 * C>();
+      if (NS > 1 && i + 1 < nt)
+        wait_copies<3 * C>();   // V of this tile, K and V of the next
       else
-        wait_copies<C>();
+        wait_copies<C>();       // V of this tile
       compute(ring + k_slot(ST), ring + v_slot(ST), kt, fullc, [&] {
-        if (i + 2 < nt) {
+        if (i + NS < nt) {
           wait_reads();   // of K's slot
-          issue(Kg, kt + 2 * kTurn, k_slot(ST));
-          wait_copies<3 * C>();
-        } else if (i + 1 < nt) {
+          issue(Kg, kt + NS * kTurn, k_slot(ST));
+          wait_copies<(2 * NS - 1) * C>();
+        } else if (NS > 1 && i + 1 < nt) {
           wait_copies<2 * C>();
         } else {
           wait_copies<0>();
         }
       });
-      if (i + 2 < nt) {
+      if (i + NS < nt) {
         wait_reads();     // of V's slot
-        issue(Vg, kt + 2 * kTurn, v_slot(ST));
+        issue(Vg, kt + NS * kTurn, v_slot(ST));
       }
     };
     int i = 0;
@@ -598,42 +616,80 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
         o[i >> 4][i & 15] = fmaf(w[(2 + i) * kWave], aj, o[i >> 4][i & 15] * a);
     }
   }
-  if (!real) return;
-  // elements 4 j .. 4 j + 3: bf16, dims 32 db + 8 j + 4 h .. + 3 of block db; fp32, dims
-  // DB (8 j + 4 h + e) + db, e = 0..3: 4 DB neighbours
-  auto at = [&](int j, int u, int e) -> float {   // e-th of the 4 channels of store u
-    if constexpr (kF32) {
-      const int x = 4 * u + e;
-      return o[x % DB][4 * j + x / DB];
-    } else {
-      return o[u][4 * j + e];
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // no visible key: 0; NaN stays
+  const bool part = p.ws_o != nullptr;
+  const int64_t base = (p.part0 + split) * static_cast<int64_t>(p.tokens) * p.heads;
+  const int d = p.heads * D, col0 = (kvh * G + hg) * D;
+  if (kF32 || part) {
+    // fp32 rows, and states, straight from the registers: 16 bytes at a time, of neighbouring ones
+    if (!real) return;
+    if (part) {
+      if (h == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * (base + qrow)) = make_float2(m, l);
+      if (m == -INFINITY) return;   // the merge takes no value of such a state
     }
-  };
-  auto dim = [&](int j, int u) {
-    return kF32 ? DB * (8 * j + 4 * h) + 4 * u : 32 * u + 8 * j + 4 * h;
-  };
-  if (p.ws_o) {
-    const int64_t all = static_cast<int64_t>(p.tokens) * p.heads;
-    const int64_t at_row = (p.part0 + split) * all + qrow;
-    if (h == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * at_row) = make_float2(m, l);
-    if (m == -INFINITY) return;   // the merge takes no value of such a state
-    float* w = p.ws_o + at_row * D;
+    const float scale = part ? 1.f : inv;
+    float* to = part ? p.ws_o + (base + qrow) * D : static_cast<float*>(p.out) + qrow * D;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int u = 0; u < DB; ++u) {
+        // elements 4 j .. 4 j + 3: bf16, dims 32 u + 8 j + 4 h .. + 3 of block u; fp32, 4 of the
+        // dims DB (8 j + 4 h) .. + 4 DB - 1 (element 4 j + x / DB of block x % DB is the x-th)
+        const int dim = kF32 ? DB * (8 * j + 4 * h) + 4 * u : 32 * u + 8 * j + 4 * h;
+        float t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = 4 * u + e;
+          t[e] = (kF32 ? o[x % DB][4 * j + x / DB] : o[u][4 * j + e]) * scale;
+        }
+        if (part || p.out_form == kOutPlain)
+          *reinterpret_cast<float4*>(to + dim) = make_float4(t[0], t[1], t[2], t[3]);
+        else
+          store_split4(static_cast<uint16_t*>(p.out), p.out_form, lo + qi, col0 + dim, d, t);
+      }
+    return;
+  }
+  if constexpr (!kF32) {
+    // bf16 results leave by rows, the wave's [32][D] floats through the ring's memory (16-byte
+    // chunks XOR-swizzled by row): a lane's own channels are 8-byte pieces, 32 rows of them to a
+    // store.  6 prompts of up to 1,203 tokens (32 heads of 128) 94 -> 74 us with q's copies above.
+    if constexpr (WR > 1) __syncthreads();   // every wave is done with its tiles
+    if (w0 >= rows) return;
+    float* stage = reinterpret_cast<float*>(lds) + wr * 32 * D;
+    constexpr int kQuads = D / 4;   // 16-byte chunks of a row of floats
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int u = 0; u < DB; ++u)
-        *reinterpret_cast<float4*>(w + dim(j, u)) =
-            make_float4(at(j, u, 0), at(j, u, 1), at(j, u, 2), at(j, u, 3));
-    return;
+        *reinterpret_cast<float4*>(stage + c * D +
+                                   4 * ((8 * u + 2 * j + h) ^ (c & (kQuads - 1)))) =
+            make_float4(o[u][4 * j] * inv, o[u][4 * j + 1] * inv, o[u][4 * j + 2] * inv,
+                        o[u][4 * j + 3] * inv);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own, in program order
+    __builtin_amdgcn_wave_barrier();
+    const int place = (qi - q_first) << 16 | hg;   // of row c, read by the lanes that store it
+    constexpr int kLanes = D / 8;                  // lanes of a row, eight channels each
+#pragma unroll 4
+    for (int r0w = 0; r0w < 32; r0w += kWave / kLanes) {
+      const int r = r0w + lane / kLanes, q = 2 * (lane % kLanes);
+      const int at = __shfl(place, r, kWave);
+      if (w0 + r >= rows) continue;
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float4*>(t + 4 * i) = *reinterpret_cast<const float4*>(
+            stage + r * D + 4 * ((q + i) ^ (r & (kQuads - 1))));
+      const int64_t token = lo + q_first + (at >> 16);
+      const int col = (kvh * G + (at & 0xffff)) * D + 4 * q;
+      uint16_t* out = static_cast<uint16_t*>(p.out);
+      if (p.out_form == kOutPlain) {
+        *reinterpret_cast<uint4*>(out + token * d + col) = pack8(t);
+      } else {
+        store_split4(out, p.out_form, token, col, d, t);
+        store_split4(out, p.out_form, token, col + 4, d, t + 4);
+      }
+    }
   }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // no visible key: 0; NaN stays
-  const int d = p.heads * D, col0 = (kvh * G + hg) * D;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int u = 0; u < DB; ++u)
-      store_out4<T>(p.out, p.out_form, lo + qi, col0 + dim(j, u), d, at(j, u, 0) * inv,
-                    at(j, u, 1) * inv, at(j, u, 2) * inv, at(j, u, 3) * inv);
 }
 
 template <typename T, int D, int WR, int WK, int KT>
@@ -791,9 +847,8 @@ Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts, bool 
 template <typename T, int D>
 int launch_tiles(const GroupedArgs* a, const bool* tall, int lists, hipStream_t st) {
   constexpr bool f32 = sizeof(T) == 4;
-  // waves of a flat block: two, but one where a ring is 64 KB.  Four (half as many blocks on a CU,
-  // one with 128 dims) were 1-40% slower.
-  constexpr int kFlatGroups = f32 && D == 128 ? 1 : 2;
+  // waves of a flat block.  Four (half as many blocks on a CU, one with 128 dims) were 1-40% slower.
+  constexpr int kFlatGroups = 2;
   GroupedPair flat{};
   int64_t n_flat = 0;
   for (int i = 0; i < lists; ++i) {
