@@ -812,33 +812,37 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
 constexpr int kMaxParts = 64;     // states that a wave of the merge holds
 constexpr int kMaxOwn = 16;       // of them for a row's own keys behind a prefix
 constexpr int kFlatFill = 512;    // blocks that fill the GPU: flat ones of 128 threads
+constexpr int kFlatFew = 256;     // (and what keeps every CU busy)
 constexpr int kTallFill = 256;    // and tall ones of 256
 constexpr int kLongPart = 1280;   // keys of a part that make up for its state's way through memory
+constexpr int kLongList = 4096;   // keys that two waves alone take too long over
 
 // How one list of tiles runs: tall blocks (4 waves, 128 rows) or flat ones (32 rows, two waves that
 // share out the keys), and in how many parts the keys are cut.  Tall blocks read a key a quarter as
 // often; flat ones are more, with fewer rows to wait for.  So: tall where they fill the GPU uncut,
-// and where flat ones would have to be cut too; flat in between.  us, flat / tall: 704 flat blocks
-// of a 700-token prompt 23 / 30 (in two parts); 72 of 17 tokens behind 4,099 keys 21 / 19; 64 of 64
-// samples behind 32,749 keys (with their own keys and the merge) 117 / 73.  Tall blocks are cut to
-// one for each CU, and to two where the parts stay long: 4 continuations of 100 tokens behind 6,000
-// keys 64 / 53 us; the 64 samples above 73 / 75, 17 tokens behind 4,099 keys 19 / 21.
+// and where flat ones would have to be cut too or have long lists; flat in between.  us, flat /
+// tall: 704 flat blocks of a 700-token prompt 23 / 30 (in two parts), 752 of a 1,500-token one (64
+// dims) 19 / 28; 540 of 467 tokens behind 11,204 keys 160 / 77; 72 of 17 tokens behind 4,099 keys
+// 21 / 19; 64 of 64 samples behind 32,749 keys (with their own keys and the merge) 117 / 73.
+// Tall blocks are cut to one for each CU, and to two where the parts stay long: 4 continuations of
+// 100 tokens behind 6,000 keys 64 / 53 us; the 64 samples above 73 / 75, 17 tokens behind 4,099
+// keys 19 / 21.
 struct Plan {
   bool tall;
   int n_tiles, n_split;
 };
 
-Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts, bool stay_flat = false) {
+Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts, int min_part,
+                bool stay_flat = false) {
   const int64_t tall = pairs * ((max_rows + 127) / 128), flat = pairs * ((max_rows + 31) / 32);
   Plan r;
   r.tall = max_rows > 32 && !stay_flat &&
-           (tall >= kTallFill || (max_parts > 1 && flat < kFlatFill));
+           (tall >= kTallFill || (max_parts > 1 && (flat < kFlatFew || slots > kLongList)));
   r.n_tiles = static_cast<int>(r.tall ? (max_rows + 127) / 128 : (max_rows + 31) / 32);
   const int64_t blocks = r.tall ? tall : flat;
   int64_t fill = r.tall ? kTallFill : kFlatFill;
   if (r.tall && (2 * fill + blocks - 1) / blocks * kLongPart <= slots) fill *= 2;
-  const int64_t want = (fill + blocks - 1) / blocks;
-  const int64_t most = (slots + 63) / 64;   // a turn of a block
+  const int64_t want = (fill + blocks - 1) / blocks, most = slots / min_part;
   const int64_t ns = want < most ? want : most;
   r.n_split = static_cast<int>(ns < 1 ? 1 : ns > max_parts ? max_parts : ns);
   return r;
@@ -918,6 +922,10 @@ int check_sizes(int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, i
   return MDL_OK;
 }
 
+// Keys of a part at least, where the merge is a launch more than without parts: 16 sequences of up to
+// 61 tokens behind 13 keys (3 heads of 128) 13.3 us in parts of 64, 8.7 uncut.
+int least_part(int dtype) { return dtype == MDL_DTYPE_F32 ? 128 : 256; }
+
 int64_t state_bytes(int parts, int64_t rows, int head_dim) {
   return parts * rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
@@ -937,7 +945,7 @@ extern "C" int64_t mdl_attn_grouped_workspace_bytes(int n_seq, int tokens, int m
     return 0;
   const Plan pl = plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
                              static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), cache_slots,
-                             kMaxParts);
+                             kMaxParts, least_part(dtype));
   return pl.n_split > 1 ? state_bytes(pl.n_split, static_cast<int64_t>(tokens) * n_heads, head_dim)
                         : 0;
 }
@@ -959,7 +967,7 @@ extern "C" int mdl_attn_grouped(const void* q, const void* k_cache, const void* 
   if (n_seq == 0 || tokens == 0 || max_q == 0) return MDL_OK;
   const Plan pl = plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
                              static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), cache_slots,
-                             workspace ? kMaxParts : 1);
+                             workspace ? kMaxParts : 1, least_part(dtype));
   const int64_t rows = static_cast<int64_t>(tokens) * n_heads;
   if (pl.n_split > 1 && workspace_bytes < state_bytes(pl.n_split, rows, head_dim))
     return MDL_ERR_WORKSPACE;
@@ -1000,10 +1008,13 @@ SharedPlan plan_shared(int batch, int n_prefix, int max_rows, int n_heads, int n
       static_cast<double>((max_rows * g + 31) / 32) * n_prefix * prefix_slots;
   const bool own_first = prefix_reads * (head_dim == 128 ? 4 : 1) <=
                          static_cast<double>(batch) * cache_slots;
+  // as much as flat blocks that fill the GPU read in some microseconds: a launch less counts for more
+  // (13 fp32 rows of three prompts of up to 221 tokens, 128 heads on 8: 32 / 19)
+  const bool little = prefix_reads * n_kv_heads * head_dim <= kFlatFill * 512 * 64;
   SharedPlan r;
   r.prefix = plan_tiles(static_cast<int64_t>(n_prefix) * n_kv_heads, max_rows * g, prefix_slots,
-                        kMaxParts - kMaxOwn, own_first);
-  r.own = plan_tiles(static_cast<int64_t>(batch) * n_kv_heads, g, cache_slots, kMaxOwn);
+                        kMaxParts - kMaxOwn, 64, own_first || little);
+  r.own = plan_tiles(static_cast<int64_t>(batch) * n_kv_heads, g, cache_slots, kMaxOwn, 64);
   return r;
 }
 
