@@ -748,19 +748,25 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
     }
   };
   load(0);
-  // sequences that start at or before the token, 64 at a time; a token of none is in no part
-  int first = 0, end = 0, before = 0;
-  for (int s0 = 0; s0 < p.n_seq; s0 += kWave) {
-    const int s = s0 + lane;
-    const int at = s < p.n_seq ? p.q_offset[s] : INT_MAX;
-    const int after = s < p.n_seq ? p.q_offset[s + 1] : INT_MAX;
-    const int k = __popcll(__ballot(at <= t));
-    if (k > 0) {
+  // the last sequence that starts at or before the token, by 64 probes at a time; `before` counts those
+  // that do (a token of none is in no part)
+  int first = 0, end = 0, before = 0, s0 = 0, span = p.n_seq;
+  while (span > 0) {
+    const int step = (span + kWave - 1) / kWave;
+    const int s = s0 + lane * step;
+    const bool in = lane * step < span;
+    const int at = in ? p.q_offset[s] : INT_MAX;
+    const int after = in && step == 1 ? p.q_offset[s + 1] : INT_MAX;
+    const int k = __popcll(__ballot(in && at <= t));
+    if (k == 0) break;
+    if (step == 1) {
       first = __builtin_amdgcn_readlane(at, k - 1);
       end = __builtin_amdgcn_readlane(after, k - 1);
+      before = s0 + k;
+      break;
     }
-    before += k;
-    if (k < kWave) break;
+    s0 += (k - 1) * step;
+    span = min(step, p.n_seq - s0);
   }
   const bool held = before > 0 && t < end && t - max(first, 0) < p.max_q;
   const int part0 = held ? 0 : p.n0;

@@ -159,6 +159,23 @@ def test_grouped_tall_blocks(dtype, D):
     c.check("tall, whole", causal=False)
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+def test_grouped_tall_blocks_in_parts(dtype, D):
+    """A few hundred rows behind thousands of keys."""
+    c = Grouped(13, dtype, D, 8, 2, [40, 17, 0, 3], [3000, 2950, 2000, 1], tail=1)
+    assert K().attn_grouped_workspace_bytes(c.q.to(DEV), c.k.to(DEV), 40) > 0
+    c.check("parts")
+    c.check("no workspace", workspace=False)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+def test_grouped_many_heads_to_one(dtype, D):
+    """More query heads to a key / value head than rows in a tile, and a number that divides none."""
+    c = Grouped(14, dtype, D, 161, 1, [3, 2], [40, 0], tail=1)
+    c.check("161 heads")
+    c.check("161 heads, no workspace", workspace=False)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_grouped_parts_and_no_workspace(dtype):
     """Few rows and many keys: cut into parts with a workspace, whole without, equal calls equal."""
@@ -190,7 +207,8 @@ def test_grouped_large_scores(dtype):
 
 @pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-def test_grouped_values_that_are_not_finite(dtype, D, bad):
+@pytest.mark.parametrize("workspace", [True, False])
+def test_grouped_values_that_are_not_finite(dtype, D, bad, workspace):
     """Values behind the keys, and in slots that only later queries see, reach nobody else."""
     c = Grouped(7, dtype, D, 6, 2, [70, 45], [0, 20])
     ref, bound = c.reference()
@@ -200,7 +218,7 @@ def test_grouped_values_that_are_not_finite(dtype, D, bad):
             t[b, :, n:] = bad
     c.v[:, 0, at, 3] = bad                      # one channel of a value
     c.k[:, 1, at] = float("nan")                # a whole key
-    out = c.run().double().cpu()
+    out = c.run(workspace=workspace).double().cpu()
     lo0, lo1 = 50, 70 + 30                      # the first rows that see the slot
     hit = torch.zeros(c.offset[-1], dtype=torch.bool)
     hit[lo0:70] = True
@@ -391,6 +409,26 @@ def test_shared_long_prefix_in_parts():
     ref, bound = c.reference()
     _check(c.run(), ref, bound, "parts")
     assert torch.equal(c.run(), c.run())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_shared_tall_prefix(dtype):
+    """Enough rows and keys for the prefixes' launch of 128-row blocks, in parts."""
+    c = Shared(8, dtype, 128, 16, 4, [0, 31, 37], [9001, 130], [(7 * i) % 40 for i in range(40)])
+    ref, bound = c.reference()
+    _check(c.run(), ref, bound, "tall")
+
+
+@pytest.mark.parametrize("n", [64, 65, 300])
+def test_shared_many_prefixes(n):
+    """A prefix for every other row, the rows between in none of them or in their neighbour's."""
+    g = _gen(n)
+    sizes = torch.randint(0, 3, (n,), generator=g).tolist()
+    edges = [1 + sum(sizes[:i]) for i in range(n + 1)]
+    c = Shared(9, BF, 64, 2, 1, edges, [1 + 5 * i % 40 for i in range(n)],
+               [i % 9 for i in range(edges[-1] + 2)])
+    ref, bound = c.reference()
+    _check(c.run(), ref, bound, "prefixes")
 
 
 def test_shared_rows_past_max_rows_have_no_prefix():
