@@ -27,8 +27,17 @@
 // Staging: key tiles of KT keys go through a ring of two LDS stages filled by direct global -> LDS
 // copies, the next tile's under this one's work.  16-byte chunks are XOR-swizzled by row (swz).
 // WR waves share a ring and split the rows; WK groups of WR waves take the tiles in turn, each with
-// a ring of its own, and merge at the end.  A launch may also cut each tile's keys in n_split parts
-// whose states (fp32 m, l, o) go to the workspace; merge_kernel joins them.
+// a ring of its own, and merge at the end: tall blocks are WR = 4, WK = 1, flat ones WR = 1, WK = 2
+// (plan_tiles chooses).  A launch may also cut each tile's keys in n_split parts whose states (fp32
+// m, l, o) go to the workspace; attn_merge_kernel joins them.
+//
+// What bounds it.  128 dims, bf16: the MFMAs at the power limit (two prompts of up to 8,192 tokens,
+// 32 heads on 8: 880 us, 1,105 TFLOP/s, 81% of a large library product on this card).  64 dims: an
+// exponential costs as much as its products, and VALU and MFMA instructions of three waves a SIMD
+// fill each other's gaps only in part (4 prompts of up to 6,000, 16 heads on 4: 251 us, 904
+// TFLOP/s).  fp32: the MFMAs, 75% of the rate of a large product (2 prompts of 4,000, 12 heads of
+// 64: 428 us).  Few rows: HBM (64 rows of up to 4,000 keys, 32 heads on 8 of 128: 143 us, 6.2 TB/s)
+// or, below some 20 MB, the launches and one block's chain of loads.
 #include <climits>
 #include <type_traits>
 
@@ -143,7 +152,8 @@ struct GroupedShape {
   static constexpr int kTile = KT * kRowBytes;            // bytes of a K or V tile
   // Two stages of K and V per group.  One for the flat fp32 blocks of 128 dims, where either product
   // of a tile (4,096 cycles) outlasts a copy: twice the waves on a CU, 16 rows of 2,000 keys (16
-  // heads) 45 -> 33 us.  With 64 dims the copies are waited for: 2 prompts of up to 731 tokens 37 -> 42.
+  // heads) 45 -> 33 us.  With 64 dims the copies are waited for: 2 prompts of up to 731 tokens 37
+  // -> 42.
   static constexpr int kStages = WR == 1 && kRowBytes == 512 ? 1 : 2;
   static constexpr int kLds = WK * 2 * kStages * kTile;
   static constexpr int kRows = 32 * WR;                   // rows of a block
@@ -748,8 +758,8 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
     }
   };
   load(0);
-  // the last sequence that starts at or before the token, by 64 probes at a time; `before` counts those
-  // that do (a token of none is in no part)
+  // the last sequence that starts at or before the token, by 64 probes at a time; `before` counts
+  // those that do (a token of none is in no part)
   int first = 0, end = 0, before = 0, s0 = 0, span = p.n_seq;
   while (span > 0) {
     const int step = (span + kWave - 1) / kWave;
