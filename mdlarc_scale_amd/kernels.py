@@ -1154,6 +1154,12 @@ def _grouped_shapes(q: torch.Tensor, k: torch.Tensor) -> tuple[tuple, tuple]:
     return shape, cache
 
 
+def _at_most(bound: int, rows: int) -> int:
+    """``bound`` on a number of the ``rows`` for an entry's C int, which would drop the high bits of a
+    large one; every negative one is -1, which the entries refuse."""
+    return max(-1, min(bound, rows))
+
+
 def _out_spec(out: torch.Tensor, q: torch.Tensor, rows: int, width: int, split: bool,
               tiled: bool) -> tuple:
     if split:
@@ -1218,8 +1224,8 @@ def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.
 def attn_grouped_workspace_bytes(q: torch.Tensor, k_cache: torch.Tensor, max_q: int) -> int:
     """Bytes of ``attn_grouped``'s workspace for tensors of these shapes (0: none is used)."""
     (tokens, heads, d), (n_seq, kv, slots, _) = _grouped_shapes(q, k_cache)
-    return _lib.lib().mdl_attn_grouped_workspace_bytes(n_seq, tokens, max_q, heads, kv, d,
-                                                       cache_dtype_code(q), slots)
+    return _lib.lib().mdl_attn_grouped_workspace_bytes(n_seq, tokens, _at_most(max_q, tokens),
+                                                       heads, kv, d, cache_dtype_code(q), slots)
 
 
 def attn_grouped(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -1251,8 +1257,8 @@ def attn_grouped(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     if tokens == 0 or n_seq == 0:
         return
     _launch(dev, "mdl_attn_grouped", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), code,
-            n_seq, tokens, max_q, heads, kv, d, slots, q_offset.data_ptr(), kv_len.data_ptr(),
-            int(causal), out.data_ptr(), split + tiled, ws, ws_bytes)
+            n_seq, tokens, _at_most(max_q, tokens), heads, kv, d, slots, q_offset.data_ptr(),
+            kv_len.data_ptr(), int(causal), out.data_ptr(), split + tiled, ws, ws_bytes)
 
 
 def attn_decode_shared_workspace_bytes(q: torch.Tensor, prefix_k: torch.Tensor,
@@ -1260,8 +1266,8 @@ def attn_decode_shared_workspace_bytes(q: torch.Tensor, prefix_k: torch.Tensor,
     """Bytes of ``attn_decode_shared``'s workspace for tensors of these shapes."""
     (batch, heads, d), (_, kv, slots, _) = _grouped_shapes(q, k_cache)
     return _lib.lib().mdl_attn_decode_shared_workspace_bytes(
-        batch, prefix_k.shape[0], max_rows, heads, kv, d, cache_dtype_code(q), prefix_k.shape[2],
-        slots)
+        batch, prefix_k.shape[0], _at_most(max_rows, batch), heads, kv, d, cache_dtype_code(q),
+        prefix_k.shape[2], slots)
 
 
 def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
@@ -1299,9 +1305,10 @@ def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     if batch == 0:
         return
     _launch(dev, "mdl_attn_decode_shared", q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(),
-            row_offset.data_ptr(), prefix_len.data_ptr(), n_prefix, prefix[2], max_rows,
-            k_cache.data_ptr(), v_cache.data_ptr(), kv_len.data_ptr(), batch, cache[2], code, heads,
-            kv, d, out.data_ptr(), split + tiled, workspace.data_ptr(), workspace.numel() * 4)
+            row_offset.data_ptr(), prefix_len.data_ptr(), n_prefix, prefix[2],
+            _at_most(max_rows, batch), k_cache.data_ptr(), v_cache.data_ptr(), kv_len.data_ptr(),
+            batch, cache[2], code, heads, kv, d, out.data_ptr(), split + tiled,
+            workspace.data_ptr(), workspace.numel() * 4)
 
 
 

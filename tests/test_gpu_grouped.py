@@ -242,6 +242,17 @@ def test_grouped_too_many_queries_stay():
         assert bool((out[9:40] == 7.0).all())
 
 
+@pytest.mark.parametrize("max_q", [2 ** 31, 2 ** 32, 2 ** 32 + 1])
+def test_grouped_bound_above_the_rows(max_q):
+    Grouped(61, BF, 64, 4, 2, [3, 40, 1], [900, 0, 1500], tail=2).check("bound", max_q=max_q)
+
+
+@pytest.mark.parametrize("max_q", [-1, -2 ** 32, -2 ** 32 + 5])
+def test_grouped_bound_below_zero_is_refused(max_q):
+    with pytest.raises((RuntimeError, ValueError)):
+        Grouped(62, BF, 64, 4, 2, [3], [9]).run(max_q=max_q)
+
+
 def test_grouped_lengths_out_of_range_are_clamped():
     c = Grouped(9, F32, 64, 4, 2, [5, 6], [10, 0])
     slots = c.k.shape[2]
@@ -435,6 +446,13 @@ def test_shared_rows_past_max_rows_have_no_prefix():
     c = Shared(3, F32, 64, 4, 2, [0, 6], [200], [5, 6, 7, 8, 9, 10])
     ref, bound = c.reference(max_rows=4)
     _check(c.run(max_rows=4), ref, bound, "max_rows")
+
+
+@pytest.mark.parametrize("max_rows", [2 ** 31, 2 ** 32, 2 ** 32 + 1])
+def test_shared_bound_above_the_rows(max_rows):
+    c = Shared(63, BF, 64, 4, 2, [0, 3, 5], [70, 33], [9, 40, 5, 64, 7])
+    ref, bound = c.reference()
+    _check(c.run(max_rows=max_rows), ref, bound, "bound")
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])

@@ -97,3 +97,22 @@ def test_wrappers_refuse_host_tensors_and_shapes():
     with pytest.raises(ValueError, match="GPU tensor"):
         K.qk_norm_rope_cache(torch.zeros(3, 640), None, off, q, (8, 8, 8, 10, 10, 12), q, q, 1e-5,
                              off, off, 1.0, q, c, c)
+
+
+@pytest.mark.parametrize("most", [2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 40])
+def test_bounds_above_the_rows_count_as_the_rows(L, most):
+    """max_q and max_rows are bounds: one that a C int does not hold is still one, no small number
+    or zero (for which the entries have nothing to do)."""
+    q, cache = torch.zeros(9, 6, 64), torch.zeros(2, 2, 4096, 64)
+    assert K.attn_grouped_workspace_bytes(q, cache, most) == \
+        K.attn_grouped_workspace_bytes(q, cache, 9) > 0
+    own = torch.zeros(9, 2, 16, 64)
+    assert K.attn_decode_shared_workspace_bytes(q, cache, own, most) == \
+        K.attn_decode_shared_workspace_bytes(q, cache, own, 9) > 0
+
+
+@pytest.mark.parametrize("most", [-1, -2 ** 31, -2 ** 32, -2 ** 32 + 5])
+def test_bounds_below_zero_need_no_workspace(L, most):
+    q, cache = torch.zeros(9, 6, 64), torch.zeros(2, 2, 4096, 64)
+    assert K.attn_grouped_workspace_bytes(q, cache, most) == 0
+    assert K.attn_decode_shared_workspace_bytes(q, cache, torch.zeros(9, 2, 16, 64), most) == 0
