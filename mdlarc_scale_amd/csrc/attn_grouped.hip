@@ -259,16 +259,17 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   // Copy j of a tile: rows (1024 / row bytes) j .. of K and of V, one kilobyte each; a lane takes
   // physical chunk lane % chunks of its row.  Rows past the last key copy that key.
   constexpr int kChunks = S::kRowBytes / 16;
-  // (fp32 reads V by whole rows, which need no swizzle: their addresses are one lane offset then.)
-  auto issue = [&](const T* src, int kt, uint32_t at) {
-    const bool plain = kF32 && src == Vg;
+  // fp32 reads V by whole rows, which need no swizzle: their addresses are one lane offset then.
+  constexpr std::false_type kSwizzled{};
+  constexpr std::bool_constant<kF32> kPlainV{};
+  auto issue = [&](const T* src, int kt, uint32_t at, auto plain) {
     const T* from = scalar_ptr(src + static_cast<int64_t>(kt) * D);
 #pragma unroll
     for (int jj = 0; jj < S::kCopies; ++jj) {
       const int j = wr + WR * jj;
       const int r = S::kRowsPerCopy * j + lane / kChunks;
       const uint32_t off = min(r, kend - 1 - kt) * S::kRowBytes +
-                           16 * ((lane % kChunks) ^ (plain ? 0 : swz<T, D>(r & 15)));
+                           16 * ((lane % kChunks) ^ (decltype(plain)::value ? 0 : swz<T, D>(r & 15)));
       const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + at + 1024 * j);
       if constexpr (WR == 1)
         dma16_stream(from, off, dst);
@@ -503,8 +504,8 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
   constexpr std::integral_constant<int, 1> kOdd{};
   if constexpr (WR > 1) {
     if (first < k1) {
-      issue(Kg, first, k_slot(0));
-      issue(Vg, first, v_slot(0));
+      issue(Kg, first, k_slot(0), kSwizzled);
+      issue(Vg, first, v_slot(0), kPlainV);
     }
     // q of the wave's 32 rows through the second stage (the first turn's barrier frees it), whole
     // rows to a copy: read into registers directly, an instruction takes 16 bytes of 64 places.
@@ -535,8 +536,8 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       __builtin_amdgcn_s_waitcnt(kWaitAll);
       asm volatile("s_barrier" ::: "memory");
       if (kt + kTurn < k1) {
-        issue(Kg, kt + kTurn, k_slot(ST ^ 1));
-        issue(Vg, kt + kTurn, v_slot(ST ^ 1));
+        issue(Kg, kt + kTurn, k_slot(ST ^ 1), kSwizzled);
+        issue(Vg, kt + kTurn, v_slot(ST ^ 1), kPlainV);
       }
       // past the part, or no row of the wave sees a key
       if (!decltype(fullc)::value && (kt >= k1 || kt > lim_hi)) return;
@@ -558,8 +559,8 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     constexpr int C = S::kCopies, NS = S::kStages;
     const int nt = first < k1 ? (k1 - first + kTurn - 1) / kTurn : 0;
     for (int i = 0; i < NS && i < nt; ++i) {
-      issue(Kg, first + i * kTurn, k_slot(i));
-      issue(Vg, first + i * kTurn, v_slot(i));
+      issue(Kg, first + i * kTurn, k_slot(i), kSwizzled);
+      issue(Vg, first + i * kTurn, v_slot(i), kPlainV);
     }
     // a wait that the compiler sees, for q: it would wait for q inside the loop otherwise, and with
     // it for every copy
@@ -574,7 +575,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       compute(ring + k_slot(ST), ring + v_slot(ST), kt, fullc, [&] {
         if (i + NS < nt) {
           wait_reads();   // of K's slot
-          issue(Kg, kt + NS * kTurn, k_slot(ST));
+          issue(Kg, kt + NS * kTurn, k_slot(ST), kSwizzled);
           wait_copies<(2 * NS - 1) * C>();
         } else if (NS > 1 && i + 1 < nt) {
           wait_copies<2 * C>();
@@ -584,7 +585,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       });
       if (i + NS < nt) {
         wait_reads();     // of V's slot
-        issue(Vg, kt + NS * kTurn, v_slot(ST));
+        issue(Vg, kt + NS * kTurn, v_slot(ST), kPlainV);
       }
     };
     int i = 0;

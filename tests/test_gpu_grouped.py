@@ -343,6 +343,24 @@ def test_grouped_graph_and_streams():
         torch.randn(1000, device=DEV).sum().item()
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("batch", ["flat", "tall"])
+def test_grouped_one_buffer_for_keys_and_values(dtype, D, batch):
+    """Keys that are the values too (one cache given for both), in either block form."""
+    if batch == "flat":
+        c = Grouped(71, dtype, D, 6, 2, [33, 1, 9], [40, 300, 0], tail=1)
+    else:
+        c = Grouped(72, dtype, D, 16, 16, [150, 300, 77, 5, 290, 33, 128, 257], [0] * 8)
+    c.v = c.k
+    ref, bound = c.reference()
+    kern = K()
+    q, cache, out = c.q.to(DEV), c.k.to(DEV), torch.full_like(c.q, 7.0, device=DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    kern.attn_grouped(q, cache, cache, i32(c.offset), i32(c.keys), max(c.n), out)
+    end = c.offset[-1]
+    _check(out[:end], ref[:end], bound[:end], batch)
+
+
 # ---- K8: shared prefixes -----------------------------------------------------------------------
 
 class Shared:
@@ -514,6 +532,17 @@ def test_shared_graph():
         torch.cuda.synchronize()
         assert torch.equal(a[9], b[9]), step
         torch.randn(1000, device=DEV).sum().item()
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+def test_shared_one_buffer_for_keys_and_values(dtype, D):
+    c = Shared(73, dtype, D, 6, 2, [0, 3, 5], [170, 33], [9, 40, 5, 64, 7])
+    c.pv, c.v = c.pk, c.k
+    ref, bound = c.reference()
+    a = c.args()
+    a[2], a[7] = a[1], a[6]
+    K().attn_decode_shared(*a)
+    _check(a[9], ref, bound, "one buffer")
 
 
 # ---- K7 ----------------------------------------------------------------------------------------
