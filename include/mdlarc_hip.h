@@ -692,7 +692,8 @@ int mdl_qk_norm_rope_cache(const void* qkv, int in_dtype, int64_t ld, const floa
  * j <= kv_len[s] - n + i:
  *   out = sum_j 2^(q . k_j) v_j / sum_j 2^(q . k_j),   0 where a query sees no slot.
  * A value that is not finite in a slot that a query does not see does not reach it.  Softmax
- * statistics and sums are fp32; bf16: the weights are rounded to bf16 for the product with V.
+ * statistics and sums are fp32; bf16: the weights are rounded to bf16 for the product with V, and
+ * those below 2^-126 of a row's reference are zero (fp32 keeps them, as mdl_attn_prefill_f32 does).
  * max_q: at least the most queries of a sequence; queries past it, and rows of q behind the last
  * sequence, are not computed and their rows of out stay as they were.  Lengths and offsets outside
  * their ranges are clamped.

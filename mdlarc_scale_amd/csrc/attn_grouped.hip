@@ -113,6 +113,13 @@ __device__ __forceinline__ float max_halves(float v) {
   return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
+// 2^x.  EXACT (fp32 data) keeps results below 2^-126; the bare instruction, which gives the same bits
+// above, makes them zero, and bf16 data has it everywhere, as in K4a and K4b.
+template <bool EXACT>
+__device__ __forceinline__ float weight_exp2(float x) {
+  return EXACT ? exp2f(x) : __builtin_amdgcn_exp2f(x);
+}
+
 __device__ __forceinline__ f32x16_t splat16(float v) {
   return f32x16_t{v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v};
 }
@@ -393,6 +400,26 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     for (int db = 0; db < DB; ++db) v[db] = 0.f;
   };
 
+  // fp32: the products of a tile's weights below 2^-126, which the bare exponential makes zero.  Rare,
+  // so a loop of its own beside the products of all weights (the scores go round once), behind the
+  // branch that moves the reference.  16 prompts of up to 811 tokens (12 heads of 64) / 2 of 4,000: 161
+  // / 430 us without and with it; exp2f for every weight 168 / 454, a choice of the exponentials in
+  // front of the products 170 / 437.  A value that is not finite is left to those products.
+  auto faint_weights = [&](f32x16_t& s, const uint8_t* Vt) {
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r) {
+      const float pr = s[0] < -126.f ? weight_exp2<true>(s[0]) : 0.f;
+      s = __builtin_shufflevector(s, s, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 0);
+      l += pr;
+      float v[DB];
+      v_row(Vt, (r & 3) + 8 * (r >> 2) + 4 * h, v);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(fabsf(v[db]) < INFINITY ? v[db] : 0.f, pr, o[db],
+                                                     0, 0, 0);
+    }
+  };
+
   auto compute = [&](const uint8_t* Kt, const uint8_t* Vt, int kt, auto fullc, auto after_qk) {
     // some row does not see the whole tile
     const bool masked = !decltype(fullc)::value && kt + KT - 1 > lim_lo;
@@ -418,6 +445,12 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
       }
     }
     after_qk();
+    // fp32: the lowest score, before the mask (whose -inf would always count as low)
+    float least = 0.f;
+    if constexpr (kF32) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) least = fminf(least, sc[0][r]);
+    }
     if (masked) {
       int x = lim - kt - 4 * h;   // the last visible key, from this lane half's first
       // a value made here keeps this a branch: as selects it would cost every tile 60 instructions
@@ -433,19 +466,23 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) lmax = fmaxf(lmax, sc[nb][r]);
-    if (__ballot(lmax > thr) != 0) {
+    if (__ballot(lmax > thr || (kF32 && least < -126.f)) != 0) {
       const float tmax = max_halves(lmax);
       if (tmax > thr) {   // the same in both lanes of a row
         const bool fresh = thr == -INFINITY;
-        const float alpha = fresh ? 0.f : __builtin_amdgcn_exp2f(-tmax);
+        const float alpha = fresh ? 0.f : weight_exp2<kF32>(-tmax);
         negm = fresh ? -tmax : negm - tmax;
         if constexpr (kKeepStart) start = splat16(negm);
         thr = kGap;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) sc[nb] -= tmax;
+        least -= tmax;
         l *= alpha;
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      }
+      if constexpr (kF32) {
+        if (__ballot(least < -126.f) != 0) faint_weights(sc[0], Vt);
       }
     }
 #pragma unroll
@@ -619,7 +656,7 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
     for (int j = 0; j < WK - 1; ++j) {
       const float* w = st + (j * WR + wr) * (2 + 16 * DB) * kWave + lane;
       const float mj = w[0], top = fmaxf(m, mj), base = top == -INFINITY ? 0.f : top;
-      const float a = __builtin_amdgcn_exp2f(m - base), aj = __builtin_amdgcn_exp2f(mj - base);
+      const float a = weight_exp2<kF32>(m - base), aj = weight_exp2<kF32>(mj - base);
       m = top;
       l = l * a + w[kWave] * aj;
 #pragma unroll
@@ -784,7 +821,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const MergeArgs p) {
   if (part0 >= n) return;   // the token is in no sequence: its row stays as it was
   const bool live = lane >= part0 && lane < n && ml.x != -INFINITY;
   const float top = wave_max(live ? ml.x : -INFINITY);
-  const float w = live ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
+  const float w = live ? weight_exp2<sizeof(T) == 4>(ml.x - top) : 0.f;
   const uint64_t mask = __ballot(live);
   const float L = wave_sum(live ? ml.y * w : 0.f);
   float O[C];

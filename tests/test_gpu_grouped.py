@@ -361,6 +361,52 @@ def test_grouped_one_buffer_for_keys_and_values(dtype, D, batch):
     _check(out[:end], ref[:end], bound[:end], batch)
 
 
+FAINT = {"flat": (2, 3, 90), "tall": (90, 300, 300), "parts": (1, 1, 2300),
+         "tall parts": (1, 140, 2300)}
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("form", FAINT)
+@pytest.mark.parametrize("heavy", ["first", "last"])
+def test_grouped_keeps_fp32_weights_below_the_normal_range(form, D, heavy):
+    """A weight of 2^-130 is a denormal fp32 number, and counts: times a value of 2^100 it is 2^-30.
+    The key of weight 1 comes before the others (their weights are formed so) or behind them (their
+    sum is rescaled, or joined, by 2^-130)."""
+    seqs, n, slots = FAINT[form]
+    q = torch.zeros(seqs * n, 1, D, device=DEV)
+    q[..., 0] = 1.0                                   # the score is the key's first channel
+    kc, vc = torch.zeros(2, seqs, 1, slots, D, device=DEV).unbind()
+    kc[..., 0], vc[..., 5] = -130.0, 2.0 ** 100
+    one = 0 if heavy == "first" else slots - 1
+    kc[:, :, one, 0], vc[:, :, one, 5] = 0.0, 0.0
+    out = torch.full_like(q, 7.0)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    ws = torch.empty(K().attn_grouped_workspace_bytes(q, kc, n) // 4, device=DEV)
+    assert (ws.numel() > 0) == ("parts" in form)
+    K().attn_grouped(q, kc, vc, i32([n * s for s in range(seqs + 1)]), i32([slots] * seqs), n, out,
+                     causal=False, workspace=ws)
+    # whole numbers of 2^-30, and a sum of weights that rounds to 1
+    assert bool((out[..., 5] == (slots - 1) * 2.0 ** -30).all())
+    assert bool((out[..., :5] == 0).all()) and bool((out[..., 6:] == 0).all())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_grouped_faint_fp32_weights_beside_values_that_are_not_finite(bad):
+    """A value that only later queries see does not reach the sums of weights of 2^-130."""
+    q = torch.zeros(70, 1, 64, device=DEV)
+    q[..., 0] = 1.0
+    kc, vc = torch.zeros(2, 1, 1, 90, 64, device=DEV).unbind()
+    kc[..., 0], vc[..., 5] = -130.0, 2.0 ** 100
+    kc[:, :, 0, 0], vc[:, :, 0, 5] = 0.0, 0.0
+    vc[:, :, 41, 5] = vc[:, :, 70:] = kc[:, :, 70:] = bad
+    out = torch.full_like(q, 7.0)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    K().attn_grouped(q, kc, vc, i32([0, 70]), i32([70]), 70, out)
+    assert bool((out[:41, 0, 5] == torch.arange(41, device=DEV) * 2.0 ** -30).all())
+    assert not bool(out[41:, 0, 5].isfinite().any())
+    assert bool((out[..., :5] == 0).all()) and bool((out[..., 6:] == 0).all())
+
+
 # ---- K8: shared prefixes -----------------------------------------------------------------------
 
 class Shared:
@@ -543,6 +589,25 @@ def test_shared_one_buffer_for_keys_and_values(dtype, D):
     a[2], a[7] = a[1], a[6]
     K().attn_decode_shared(*a)
     _check(a[9], ref, bound, "one buffer")
+
+
+@pytest.mark.parametrize("heavy", ["first", "last"])
+def test_shared_keeps_fp32_weights_below_the_normal_range(heavy):
+    """The same over a prefix and the row's own keys: the key of weight 1 is one or the other's."""
+    q = torch.zeros(3, 1, 64, device=DEV)
+    q[..., 0] = 1.0
+    pk, pv = torch.zeros(2, 1, 1, 500, 64, device=DEV).unbind()
+    kc, vc = torch.zeros(2, 3, 1, 70, 64, device=DEV).unbind()
+    for k, v in ((pk, pv), (kc, vc)):
+        k[..., 0], v[..., 5] = -130.0, 2.0 ** 100
+    k, v = (pk, pv) if heavy == "first" else (kc, vc)
+    k[:, :, 3, 0], v[:, :, 3, 5] = 0.0, 0.0
+    out = torch.full_like(q, 7.0)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    ws = torch.empty(K().attn_decode_shared_workspace_bytes(q, pk, kc, 3) // 4, device=DEV)
+    K().attn_decode_shared(q, pk, pv, i32([0, 3]), i32([500]), 3, kc, vc, i32([70, 9, 40]), out, ws)
+    want = torch.tensor([569.0, 508.0, 539.0], device=DEV) * 2.0 ** -30
+    assert bool((out[:, 0, 5] == want).all())
 
 
 # ---- K7 ----------------------------------------------------------------------------------------
