@@ -1189,6 +1189,8 @@ def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.
     if len(shape) != 2:
         raise ValueError("qkv must be [rows, (n_heads + 2 * n_kv_heads) * head_dim]")
     rows, width = shape
+    if rows and not batch:
+        raise ValueError("a cache with batch 0 has no row for the tokens of qkv")
     heads = width // d - 2 * kv
     if not kv or width % d or heads <= 0 or heads % kv:
         raise ValueError(f"qkv rows of {width} do not hold a multiple of {kv} query heads, {kv} key "
@@ -1212,7 +1214,7 @@ def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.
         (token_row, "token_row", I32, rows), (token_slot, "token_slot", I32, rows),
         (q_out, "q_out", out, rows * heads * d), (k_cache, "k_cache", out, 0),
         (v_cache, "v_cache", out, 0)))
-    if rows == 0 or batch == 0:
+    if rows == 0:
         return
     _launch(dev, "mdl_qk_norm_rope_cache", qkv.data_ptr(), in_dt, ld,
             None if rstd is None else rstd.data_ptr(), pos.data_ptr(), rope_tab.data_ptr(), rows,

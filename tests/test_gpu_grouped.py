@@ -712,6 +712,27 @@ def test_qk_norm_streaming_rows_and_far_slots():
         _check(got, ref, err * (1 + half) + half * ref.abs() + 1e-30)
 
 
+def test_qk_norm_refuses_a_cache_without_rows():
+    """q_out is written for every token, in the cache or not, so a call that would leave it as it was
+    is an error; one without tokens has nothing to write."""
+    D, heads, kv = 64, 4, 2
+    tab, geom = _rope(D)
+    ones = torch.ones(D, device=DEV)
+    for rows in (3, 0):
+        qkv = torch.zeros(rows, (heads + 2 * kv) * D, device=DEV)
+        pos = torch.zeros(rows, 3, dtype=torch.int64, device=DEV)
+        at = torch.zeros(rows, dtype=torch.int32, device=DEV)
+        q = torch.full((rows, heads, D), 7.0, device=DEV)
+        cache = torch.zeros(0, kv, 8, D, device=DEV)
+        args = (qkv, None, pos, tab.to(DEV), geom, ones, ones, 1e-5, at, at, 1.0, q, cache,
+                torch.zeros_like(cache))
+        if rows:
+            with pytest.raises(ValueError, match="batch"):
+                K().qk_norm_rope_cache(*args)
+        else:
+            K().qk_norm_rope_cache(*args)
+
+
 # ---- together ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [BF, F32])

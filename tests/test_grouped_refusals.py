@@ -116,3 +116,13 @@ def test_bounds_below_zero_need_no_workspace(L, most):
     q, cache = torch.zeros(9, 6, 64), torch.zeros(2, 2, 4096, 64)
     assert K.attn_grouped_workspace_bytes(q, cache, most) == 0
     assert K.attn_decode_shared_workspace_bytes(q, cache, torch.zeros(9, 2, 16, 64), most) == 0
+
+
+def test_qk_norm_refuses_a_cache_without_rows():
+    """q_out is written for every token, whether its slot is in the cache or not, so the wrapper does
+    not pass over tokens that no cache row can hold."""
+    qkv, none = torch.zeros(3, 8 * 64), torch.zeros(0, 2, 8, 64)
+    off, gain = torch.zeros(3, dtype=torch.int32), torch.ones(64)
+    with pytest.raises(ValueError, match="batch 0"):
+        K.qk_norm_rope_cache(qkv, None, off, gain, (8, 8, 8, 10, 10, 12), gain, gain, 1e-5, off, off,
+                             1.0, torch.zeros(3, 4, 64), none, none)
