@@ -1102,12 +1102,13 @@ extern "C" int mdl_attn_decode_shared(const void* q, const void* prefix_k, const
   if (!q || !prefix_k || !prefix_v || !row_offset || !prefix_len || !k_cache || !v_cache ||
       !kv_len || !out || !workspace)
     return MDL_ERR_NULL;
-  int bad = check_sizes(n_prefix, batch, max_rows, n_heads, n_kv_heads, head_dim, dtype,
-                        prefix_slots);
+  // a group has at most the batch's rows
+  int bad = check_sizes(n_prefix, batch, max_rows < batch ? max_rows : batch, n_heads, n_kv_heads,
+                        head_dim, dtype, prefix_slots);
   if (bad == MDL_OK)
     bad = check_sizes(batch, batch, 1, n_heads, n_kv_heads, head_dim, dtype, cache_slots);
   if (bad != MDL_OK) return bad;
-  if (n_prefix == 0 || max_rows == 0 || out_form < MDL_OUT_PLAIN || out_form > MDL_OUT_SPLIT_TILES)
+  if (n_prefix == 0 || max_rows <= 0 || out_form < MDL_OUT_PLAIN || out_form > MDL_OUT_SPLIT_TILES)
     return MDL_ERR_SHAPE;
   if (!aligned16(q) || !aligned16(prefix_k) || !aligned16(prefix_v) || !aligned16(k_cache) ||
       !aligned16(v_cache) || !aligned16(out) || !aligned16(workspace) || !aligned4(row_offset) ||

@@ -126,3 +126,17 @@ def test_qk_norm_refuses_a_cache_without_rows():
     with pytest.raises(ValueError, match="batch 0"):
         K.qk_norm_rope_cache(qkv, None, off, gain, (8, 8, 8, 10, 10, 12), gain, gain, 1e-5, off, off,
                              1.0, torch.zeros(3, 4, 64), none, none)
+
+
+@pytest.mark.parametrize("most", [5, 2 ** 20, 2 ** 31 - 1])
+def test_shared_bound_above_the_rows_is_their_number(L, most):
+    """The entry takes every bound that its workspace function does (and stops at a workspace of 0
+    bytes here); the refusals of a batch below zero or a bound of none stay."""
+    need = L.mdl_attn_decode_shared_workspace_bytes
+    assert need(4, 1, most, 6, 2, 64, 1, 512, 64) == need(4, 1, 4, 6, 2, 64, 1, 512, 64) > 0
+    call = L.mdl_attn_decode_shared
+    assert call(*{**SH, "max_rows": most}.values()) == WORKSPACE
+    assert call(*{**SH, "max_rows": most, "batch": 0}.values()) == 0
+    assert call(*{**SH, "max_rows": most, "batch": -1}.values()) == SHAPE
+    assert call(*{**SH, "max_rows": 0, "batch": 0}.values()) == SHAPE
+    assert call(*{**SH, "max_rows": -1}.values()) == SHAPE
