@@ -877,7 +877,10 @@ constexpr int kLongList = 4096;   // keys that two waves alone take too long ove
 // and where flat ones would have to be cut too or have long lists; flat in between.  us, flat /
 // tall: 704 flat blocks of a 700-token prompt 23 / 30 (in two parts), 752 of a 1,500-token one (64
 // dims) 19 / 28; 540 of 467 tokens behind 11,204 keys 160 / 77; 72 of 17 tokens behind 4,099 keys
-// 21 / 19; 64 of 64 samples behind 32,749 keys (with their own keys and the merge) 117 / 73.
+// 21 / 19; 64 of 64 samples behind 32,749 keys (with their own keys and the merge) 117 / 73.  Where the
+// keys are too few to be cut, flat, as without a workspace: 116 flat blocks of a 300-token prompt in
+// 337 slots 6.9 / 7.9 (64 dims), 10.8 / 10.2 (128); 152 of two fp32 ones of 200 14.8 / 19.8; the own keys
+// of 8 samples, 40 heads to a kv head in 100 slots, in one launch with their prefix 8.4 / 13.4.
 // Tall blocks are cut to one for each CU, and to two where the parts stay long: 4 continuations of
 // 100 tokens behind 6,000 keys 64 / 53 us; the 64 samples above 73 / 75, 17 tokens behind 4,099
 // keys 19 / 21.
@@ -889,14 +892,16 @@ struct Plan {
 Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts, int min_part,
                 bool stay_flat = false) {
   const int64_t tall = pairs * ((max_rows + 127) / 128), flat = pairs * ((max_rows + 31) / 32);
+  const int64_t most = slots / min_part;
+  const bool can_cut = max_parts > 1 && most > 1;
   Plan r;
   r.tall = max_rows > 32 && !stay_flat &&
-           (tall >= kTallFill || (max_parts > 1 && (flat < kFlatFew || slots > kLongList)));
+           (tall >= kTallFill || (can_cut && (flat < kFlatFew || slots > kLongList)));
   r.n_tiles = static_cast<int>(r.tall ? (max_rows + 127) / 128 : (max_rows + 31) / 32);
   const int64_t blocks = r.tall ? tall : flat;
   int64_t fill = r.tall ? kTallFill : kFlatFill;
   if (r.tall && (2 * fill + blocks - 1) / blocks * kLongPart <= slots) fill *= 2;
-  const int64_t want = (fill + blocks - 1) / blocks, most = slots / min_part;
+  const int64_t want = (fill + blocks - 1) / blocks;
   const int64_t ns = want < most ? want : most;
   r.n_split = static_cast<int>(ns < 1 ? 1 : ns > max_parts ? max_parts : ns);
   return r;

@@ -407,6 +407,27 @@ def test_grouped_faint_fp32_weights_beside_values_that_are_not_finite(bad):
     assert bool((out[..., :5] == 0).all()) and bool((out[..., 6:] == 0).all())
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("tokens,slots", [(300, 337), (200, 255), (130, 140)])
+def test_grouped_a_workspace_that_is_not_used_changes_nothing(dtype, D, tokens, slots):
+    """Where a call needs no workspace (keys too few to be cut), the one that a program keeps for its
+    other calls gives the bits of none."""
+    if dtype == F32:
+        tokens, slots = tokens // 2, slots // 2
+    c = Grouped(81, dtype, D, 12, 4, [tokens], [0], spare=slots - tokens)
+    q, k, v = c.q.to(DEV), c.k.to(DEV), c.v.to(DEV)
+    assert k.shape[2] == slots and K().attn_grouped_workspace_bytes(q, k, tokens) == 0
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    out = []
+    for ws in (None, torch.empty(1 << 20, device=DEV)):
+        out.append(torch.full_like(q, 7.0))
+        K().attn_grouped(q, k, v, i32([0, tokens]), i32([tokens]), tokens, out[-1], workspace=ws)
+    ref, bound = c.reference()
+    _check(out[0], ref, bound, "no workspace")
+    _check(out[1], ref, bound, "workspace")
+    assert torch.equal(out[0], out[1])
+
+
 # ---- K8: shared prefixes -----------------------------------------------------------------------
 
 class Shared:
