@@ -1154,6 +1154,9 @@ def _grouped_shapes(q: torch.Tensor, k: torch.Tensor) -> tuple[tuple, tuple]:
     return shape, cache
 
 
+C_INT_MAX = 2 ** 31 - 1
+
+
 def _at_most(bound: int, rows: int) -> int:
     """``bound`` on a number of the ``rows`` for an entry's C int, which would drop the high bits of a
     large one; every negative one is -1, which the entries refuse."""
@@ -1202,7 +1205,7 @@ def qk_norm_rope_cache(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.
         raise ValueError("the rows of qkv must be contiguous")
     if rows <= 1:
         ld = width
-    mx, my, mz, px, py, pz = rope_geom
+    mx, my, mz, px, py, pz = (_at_most(n, C_INT_MAX) for n in rope_geom)   # larger: refused
     out = k_cache.dtype
     in_dt, out_dt = cache_dtype_code(qkv), cache_dtype_code(k_cache)
     if rstd is not None:

@@ -140,3 +140,24 @@ def test_shared_bound_above_the_rows_is_their_number(L, most):
     assert call(*{**SH, "max_rows": most, "batch": -1}.values()) == SHAPE
     assert call(*{**SH, "max_rows": 0, "batch": 0}.values()) == SHAPE
     assert call(*{**SH, "max_rows": -1}.values()) == SHAPE
+
+
+@pytest.mark.parametrize("geom,sent", [
+    ((2 ** 32 + 32, 1, 1, 1, 31, 0), (2 ** 31 - 1, 1, 1, 1, 31, 0)),
+    ((1, -2 ** 32 + 32, 1, 0, 32, 0), (1, -1, 1, 0, 32, 0)),
+    ((32, 32, 8, -2 ** 32 + 10, 10, 12), (32, 32, 8, -1, 10, 12)),
+    ((32, 32, 8, 10, 2 ** 32 + 10, 12), (32, 32, 8, 10, 2 ** 31 - 1, 12))])
+def test_axes_that_a_c_int_does_not_hold_are_refused(L, monkeypatch, geom, sent):
+    """They reach the entry as numbers that it refuses, not as their low 32 bits, for which the table
+    was not checked."""
+    got = []
+    monkeypatch.setattr(K, "_need_all", lambda dev, specs: None)
+    monkeypatch.setattr(K, "_launch", lambda dev, name, *args: got.append(args))
+    n, gain = torch.zeros(3, dtype=torch.int32), torch.ones(64)
+    cache = torch.zeros(2, 2, 8, 64)
+    K.qk_norm_rope_cache(torch.zeros(3, 8 * 64), None, n, gain, geom, gain, gain, 1e-5, n, n, 1.0,
+                         torch.zeros(3, 4, 64), cache, cache)
+    at = list(QK).index("mx") - list(QK).index("in_dtype") + 1
+    assert got[0][at:at + 6] == sent
+    fake = {**QK, **dict(zip(("mx", "my", "mz", "px", "py", "pz"), sent))}
+    assert L.mdl_qk_norm_rope_cache(*fake.values()) == SHAPE
