@@ -428,6 +428,71 @@ def test_grouped_a_workspace_that_is_not_used_changes_nothing(dtype, D, tokens, 
     assert torch.equal(out[0], out[1])
 
 
+def _whole_reference(c):
+    """Grouped.reference, causal, by matrix products in float64 on the GPU (long sequences)."""
+    ref = torch.zeros(c.tokens, c.heads, c.D, dtype=torch.float64, device=DEV)
+    bound = torch.zeros_like(ref)
+    r = c.heads // c.kv
+    for b, (n, keys) in enumerate(zip(c.n, c.keys)):
+        a = c.offset[b]
+        unseen = torch.arange(keys, device=DEV)[None] > \
+            keys - n + torch.arange(n, device=DEV)[:, None]
+        for h in range(c.heads):
+            q = c.q[a:a + n, h].to(DEV).double()
+            k, v = (t[b, h // r, :keys].to(DEV).double() for t in (c.k, c.v))
+            kt = k.t().contiguous()
+            s = (q @ kt).masked_fill(unseen, float("-inf"))
+            w = torch.softmax(s * math.log(2.0), -1)
+            ds = (q.abs() @ kt.abs()).masked_fill(unseen, 0.0).amax(-1, keepdim=True)
+            ref[a:a + n, h] = w @ v
+            bound[a:a + n, h] = _bound(ref[a:a + n, h], w @ v.abs(), 2 * c.D * 2.0 ** -23 * ds, keys,
+                                       c.dtype)
+    return ref.cpu(), bound.cpu()
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("blocks,seqs,heads,kv,longest", [
+    (511, 7, 4, 1, 2331), (512, 4, 8, 1, 2047), (513, 9, 12, 3, 607), (546, 13, 12, 3, 447),
+    (1053, 13, 9, 3, 1150)])
+def test_grouped_order_of_many_tall_blocks(dtype, D, blocks, seqs, heads, kv, longest):
+    """Launches around two blocks for each of the 256 CUs and above, whose second 256 blocks run
+    backwards and whose pairs of sequence and head move over the XCDs from the sixth tile on: every
+    row is some block's, once."""
+    n = [longest - 37 * (b % 5) for b in range(seqs)]
+    c = Grouped(blocks, dtype, D, heads, kv, n, [0] * seqs, tail=2)
+    assert blocks == seqs * kv * -(-longest * heads // kv // 128)
+    ref, bound = _whole_reference(c)
+    out = c.run()
+    end = c.offset[-1]
+    _check(out[:end], ref[:end], bound[:end], blocks)
+    assert bool((out[end:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tiled", [False, True])
+@pytest.mark.parametrize("form", ["flat", "parts", "tall", "tall parts"])
+def test_grouped_split_output_of_each_block_form(dtype, D, tiled, form):
+    n, past, heads, kv = {"flat": ([3, 18], [0, 0], 4, 2), "parts": ([3, 1], [2200, 1900], 4, 2),
+                          "tall": ([150, 300, 77, 5, 290, 33, 128, 257], [0] * 8, 16, 16),
+                          "tall parts": ([40, 17], [3000, 2950], 8, 2)}[form]
+    c = Grouped(91, dtype, D, heads, kv, n, past, tail=2)
+    ws = K().attn_grouped_workspace_bytes(c.q.to(DEV), c.k.to(DEV), max(n))
+    assert (ws > 0) == ("parts" in form)
+    ref, bound = _whole_reference(c)
+    width, rows = heads * D, c.tokens
+    pad = -(-rows // 16) * 16 if tiled else rows
+    out = torch.full((pad, 2 * width), 3.0, dtype=BF, device=DEV)
+    got = c.run(out=out, split=True, tiled=tiled)
+    got = (K().untile_matrix(out, rows, 2 * width) if tiled else got)[:rows].double().cpu()
+    value = (got[:, :width] + got[:, width:]).view(rows, heads, D)
+    end = c.offset[-1]
+    # hi + lo is within 2^-8 2^-8 of the fp32 value
+    extra = 2.0 ** -16 * ref.abs() - (HALF_STEP[BF] * ref.abs() if dtype == BF else 0)
+    _check(value[:end], ref[:end], (bound + extra)[:end], form)
+    assert bool((got[end:] == 3.0).all())
+
+
 # ---- K8: shared prefixes -----------------------------------------------------------------------
 
 class Shared:
@@ -629,6 +694,75 @@ def test_shared_keeps_fp32_weights_below_the_normal_range(heavy):
     K().attn_decode_shared(q, pk, pv, i32([0, 3]), i32([500]), 3, kc, vc, i32([70, 9, 40]), out, ws)
     want = torch.tensor([569.0, 508.0, 539.0], device=DEV) * 2.0 ** -30
     assert bool((out[:, 0, 5] == want).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tiled", [False, True])
+def test_shared_split_output_of_each_type(dtype, D, tiled):
+    c = Shared(92, dtype, D, 6, 2, [0, 3, 7], [300, 77], [9, 40, 5, 1, 70, 2, 130, 6])
+    ref, bound = c.reference()
+    a = c.args()
+    rows, width = 8, c.heads * D
+    a[9] = torch.zeros(16 if tiled else rows, 2 * width, dtype=BF, device=DEV)
+    K().attn_decode_shared(*a, split=True, tiled=tiled)
+    got = (K().untile_matrix(a[9], rows, 2 * width) if tiled else a[9]).double().cpu()
+    value = (got[:, :width] + got[:, width:]).view(rows, c.heads, D)
+    extra = 2.0 ** -16 * ref.abs() - (HALF_STEP[BF] * ref.abs() if dtype == BF else 0)
+    _check(value, ref, bound + extra, "split")
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("heads,kv", [(80, 2), (33, 1), (161, 1)])
+def test_shared_many_heads_to_one(dtype, D, heads, kv):
+    """More query heads to a key / value head than rows in a flat tile: the rows' own keys run in tall
+    blocks too."""
+    c = Shared(93, dtype, D, heads, kv, [0, 5, 7], [2500, 60], [1, 300, 2, 0, 129, 90, 64, 200])
+    ref, bound = c.reference()
+    _check(c.run(), ref, bound, f"{heads} heads on {kv}")
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("heads", [4, 80])
+def test_shared_values_that_are_not_finite_of_each_type(dtype, D, bad, heads):
+    """In slots behind the ends, in a value of the prefix's or a row's own, in a key of either."""
+    c = Shared(94, dtype, D, heads, 2, [0, 3, 6], [700, 33], [9, 40, 5, 64, 0, 150, 7])
+    ref, bound = c.reference()
+    for t, lens in ((c.pk, c.prefix), (c.pv, c.prefix), (c.k, c.own), (c.v, c.own)):
+        for b, n in enumerate(lens):
+            t[b, :, n:] = bad
+    half = heads // 2
+    c.v[1, 1, 39, 2] = bad                       # the last own slot of row 1, second kv head
+    c.pv[1, 0, 32, 5] = bad                      # the last slot of prefix 1, first kv head
+    c.k[6, 0, 3] = float("nan")                  # a whole own key of row 6
+    c.pk[0, 0, 100] = float("nan")               # a whole key of prefix 0
+    out = c.run().double().cpu()
+    hit = torch.zeros_like(ref, dtype=torch.bool)
+    hit[1, half:, 2] = hit[3:6, :half, 5] = True
+    hit[6, :half] = hit[:3, :half] = True
+    _check(torch.where(hit, ref, out), ref, bound, "others")
+    for got in (out[1, half:, 2], out[3:6, :half, 5]):
+        assert bool(got.isnan().all() if math.isnan(bad) else (got == bad).all())
+    assert bool(out[6, :half].isnan().all()) and bool(out[:3, :half].isnan().all())
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+def test_caches_with_many_more_slots_than_keys(dtype, D):
+    """Caches that hold a whole output ahead: plans for their slots, most parts without a key."""
+    c = Shared(95, dtype, D, 8, 2, [0, 3, 6], [70, 1], [1, 0, 5, 64, 2, 9, 33])
+
+    def wide(t, n):
+        return torch.cat([t, torch.full((*t.shape[:2], n, D), float("nan"), dtype=dtype)], 2)
+
+    c.pk, c.pv, c.k, c.v = wide(c.pk, 9000), wide(c.pv, 9000), wide(c.k, 4096), wide(c.v, 4096)
+    ref, bound = c.reference()
+    _check(c.run(), ref, bound, "shared")
+    for n, past in (([1, 1, 1], [0, 40, 129]), ([40, 7, 0], [0, 300, 0])):
+        g = Grouped(96, dtype, D, 8, 2, n, past, tail=1)
+        g.k, g.v = wide(g.k, 9000), wide(g.v, 9000)
+        g.check("parts")
+        g.check("no workspace", workspace=False)
 
 
 # ---- K7 ----------------------------------------------------------------------------------------
