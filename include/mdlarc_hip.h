@@ -700,8 +700,9 @@ int mdl_qk_norm_rope_cache(const void* qkv, int in_dtype, int64_t ld, const floa
  * workspace (16-byte aligned) lets launches with few rows cut their keys into parts that a second
  * launch joins; mdl_attn_grouped_workspace_bytes of the same sizes (0: not used).  NULL: never
  * cut.  Smaller than that: MDL_ERR_WORKSPACE.  Calls that may overlap in time need workspaces of
- * their own.  The sums of a row are split by n_seq, max_q and cache_slots, so their order, and
- * with it the last bits, may change with those; equal calls give equal bits.
+ * their own.  The sums of a row are split by n_seq, max_q, cache_slots and whether there is a
+ * workspace, so their order, and with it the last bits, may change with those; equal calls give
+ * equal bits.
  */
 int mdl_attn_grouped(const void* q, const void* k_cache, const void* v_cache, int dtype, int n_seq,
                      int tokens, int max_q, int n_heads, int n_kv_heads, int head_dim,

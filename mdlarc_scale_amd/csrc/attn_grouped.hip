@@ -31,13 +31,14 @@
 // (plan_tiles chooses).  A launch may also cut each tile's keys in n_split parts whose states (fp32
 // m, l, o) go to the workspace; attn_merge_kernel joins them.
 //
-// What bounds it.  128 dims, bf16: the MFMAs at the power limit (two prompts of up to 8,192 tokens,
-// 32 heads on 8: 880 us, 1,105 TFLOP/s, 81% of a large library product on this card).  64 dims: an
-// exponential costs as much as its products, and VALU and MFMA instructions of three waves a SIMD
-// fill each other's gaps only in part (4 prompts of up to 6,000, 16 heads on 4: 251 us, 904
-// TFLOP/s).  fp32: the MFMAs, 75% of the rate of a large product (2 prompts of 4,000, 12 heads of
-// 64: 428 us).  Few rows: HBM (64 rows of up to 4,000 keys, 32 heads on 8 of 128: 143 us, 6.2 TB/s)
-// or, below some 20 MB, the launches and one block's chain of loads.
+// What bounds it.  128 dims, bf16: the clock, 1.5 GHz under this as under a large library product
+// (2.4 in launches that wait for memory), at which the MFMAs are busy 61% of the cycles, MFMAs or
+// VALU 90% and the LDS 31% (two prompts of up to 8,192 tokens, 32 heads on 8: 870 to 912 us, 1,066
+// to 1,117 TFLOP/s, some 80% of that product).  64 dims: an exponential costs as much as its
+// products; VALU busy 61%, MFMAs 45%, one or the other 87% (4 prompts of up to 6,000, 16 heads on 4:
+// 251 us, 904 TFLOP/s).  fp32: the MFMAs, busy 71%, 75% of the rate of a large product (2 prompts of
+// 4,000, 12 heads of 64: 432 us).  Few rows: HBM (64 rows of up to 4,000 keys, 32 heads on 8 of 128:
+// 143 us, 6.2 TB/s) or, below some 20 MB, the launches and one block's chain of loads.
 #include <climits>
 #include <type_traits>
 
@@ -113,8 +114,8 @@ __device__ __forceinline__ float max_halves(float v) {
   return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
-// 2^x.  EXACT (fp32 data) keeps results below 2^-126; the bare instruction, which gives the same bits
-// above, makes them zero, and bf16 data has it everywhere, as in K4a and K4b.
+// 2^x.  EXACT (fp32 data) keeps results below 2^-126; the bare instruction, which gives the same
+// bits above, makes them zero, and bf16 data has it everywhere, as in K4a and K4b.
 template <bool EXACT>
 __device__ __forceinline__ float weight_exp2(float x) {
   return EXACT ? exp2f(x) : __builtin_amdgcn_exp2f(x);
@@ -402,9 +403,9 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
 
   // fp32: the products of a tile's weights below 2^-126, which the bare exponential makes zero.  Rare,
   // so a loop of its own beside the products of all weights (the scores go round once), behind the
-  // branch that moves the reference.  16 prompts of up to 811 tokens (12 heads of 64) / 2 of 4,000: 161
-  // / 430 us without and with it; exp2f for every weight 168 / 454, a choice of the exponentials in
-  // front of the products 170 / 437.  A value that is not finite is left to those products.
+  // branch that moves the reference.  16 prompts of up to 811 tokens (12 heads of 64) / 2 of 4,000:
+  // 161 / 430 us without it, 162 / 432 with it; exp2f for every weight 168 / 454, a choice of the
+  // exponentials in front of the products 170 / 437.  A value that is not finite is left to those products.
   auto faint_weights = [&](f32x16_t& s, const uint8_t* Vt) {
 #pragma unroll 1
     for (int r = 0; r < 16; ++r) {
@@ -516,7 +517,10 @@ __device__ __forceinline__ void grouped_block(const GroupedArgs& p, int block, u
           const bf16x8_t pb = {(__bf16)t[8 * s], (__bf16)t[8 * s + 1], (__bf16)t[8 * s + 2],
                                (__bf16)t[8 * s + 3], (__bf16)t[8 * s + 4], (__bf16)t[8 * s + 5],
                                (__bf16)t[8 * s + 6], (__bf16)t[8 * s + 7]};
-          // the sum of the rounded weights that the product below takes, a pair at a time
+          // The weights are rounded to bf16, as the MFMA takes them: outputs are 2.0e-3 to 2.3e-3 from
+          // the definition where one rounding of the output alone makes 1.6e-3 to 1.7e-3.  A second
+          // product of what the rounding drops would be half as many MFMAs again.  The sum is of the
+          // rounded weights, so that their errors do not move the mean of the values.
           const uint4 pw = __builtin_bit_cast(uint4, pb);
           l = add_pair(add_pair(add_pair(add_pair(l, pw.x), pw.y), pw.z), pw.w);
           uint4 va[DB];
@@ -879,8 +883,8 @@ constexpr int kLongList = 4096;   // keys that two waves alone take too long ove
 // dims) 19 / 28; 540 of 467 tokens behind 11,204 keys 160 / 77; 72 of 17 tokens behind 4,099 keys
 // 21 / 19; 64 of 64 samples behind 32,749 keys (with their own keys and the merge) 117 / 73.  Where the
 // keys are too few to be cut, flat, as without a workspace: 116 flat blocks of a 300-token prompt in
-// 337 slots 6.9 / 7.9 (64 dims), 10.8 / 10.2 (128); 152 of two fp32 ones of 200 14.8 / 19.8; the own keys
-// of 8 samples, 40 heads to a kv head in 100 slots, in one launch with their prefix 8.4 / 13.4.
+// 337 slots 6.9 / 7.9 (64 dims), 10.8 / 10.2 (128); 152 of two fp32 ones of 200 14.8 / 19.8; the own
+// keys of 8 samples, 40 heads to a kv head in 100 slots, in a launch with their prefix 8.4 / 13.4.
 // Tall blocks are cut to one for each CU, and to two where the parts stay long: 4 continuations of
 // 100 tokens behind 6,000 keys 64 / 53 us; the 64 samples above 73 / 75, 17 tokens behind 4,099
 // keys 19 / 21.
