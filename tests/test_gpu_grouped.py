@@ -493,6 +493,77 @@ def test_grouped_split_output_of_each_block_form(dtype, D, tiled, form):
     assert bool((got[end:] == 3.0).all())
 
 
+@pytest.mark.parametrize("tiled", [None, True])
+def test_grouped_far_rows(tiled):
+    """q and out of more than 2^31 elements: the last rows, and one in the middle."""
+    D, heads, tokens = 128, 256, 66_000
+    q = torch.zeros(tokens, heads, D, dtype=BF, device=DEV)
+    assert q.numel() > 2 ** 31
+    c = Grouped(97, BF, D, heads, 1, [3], [60])
+    at = [30_000, 65_998, 65_999]                       # rows that get the queries of c
+    q[at] = c.q.to(DEV)
+    k, v = c.k.to(DEV), c.v.to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    width = heads * D
+    out = torch.zeros(tokens, 2 * width if tiled else width, dtype=BF, device=DEV)
+    K().attn_grouped(q, k, v, i32([0, tokens]), i32([63]), tokens, out, causal=False,
+                     split=bool(tiled), tiled=bool(tiled))
+    ref, bound = c.reference(causal=False)
+    if tiled:
+        first = [(a // 16) * 16 for a in at]             # blocks of sixteen rows
+        got = torch.stack([K().untile_matrix(out.view(-1)[2 * f * width:2 * (f + 16) * width], 16,
+                                             2 * width)[a - f] for f, a in zip(first, at)]).double()
+        got = (got[:, :width] + got[:, width:]).view(3, heads, D)
+        bound = bound + 2.0 ** -16 * ref.abs()
+    else:
+        got = out.view(tokens, heads, D)[at]
+    _check(got, ref, bound, "far rows")
+    # a query of zeros sees every key alike: the mean of the values
+    if not tiled:
+        want = c.v[0, 0, :63].double().mean(0).expand(heads, D)
+        mass = c.v[0, 0, :63].double().abs().mean(0)
+        _check(out.view(tokens, heads, D)[65_997], want,
+               2.0 ** -8 * want.abs() + (63 + 64) * 2.0 ** -23 * mass * 1.01, "mean")
+
+
+def test_grouped_calls_at_once():
+    """Two streams, a workspace each, and two captured graphs replayed side by side."""
+    kern = K()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    calls = []
+    for seed in (98, 99):
+        c = Grouped(seed, BF, 128, 8, 2, [3, 40, 1], [2900, 10, 1500])
+        q, k, v = c.q.to(DEV), c.k.to(DEV), c.v.to(DEV)
+        ws = torch.empty(kern.attn_grouped_workspace_bytes(q, k, 40) // 4, device=DEV)
+        assert ws.numel() > 0
+        calls.append((c, torch.cuda.Stream(), ws, (q, k, v, i32(c.offset), i32(c.keys), 40,
+                                                   torch.full_like(q, 7.0))))
+    refs = [c.reference() for c, _, _, _ in calls]
+    torch.cuda.synchronize()
+
+    def check(what):
+        torch.cuda.synchronize()
+        for (ref, bound), (_, _, _, a) in zip(refs, calls):
+            _check(a[6], ref, bound, what)
+            a[6].fill_(7.0)
+        torch.cuda.synchronize()
+    for _ in range(4):
+        for _, side, ws, a in calls:
+            with torch.cuda.stream(side):
+                kern.attn_grouped(*a, workspace=ws)
+    check("streams")
+    graphs = []
+    for _, side, ws, a in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            kern.attn_grouped(*a, workspace=ws)
+    for step in range(3):
+        for g, (_, side, _, _) in zip(graphs, calls):
+            with torch.cuda.stream(side):
+                g.replay()
+        check(f"graphs, replay {step}")
+
+
 # ---- K8: shared prefixes -----------------------------------------------------------------------
 
 class Shared:
@@ -765,6 +836,18 @@ def test_caches_with_many_more_slots_than_keys(dtype, D):
         g.check("no workspace", workspace=False)
 
 
+def test_shared_another_stream():
+    c = Shared(100, F32, 64, 4, 2, [0, 3, 5], [700, 33], [9, 40, 5, 64, 7])
+    a = c.args()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K().attn_decode_shared(*a)
+    torch.cuda.current_stream().wait_stream(side)
+    ref, bound = c.reference()
+    _check(a[9], ref, bound, "other stream")
+
+
 # ---- K7 ----------------------------------------------------------------------------------------
 
 def _rope(D, sizes=(32, 32, 8)):
@@ -886,6 +969,69 @@ def test_qk_norm_refuses_a_cache_without_rows():
                 K().qk_norm_rope_cache(*args)
         else:
             K().qk_norm_rope_cache(*args)
+
+
+def test_qk_norm_far_rows():
+    """qkv and q_out of more than 2^31 elements."""
+    D, heads, kv, rows = 128, 256, 1, 66_000
+    g = _gen(101)
+    tab, geom = _rope(D)
+    gain = torch.ones(D)
+    last = _rand(g, 4, (heads + 2 * kv) * D).to(BF)
+    qkv = torch.ones(rows, (heads + 2 * kv) * D, dtype=BF, device=DEV)
+    qkv[-4:] = last.to(DEV)
+    pos = torch.randint(0, 30, (rows, 3), generator=g)
+    slot = torch.arange(rows).int()
+    q = torch.empty(rows, heads, D, dtype=BF, device=DEV)
+    assert q.numel() > 2 ** 31
+    kc, vc = torch.zeros(2, 1, kv, rows, D, dtype=BF, device=DEV).unbind()
+    K().qk_norm_rope_cache(qkv, None, pos.to(DEV), tab.to(DEV), geom, gain.to(DEV), gain.to(DEV),
+                           1e-5, torch.zeros(rows, dtype=torch.int32, device=DEV), slot.to(DEV), 0.5,
+                           q, kc, vc)
+    refs = _qk_norm_reference(last, None, pos[-4:], tab, geom, gain, gain, 1e-5, heads, kv, D, 0.5)
+    half = HALF_STEP[BF]
+    for got, (ref, err) in zip((q[-4:], kc[0, :, -4:].transpose(0, 1), vc[0, :, -4:].transpose(0, 1)),
+                               refs):
+        _check(got, ref, err * (1 + half) + half * ref.abs() + 1e-30)
+
+
+def test_qk_norm_graph_and_streams():
+    """Captured once, replayed with other tokens and slots between eager work; another stream."""
+    kern = K()
+    D, heads, kv, rows, slots = 64, 6, 2, 16, 50
+    g = _gen(102)
+    tab, geom = _rope(D)
+    ones = torch.ones(D, device=DEV)
+    qkv = _rand(g, rows, (heads + 2 * kv) * D).to(DEV)
+    pos = torch.randint(0, 30, (rows, 3), generator=g).to(DEV)
+    row = torch.arange(rows, dtype=torch.int32, device=DEV)
+    slot = torch.full_like(row, 3)
+    new = lambda: (torch.full((rows, heads, D), 7.0, dtype=BF, device=DEV),  # noqa: E731
+                   *torch.zeros(2, rows, kv, slots, D, dtype=BF, device=DEV).unbind())
+    tab = tab.to(DEV)
+    run = lambda o: kern.qk_norm_rope_cache(qkv, None, pos, tab, geom, ones, ones, 1e-5, row, slot,  # noqa: E731
+                                            0.2, *o)
+    a, b = new(), new()
+    run(a)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(b)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(a)
+    for step in range(3):
+        qkv.copy_(torch.randn_like(qkv))
+        pos.add_(1)
+        slot.add_(7)
+        run(b)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(a, b)), step
+        torch.randn(1000, device=DEV).sum().item()
 
 
 # ---- together ----------------------------------------------------------------------------------
