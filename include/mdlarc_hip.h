@@ -64,6 +64,7 @@ extern "C" {
 
 #define MDL_DTYPE_F32 0
 #define MDL_DTYPE_BF16 1
+#define MDL_DTYPE_FP4 2            /* pages alone: e2m1 pairs with an e8m0 power for 32 channels */
 
 /* How mdl_attn_grouped / mdl_attn_decode_shared write their output (their out_form argument): in the
  * type of q, row-major [rows, n_heads * head_dim], or as the split input of a projection. */
@@ -735,6 +736,89 @@ int mdl_attn_decode_shared(const void* q, const void* prefix_k, const void* pref
 int64_t mdl_attn_decode_shared_workspace_bytes(int batch, int n_prefix, int max_rows, int n_heads,
                                                int n_kv_heads, int head_dim, int dtype,
                                                int prefix_slots, int cache_slots);
+
+/*
+ * Paged caches (K9, K10): a pool [n_pages, n_kv_heads, page_slots, head_dim] of K and one of V, and
+ * page_table int32 [n_seq, table_width] (row stride table_ld elements): slot j of sequence s is slot
+ * j % page_slots of page page_table[s][j / page_slots].  page_slots is a multiple of 16, 16 to 4,096.
+ * Sequences take pages as they grow, in any order; a page may be in several sequences (a prefix that
+ * they share, which none of them appends to).  page_dtype: MDL_DTYPE_F32, MDL_DTYPE_BF16, or
+ * MDL_DTYPE_FP4 -- uint8 pools [.., head_dim / 2] of e2m1 numbers (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their
+ * negatives; the even channel in the low four bits) and uint8 k_scale / v_scale [n_pages, n_kv_heads,
+ * page_slots, head_dim / 32] of powers of two (e8m0: byte b is 2^(b - 127), 255 is NaN) by which the
+ * 32 channels are multiplied: 17/32 of a byte a value.
+ * No counterpart in the reference, whose StaticKVCache (src/inference.py:51-96) gives every row as
+ * many slots as the longest.
+ *
+ * K9, append: mdl_qk_norm_rope_cache with the pages of token m's sequence token_row[m] in place of a
+ * cache row, and norms only where q_gamma and k_gamma are not NULL (both or neither).  A slot outside
+ * the table, a sequence outside it and a page number outside the pool are not written.  q_out is of
+ * q_dtype, the pages' type unless those are MDL_DTYPE_FP4.  4 bits: the 32 channels' power is the
+ * smallest 2^k, -100 <= k <= 125, by which all their magnitudes are below 7, and each value times
+ * 2^-k goes to the nearest number (ties to even); 32 channels with a value that is not finite become
+ * NaN.
+ */
+int mdl_rope_cache_paged(const void* qkv, int in_dtype, int64_t ld, const float* rstd,
+                         const int64_t* pos, const float* rope_tab, int64_t rows,
+                         const int32_t* token_row, const int32_t* token_slot,
+                         const int32_t* page_table, int64_t table_ld, int n_seq, int table_width,
+                         int n_pages, int page_slots, int n_heads, int n_kv_heads, int head_dim,
+                         int max_x, int max_y, int max_z, int px, int py, int pz,
+                         const float* q_gamma, const float* k_gamma, float eps, float q_scale,
+                         void* q_out, int q_dtype, void* k_pages, void* v_pages, int page_dtype,
+                         uint8_t* k_scale, uint8_t* v_scale, void* stream);
+
+/*
+ * K9, read: k_out / v_out [n_seq, n_kv_heads, run, head_dim]: row i < count[s] of sequence s is its
+ * slot start[s] + i (int32 [n_seq] each).  Rows from count[s] on, and rows whose slot is outside the
+ * table or in a page outside the pool, stay as they were.  out_dtype is the pages' type, or
+ * MDL_DTYPE_BF16 or MDL_DTYPE_F32 for 4-bit pages, whose values both hold exactly.
+ */
+int mdl_paged_rows(const void* k_pages, const void* v_pages, int page_dtype,
+                   const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* page_table,
+                   int64_t table_ld, int n_seq, int table_width, int n_pages, int page_slots,
+                   int n_kv_heads, int head_dim, const int32_t* start, const int32_t* count, int run,
+                   void* k_out, void* v_out, int out_dtype, void* stream);
+
+/*
+ * K10: mdl_attn_grouped with the pages of a sequence in place of its cache row; cache_slots is
+ * table_width * page_slots.  q (and out) are of dtype, the pages' type unless those are
+ * MDL_DTYPE_FP4, whose values enter the products as they are.  A sequence that has a page number
+ * outside the pool among the pages of its keys reads no memory outside the pool and gives NaN in every
+ * row that sees such a page (and may in its other rows).
+ */
+int mdl_attn_paged(const void* q, int dtype, const void* k_pages, const void* v_pages,
+                   int page_dtype, const uint8_t* k_scale, const uint8_t* v_scale, int n_pages,
+                   int page_slots, const int32_t* page_table, int64_t table_ld, int table_width,
+                   int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, int head_dim,
+                   const int32_t* q_offset, const int32_t* kv_len, int causal, void* out,
+                   int out_form, float* workspace, int64_t workspace_bytes, void* stream);
+int64_t mdl_attn_paged_workspace_bytes(int n_seq, int tokens, int max_q, int n_heads,
+                                       int n_kv_heads, int head_dim, int dtype, int page_dtype,
+                                       int table_width, int page_slots);
+
+/*
+ * K11: one token a row, sampled from logits [rows, vocab] (MDL_DTYPE_F32 or MDL_DTYPE_BF16, row stride
+ * ld elements; vocab at most 2^20).  Tokens are ordered by value, larger first, equal ones by index,
+ * lower first; weights are w = e^((x - max) / temperature[r]):
+ *   top_k[r] > 0    the first top_k[r] of the order are kept;
+ *   top_p[r] < 1    of those, the ones before which the sum is below top_p[r] times the sum of all;
+ *   min_p[r] > 0    of those, the ones with w >= min_p[r] (the largest w is 1);
+ *   token_out[r]    int64: the first index whose sum of kept weights up to it is above uniform[r] times
+ *                   the sum of all (uniform[r] in [0, 1));
+ *   logprob_out[r]  (may be NULL) ln of the token's share of the kept weights.
+ * temperature, top_k, top_p and min_p are device arrays of a number a row; NULL is 1 and no filter.  A
+ * temperature of 0 or below (or NaN), a top_k of 1, a top_p of 0 or below and a min_p above 1 give the
+ * first of the order, with logprob 0.  NaN logits count as -inf, which is never taken; a row of nothing
+ * else gives token 0 and logprob -inf.  Weights are of 64 bits and are summed as multiples of 2^-44 of
+ * the largest, so equal calls give equal tokens and no order of the sums moves one.
+ * Replaces: the temperature / top-k branch of generate_output (src/inference.py:573-583) with the
+ *           random number as an input, so a sampled step can be captured and repeated.
+ */
+int mdl_sample_tokens(const void* logits, int dtype, int64_t ld, int rows, int vocab,
+                      const float* uniform, const float* temperature, const int32_t* top_k,
+                      const float* top_p, const float* min_p, int64_t* token_out,
+                      float* logprob_out, void* stream);
 
 /*
  * Every layer of a prompt or decode step from one call (host code over the entries above, which

@@ -146,6 +146,17 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mdl_attn_decode_shared": (c_int, [P, P, P, P, P, c_int, c_int, c_int, P, P, P, c_int, c_int,
                                        c_int, c_int, c_int, c_int, P, c_int, P, c_int64, P]),
     "mdl_attn_decode_shared_workspace_bytes": (c_int64, [c_int] * 9),
+    "mdl_rope_cache_paged": (c_int, [P, c_int, c_int64, P, P, P, c_int64, P, P, P, c_int64, c_int,
+                                     c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                     c_int, c_int, c_int, P, P, c_float, c_float, P, c_int, P, P,
+                                     c_int, P, P, P]),
+    "mdl_paged_rows": (c_int, [P, P, c_int, P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int,
+                               c_int, P, P, c_int, P, P, c_int, P]),
+    "mdl_attn_paged": (c_int, [P, c_int, P, P, c_int, P, P, c_int, c_int, P, c_int64, c_int, c_int,
+                               c_int, c_int, c_int, c_int, c_int, P, P, c_int, P, c_int, P, c_int64,
+                               P]),
+    "mdl_attn_paged_workspace_bytes": (c_int64, [c_int] * 10),
+    "mdl_sample_tokens": (c_int, [P, c_int, c_int64, c_int, c_int, P, P, P, P, P, P, P, P]),
     "mdl_lm_head": (c_int, [P, P, c_int, c_int, P, c_float, P, c_int, P, P, CONS, c_int, P]),
     "mdl_decode_head": (c_int, [P, c_int, c_int, P, c_float, P, c_int, P, P, P, c_int64, c_int,
                                 P, P, c_int, c_int, CONS, c_int, P]),

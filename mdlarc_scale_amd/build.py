@@ -32,7 +32,10 @@ SOURCES = [
     "attn_prefill.hip",
     "attn_f32.hip",
     "attn_grouped.hip",
+    "attn_paged.hip",
     "qk_norm.hip",
+    "paged_cache.hip",
+    "sample.hip",
     "head_state.hip",
     "prompt_build.hip",
     "split_gemm.hip",

@@ -16,6 +16,8 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // vmcnt(0) lgkmcnt(0).  Issued through __builtin_amdgcn_s_waitcnt, the wait is visible to the
 // compiler's own wait insertion, which then counts every load it issued before as complete.
 constexpr int kWaitAll = 0x0070;
+// lgkmcnt(0) alone: the wave's LDS operations are done, its vector loads may be in flight.
+constexpr int kWaitLds = 0xc07f;
 
 // 16 bytes per lane from global memory straight into LDS: lane l's bytes land at lds + 16 l
 // (lds wave-uniform, through M0).  Issued as inline assembly, so the compiler neither sees nor

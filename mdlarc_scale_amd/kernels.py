@@ -1316,6 +1316,230 @@ def attn_decode_shared(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
             workspace.data_ptr(), workspace.numel() * 4)
 
 
+# --- paged caches (K9, K10) ----------------------------------------------------------------------
+
+FP4_GROUP = 32      # channels of a 4-bit page that share a power
+PAGE_FP4 = 2        # MDL_DTYPE_FP4
+
+
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor | None,
+           v_scale: torch.Tensor | None, page_table: torch.Tensor,
+           dtype: torch.dtype) -> tuple[tuple, int, list, tuple]:
+    """Checks of a paged cache for rows of ``dtype``: its (pages, kv_heads, page slots, head dim),
+    the pages' type code, the specs of its tensors, and the table's (sequences, width, row stride)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError("k_pages and v_pages must both be [pages, kv_heads, page_slots, head_dim] "
+                         f"(got {tuple(shape)} and {tuple(v_pages.shape)})")
+    n, kv, slots, d = shape
+    fp4 = k_pages.dtype is U8
+    if fp4:
+        d *= 2
+    if d not in GROUPED_HEAD_DIMS:
+        raise ValueError(f"pages must have a head_dim of 64 or 128, 4-bit ones half as many bytes "
+                         f"(got {tuple(shape)} of {k_pages.dtype})")
+    if not n or not kv or slots < 16 or slots > 4096 or slots % 16:
+        raise ValueError("a pool needs pages, key / value heads, and 16 to 4096 slots a page, in "
+                         f"multiples of 16 (got {tuple(shape)})")
+    if len(page_table.shape) != 2:
+        raise ValueError(f"page_table must be [sequences, pages] (got {tuple(page_table.shape)})")
+    n_seq, width = page_table.shape
+    ld, step = page_table.stride()
+    if page_table.dtype is not I32 or (width > 1 and step != 1) or (n_seq > 1 and ld < width):
+        raise ValueError("page_table must be int32 with contiguous rows that do not overlap")
+    code = PAGE_FP4 if fp4 else cache_dtype_code(k_pages)
+    specs = [(k_pages, "k_pages", U8 if fp4 else dtype, 0),
+             (v_pages, "v_pages", U8 if fp4 else dtype, 0)]
+    if fp4:
+        scales = (n, kv, slots, d // FP4_GROUP)
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t is None or t.shape != scales:
+                raise ValueError(f"{name} must be {list(scales)} for 4-bit pages (got "
+                                 f"{None if t is None else tuple(t.shape)})")
+            specs.append((t, name, U8, 0))
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("only 4-bit (uint8) pages have scales")
+    return (n, kv, slots, d), code, specs, (n_seq, width, ld if n_seq > 1 else max(width, 1))
+
+
+def _on(dev: int, t: torch.Tensor, name: str) -> None:
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, another tensor on GPU {dev}: one call runs on "
+                         "one device")
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def rope_cache_paged(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.Tensor,
+                     rope_tab: torch.Tensor, rope_geom: tuple[int, int, int, int, int, int],
+                     token_row: torch.Tensor, token_slot: torch.Tensor, page_table: torch.Tensor,
+                     q_scale: float, q_out: torch.Tensor, k_pages: torch.Tensor,
+                     v_pages: torch.Tensor, k_scale: torch.Tensor | None = None,
+                     v_scale: torch.Tensor | None = None, q_gamma: torch.Tensor | None = None,
+                     k_gamma: torch.Tensor | None = None, eps: float = 1e-5) -> None:
+    """``qk_norm_rope_cache`` into pages: the tokens' keys and values go to slot token_slot[m] of
+    sequence token_row[m], which is slot j % P of page page_table[row, j // P] of pools [pages,
+    kv_heads, P, D] (bf16, fp32, or 4 bits: uint8 [.., D / 2] with ``k_scale`` / ``v_scale`` uint8
+    [.., D / 32]).  page_table: int32 [sequences, width], rows may be strided (``table[:, :n]``).  Head
+    norms only with ``q_gamma`` and ``k_gamma``.  Slots, sequences and pages that do not exist are not
+    written.  q_out: the pages' type; bf16 or fp32 with 4-bit pages."""
+    out, shape = q_out.dtype, qkv.shape
+    (n_pages, kv, slots, d), code, specs, (n_seq, width, ld) = _pages(
+        k_pages, v_pages, k_scale, v_scale, page_table, out)
+    if len(shape) != 2:
+        raise ValueError("qkv must be [rows, (n_heads + 2 * n_kv_heads) * head_dim]")
+    rows, columns = shape
+    heads = columns // d - 2 * kv
+    if columns % d or heads <= 0 or heads % kv:
+        raise ValueError(f"qkv rows of {columns} do not hold a multiple of {kv} query heads, {kv} "
+                         f"key heads and {kv} value heads of {d}")
+    if (q_gamma is None) != (k_gamma is None):
+        raise ValueError("q_gamma and k_gamma are given together or not at all")
+    dev = qkv.get_device()
+    row_ld, step = qkv.stride()
+    if step != 1:
+        raise ValueError("the rows of qkv must be contiguous")
+    if rows <= 1:
+        row_ld = columns
+    mx, my, mz, px, py, pz = (_at_most(n, C_INT_MAX) for n in rope_geom)   # larger: refused
+    in_dt, out_dt = cache_dtype_code(qkv), cache_dtype_code(q_out)
+    specs += [(pos, "pos", I64, rows * 3),
+              (rope_tab, "rope_tab", F32, 2 * (mx * px + my * py + mz * pz)),
+              (token_row, "token_row", I32, rows), (token_slot, "token_slot", I32, rows),
+              (q_out, "q_out", out, rows * heads * d)]
+    if rstd is not None:
+        specs.append((rstd, "rstd", F32, rows))
+    if q_gamma is not None:
+        specs += [(q_gamma, "q_gamma", F32, d), (k_gamma, "k_gamma", F32, d)]
+    _need_all(dev, specs)
+    _on(dev, page_table, "page_table")
+    if rows == 0:
+        return
+    _launch(dev, "mdl_rope_cache_paged", qkv.data_ptr(), in_dt, row_ld, _ptr(rstd), pos.data_ptr(),
+            rope_tab.data_ptr(), rows, token_row.data_ptr(), token_slot.data_ptr(),
+            page_table.data_ptr(), ld, n_seq, width, n_pages, slots, heads, kv, d, mx, my, mz, px,
+            py, pz, _ptr(q_gamma), _ptr(k_gamma), eps, q_scale, q_out.data_ptr(), out_dt,
+            k_pages.data_ptr(), v_pages.data_ptr(), code, _ptr(k_scale), _ptr(v_scale))
+
+
+def paged_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+               start: torch.Tensor, count: torch.Tensor, k_out: torch.Tensor,
+               v_out: torch.Tensor, k_scale: torch.Tensor | None = None,
+               v_scale: torch.Tensor | None = None) -> None:
+    """Slots start[s] .. start[s] + count[s] - 1 of each sequence (int32) out of its pages into rows 0
+    .. count[s] - 1 of k_out and v_out [sequences, kv_heads, run, D]; other rows stay as they were.
+    The rows are of the pages' type, or bf16 or fp32 (both exact) for 4-bit pages: a prompt written to
+    pages can so become the prefix that ``attn_decode_shared`` reads."""
+    out, shape = k_out.dtype, k_out.shape
+    (n_pages, kv, slots, d), code, specs, (n_seq, width, ld) = _pages(
+        k_pages, v_pages, k_scale, v_scale, page_table, out)
+    if v_out.shape != shape or len(shape) != 4 or (shape[0], shape[1], shape[3]) != (n_seq, kv, d):
+        raise ValueError(f"k_out and v_out must both be [{n_seq}, {kv}, run, {d}] (got "
+                         f"{tuple(shape)} and {tuple(v_out.shape)})")
+    if start.numel() != n_seq or count.numel() != n_seq:
+        raise ValueError(f"start and count must have {n_seq} elements")
+    dev = k_pages.get_device()
+    specs += [(start, "start", I32, 0), (count, "count", I32, 0), (k_out, "k_out", out, 0),
+              (v_out, "v_out", out, 0)]
+    _need_all(dev, specs)
+    _on(dev, page_table, "page_table")
+    if n_seq == 0 or shape[2] == 0:
+        return
+    _launch(dev, "mdl_paged_rows", k_pages.data_ptr(), v_pages.data_ptr(), code, _ptr(k_scale),
+            _ptr(v_scale), page_table.data_ptr(), ld, n_seq, width, n_pages, slots, kv, d,
+            start.data_ptr(), count.data_ptr(), shape[2], k_out.data_ptr(), v_out.data_ptr(),
+            cache_dtype_code(k_out))
+
+
+def _paged_q(q: torch.Tensor, kv: int, d: int) -> tuple[int, int]:
+    """Tokens and heads of q [tokens, n_heads, D] for pages of ``kv`` heads of ``d``."""
+    if len(q.shape) != 3 or q.shape[2] != d or not q.shape[1] or q.shape[1] % kv:
+        raise ValueError(f"q must be [tokens, a multiple of {kv} heads, {d}] (got {tuple(q.shape)})")
+    return q.shape[0], q.shape[1]
+
+
+def attn_paged_workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor,
+                               max_q: int) -> int:
+    """Bytes of ``attn_paged``'s workspace for tensors of these shapes (0: none is used)."""
+    _, kv, slots, d = k_pages.shape
+    fp4 = k_pages.dtype is U8
+    d = 2 * d if fp4 else d
+    tokens, heads = _paged_q(q, kv, d)
+    code = cache_dtype_code(q)
+    return _lib.lib().mdl_attn_paged_workspace_bytes(
+        page_table.shape[0], tokens, _at_most(max_q, tokens), heads, kv, d, code,
+        PAGE_FP4 if fp4 else code, page_table.shape[1], slots)
+
+
+def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+               page_table: torch.Tensor, q_offset: torch.Tensor, kv_len: torch.Tensor, max_q: int,
+               out: torch.Tensor, causal: bool = True, workspace: torch.Tensor | None = None,
+               k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+               split: bool = False, tiled: bool = False) -> None:
+    """``attn_grouped`` over pages (``rope_cache_paged``'s pools and page_table): sequence s has the
+    rows q_offset[s] .. q_offset[s + 1] - 1 of q [tokens, n_heads, D] (single tokens, continuations,
+    whole prompts) and the keys in its slots [0, kv_len[s]).  q and out are of the pages' type; bf16 or
+    fp32 with 4-bit pages.  ``workspace``: fp32, attn_paged_workspace_bytes; it depends on the table's
+    width, so a table cut to the pages in use (``table[:, :n]``) splits the keys better.  A page number
+    outside the pool among a sequence's keys gives NaN in the rows that see it."""
+    dt = q.dtype
+    (n_pages, kv, slots, d), page_code, specs, (n_seq, width, ld) = _pages(
+        k_pages, v_pages, k_scale, v_scale, page_table, dt)
+    tokens, heads = _paged_q(q, kv, d)
+    if q_offset.numel() != n_seq + 1 or kv_len.numel() != n_seq:
+        raise ValueError(f"q_offset and kv_len must have {n_seq + 1} and {n_seq} elements")
+    dev, code = q.get_device(), cache_dtype_code(q)
+    specs += [(q, "q", dt, 0), (q_offset, "q_offset", I32, 0), (kv_len, "kv_len", I32, 0),
+              _out_spec(out, q, tokens, heads * d, split, tiled)]
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        specs.append((workspace, "workspace", F32, 0))
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * 4
+    _need_all(dev, specs)
+    _on(dev, page_table, "page_table")
+    if tokens == 0 or n_seq == 0:
+        return
+    _launch(dev, "mdl_attn_paged", q.data_ptr(), code, k_pages.data_ptr(), v_pages.data_ptr(),
+            page_code, _ptr(k_scale), _ptr(v_scale), n_pages, slots, page_table.data_ptr(), ld,
+            width, n_seq, tokens, _at_most(max_q, tokens), heads, kv, d, q_offset.data_ptr(),
+            kv_len.data_ptr(), int(causal), out.data_ptr(), split + tiled, ws, ws_bytes)
+
+
+# --- sampling (K11) ------------------------------------------------------------------------------
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, token_out: torch.Tensor,
+                  temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+                  top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+                  logprob_out: torch.Tensor | None = None) -> None:
+    """One token a row (int64 token_out) from logits [rows, vocab] (fp32 or bf16, rows may be strided)
+    at the random numbers ``uniform`` [rows] in [0, 1), after temperature, top-k, top-p and min-p (a
+    number a row each: fp32, int32, fp32, fp32; None: 1 and no filter), in that order; ``logprob_out``
+    (fp32): the log of the token's share of what the filters keep.  A temperature of 0 is greedy.  Ties
+    go to the lowest index; NaN logits count as -inf."""
+    if len(logits.shape) != 2 or not logits.shape[1]:
+        raise ValueError(f"logits must be [rows, vocab] (got {tuple(logits.shape)})")
+    rows, vocab = logits.shape
+    ld, step = logits.stride()
+    if (vocab > 1 and step != 1) or (rows > 1 and ld < vocab):
+        raise ValueError("the rows of logits must be contiguous and not overlap")
+    if rows <= 1:
+        ld = vocab
+    code, dev = cache_dtype_code(logits), logits.get_device()
+    specs = [(uniform, "uniform", F32, rows), (token_out, "token_out", I64, rows)]
+    for t, name, dt in ((temperature, "temperature", F32), (top_k, "top_k", I32),
+                        (top_p, "top_p", F32), (min_p, "min_p", F32),
+                        (logprob_out, "logprob_out", F32)):
+        if t is not None:
+            specs.append((t, name, dt, rows))
+    _need_all(dev, specs)
+    if rows == 0:
+        return
+    _launch(dev, "mdl_sample_tokens", logits.data_ptr(), code, ld, rows, vocab, uniform.data_ptr(),
+            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), token_out.data_ptr(),
+            _ptr(logprob_out))
+
 
 class HeadConstraints:
     """Device form of DecodingConstraints for the head kernels (``mdl_logit_constraints``):
