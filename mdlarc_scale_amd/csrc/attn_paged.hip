@@ -40,6 +40,310 @@ int launch_source(const PagedArgs& a, bool fp4, bool tall, unsigned blocks, hipS
              : launch_paged<T, D, kPages>(a, tall, blocks, st);
 }
 
+// ---- single tokens over 4-bit pages ------------------------------------------------------------
+
+// One query a sequence and up to 16 of its heads to a key / value head: rows of 16 x 16 x 32 MFMAs
+// (lane c = lane % 16, g = lane / 16), KT keys at a time.
+//   S^T = K Q^T, 16 keys a block: the k index of an MFMA is whatever both operands agree on, so lane
+//     group g takes dims g D / 4 .. of its key, which are neighbouring bytes: a block is one load a
+//     lane, and its codes become the operand in registers.  Lane c, g holds the scores of row c with
+//     keys 4 g .. 4 g + 3 of each block.
+//   O^T = V^T P^T, 32 keys a step: the weights are the operand where they are; V^T comes from the
+//     wave's own tile of bf16 values in LDS by transposing reads.
+// fp32 queries (PARTS 3): codes are exact in bf16, so q and the weights go as sums of three bf16
+// numbers each (24 bits), and the products are fp32's.  Weights below 2^-126 are zero in either form.
+// The waves of a block take the tiles in turn and merge at the end.  A value that is not finite is
+// seen by every row or (keys behind the last) set to zero.
+template <int D>
+struct TokenShape {
+  static constexpr int kTile = D == 128 ? 32 : 64;     // keys of a tile
+  static constexpr int kBlocks = kTile / 16;
+  static constexpr int kBytes = D / 8;                 // of codes in a lane's piece of a row
+  static constexpr int kWords = kBytes / 4;
+  static constexpr int kAhead = 2;                     // tiles in flight
+  static constexpr int kWaves = 4;
+  static constexpr int kLd = D + 8;                    // bf16 elements of a row of V in LDS
+  static constexpr int kStateLd = D + 4;               // floats of a row of a wave's state
+  static constexpr int kWaveBytes =
+      kTile * kLd * 2 > 16 * kStateLd * 4 ? kTile * kLd * 2 : 16 * kStateLd * 4;
+};
+
+template <int D, int PARTS>
+__global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel(const PagedArgs p) {
+  using S = TokenShape<D>;
+  constexpr int KT = S::kTile, NB = S::kBlocks, W = S::kWords, DB = D / 16, kTurn = KT * S::kWaves;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kWaves * S::kWaveBytes];
+  __shared__ float states[S::kWaves][2][16];
+  const int block = blockIdx.x;
+  const int pairs = p.n_seq * p.kv_heads;
+  const int split = quotient(block, p.by_pairs), pair = block - split * pairs;
+  const int seq = quotient(pair, p.by_kv), kvh = pair - seq * p.kv_heads;
+  const int lo = min(max(p.q_offset[seq], 0), p.tokens);
+  if (min(max(p.q_offset[seq + 1], lo), p.tokens) == lo) return;
+  const int G = p.group;
+  const int kend = min(max(p.kv_len[seq], 0), p.slots);
+  const int per = ((kend + p.n_split - 1) / p.n_split + kTurn - 1) / kTurn * kTurn;
+  const int k0 = min(split * per, kend), k1 = min(k0 + per, kend);
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t qrow = static_cast<int64_t>(lo) * p.heads + kvh * G;
+
+  // q of row c (rows past G: the last one's), dims g D / 4 + 8 s .. + 7 of step s
+  bf16x8_t qf[PARTS][D / 32];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    const int64_t at = (qrow + min(c, G - 1)) * D + g * (D / 4) + 8 * s;
+    if constexpr (PARTS == 1) {
+      qf[0][s] = as_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at));
+    } else {
+      float f[8];
+      load8f(static_cast<const float*>(p.q) + at, f);
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        uint4 hi, rest;
+        split8(f, hi, rest);
+        qf[i][s] = as_bf16x8(hi);
+        float h[8];
+        unpack8(hi, h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] -= h[e];
+      }
+    }
+  }
+
+  // the numbers of 64 pages from `page0` on, one a lane (as in attn_tiles.h)
+  int page0 = 0, page_no = 0;
+  bool astray = false;
+  auto load_pages = [&](int page) {
+    page0 = page;
+    const int last = quotient(kend - 1, p.by_page);
+    page_no = p.table[seq * p.table_ld + min(page + lane, last)];
+    const bool bad = page_no < 0 || page_no >= p.n_pages;
+    astray = astray || __ballot(bad) != 0;
+    page_no = bad ? 0 : page_no;
+  };
+  struct Tile {
+    uint32_t k[NB][W], v[NB][W], kp[NB], vp[NB];
+  };
+  Tile tiles[S::kAhead];
+  // lane's places in a block: K, key c and piece g; V, key lane / 4 and piece lane % 4
+  const uint32_t k_at = c * (D / 2) + g * S::kBytes, v_at = lane * S::kBytes;
+  const uint32_t kp_at = c * (D / 32) + g * (D / 4) / 32;
+  const uint32_t vp_at = (lane >> 2) * (D / 32) + (lane & 3) * (D / 4) / 32;
+  auto piece = [&](const uint8_t* from, uint32_t (&t)[W]) {
+    if constexpr (W == 4) {
+      const uint4 u = load_nt16(from);
+      t[0] = u.x; t[1] = u.y; t[2] = u.z; t[3] = u.w;
+    } else {
+      const u32x2_t u = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(from));
+      t[0] = u.x; t[1] = u.y;
+    }
+  };
+  auto fetch = [&](Tile& t, int kt) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int key = min(kt + 16 * b, (kend - 1) & ~15);
+      const int page = quotient(key, p.by_page);
+      if (static_cast<uint32_t>(page - page0) >= kWave) load_pages(page);
+      const int64_t no = __builtin_amdgcn_readlane(page_no, page - page0);
+      const int64_t row = (no * p.kv_heads + kvh) * p.page_slots + key - page * p.page_slots;
+      piece(static_cast<const uint8_t*>(p.k) + row * (D / 2) + k_at, t.k[b]);
+      piece(static_cast<const uint8_t*>(p.v) + row * (D / 2) + v_at, t.v[b]);
+      t.kp[b] = (p.k_scale + row * (D / 32))[kp_at];
+      t.vp[b] = (p.v_scale + row * (D / 32))[vp_at];
+    }
+  };
+
+  float negm = 0.f, thr = -INFINITY, l = 0.f;   // l: of this lane's keys
+  f32x4_t o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  uint16_t* vt = reinterpret_cast<uint16_t*>(lds + wave * S::kWaveBytes);
+
+  auto work = [&](Tile& t, int kt) {
+    const bool whole = kt + KT <= k1;
+    f32x4_t sc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      sc[b] = f32x4_t{negm, negm, negm, negm};
+      const float power = __uint_as_float(t.kp[b] << 23);
+#pragma unroll
+      for (int s = 0; s < W; ++s) {
+        uint32_t u[8];
+        fp4_values<uint16_t>(t.k[b][s], power, u);
+        const bf16x8_t a = as_bf16x8(make_uint4(u[0], u[1], u[2], u[3]));
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[i][s], sc[b], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);   // one block's values in registers at a time
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const bool there = whole || kt + 16 * b + (lane >> 2) < k1;
+      const float power = there ? __uint_as_float(t.vp[b] << 23) : 1.f;
+#pragma unroll
+      for (int s = 0; s < W; ++s) {
+        uint32_t u[8];
+        fp4_values<uint16_t>(there ? t.v[b][s] : 0u, power, u);
+        *reinterpret_cast<uint4*>(vt + (16 * b + (lane >> 2)) * S::kLd + (lane & 3) * (D / 4) +
+                                  8 * s) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!whole) {
+      const int x = k1 - kt - 4 * g;   // keys of the tile, from this lane's first
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * b + r >= x) sc[b][r] = -INFINITY;
+    }
+    float lmax = sc[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) lmax = fmaxf(lmax, sc[b][r]);
+    if (__ballot(lmax > thr) != 0) {
+      const float tmax = max_over_groups(lmax);
+      if (tmax > thr) {   // the same in the four lanes of a row
+        const bool fresh = thr == -INFINITY;
+        const float alpha = fresh ? 0.f : __builtin_amdgcn_exp2f(-tmax);
+        negm = fresh ? -tmax : negm - tmax;
+        thr = kGap;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) sc[b] -= tmax;
+        l *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sc[b][r] = __builtin_amdgcn_exp2f(sc[b][r]);
+#pragma unroll
+    for (int kk = 0; kk < NB / 2; ++kk) {
+      bf16x8_t pb[PARTS];
+      if constexpr (PARTS == 1) {
+        // rounded to bf16, and the sum is of the rounded weights, as in attn_tiles.h
+        pb[0] = pt_operand(sc[2 * kk], sc[2 * kk + 1]);
+        const uint4 pw = __builtin_bit_cast(uint4, pb[0]);
+        l = add_pair(add_pair(add_pair(add_pair(l, pw.x), pw.y), pw.z), pw.w);
+      } else {
+        float f[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f[r] = sc[2 * kk][r];
+          f[4 + r] = sc[2 * kk + 1][r];
+          l += f[r] + f[4 + r];
+        }
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          uint4 hi, rest;
+          split8(f, hi, rest);
+          pb[i] = as_bf16x8(hi);
+          float h[8];
+          unpack8(hi, h);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] -= h[e];
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const bf16x8_t a = vt_operand(vt, S::kLd, kk, db, c, g);
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+          o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[i], o[db], 0, 0, 0);
+        if (db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  const int first = k0 + KT * wave;
+  const int nt = first < k1 ? (k1 - first + kTurn - 1) / kTurn : 0;
+  if (nt > 0) {
+    load_pages(quotient(first, p.by_page));
+#pragma unroll
+    for (int j = 0; j < S::kAhead; ++j) fetch(tiles[j], first + min(j, nt - 1) * kTurn);
+    for (int i = 0; i < nt; i += S::kAhead) {   // a tile past the last one has no keys
+#pragma unroll
+      for (int j = 0; j < S::kAhead; ++j) {
+        work(tiles[j], first + (i + j) * kTurn);
+        if (i + j + S::kAhead < nt) fetch(tiles[j], first + (i + j + S::kAhead) * kTurn);
+      }
+    }
+  }
+
+  // sum of the row's four lanes
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  if (astray) l = __uint_as_float(0x7fc00000u);
+  float* st = reinterpret_cast<float*>(lds + wave * S::kWaveBytes);
+  // -inf marks a state without keys (scores that are all NaN make one with keys)
+  if (g == 0) {
+    states[wave][0][c] = thr == -INFINITY && l == 0.f ? -INFINITY : -negm;
+    states[wave][1][c] = l;
+  }
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+    *reinterpret_cast<float4*>(st + c * S::kStateLd + 16 * db + 4 * g) =
+        make_float4(o[db][0], o[db][1], o[db][2], o[db][3]);
+  __syncthreads();
+  const bool part = p.ws_o != nullptr;
+  const int64_t base = split * static_cast<int64_t>(p.tokens) * p.heads + qrow;
+  for (int i = threadIdx.x; i < G * (D / 4); i += 256) {
+    const int row = i / (D / 4), dim = 4 * (i - row * (D / 4));
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < S::kWaves; ++w) top = fmaxf(top, states[w][0][row]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < S::kWaves; ++w) {
+      const float m = states[w][0][row];
+      if (m == -INFINITY) continue;
+      const float a = __builtin_amdgcn_exp2f(m - ref);
+      sum = fmaf(states[w][1][row], a, sum);
+      const float4 v = *reinterpret_cast<const float4*>(
+          reinterpret_cast<const float*>(lds + w * S::kWaveBytes) + row * S::kStateLd + dim);
+      t[0] = fmaf(v.x, a, t[0]); t[1] = fmaf(v.y, a, t[1]);
+      t[2] = fmaf(v.z, a, t[2]); t[3] = fmaf(v.w, a, t[3]);
+    }
+    if (part) {
+      if (dim == 0)
+        *reinterpret_cast<float2*>(p.ws_ml + 2 * (base + row)) = make_float2(top, sum);
+      if (top == -INFINITY) continue;   // the merge takes no value of such a state
+      *reinterpret_cast<float4*>(p.ws_o + (base + row) * D + dim) =
+          make_float4(t[0], t[1], t[2], t[3]);
+      continue;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // no key: 0; NaN stays
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] *= inv;
+    if (p.out_form != kOutPlain)
+      store_split4(static_cast<uint16_t*>(p.out), p.out_form, lo, (kvh * G + row) * D + dim,
+                   p.heads * D, t);
+    else if constexpr (PARTS == 1)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (qrow + row) * D + dim) =
+          make_uint2(pack_bf2(t[0], t[1]), pack_bf2(t[2], t[3]));
+    else
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + (qrow + row) * D + dim) =
+          make_float4(t[0], t[1], t[2], t[3]);
+  }
+}
+
+int launch_token_fp4(const PagedArgs& a, int dtype, int head_dim, unsigned blocks, hipStream_t st) {
+  if (dtype == MDL_DTYPE_F32) {
+    if (head_dim == 64) attn_token_fp4_kernel<64, 3><<<blocks, 256, 0, st>>>(a);
+    else attn_token_fp4_kernel<128, 3><<<blocks, 256, 0, st>>>(a);
+  } else {
+    if (head_dim == 64) attn_token_fp4_kernel<64, 1><<<blocks, 256, 0, st>>>(a);
+    else attn_token_fp4_kernel<128, 1><<<blocks, 256, 0, st>>>(a);
+  }
+  return launch_status();
+}
+
 // sizes that both entries take
 int check_paged(int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, int head_dim,
                 int dtype, int table_width, int page_slots) {
@@ -50,8 +354,23 @@ int check_paged(int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, i
                      table_width * page_slots);
 }
 
-Plan plan_paged(int n_seq, int max_q, int n_heads, int n_kv_heads, int dtype, int slots,
-                int max_parts) {
+constexpr int kTokenFill = 1536;   // blocks of single tokens over 4-bit pages that fill the GPU
+constexpr int kTokenPart = 512;    // keys of a part at least
+
+// Single tokens over 4-bit pages with no more heads to a key / value head than rows of their kernel.
+bool takes_tokens(int page_dtype, int max_q, int n_heads, int n_kv_heads) {
+  return page_dtype == MDL_DTYPE_FP4 && max_q == 1 && n_heads / n_kv_heads <= 16;
+}
+
+Plan plan_paged(int n_seq, int max_q, int n_heads, int n_kv_heads, int dtype, int page_dtype,
+                int slots, int max_parts) {
+  if (takes_tokens(page_dtype, max_q, n_heads, n_kv_heads)) {
+    const int64_t pairs = static_cast<int64_t>(n_seq) * n_kv_heads;
+    int64_t ns = (kTokenFill + pairs - 1) / pairs;
+    const int64_t most = slots / kTokenPart < max_parts ? slots / kTokenPart : max_parts;
+    ns = ns < most ? ns : most;
+    return Plan{false, 1, static_cast<int>(ns < 1 ? 1 : ns)};
+  }
   return plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
                     static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), slots, max_parts,
                     least_part(dtype));
@@ -72,8 +391,8 @@ extern "C" int64_t mdl_attn_paged_workspace_bytes(int n_seq, int tokens, int max
                   page_slots) != MDL_OK ||
       (page_dtype != dtype && page_dtype != MDL_DTYPE_FP4) || n_seq == 0 || max_q == 0)
     return 0;
-  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, dtype, table_width * page_slots,
-                             kMaxParts);
+  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, dtype, page_dtype,
+                             table_width * page_slots, kMaxParts);
   return pl.n_split > 1 ? state_bytes(pl.n_split, static_cast<int64_t>(tokens) * n_heads, head_dim)
                         : 0;
 }
@@ -102,7 +421,7 @@ extern "C" int mdl_attn_paged(const void* q, int dtype, const void* k_pages, con
     return MDL_ERR_ALIGN;
   if (n_seq == 0 || tokens == 0 || max_q == 0) return MDL_OK;
   const int slots = table_width * page_slots;
-  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, dtype, slots,
+  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, dtype, page_dtype, slots,
                              workspace ? kMaxParts : 1);
   const int64_t rows = static_cast<int64_t>(tokens) * n_heads;
   if (pl.n_split > 1 && workspace_bytes < state_bytes(pl.n_split, rows, head_dim))
@@ -129,7 +448,9 @@ extern "C" int mdl_attn_paged(const void* q, int dtype, const void* k_pages, con
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned n = static_cast<unsigned>(blocks);
   int rc;
-  if (dtype == MDL_DTYPE_F32)
+  if (takes_tokens(page_dtype, max_q, n_heads, n_kv_heads))
+    rc = launch_token_fp4(a, dtype, head_dim, n, st);
+  else if (dtype == MDL_DTYPE_F32)
     rc = head_dim == 64 ? launch_source<float, 64>(a, fp4, pl.tall, n, st)
                         : launch_source<float, 128>(a, fp4, pl.tall, n, st);
   else
