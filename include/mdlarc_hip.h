@@ -810,15 +810,18 @@ int64_t mdl_attn_paged_workspace_bytes(int n_seq, int tokens, int max_q, int n_h
  * temperature, top_k, top_p and min_p are device arrays of a number a row; NULL is 1 and no filter.  A
  * temperature of 0 or below (or NaN), a top_k of 1, a top_p of 0 or below and a min_p above 1 give the
  * first of the order, with logprob 0.  NaN logits count as -inf, which is never taken; a row of nothing
- * else gives token 0 and logprob -inf.  Weights are of 64 bits and are summed as multiples of 2^-44 of
- * the largest, so equal calls give equal tokens and no order of the sums moves one.
+ * else gives token 0 and logprob -inf.  Weights are of 64 bits and their sums do not depend on an order,
+ * so equal calls give equal tokens; tokens below 2^-43 of the largest may count as nothing.
+ * workspace (8-byte aligned): mdl_sample_workspace_bytes of the same sizes, 0 up to 4,096 tokens; calls
+ * that may overlap in time need workspaces of their own.
  * Replaces: the temperature / top-k branch of generate_output (src/inference.py:573-583) with the
  *           random number as an input, so a sampled step can be captured and repeated.
  */
 int mdl_sample_tokens(const void* logits, int dtype, int64_t ld, int rows, int vocab,
                       const float* uniform, const float* temperature, const int32_t* top_k,
                       const float* top_p, const float* min_p, int64_t* token_out,
-                      float* logprob_out, void* stream);
+                      float* logprob_out, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t mdl_sample_workspace_bytes(int rows, int vocab);
 
 /*
  * Every layer of a prompt or decode step from one call (host code over the entries above, which

@@ -156,7 +156,9 @@ SIGNATURES: dict[str, tuple[object, list]] = {
                                c_int, c_int, c_int, c_int, c_int, P, P, c_int, P, c_int, P, c_int64,
                                P]),
     "mdl_attn_paged_workspace_bytes": (c_int64, [c_int] * 10),
-    "mdl_sample_tokens": (c_int, [P, c_int, c_int64, c_int, c_int, P, P, P, P, P, P, P, P]),
+    "mdl_sample_tokens": (c_int, [P, c_int, c_int64, c_int, c_int, P, P, P, P, P, P, P, P, c_int64,
+                                  P]),
+    "mdl_sample_workspace_bytes": (c_int64, [c_int, c_int]),
     "mdl_lm_head": (c_int, [P, P, c_int, c_int, P, c_float, P, c_int, P, P, CONS, c_int, P]),
     "mdl_decode_head": (c_int, [P, c_int, c_int, P, c_float, P, c_int, P, P, P, c_int64, c_int,
                                 P, P, c_int, c_int, CONS, c_int, P]),

@@ -10,6 +10,8 @@
 // registers one tile ahead, two conversions of four values to an instruction write bf16 (or fp32)
 // values into the ring, and everything behind it is K8's.  The conversions are exact: a code times a
 // power is a bf16 number.
+#include <algorithm>
+
 #include "attn_tiles.h"
 #include "lds_dma.h"
 
@@ -62,30 +64,47 @@ struct TokenShape {
   static constexpr int kWords = kBytes / 4;
   static constexpr int kAhead = 2;                     // tiles in flight
   static constexpr int kWaves = 4;
+  static constexpr int kTurn = kTile * kWaves;
   static constexpr int kLd = D + 8;                    // bf16 elements of a row of V in LDS
   static constexpr int kStateLd = D + 4;               // floats of a row of a wave's state
   static constexpr int kWaveBytes =
       kTile * kLd * 2 > 16 * kStateLd * 4 ? kTile * kLd * 2 : 16 * kStateLd * 4;
 };
 
+// The bytes at base + off + at: base and off are the same for the wave, so the load takes their sum from
+// scalar registers (the empty assembly keeps it there) and a lane's 32-bit offset.
+template <typename T>
+__device__ __forceinline__ T load_at(const void* base, int64_t off, uint32_t at) {
+  uint64_t a = reinterpret_cast<uint64_t>(base) + off;
+  asm volatile("" : "+s"(a));
+  return __builtin_nontemporal_load(
+      (const __attribute__((address_space(1))) T*)((const __attribute__((address_space(1))) uint8_t*)a + at));
+}
+
 template <int D, int PARTS>
 __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel(const PagedArgs p) {
   using S = TokenShape<D>;
-  constexpr int KT = S::kTile, NB = S::kBlocks, W = S::kWords, DB = D / 16, kTurn = KT * S::kWaves;
+  constexpr int KT = S::kTile, NB = S::kBlocks, W = S::kWords, DB = D / 16, kTurn = S::kTurn;
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::kWaves * S::kWaveBytes];
   __shared__ float states[S::kWaves][2][16];
   const int block = blockIdx.x;
   const int pairs = p.n_seq * p.kv_heads;
   const int split = quotient(block, p.by_pairs), pair = block - split * pairs;
   const int seq = quotient(pair, p.by_kv), kvh = pair - seq * p.kv_heads;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Uncut keys: the numbers of the first pages on their way before the lengths are known.  A block's
+  // chain of reads is much of its life where each has a few tiles.
+  int early = 0;
+  const int early0 = quotient(KT * wave, p.by_page);
+  if (p.n_split == 1 && p.slots > 0)
+    early = p.table[seq * p.table_ld + min(early0 + lane, quotient(p.slots - 1, p.by_page))];
   const int lo = min(max(p.q_offset[seq], 0), p.tokens);
   if (min(max(p.q_offset[seq + 1], lo), p.tokens) == lo) return;
   const int G = p.group;
   const int kend = min(max(p.kv_len[seq], 0), p.slots);
   const int per = ((kend + p.n_split - 1) / p.n_split + kTurn - 1) / kTurn * kTurn;
   const int k0 = min(split * per, kend), k1 = min(k0 + per, kend);
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t qrow = static_cast<int64_t>(lo) * p.heads + kvh * G;
 
   // q of row c (rows past G: the last one's), dims g D / 4 + 8 s .. + 7 of step s
@@ -111,16 +130,24 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
     }
   }
 
-  // the numbers of 64 pages from `page0` on, one a lane (as in attn_tiles.h)
-  int page0 = 0, page_no = 0;
+  // The pool's rows at which 64 pages from `page0` on begin, one a lane; a page number outside the
+  // pool as in attn_tiles.h
+  int page0 = 0;
+  uint32_t row_lo = 0, row_hi = 0;
   bool astray = false;
-  auto load_pages = [&](int page) {
+  auto take_pages = [&](int page, int no) {
     page0 = page;
-    const int last = quotient(kend - 1, p.by_page);
-    page_no = p.table[seq * p.table_ld + min(page + lane, last)];
-    const bool bad = page_no < 0 || page_no >= p.n_pages;
+    const bool used = page + lane <= quotient(kend - 1, p.by_page);
+    const bool bad = used && (no < 0 || no >= p.n_pages);
     astray = astray || __ballot(bad) != 0;
-    page_no = bad ? 0 : page_no;
+    const uint64_t row =
+        (static_cast<uint64_t>(used && !bad ? no : 0) * p.kv_heads + kvh) * p.page_slots;
+    row_lo = static_cast<uint32_t>(row);
+    row_hi = static_cast<uint32_t>(row >> 32);
+  };
+  auto load_pages = [&](int page) {
+    const int last = quotient(kend - 1, p.by_page);
+    take_pages(page, p.table[seq * p.table_ld + min(page + lane, last)]);
   };
   struct Tile {
     uint32_t k[NB][W], v[NB][W], kp[NB], vp[NB];
@@ -130,31 +157,40 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
   const uint32_t k_at = c * (D / 2) + g * S::kBytes, v_at = lane * S::kBytes;
   const uint32_t kp_at = c * (D / 32) + g * (D / 4) / 32;
   const uint32_t vp_at = (lane >> 2) * (D / 32) + (lane & 3) * (D / 4) / 32;
-  auto piece = [&](const uint8_t* from, uint32_t (&t)[W]) {
+  auto piece = [&](const void* base, int64_t off, uint32_t at, uint32_t (&t)[W]) {
     if constexpr (W == 4) {
-      const uint4 u = load_nt16(from);
+      const u32x4_t u = load_at<u32x4_t>(base, off, at);
       t[0] = u.x; t[1] = u.y; t[2] = u.z; t[3] = u.w;
     } else {
-      const u32x2_t u = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(from));
+      const u32x2_t u = load_at<u32x2_t>(base, off, at);
       t[0] = u.x; t[1] = u.y;
     }
   };
   auto fetch = [&](Tile& t, int kt) {
+    const int last_key = (kend - 1) & ~15;
+    const int page_a = quotient(min(kt, last_key), p.by_page);
+    const int page_b = quotient(min(kt + KT - 16, last_key), p.by_page);
+    if (page_a < page0 || page_b >= page0 + kWave) load_pages(page_a);
+    // 32-bit offsets to the loads: the compiler otherwise widens them outside the loop
+    uint32_t ka = k_at, va = v_at, kpa = kp_at, vpa = vp_at;
+    asm volatile("" : "+v"(ka), "+v"(va), "+v"(kpa), "+v"(vpa));
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int key = min(kt + 16 * b, (kend - 1) & ~15);
+      const int key = min(kt + 16 * b, last_key);
       const int page = quotient(key, p.by_page);
-      if (static_cast<uint32_t>(page - page0) >= kWave) load_pages(page);
-      const int64_t no = __builtin_amdgcn_readlane(page_no, page - page0);
-      const int64_t row = (no * p.kv_heads + kvh) * p.page_slots + key - page * p.page_slots;
-      piece(static_cast<const uint8_t*>(p.k) + row * (D / 2) + k_at, t.k[b]);
-      piece(static_cast<const uint8_t*>(p.v) + row * (D / 2) + v_at, t.v[b]);
-      t.kp[b] = (p.k_scale + row * (D / 32))[kp_at];
-      t.vp[b] = (p.v_scale + row * (D / 32))[vp_at];
+      const uint32_t lo32 = __builtin_amdgcn_readlane(row_lo, page - page0);
+      const uint32_t hi32 = __builtin_amdgcn_readlane(row_hi, page - page0);
+      const int64_t row = static_cast<int64_t>(static_cast<uint64_t>(hi32) << 32 | lo32) + key -
+                          page * p.page_slots;
+      piece(p.k, row * (D / 2), ka, t.k[b]);
+      piece(p.v, row * (D / 2), va, t.v[b]);
+      t.kp[b] = load_at<uint8_t>(p.k_scale, row * (D / 32), kpa);
+      t.vp[b] = load_at<uint8_t>(p.v_scale, row * (D / 32), vpa);
     }
   };
 
   float negm = 0.f, thr = -INFINITY, l = 0.f;   // l: of this lane's keys
+  f32x4_t start = {0.f, 0.f, 0.f, 0.f};         // negm in every element
   f32x4_t o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -165,7 +201,6 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
     f32x4_t sc[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      sc[b] = f32x4_t{negm, negm, negm, negm};
       const float power = __uint_as_float(t.kp[b] << 23);
 #pragma unroll
       for (int s = 0; s < W; ++s) {
@@ -174,25 +209,37 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
         const bf16x8_t a = as_bf16x8(make_uint4(u[0], u[1], u[2], u[3]));
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
-          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[i][s], sc[b], 0, 0, 0);
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[i][s],
+                                                          s + i == 0 ? start : sc[b], 0, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);   // one block's values in registers at a time
     }
+    if (!whole) {   // no values behind the keys
+      int x = k1 - kt - (lane >> 2);
+      asm volatile("" : "+v"(x));   // keeps this a branch
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        if (16 * b >= x) {
+          t.vp[b] = 127;
+#pragma unroll
+          for (int s = 0; s < W; ++s) t.v[b][s] = 0;
+        }
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const bool there = whole || kt + 16 * b + (lane >> 2) < k1;
-      const float power = there ? __uint_as_float(t.vp[b] << 23) : 1.f;
+      const float power = __uint_as_float(t.vp[b] << 23);
 #pragma unroll
       for (int s = 0; s < W; ++s) {
         uint32_t u[8];
-        fp4_values<uint16_t>(there ? t.v[b][s] : 0u, power, u);
+        fp4_values<uint16_t>(t.v[b][s], power, u);
         *reinterpret_cast<uint4*>(vt + (16 * b + (lane >> 2)) * S::kLd + (lane & 3) * (D / 4) +
                                   8 * s) = make_uint4(u[0], u[1], u[2], u[3]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     if (!whole) {
-      const int x = k1 - kt - 4 * g;   // keys of the tile, from this lane's first
+      int x = k1 - kt - 4 * g;   // keys of the tile, from this lane's first
+      asm volatile("" : "+v"(x));
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -210,6 +257,7 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
         const bool fresh = thr == -INFINITY;
         const float alpha = fresh ? 0.f : __builtin_amdgcn_exp2f(-tmax);
         negm = fresh ? -tmax : negm - tmax;
+        start = f32x4_t{negm, negm, negm, negm};
         thr = kGap;
 #pragma unroll
         for (int b = 0; b < NB; ++b) sc[b] -= tmax;
@@ -263,7 +311,10 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
   const int first = k0 + KT * wave;
   const int nt = first < k1 ? (k1 - first + kTurn - 1) / kTurn : 0;
   if (nt > 0) {
-    load_pages(quotient(first, p.by_page));
+    if (p.n_split == 1)
+      take_pages(early0, early);
+    else
+      load_pages(quotient(first, p.by_page));
 #pragma unroll
     for (int j = 0; j < S::kAhead; ++j) fetch(tiles[j], first + min(j, nt - 1) * kTurn);
     for (int i = 0; i < nt; i += S::kAhead) {   // a tile past the last one has no keys
@@ -354,22 +405,26 @@ int check_paged(int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, i
                      table_width * page_slots);
 }
 
-constexpr int kTokenFill = 1536;   // blocks of single tokens over 4-bit pages that fill the GPU
-constexpr int kTokenPart = 512;    // keys of a part at least
-
 // Single tokens over 4-bit pages with no more heads to a key / value head than rows of their kernel.
 bool takes_tokens(int page_dtype, int max_q, int n_heads, int n_kv_heads) {
   return page_dtype == MDL_DTYPE_FP4 && max_q == 1 && n_heads / n_kv_heads <= 16;
 }
 
-Plan plan_paged(int n_seq, int max_q, int n_heads, int n_kv_heads, int dtype, int page_dtype,
-                int slots, int max_parts) {
+Plan plan_paged(int n_seq, int max_q, int n_heads, int n_kv_heads, int head_dim, int dtype,
+                int page_dtype, int slots, int max_parts) {
   if (takes_tokens(page_dtype, max_q, n_heads, n_kv_heads)) {
+    // Parts of the keys, which a second launch joins (some 3 us): to two blocks a CU, if the keys are
+    // worth three parts of two turns of the block's waves at least; to eight a CU in parts of 2,048
+    // keys or more.  us, so / in more or fewer parts: 64 rows of 32,750 keys (32 heads on 8 of 128) in
+    // 4 286 / in 2 335 / in 6 285; 64 of 2,000 uncut 26 / in 3 33; 4 of 2,000 in 7 8.5 / uncut 16; 16
+    // of 811 (12 heads on 4 of 64) uncut 7.7 / in 3 8.6; 16 of 20,000 (12 heads of 64) in 9 58 / in 6
+    // 63 / in 32 65.
     const int64_t pairs = static_cast<int64_t>(n_seq) * n_kv_heads;
-    int64_t ns = (kTokenFill + pairs - 1) / pairs;
-    const int64_t most = slots / kTokenPart < max_parts ? slots / kTokenPart : max_parts;
-    ns = ns < most ? ns : most;
-    return Plan{false, 1, static_cast<int>(ns < 1 ? 1 : ns)};
+    const int turn = head_dim == 128 ? TokenShape<128>::kTurn : TokenShape<64>::kTurn;
+    const int64_t few = slots / (2 * turn), many = slots / 2048;
+    int64_t ns = few < 3 ? 1 : std::min<int64_t>((512 + pairs - 1) / pairs, few);
+    ns = std::max(ns, std::min<int64_t>((2048 + pairs - 1) / pairs, many));
+    return Plan{false, 1, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ns, max_parts)))};
   }
   return plan_tiles(static_cast<int64_t>(n_seq) * n_kv_heads,
                     static_cast<int64_t>(max_q) * (n_heads / n_kv_heads), slots, max_parts,
@@ -391,7 +446,7 @@ extern "C" int64_t mdl_attn_paged_workspace_bytes(int n_seq, int tokens, int max
                   page_slots) != MDL_OK ||
       (page_dtype != dtype && page_dtype != MDL_DTYPE_FP4) || n_seq == 0 || max_q == 0)
     return 0;
-  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, dtype, page_dtype,
+  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, head_dim, dtype, page_dtype,
                              table_width * page_slots, kMaxParts);
   return pl.n_split > 1 ? state_bytes(pl.n_split, static_cast<int64_t>(tokens) * n_heads, head_dim)
                         : 0;
@@ -421,7 +476,7 @@ extern "C" int mdl_attn_paged(const void* q, int dtype, const void* k_pages, con
     return MDL_ERR_ALIGN;
   if (n_seq == 0 || tokens == 0 || max_q == 0) return MDL_OK;
   const int slots = table_width * page_slots;
-  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, dtype, page_dtype, slots,
+  const Plan pl = plan_paged(n_seq, max_q, n_heads, n_kv_heads, head_dim, dtype, page_dtype, slots,
                              workspace ? kMaxParts : 1);
   const int64_t rows = static_cast<int64_t>(tokens) * n_heads;
   if (pl.n_split > 1 && workspace_bytes < state_bytes(pl.n_split, rows, head_dim))

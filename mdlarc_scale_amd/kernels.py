@@ -1509,15 +1509,24 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
 # --- sampling (K11) ------------------------------------------------------------------------------
 
+SAMPLE_LIST = 4096   # tokens of a row that need no workspace
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    """Bytes of ``sample_tokens``'s workspace (0 up to 4,096 tokens: none is used)."""
+    return _lib.lib().mdl_sample_workspace_bytes(min(rows, C_INT_MAX), min(vocab, C_INT_MAX))
+
+
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, token_out: torch.Tensor,
                   temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
                   top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
-                  logprob_out: torch.Tensor | None = None) -> None:
+                  logprob_out: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> None:
     """One token a row (int64 token_out) from logits [rows, vocab] (fp32 or bf16, rows may be strided)
     at the random numbers ``uniform`` [rows] in [0, 1), after temperature, top-k, top-p and min-p (a
     number a row each: fp32, int32, fp32, fp32; None: 1 and no filter), in that order; ``logprob_out``
     (fp32): the log of the token's share of what the filters keep.  A temperature of 0 is greedy.  Ties
-    go to the lowest index; NaN logits count as -inf."""
+    go to the lowest index; NaN logits count as -inf.  ``workspace``: uint8, sample_workspace_bytes;
+    None takes one from torch's allocator where the rows need it."""
     if len(logits.shape) != 2 or not logits.shape[1]:
         raise ValueError(f"logits must be [rows, vocab] (got {tuple(logits.shape)})")
     rows, vocab = logits.shape
@@ -1533,12 +1542,16 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, token_out: torch.
                         (logprob_out, "logprob_out", F32)):
         if t is not None:
             specs.append((t, name, dt, rows))
+    if workspace is not None:
+        specs.append((workspace, "workspace", U8, 0))
     _need_all(dev, specs)
     if rows == 0:
         return
+    if workspace is None and vocab > SAMPLE_LIST:
+        workspace = torch.empty(sample_workspace_bytes(rows, vocab), dtype=U8, device=logits.device)
     _launch(dev, "mdl_sample_tokens", logits.data_ptr(), code, ld, rows, vocab, uniform.data_ptr(),
             _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), token_out.data_ptr(),
-            _ptr(logprob_out))
+            _ptr(logprob_out), _ptr(workspace), 0 if workspace is None else workspace.numel())
 
 
 class HeadConstraints:

@@ -81,6 +81,10 @@ def test_filters(dtype, vocab):
     check(x, u, top_k=k)
     check(x, u, top_p=p)
     check(x, u, min_p=m)
+    check(x, u, temperature=heat, top_k=k, top_p=p, min_p=m)
+    check(x, u, temperature=heat, top_k=k, top_p=p)
+    check(x, u, top_k=k, min_p=5 * m)
+    check(x, u, top_p=p, min_p=5 * m)
     # each filter off in some rows
     k[::3], p[1::3], m[2::3], heat[5::7] = 0, 1.0, 0.0, 0.0
     check(x, u, temperature=heat, top_k=k, top_p=p, min_p=m)

@@ -88,16 +88,26 @@ def test_attention_workspace(L):
 
 
 SA = dict(logits=FAKE, dtype=0, ld=100, rows=4, vocab=100, u=FAKE, t=None, k=None, p=None, m=None,
-          token=FAKE, logprob=None, stream=None)
+          token=FAKE, logprob=None, ws=None, ws_bytes=0, stream=None)
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(logits=None), NULL), (dict(u=None), NULL), (dict(token=None), NULL), (dict(dtype=2), DTYPE),
     (dict(rows=-1), SHAPE), (dict(vocab=0), SHAPE), (dict(ld=99), SHAPE),
     (dict(vocab=2 ** 20 + 1, ld=2 ** 21), SHAPE), (dict(logits=FAKE + 2), ALIGN),
-    (dict(dtype=1, logits=FAKE + 1), ALIGN), (dict(token=FAKE + 4), ALIGN), (dict(k=FAKE + 2), ALIGN)])
+    (dict(dtype=1, logits=FAKE + 1), ALIGN), (dict(token=FAKE + 4), ALIGN), (dict(k=FAKE + 2), ALIGN),
+    (dict(ws=FAKE + 4), ALIGN), (dict(vocab=5000, ld=5000), WORKSPACE),
+    (dict(vocab=5000, ld=5000, ws=FAKE, ws_bytes=100), WORKSPACE),
+    (dict(vocab=5000, ld=5000, ws=FAKE, rows=2 ** 31 - 1), SHAPE)])
 def test_sample_refusals(L, change, code):
     assert L.mdl_sample_tokens(*{**SA, **change}.values()) == code
+
+
+def test_sample_workspace(L):
+    need = L.mdl_sample_workspace_bytes
+    assert need(64, 4096) == need(0, 9000) == need(5, 2 ** 20 + 1) == 0
+    assert need(1, 4097) > 0 and need(64, 2 ** 20) >= 64 * 64 * 8192
+    assert K.sample_workspace_bytes(3, 10 ** 5) == need(3, 10 ** 5)
 
 
 def test_empty_calls_have_nothing_to_do(L):
