@@ -16,14 +16,17 @@
 //
 // Three sizes of rows:
 //   up to 64 tokens: a wave a row, a token a lane; the order comes from comparing every pair;
-//   up to 4,096: a block a row, all tokens sorted in LDS;
-//   longer: a row in parts of up to 16,384 tokens.  One launch finds each part's largest value and
-//   counts and sums its weights in 1,024 bins of 1/16 octave (on a grid that does not depend on the
-//   part, so the bins of parts add up; in a bin a weight is its top times 2^-f/16, a short
-//   polynomial).  A second launch, a block a row, finds from the bins which of them the filters reach
-//   into.  If those and the ones before hold up to 4,096 tokens, it reads the row once more, sorts them
-//   and is done; otherwise it looks for the border in its bin alone, takes the parts' kept sums from
-//   their bins and reads the tokens of the part that holds the result.
+//   up to 4,096: a block a row, its tokens in LDS;
+//   longer: a row in parts of up to 16,384 tokens, whose bins (below) a first launch makes; a second,
+//   a block a row, adds them up and reads the row once more for the tokens in bins up to the last that
+//   is kept, up to 4,096 of them, to LDS.
+// Counts and sums of weights in 1,024 bins of 1/16 octave say which bins the filters reach into.  (The
+// bins lie on a grid that does not depend on the part, so those of parts add up; in a bin a weight is
+// its top times 2^(-f / 16), a short polynomial.)  Inside such a bin tokens are compared pair by pair, or
+// sorted where they are many.  The kept weights are then summed by stretches of indexes, and the tokens
+// of the stretch that holds the result compared by index.  Where more than 4,096 tokens are kept the
+// row's second launch looks for the borders in their bins alone, cut by the digits of value and index
+// where thousands are equal, and takes the parts' kept sums from their bins.
 //
 #include <cfloat>
 
@@ -211,7 +214,7 @@ struct Stretch {
 #pragma unroll
       for (int e = 0; e < kEach; ++e) f(v[e], head + c * kEach + e);
     };
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;
     int c = t;
     for (; c + (kAhead - 1) * kThreads < pieces; c += kAhead * kThreads) {
       uint4 u[kAhead];
@@ -267,72 +270,287 @@ __device__ __forceinline__ void sort_list(u64* list, int n) {
   __syncthreads();
 }
 
-struct ListLds {
-  u64 list[kList];
-  u64 part[kWaves];
-  int n, kept, found;
+constexpr int kBins = 1024;            // one a thread
+constexpr double kBinsOctave = 16.0;
+static_assert(kBins == kThreads, "a bin a thread");
+
+// The row's bins: 1/16 octave each, bin 0 with the largest value; kBins for values below all of them.
+// A logit lies at -x times the scale, in bins; `base` is where bin 0 begins.
+struct Grid {
+  double scale, at_top, base;
+  bool huge;      // the largest value is infinite: it alone has a weight, in bin 0
+
+  __device__ __forceinline__ Grid(float top, double c) : scale(c * kBinsOctave) {
+    huge = top == INFINITY;
+    at_top = huge ? 0.0 : at(top);
+    base = floor(at_top);
+  }
+  __device__ __forceinline__ double at(float x) const { return -static_cast<double>(x) * scale; }
+  __device__ __forceinline__ int bin(float x) const {
+    if (huge) return x == INFINITY ? 0 : kBins;
+    const double d = floor(at(x)) - base;
+    return d < kBins ? static_cast<int>(d) : kBins;
+  }
+  // a bound below every value in bins up to `last` (a few roundings of fp32 lower)
+  __device__ __forceinline__ float least(int last) const {
+    if (huge) return INFINITY;
+    const double x = -(base + last + 1) / scale;
+    return static_cast<float>(x - fabs(x) * 0x1p-20);
+  }
 };
 
-// The token of a row whose first n <= kList tokens of the order (all that the filters can keep) are
-// in s.list, as places in any order.  `cut`: top-k keeps fewer than there are.  `sum`: of the weights
-// that top-k keeps, 0 where they are all in the list.
-__device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, const Filters& f, int row,
-                                            int n, float top, bool cut, u64 sum) {
+// What a token adds to its bin: a count in the upper 16 bits, and the weight over that of the bin's
+// top, 2^(-f / 16) with 0 <= f < 1, to the nearest 2^-33.
+__device__ __forceinline__ u64 bin_entry(double f) {
+  const double y = f * (-0.69314718055994530942 / kBinsOctave);
+  double w = 1.0 / 720;          // e^y for -0.044 < y <= 0: y^7 / 5040 is below 2^-43
+  w = fma(w, y, 1.0 / 120);
+  w = fma(w, y, 1.0 / 24);
+  w = fma(w, y, 1.0 / 6);
+  w = fma(w, y, 0.5);
+  w = fma(w, y, 1.0);
+  w = fma(w, y, 1.0);
+  return (u64{1} << 48) + __builtin_bit_cast(u64, w + 524288.0) -
+         __builtin_bit_cast(u64, 524288.0);
+}
+
+constexpr u64 kEntrySum = (u64{1} << 48) - 1;
+
+__device__ __forceinline__ void add_to_bins(u64* bins, const Grid& g, float x) {
+  if (!(x > -INFINITY)) return;
+  if (g.huge) {
+    if (x == INFINITY) atomicAdd(&bins[0], bin_entry(0.0));
+    return;
+  }
+  const double q = g.at(x), b = floor(q);
+  if (b - g.base < kBins) atomicAdd(&bins[static_cast<int>(b - g.base)], bin_entry(q - b));
+}
+
+// The sum of weights of bin `bin` with the entries' sum `e`, in multiples of 2^-43; scale: the weight of
+// the bin's top.
+__device__ __forceinline__ u64 bin_sum(u64 e, double scale) {
+  return static_cast<u64>(static_cast<double>(e & kEntrySum) * scale * 0x1p10 + 0.5);
+}
+
+__device__ __forceinline__ double bin_scale(const Grid& g, int bin) {
+  return exp2((g.at_top - g.base - bin) * (1.0 / kBinsOctave));
+}
+
+struct Border {
+  u64 last;    // the place of the last token that is kept
+  u64 sum;     // of the weights up to it
+};
+
+struct ListLds {
+  u64 list[kList];
+  u64 few[kThreads], few_sum[kThreads];
+  u64 part[kWaves];
+  u64 last, sum;
+  int n, found, bin_k, bin_p, upto;
+};
+
+constexpr int kCompared = 192;   // tokens of a bin that are compared pair by pair, more are sorted
+
+// What each filter makes of the bins: those that the filters reach into (kBins: none), and the thread's
+// bin.
+struct Bins {
+  u64 count, sum;                  // of the thread's bin
+  u64 count_before, sum_before;    // of the bins before it
+  u64 total;
+  bool cut, by_p, by_m;            // top-k keeps fewer than there are; top-p; min-p
+  int bin_k, bin_p, bin_m, last;
+
+  // the bin in which the sum reaches `goal`, at most the sum of all; a call of all threads
+  __device__ __forceinline__ int by_sum(ListLds& s, u64 goal) const {
+    __syncthreads();
+    if (sum_before < goal && sum_before + sum >= goal) s.bin_p = threadIdx.x;
+    __syncthreads();
+    return s.bin_p;
+  }
+
+  __device__ __forceinline__ Bins(ListLds& s, const Filters& f, const Grid& g, u64 n, u64 m)
+      : count(n), sum(m) {
+    u64 tokens;
+    count_before = block_scan(count, s.part, tokens);
+    sum_before = block_scan(sum, s.part, total);
+    cut = f.top_k > 0 && tokens > static_cast<u64>(f.top_k);
+    by_p = f.top_p < 1.0;
+    by_m = f.min_p > 0.0;
+    // the first bin with weights below min_p, but for roundings: a bin more is looked at either side
+    const double low = by_m ? g.at_top - g.base - kBinsOctave * log2(f.min_p) : kBins;
+    bin_m = low < kBins ? static_cast<int>(low) : kBins;
+    bin_k = bin_p = kBins;
+    if (cut) {
+      if (count_before < static_cast<u64>(f.top_k) &&
+          count_before + count >= static_cast<u64>(f.top_k))
+        s.bin_k = threadIdx.x;
+      __syncthreads();
+      bin_k = s.bin_k;
+    } else if (by_p) {
+      bin_p = by_sum(s, share_of(f.top_p, total));
+    }
+    // everything that is kept is in bins up to `last`, and so is what top-p's share is of: all that
+    // top-k keeps, or the total
+    last = cut && by_p ? bin_k : min(min(bin_k, bin_p), min(bin_m + 1, kBins - 1));
+    if (threadIdx.x == last) s.upto = static_cast<int>(count_before + count);
+    __syncthreads();
+  }
+};
+
+// The last token of a sorted list of n before which there is less than `goal`, tokens (by_count) or
+// sums; c and m lie before the list.
+__device__ __forceinline__ Border border_sorted(ListLds& s, const u64* list, int n, float top,
+                                                const Filters& f, bool by_count, u64 c, u64 m,
+                                                u64 goal) {
   const int t = threadIdx.x;
-  sort_list(s.list, n);
-  u64 w[kEachList], mine = 0;
+  u64 w[kEachList], mine = 0, all;
 #pragma unroll
   for (int e = 0; e < kEachList; ++e) {
     const int i = kEachList * t + e;
-    w[e] = i < n && (!cut || i < f.top_k) ? fixed(weight(value_at(s.list[i]), top, f.c)) : 0;
+    w[e] = i < n ? fixed(weight(value_at(list[i]), top, f.c)) : 0;
     mine += w[e];
     __builtin_amdgcn_sched_barrier(0);
   }
-  u64 all;
-  u64 before = block_scan(mine, s.part, all);
-  const u64 goal = f.top_p < 1.0 ? share_of(f.top_p, sum ? sum : all) : ~u64{0};
-  if (t == 0) s.kept = 1;
-  __syncthreads();
-  int kept = 0;   // the tokens of the thread that stay: each filter keeps a run from the first on
+  if (t == 0) s.found = 0;
+  const u64 first = m + block_scan(mine, s.part, all);
+  u64 before = first;
+  int found = 0;
 #pragma unroll
   for (int e = 0; e < kEachList; ++e) {
     const int i = kEachList * t + e;
-    if (w[e] != 0 && before < goal && weight(value_at(s.list[min(i, n - 1)]), top, f.c) >= f.min_p)
-      kept = i + 1;
+    if (i < n && (by_count ? c + i : before) < goal) found = i;
     before += w[e];
+  }
+  if (found > 0) atomicMax(&s.found, found);
+  __syncthreads();
+  before = first;
+#pragma unroll
+  for (int e = 0; e < kEachList; ++e) {
+    before += w[e];
+    if (kEachList * t + e == s.found) {
+      s.last = list[s.found];
+      s.sum = before;
+    }
+  }
+  __syncthreads();
+  return Border{s.last, s.sum};
+}
+
+// The token of a row whose tokens in bins up to b.last, n <= kList of them, are in s.list as places in
+// any order.
+__device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, const Filters& f, int row,
+                                            int n, float top, const Grid& g, const Bins& b) {
+  const int t = threadIdx.x;
+  u64 mine[kEachList];
+  int bin[kEachList];
+#pragma unroll
+  for (int e = 0; e < kEachList; ++e) {
+    const int i = t + e * kThreads;
+    mine[e] = i < n ? s.list[i] : ~u64{0};
+    bin[e] = i < n ? g.bin(value_at(mine[e])) : kBins;
+  }
+  // the border in bin `at`
+  auto border_in = [&](int at, bool by_count, u64 goal) {
+    __syncthreads();
+    if (t == at) {
+      s.sum = b.sum_before;
+      s.last = b.count_before;
+      s.upto = static_cast<int>(b.count);
+    }
+    if (t == 0) s.n = 0;
+    __syncthreads();
+    const u64 c = s.last, m = s.sum;
+    if (s.upto > kThreads) {   // thousands of tokens in a bin: the whole list in order
+      sort_list(s.list, n);
+      return border_sorted(s, s.list, n, top, f, by_count, 0, 0, goal);
+    }
+#pragma unroll
+    for (int e = 0; e < kEachList; ++e)
+      if (bin[e] == at) {
+        const int i = atomicAdd(&s.n, 1);
+        s.few[i] = mine[e];
+        s.few_sum[i] = fixed(weight(value_at(mine[e]), top, f.c));
+      }
+    __syncthreads();
+    const int some = s.n;
+    if (some > kCompared) {
+      sort_list(s.few, some);
+      return border_sorted(s, s.few, some, top, f, by_count, c, m, goal);
+    }
+    if (t == 0) s.found = 0;
+    u64 rank = 0, before = 0, my = 0;
+    if (t < some) {
+      my = s.few[t];
+      for (int j = 0; j < some; ++j) {
+        const bool ahead = s.few[j] < my;
+        rank += ahead;
+        before += ahead ? s.few_sum[j] : 0;
+      }
+    }
+    __syncthreads();
+    if (t < some && (by_count ? c + rank : m + before) < goal)
+      atomicMax(&s.found, static_cast<int>(rank));
+    __syncthreads();
+    if (t < some && static_cast<int>(rank) == s.found) {
+      s.last = my;
+      s.sum = m + before + s.few_sum[t];
+    }
+    __syncthreads();
+    return Border{s.last, s.sum};
+  };
+  // (a border past the last bin of the list is past what min-p keeps)
+  Border border{~u64{0}, b.total};
+  if (b.cut && b.bin_k <= b.last) border = border_in(b.bin_k, true, f.top_k);
+  if (b.by_p) {
+    const u64 goal = share_of(f.top_p, border.sum);
+    const int at = b.cut ? b.by_sum(s, goal) : b.bin_p;
+    if (at <= b.last) {
+      const Border other = border_in(at, false, goal);
+      if (other.last < border.last) border = other;
+    }
+  }
+  // sums of the kept tokens by stretches of indexes, a thread each; then the tokens of one stretch
+  const int stretch = (p.vocab + kThreads - 1) / kThreads;
+  __syncthreads();
+  s.few_sum[t] = 0;
+  if (t == 0) s.n = 0;
+  __syncthreads();
+  u64 w[kEachList];
+#pragma unroll
+  for (int e = 0; e < kEachList; ++e) {
+    const bool there = bin[e] <= b.last && mine[e] <= border.last;
+    const double x = there ? weight(value_at(mine[e]), top, f.c) : 0.0;
+    w[e] = x >= f.min_p ? fixed(x) : 0;
+    if (w[e] != 0) atomicAdd(&s.few_sum[static_cast<uint32_t>(mine[e]) / stretch], w[e]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  if (kept > 0) atomicMax(&s.kept, kept);
   __syncthreads();
-  // the kept ones by index: index above, value below
-  n = s.kept;
-  u64 v[kEachList];
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) v[e] = s.list[min(t + e * kThreads, n - 1)];
+  const u64 here = s.few_sum[t];
+  u64 total;
+  const u64 ahead = block_scan(here, s.part, total);
+  const u64 goal = target_of(p.uniform[row], total);
+  if (ahead <= goal && goal < ahead + here) {   // one thread
+    s.found = t;
+    s.sum = ahead;
+  }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < kEachList; ++e)
-    if (t + e * kThreads < n)
-      s.list[t + e * kThreads] = v[e] << 32 | __float_as_uint(value_at(v[e]));
-  sort_list(s.list, n);
-  mine = 0;
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    const int i = kEachList * t + e;
-    w[e] = i < n ? fixed(weight(__uint_as_float(static_cast<uint32_t>(s.list[i])), top, f.c)) : 0;
-    mine += w[e];
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  before = block_scan(mine, s.part, all);
-  const u64 at = target_of(p.uniform[row], all);
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    if (before <= at && at < before + w[e]) {
-      const u64 k = s.list[kEachList * t + e];
-      leave(p, row, static_cast<int>(k >> 32),
-            weight(__uint_as_float(static_cast<uint32_t>(k)), top, f.c), all);
+    if (w[e] != 0 && static_cast<int>(static_cast<uint32_t>(mine[e]) / stretch) == s.found)
+      s.list[atomicAdd(&s.n, 1)] = mine[e];
+  __syncthreads();
+  n = s.n;
+  for (int i = t; i < n; i += kThreads) {
+    const u64 my = s.list[i];
+    u64 before = s.sum;
+    for (int j = 0; j < n; ++j) {
+      const u64 o = s.list[j];
+      if (static_cast<uint32_t>(o) < static_cast<uint32_t>(my))
+        before += fixed(weight(value_at(o), top, f.c));
     }
-    before += w[e];
+    const double x = weight(value_at(my), top, f.c);
+    if (before <= goal && goal < before + fixed(x))
+      leave(p, row, static_cast<int>(static_cast<uint32_t>(my)), x, total);
   }
 }
 
@@ -379,60 +597,45 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(const SampleArgs 
   const int row = blockIdx.x, t = threadIdx.x;
   const Filters f = filters_of(p, row);
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-  float top = -INFINITY;
+  float v[kEachList], top = -INFINITY;
   int at = 0x7fffffff;
 #pragma unroll
   for (int e = 0; e < kEachList; ++e) {
     const int i = t + e * kThreads;
-    if (i >= p.vocab) break;
-    float v = logit(x, i);
-    v = v > -INFINITY ? v : -INFINITY;   // no NaN
-    s.list[i] = place(v, i);
-    if (v > top) {
-      top = v;
+    v[e] = i < p.vocab ? logit(x, i) : -INFINITY;
+    v[e] = v[e] > -INFINITY ? v[e] : -INFINITY;   // no NaN
+    if (i < p.vocab) s.list[i] = place(v[e], i);
+    if (v[e] > top) {
+      top = v[e];
       at = i;
     }
   }
+  s.few[t] = 0;
   block_top(top, at, part_top, part_at);
   if (leave_first(p, f, row, top, at)) return;
-  finish_list(s, p, f, row, p.vocab, top, f.top_k > 0 && f.top_k < p.vocab, 0);
+  const Grid g(top, f.c);
+#pragma unroll
+  for (int e = 0; e < kEachList; ++e) {
+    add_to_bins(s.few, g, v[e]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  const u64 entries = s.few[t];
+  const Bins b(s, f, g, entries >> 48, bin_sum(entries, bin_scale(g, t)));
+  finish_list(s, p, f, row, p.vocab, top, g, b);
 }
 
 // ---- a row in parts ----------------------------------------------------------------------------
 
-constexpr int kBins = 1024;            // one a thread
-constexpr double kBinsOctave = 16.0;
 constexpr int kDigit = 10;             // bits of a digit, kBins values
 constexpr int kPart = 16384;           // tokens of a part: their sum stays below 2^48 (bin_entry)
 constexpr int kMaxParts = 64;
-static_assert(kBins == kThreads && kBins == 1 << kDigit, "a bin, and a digit, a thread");
-
-// Where a logit lies on the grid of bins: larger numbers for smaller logits, in bins.
-__device__ __forceinline__ double grid_at(float x, double c) {
-  return -static_cast<double>(x) * (c * kBinsOctave);
-}
-
-// What a token adds to its bin: a count in the upper 16 bits, and the weight over that of the bin's
-// top, 2^(-f / 16) with 0 <= f < 1, to the nearest 2^-33.
-__device__ __forceinline__ u64 bin_entry(double f) {
-  const double y = f * (-0.69314718055994530942 / kBinsOctave);
-  double w = 1.0 / 720;          // e^y for -0.044 < y <= 0: y^7 / 5040 is below 2^-43
-  w = fma(w, y, 1.0 / 120);
-  w = fma(w, y, 1.0 / 24);
-  w = fma(w, y, 1.0 / 6);
-  w = fma(w, y, 0.5);
-  w = fma(w, y, 1.0);
-  w = fma(w, y, 1.0);
-  return (u64{1} << 48) + __builtin_bit_cast(u64, w + 524288.0) -
-         __builtin_bit_cast(u64, 524288.0);
-}
-
-constexpr u64 kEntrySum = (u64{1} << 48) - 1;
+static_assert(kBins == 1 << kDigit, "a digit a thread");
 
 struct Parts {
   u64* bins;      // [rows][parts][kBins]
   float* top;     // [rows][parts] largest value
-  int* at;        // and its index in the row
+  int* at;        // and its index in the row (greedy rows)
   int n, size;    // parts of a row, tokens of a part
 };
 
@@ -447,52 +650,75 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
                      min(parts.size, p.vocab - first));
   const Filters f = filters_of(p, row);
   bins[t] = 0;
-  float top = -INFINITY;
-  int at = 0x7fffffff;
-  x.each([&](float v, int i) {
-    if (v > top || (v == top && i < at)) {
-      top = v;
-      at = i;
+  if (f.greedy) {
+    float top = -INFINITY;
+    int at = 0x7fffffff;
+    x.each([&](float v, int i) {
+      if (v > top || (v == top && i < at)) {
+        top = v;
+        at = i;
+      }
+    });
+    block_top(top, at, part_top, part_at);
+    if (t == 0) {
+      parts.top[blockIdx.x] = top;
+      parts.at[blockIdx.x] = first + at;
     }
-  });
+    return;
+  }
+  // the thread's tokens stay in registers between the two passes
+  constexpr int kPieces = kPart / kThreads / Stretch<T>::kEach;
+  uint4 u[kPieces];
+  const uint4* from = reinterpret_cast<const uint4*>(x.x + x.head);
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) {
+    const int c = t + j * kThreads;
+    const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;   // -inf
+    u[j] = c < x.pieces ? from[c] : make_uint4(none, none, none, none);
+  }
+  const int rest = x.head + x.pieces * Stretch<T>::kEach + t;
+  const float v0 = t < x.head ? logit(x.x, t) : -INFINITY;
+  const float v1 = rest < x.n ? logit(x.x, rest) : -INFINITY;
+  float top = fmaxf(fmaxf(v0, v1), -INFINITY);   // fmaxf passes over NaN
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) {
+    float v[Stretch<T>::kEach];
+    x.values(u[j], v);
+#pragma unroll
+    for (int e = 0; e < Stretch<T>::kEach; ++e) top = fmaxf(top, v[e]);
+  }
+  int at = 0;
   block_top(top, at, part_top, part_at);
   if (t == 0) {
     parts.top[blockIdx.x] = top;
-    parts.at[blockIdx.x] = first + at;
+    parts.at[blockIdx.x] = 0;
   }
-  if (top == -INFINITY || f.greedy) return;
-  const bool huge = top == INFINITY;   // then infinite logits alone have a weight
-  const double base = floor(grid_at(top, f.c));
-  x.each([&](float v, int) {
-    if (!(v > -INFINITY)) return;
-    if (huge) {
-      if (v == INFINITY) atomicAdd(&bins[0], bin_entry(0.0));
-      return;
+  if (top == -INFINITY) return;
+  const Grid g(top, f.c);
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) {
+    float v[Stretch<T>::kEach];
+    x.values(u[j], v);
+#pragma unroll
+    for (int e = 0; e < Stretch<T>::kEach; ++e) {
+      add_to_bins(bins, g, v[e]);
+      if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // a few tokens' registers at a time
     }
-    const double q = grid_at(v, f.c), b = floor(q);
-    if (b - base < kBins) atomicAdd(&bins[static_cast<int>(b - base)], bin_entry(q - b));
-  });
+  }
+  add_to_bins(bins, g, v0);
+  add_to_bins(bins, g, v1);
   __syncthreads();
   parts.bins[static_cast<int64_t>(blockIdx.x) * kBins + t] = bins[t];
 }
 
 struct RowLds {
   ListLds l;
-  u64 sum[kBins];            // digits' counts and sums; then sums of the tokens up to a thread's
-  uint32_t count[kBins];
   double scale[kBins];       // weight of a bin's top
   u64 part_sum[kMaxParts];
   int shift[kMaxParts];      // of a part's bins against the row's
   float part_top[kWaves];
   int part_at[kWaves];
-  int bin_k, bin_p, upto;
-  u64 before;
-  uint32_t count_before;
-};
-
-struct Border {
-  u64 last;    // the place of the last token that is kept
-  u64 sum;     // of the weights up to it
+  int digit;
 };
 
 template <typename T>
@@ -509,131 +735,99 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
   int at = t < parts.n ? parts.at[row * parts.n + t] : 0x7fffffff;
   block_top(top, at, s.part_top, s.part_at);
   if (leave_first(p, f, row, top, at)) return;
-  const bool huge = top == INFINITY;
-  const double q_top = huge ? 0.0 : grid_at(top, f.c), base = floor(q_top);
+  const Grid g(top, f.c);
   if (t < parts.n) {
-    const double d = my_top == -INFINITY || (huge && my_top != INFINITY)
-                         ? kBins : huge ? 0.0 : floor(grid_at(my_top, f.c)) - base;
+    const double d = my_top == -INFINITY || (g.huge && my_top != INFINITY)
+                         ? kBins : g.huge ? 0.0 : floor(g.at(my_top)) - g.base;
     s.shift[t] = d < kBins ? static_cast<int>(d) : kBins;
   }
-  // the row's bin of a value above -inf, kBins for those below all bins
-  auto bin_of = [&](float v) {
-    if (huge) return v == INFINITY ? 0 : kBins;
-    const double d = floor(grid_at(v, f.c)) - base;
-    return d < kBins ? static_cast<int>(d) : kBins;
-  };
   const u64* bins = parts.bins + static_cast<int64_t>(row) * parts.n * kBins;
-  s.scale[t] = exp2((q_top - base - t) * (1.0 / kBinsOctave));
+  const double scale = bin_scale(g, t);
+  s.scale[t] = scale;
   __syncthreads();
-  auto bin_sum = [&](u64 entries, int bin) {   // of a bin's weights
-    return static_cast<u64>(static_cast<double>(entries) * s.scale[bin] * 0x1p10 + 0.5);
-  };
-  // this thread's bin, and what lies before it
-  uint32_t count = 0;
-  u64 sum = 0;
+  u64 count = 0, sum = 0;
+#pragma unroll 4
   for (int i = 0; i < parts.n; ++i) {
-    if (t < s.shift[i]) continue;
-    const u64 e = bins[i * kBins + t - s.shift[i]];
-    count += static_cast<uint32_t>(e >> 48);
-    sum += bin_sum(e & kEntrySum, t);
+    const int from = t - s.shift[i];
+    const u64 e = from >= 0 ? bins[i * kBins + from] : 0;
+    count += e >> 48;
+    sum += bin_sum(e, scale);
   }
-  u64 tokens, total;
-  const u64 count_before = block_scan(count, s.l.part, tokens);
-  const u64 sum_before = block_scan(sum, s.l.part, total);
-  const bool cut = f.top_k > 0 && tokens > static_cast<u64>(f.top_k), by_p = f.top_p < 1.0;
-  const bool by_m = f.min_p > 0.0;
-  // the first bin with weights below min_p, but for roundings: a bin more is looked at on either side
-  const double low = by_m ? q_top - base - kBinsOctave * log2(f.min_p) : kBins;
-  const int bin_m = low < kBins ? static_cast<int>(low) : kBins;
-
-  auto by_sum = [&](u64 goal) {          // the bin in which the sum reaches goal; for all threads
+  const Bins b(s.l, f, g, count, sum);
+  if ((b.cut || b.by_p || b.by_m) && s.l.upto <= kList) {
+    const int n = s.l.upto;
+    if (t == 0) s.l.n = 0;
     __syncthreads();
-    if (sum_before < goal && sum_before + sum >= goal) s.bin_p = t;
-    __syncthreads();
-    return s.bin_p;
-  };
-  int bin_k = kBins, bin_p = kBins;
-  if (cut) {
-    if (count_before < static_cast<u64>(f.top_k) && count_before + count >= static_cast<u64>(f.top_k))
-      s.bin_k = t;
-    __syncthreads();
-    bin_k = s.bin_k;
-  } else if (by_p) {
-    bin_p = by_sum(share_of(f.top_p, total));
-  }
-  // everything that is kept is in bins up to `last`, and so is what top-p's share is of: all that top-k
-  // keeps, or the total
-  const int last = cut && by_p ? bin_k : min(min(bin_k, bin_p), min(bin_m + 1, kBins - 1));
-  if (t == last) s.upto = static_cast<int>(count_before + count);
-  if (t == 0) s.l.n = 0;
-  __syncthreads();
-  if ((cut || by_p || by_m) && s.upto <= kList) {
+    const float least = g.least(b.last);
     x.each([&](float v, int i) {
-      if (v > -INFINITY && bin_of(v) <= last) s.l.list[atomicAdd(&s.l.n, 1)] = place(v, i);
+      if (v >= least && g.bin(v) <= b.last) s.l.list[atomicAdd(&s.l.n, 1)] = place(v, i);
     });
-    finish_list(s.l, p, f, row, s.upto, top, cut, cut ? 0 : total);
+    __syncthreads();
+    finish_list(s.l, p, f, row, n, top, g, b);
     return;
   }
 
-  // The border in bin `bin`, before which there are `c` tokens and `m`, and in which there are
-  // `inside`: the last token of the order before which there is less than `goal`, which the bin reaches.
-  auto border_in = [&](int bin, uint32_t c, u64 m, uint32_t inside, bool by_count, u64 goal) {
+  // The border in bin `bin`: the last token of the order before which there is less than `goal`, which
+  // the bin reaches.
+  auto border_in = [&](int bin, bool by_count, u64 goal) {
+    __syncthreads();
+    if (t == bin) {
+      s.l.sum = b.sum_before;
+      s.l.last = b.count_before;
+      s.l.upto = static_cast<int>(b.count);
+    }
+    __syncthreads();
+    u64 c = s.l.last, m = s.l.sum;
+    int inside = s.l.upto;
     u64 prefix = 0;      // the places' upper bits from `shift` on, once digits are taken
     int shift = 64;
+    u64* sums = s.l.few_sum;
+    u64* counts = s.l.few;
     while (inside > kList) {
       const int next = max(shift - kDigit, 0);
       __syncthreads();
-      s.sum[t] = 0;
-      s.count[t] = 0;
+      sums[t] = 0;
+      counts[t] = 0;
       __syncthreads();
       x.each([&](float v, int i) {
-        if (!(v > -INFINITY) || bin_of(v) != bin) return;
+        if (!(v > -INFINITY) || g.bin(v) != bin) return;
         const u64 a = place(v, i);
         if (shift < 64 && a >> shift != prefix) return;
         const int digit = static_cast<int>((a >> next) & ((u64{1} << (shift - next)) - 1));
-        atomicAdd(&s.count[digit], 1u);
-        atomicAdd(&s.sum[digit], fixed(weight(v, top, f.c)));
+        atomicAdd(&counts[digit], u64{1});
+        atomicAdd(&sums[digit], fixed(weight(v, top, f.c)));
       });
+      if (t == 0) s.digit = -1;
       __syncthreads();
       u64 all;
-      const u64 dc = s.count[t], dm = s.sum[t];
+      const u64 dc = counts[t], dm = sums[t];
       const u64 cb = c + block_scan(dc, s.l.part, all), mb = m + block_scan(dm, s.l.part, all);
       const u64 have = by_count ? cb : mb, more = by_count ? dc : dm;
-      if (t == 0) s.bin_k = -1;
-      __syncthreads();
-      if (have < goal && have + more >= goal) {
-        s.bin_k = t;
-        s.before = mb;
-        s.count_before = static_cast<uint32_t>(cb);
-      }
+      if (have < goal && have + more >= goal) s.digit = t;
       __syncthreads();
       // sums of single weights and of bins differ in their last bits: a goal past the last digit is in
       // the last one that has tokens
-      const bool none = s.bin_k < 0;
+      const bool none = s.digit < 0;
       __syncthreads();
-      if (none) {
-        if (dc > 0) atomicMax(&s.bin_k, t);
-        __syncthreads();
-        if (t == s.bin_k) {
-          s.before = mb;
-          s.count_before = static_cast<uint32_t>(cb);
-        }
-        __syncthreads();
+      if (none && dc > 0) atomicMax(&s.digit, t);
+      __syncthreads();
+      if (t == s.digit) {
+        s.l.sum = mb;
+        s.l.last = cb;
+        s.l.upto = static_cast<int>(dc);
       }
-      prefix = prefix << (shift - next) | static_cast<u64>(s.bin_k);
+      __syncthreads();
+      prefix = prefix << (shift - next) | static_cast<u64>(s.digit);
       shift = next;
-      c = s.count_before;
-      m = s.before;
-      inside = s.count[s.bin_k];
+      c = s.l.last;
+      m = s.l.sum;
+      inside = s.l.upto;
     }
     __syncthreads();
-    if (t == 0) {
-      s.l.n = 0;
-      s.l.found = 0;
-    }
+    if (t == 0) s.l.n = 0;
     __syncthreads();
     x.each([&](float v, int i) {
-      if (!(v > -INFINITY) || bin_of(v) != bin) return;
+      if (!(v > -INFINITY) || g.bin(v) != bin) return;
       const u64 a = place(v, i);
       if (shift < 64 && a >> shift != prefix) return;
       s.l.list[atomicAdd(&s.l.n, 1)] = a;
@@ -641,72 +835,32 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     __syncthreads();
     const int n = s.l.n;
     sort_list(s.l.list, n);
-    u64 w[kEachList], mine = 0, all;
-#pragma unroll
-    for (int e = 0; e < kEachList; ++e) {
-      const int i = kEachList * t + e;
-      w[e] = i < n ? fixed(weight(value_at(s.l.list[i]), top, f.c)) : 0;
-      mine += w[e];
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    const u64 first = m + block_scan(mine, s.l.part, all);
-    u64 before = first;
-    int found = 0;
-#pragma unroll
-    for (int e = 0; e < kEachList; ++e) {
-      const int i = kEachList * t + e;
-      if (i < n && (by_count ? static_cast<u64>(c) + i : before) < goal) found = i;
-      before += w[e];
-    }
-    if (found > 0) atomicMax(&s.l.found, found);
-    __syncthreads();
-    before = first;
-#pragma unroll
-    for (int e = 0; e < kEachList; ++e) {
-      before += w[e];
-      if (kEachList * t + e == s.l.found) s.before = before;
-    }
-    __syncthreads();
-    return Border{s.l.list[s.l.found], s.before};
-  };
-  // what lies before bin `bin`, from its thread
-  auto border_at = [&](int bin, bool by_count, u64 goal) {
-    __syncthreads();
-    if (t == bin) {
-      s.count_before = static_cast<uint32_t>(count_before);
-      s.before = sum_before;
-      s.upto = static_cast<int>(count);
-    }
-    __syncthreads();
-    const uint32_t c = s.count_before, inside = s.upto;
-    const u64 m = s.before;
-    __syncthreads();
-    return border_in(bin, c, m, inside, by_count, goal);
+    return border_sorted(s.l, s.l.list, n, top, f, by_count, c, m, goal);
   };
 
-  Border border{~u64{0}, total};
-  int full = by_m ? max(bin_m - 1, 0) : kBins;       // bins that are kept whole
-  if (cut) {
-    border = border_at(bin_k, true, f.top_k);
-    full = min(full, bin_k);
+  Border border{~u64{0}, b.total};
+  int full = b.by_m ? max(b.bin_m - 1, 0) : kBins;   // bins that are kept whole
+  if (b.cut) {
+    border = border_in(b.bin_k, true, f.top_k);
+    full = min(full, b.bin_k);
   }
-  if (by_p) {
+  if (b.by_p) {
     const u64 goal = share_of(f.top_p, border.sum);
-    const int bin = by_sum(goal);
-    const Border b = border_at(bin, false, goal);
-    if (b.last < border.last) border = b;
+    const int bin = b.by_sum(s.l, goal);
+    const Border other = border_in(bin, false, goal);
+    if (other.last < border.last) border = other;
     full = min(full, bin);
   }
   auto kept = [&](float v, int i, double& w) {
-    if (!(v > -INFINITY) || place(v, i) > border.last || bin_of(v) == kBins) return false;
+    if (!(v > -INFINITY) || place(v, i) > border.last || g.bin(v) == kBins) return false;
     w = weight(v, top, f.c);
     return w >= f.min_p;
   };
   // the parts' kept sums: whole bins, then tokens of the others
   for (int i = wave; i < parts.n; i += kWaves) {
     u64 m = 0;
-    for (int b = lane; b < full; b += kWave)
-      if (b >= s.shift[i]) m += bin_sum(bins[i * kBins + b - s.shift[i]] & kEntrySum, b);
+    for (int bin = lane; bin < full; bin += kWave)
+      if (bin >= s.shift[i]) m += bin_sum(bins[i * kBins + bin - s.shift[i]], s.scale[bin]);
     m = wave_sum64(m);
     if (lane == 0) s.part_sum[i] = m;
   }
@@ -714,11 +868,11 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
   if (full < kBins)
     x.each([&](float v, int i) {
       double w;
-      if (v > -INFINITY && bin_of(v) >= full && kept(v, i, w))
+      if (v > -INFINITY && g.bin(v) >= full && kept(v, i, w))
         atomicAdd(&s.part_sum[i / parts.size], fixed(w));
     });
   __syncthreads();
-  total = 0;
+  u64 total = 0;
   for (int i = 0; i < parts.n; ++i) total += s.part_sum[i];
   u64 goal = target_of(p.uniform[row], total);
   int part = 0;
@@ -728,12 +882,16 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
   const double want = static_cast<double>(goal) / kOne;
   const int end = min((part + 1) * parts.size, p.vocab), run = (parts.size + kThreads - 1) / kThreads;
   const int i0 = min(part * parts.size + t * run, end), i1 = min(i0 + run, end);
+  constexpr int kRun = kPart / kThreads;
+  float v[kRun];
+#pragma unroll
+  for (int e = 0; e < kRun; ++e) v[e] = i0 + e < i1 ? logit(logits, i0 + e) : -INFINITY;
   double mine = 0.0;
-#pragma unroll 1
-  for (int i = i0; i < i1; ++i) {
+#pragma unroll
+  for (int e = 0; e < kRun; ++e) {
     double w;
-    const float v = logit(logits, i);
-    if (kept(v, i, w)) mine += w;
+    if (kept(v[e], i0 + e, w)) mine += w;
+    __builtin_amdgcn_sched_barrier(0);
   }
   double upto = mine;
 #pragma unroll
@@ -742,21 +900,21 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     if (lane >= o) upto += d;
   }
   __syncthreads();
-  double* ends = reinterpret_cast<double*>(s.sum);
+  double* ends = reinterpret_cast<double*>(s.l.few_sum);
   ends[t] = upto;
   if (t == 0) {
-    s.bin_k = kThreads;   // the first thread whose tokens pass `want`
-    s.bin_p = -1;         // the last one that has tokens
+    s.l.bin_k = kThreads;   // the first thread whose tokens pass `want`
+    s.l.bin_p = -1;         // the last one that has tokens
   }
   __syncthreads();
   double wave0 = 0.0;
   for (int w = 0; w < wave; ++w) wave0 += ends[kWave * w + kWave - 1];
   if (mine > 0.0) {
-    if (wave0 + upto > want) atomicMin(&s.bin_k, t);
-    atomicMax(&s.bin_p, t);
+    if (wave0 + upto > want) atomicMin(&s.l.bin_k, t);
+    atomicMax(&s.l.bin_p, t);
   }
   __syncthreads();
-  if (t != (s.bin_k < kThreads ? s.bin_k : s.bin_p)) return;
+  if (t != (s.l.bin_k < kThreads ? s.l.bin_k : s.l.bin_p)) return;
   double sums = wave0 + (upto - mine), won = 0.0;
   int token = i0;
 #pragma unroll 1
