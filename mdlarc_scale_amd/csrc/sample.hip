@@ -202,33 +202,41 @@ struct Stretch {
       unpack8(u, v);
     }
   }
-  // f(value, index) for the thread's tokens, in ascending order but for the first and last few
+  // f(value, index) for every token of the block's with least <= value <= most.  The loop over the row
+  // compares and no more: few tokens pass, and f works on them (read again) in a loop of its own, of
+  // which there is one copy.
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each_between(float least, float most, F f) const {
     const int t = threadIdx.x;
-    if (t < head) f(logit(x, t), t);
+    const int rest = head + pieces * kEach + t;
+    constexpr int kAhead = 32 / kEach;
     const uint4* from = reinterpret_cast<const uint4*>(x + head);
-    auto some = [&](uint4 u, int c) {
-      float v[kEach];
-      values(u, v);
+    auto in = [&](float v) { return v >= least && v <= most; };   // not NaN
+    for (int c = t - kAhead * kThreads; c < pieces; c += kAhead * kThreads) {
+      uint32_t hits = 0;
+      if (c < 0) {   // once, before the pieces: the first and last few tokens
+        hits = (t < head && in(logit(x, t)) ? 1u : 0u) | (rest < n && in(logit(x, rest)) ? 2u : 0u);
+      } else {
+        uint4 u[kAhead];
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) f(v[e], head + c * kEach + e);
-    };
-    constexpr int kAhead = 4;
-    int c = t;
-    for (; c + (kAhead - 1) * kThreads < pieces; c += kAhead * kThreads) {
-      uint4 u[kAhead];
+        for (int j = 0; j < kAhead; ++j) u[j] = from[min(c + j * kThreads, pieces - 1)];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) u[j] = from[c + j * kThreads];
+        for (int j = 0; j < kAhead; ++j) {
+          float v[kEach];
+          values(u[j], v);
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        some(u[j], c + j * kThreads);
-        __builtin_amdgcn_sched_barrier(0);   // one piece's registers at a time
+          for (int i = 0; i < kEach; ++i)
+            hits |= in(v[i]) && c + j * kThreads < pieces ? 1u << (j * kEach + i) : 0u;
+        }
+      }
+#pragma unroll 1
+      for (; hits != 0; hits &= hits - 1) {
+        const int b = __ffs(hits) - 1;
+        const int i = c < 0 ? (b == 0 ? t : rest)
+                            : head + (c + b / kEach * kThreads) * kEach + b % kEach;
+        f(logit(x, i), i);
       }
     }
-    for (; c < pieces; c += kThreads) some(from[c], c);
-    const int i = head + pieces * kEach + t;
-    if (i < n) f(logit(x, i), i);
   }
 };
 
@@ -291,11 +299,16 @@ struct Grid {
     const double d = floor(at(x)) - base;
     return d < kBins ? static_cast<int>(d) : kBins;
   }
-  // a bound below every value in bins up to `last` (a few roundings of fp32 lower)
+  // bounds of the values in bins `first` .. `last` (a few roundings of fp32 wider)
   __device__ __forceinline__ float least(int last) const {
     if (huge) return INFINITY;
     const double x = -(base + last + 1) / scale;
     return static_cast<float>(x - fabs(x) * 0x1p-20);
+  }
+  __device__ __forceinline__ float most(int first) const {
+    if (huge || first == 0) return INFINITY;
+    const double x = -(base + first) / scale;
+    return static_cast<float>(x + fabs(x) * 0x1p-20);
   }
 };
 
@@ -650,22 +663,6 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
                      min(parts.size, p.vocab - first));
   const Filters f = filters_of(p, row);
   bins[t] = 0;
-  if (f.greedy) {
-    float top = -INFINITY;
-    int at = 0x7fffffff;
-    x.each([&](float v, int i) {
-      if (v > top || (v == top && i < at)) {
-        top = v;
-        at = i;
-      }
-    });
-    block_top(top, at, part_top, part_at);
-    if (t == 0) {
-      parts.top[blockIdx.x] = top;
-      parts.at[blockIdx.x] = first + at;
-    }
-    return;
-  }
   // the thread's tokens stay in registers between the two passes
   constexpr int kPieces = kPart / kThreads / Stretch<T>::kEach;
   uint4 u[kPieces];
@@ -687,13 +684,25 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
 #pragma unroll
     for (int e = 0; e < Stretch<T>::kEach; ++e) top = fmaxf(top, v[e]);
   }
-  int at = 0;
+  int at = 0x7fffffff;
+  if (f.greedy) {   // the first of the largest
+    if (v1 == top) at = rest;
+#pragma unroll
+    for (int j = kPieces - 1; j >= 0; --j) {
+      float v[Stretch<T>::kEach];
+      x.values(u[j], v);
+#pragma unroll
+      for (int e = Stretch<T>::kEach - 1; e >= 0; --e)
+        if (v[e] == top) at = x.head + (t + j * kThreads) * Stretch<T>::kEach + e;
+    }
+    if (v0 == top) at = t;
+  }
   block_top(top, at, part_top, part_at);
   if (t == 0) {
     parts.top[blockIdx.x] = top;
-    parts.at[blockIdx.x] = 0;
+    parts.at[blockIdx.x] = first + at;
   }
-  if (top == -INFINITY) return;
+  if (top == -INFINITY || f.greedy) return;
   const Grid g(top, f.c);
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
@@ -754,21 +763,26 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     sum += bin_sum(e, scale);
   }
   const Bins b(s.l, f, g, count, sum);
-  if ((b.cut || b.by_p || b.by_m) && s.l.upto <= kList) {
-    const int n = s.l.upto;
+  // the tokens of bins `first` .. `last` to the list, which holds them; a call of all threads
+  auto gather = [&](int first, int last) {
+    __syncthreads();
     if (t == 0) s.l.n = 0;
     __syncthreads();
-    const float least = g.least(b.last);
-    x.each([&](float v, int i) {
-      if (v >= least && g.bin(v) <= b.last) s.l.list[atomicAdd(&s.l.n, 1)] = place(v, i);
+    x.each_between(g.least(last), g.most(first), [&](float v, int i) {
+      const int bin = g.bin(v);
+      if (bin >= first && bin <= last) s.l.list[atomicAdd(&s.l.n, 1)] = place(v, i);
     });
     __syncthreads();
-    finish_list(s.l, p, f, row, n, top, g, b);
+  };
+  if ((b.cut || b.by_p || b.by_m) && s.l.upto <= kList) {
+    gather(0, b.last);
+    finish_list(s.l, p, f, row, s.l.n, top, g, b);
     return;
   }
 
   // The border in bin `bin`: the last token of the order before which there is less than `goal`, which
   // the bin reaches.
+  int listed = -1;   // the bin whose tokens the list holds
   auto border_in = [&](int bin, bool by_count, u64 goal) {
     __syncthreads();
     if (t == bin) {
@@ -789,8 +803,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       sums[t] = 0;
       counts[t] = 0;
       __syncthreads();
-      x.each([&](float v, int i) {
-        if (!(v > -INFINITY) || g.bin(v) != bin) return;
+      x.each_between(g.least(bin), g.most(bin), [&](float v, int i) {
+        if (g.bin(v) != bin) return;
         const u64 a = place(v, i);
         if (shift < 64 && a >> shift != prefix) return;
         const int digit = static_cast<int>((a >> next) & ((u64{1} << (shift - next)) - 1));
@@ -823,16 +837,20 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       m = s.l.sum;
       inside = s.l.upto;
     }
-    __syncthreads();
-    if (t == 0) s.l.n = 0;
-    __syncthreads();
-    x.each([&](float v, int i) {
-      if (!(v > -INFINITY) || g.bin(v) != bin) return;
-      const u64 a = place(v, i);
-      if (shift < 64 && a >> shift != prefix) return;
-      s.l.list[atomicAdd(&s.l.n, 1)] = a;
-    });
-    __syncthreads();
+    if (shift == 64) {
+      gather(bin, bin);
+    } else {
+      __syncthreads();
+      if (t == 0) s.l.n = 0;
+      __syncthreads();
+      x.each_between(g.least(bin), g.most(bin), [&](float v, int i) {
+        if (g.bin(v) != bin) return;
+        const u64 a = place(v, i);
+        if (a >> shift == prefix) s.l.list[atomicAdd(&s.l.n, 1)] = a;
+      });
+      __syncthreads();
+    }
+    listed = shift == 64 ? bin : -1;
     const int n = s.l.n;
     sort_list(s.l.list, n);
     return border_sorted(s.l, s.l.list, n, top, f, by_count, c, m, goal);
@@ -865,68 +883,62 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     if (lane == 0) s.part_sum[i] = m;
   }
   __syncthreads();
-  if (full < kBins)
-    x.each([&](float v, int i) {
-      double w;
-      if (v > -INFINITY && g.bin(v) >= full && kept(v, i, w))
-        atomicAdd(&s.part_sum[i / parts.size], fixed(w));
-    });
+  if (full < kBins) {
+    int to = border.last == ~u64{0} ? kBins - 1 : g.bin(value_at(border.last));   // the last bin kept
+    if (b.by_m) to = min(to, b.bin_m + 1);
+    if (to == full && listed == full) {
+      for (int i = t; i < s.l.n; i += kThreads) {
+        const u64 a = s.l.list[i];
+        const int at_i = static_cast<int>(static_cast<uint32_t>(a));
+        double w;
+        if (kept(value_at(a), at_i, w)) atomicAdd(&s.part_sum[at_i / parts.size], fixed(w));
+      }
+    } else {
+      x.each_between(g.least(min(to, kBins - 1)), g.most(full), [&](float v, int i) {
+        double w;
+        if (g.bin(v) >= full && kept(v, i, w))
+          atomicAdd(&s.part_sum[i / parts.size], fixed(w));
+      });
+    }
+  }
   __syncthreads();
   u64 total = 0;
   for (int i = 0; i < parts.n; ++i) total += s.part_sum[i];
   u64 goal = target_of(p.uniform[row], total);
   int part = 0;
   while (part < parts.n - 1 && goal >= s.part_sum[part]) goal -= s.part_sum[part++];
-  // The part's tokens in order, an equal run to each thread.  Weights too small for a multiple of 2^-43
-  // count here, in 64 bits, as they do in the bins.
-  const double want = static_cast<double>(goal) / kOne;
-  const int end = min((part + 1) * parts.size, p.vocab), run = (parts.size + kThreads - 1) / kThreads;
-  const int i0 = min(part * parts.size + t * run, end), i1 = min(i0 + run, end);
-  constexpr int kRun = kPart / kThreads;
-  float v[kRun];
-#pragma unroll
-  for (int e = 0; e < kRun; ++e) v[e] = i0 + e < i1 ? logit(logits, i0 + e) : -INFINITY;
-  double mine = 0.0;
-#pragma unroll
-  for (int e = 0; e < kRun; ++e) {
+  // The part's tokens: sums by runs of neighbours, a thread each, then the run that holds the result in
+  // order.  Weights are those against the part's own largest, which is kept where any of its tokens is.
+  const float best = parts.top[row * parts.n + part];
+  const double against = weight(best, top, f.c);
+  const int first = part * parts.size, run = (parts.size + kThreads - 1) / kThreads;
+  const Stretch<T> y(logits + first, min(parts.size, p.vocab - first));
+  auto share = [&](float v, int i) -> u64 {
     double w;
-    if (kept(v[e], i0 + e, w)) mine += w;
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  double upto = mine;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const double d = __shfl_up(upto, o, kWave);
-    if (lane >= o) upto += d;
-  }
+    return kept(v, i, w) ? fixed(weight(v, best, f.c)) : 0;
+  };
+  s.l.few_sum[t] = 0;
   __syncthreads();
-  double* ends = reinterpret_cast<double*>(s.l.few_sum);
-  ends[t] = upto;
-  if (t == 0) {
-    s.l.bin_k = kThreads;   // the first thread whose tokens pass `want`
-    s.l.bin_p = -1;         // the last one that has tokens
-  }
+  y.each_between(g.least(kBins - 1), INFINITY, [&](float v, int i) {
+    const u64 w = share(v, first + i);
+    if (w != 0) atomicAdd(&s.l.few_sum[i / run], w);
+  });
   __syncthreads();
-  double wave0 = 0.0;
-  for (int w = 0; w < wave; ++w) wave0 += ends[kWave * w + kWave - 1];
-  if (mine > 0.0) {
-    if (wave0 + upto > want) atomicMin(&s.l.bin_k, t);
-    atomicMax(&s.l.bin_p, t);
-  }
-  __syncthreads();
-  if (t != (s.l.bin_k < kThreads ? s.l.bin_k : s.l.bin_p)) return;
-  double sums = wave0 + (upto - mine), won = 0.0;
-  int token = i0;
+  u64 sums;
+  const u64 here = s.l.few_sum[t], ahead = block_scan(here, s.l.part, sums);
+  const double want = static_cast<double>(goal) / against;
+  const u64 at_sum = want < static_cast<double>(sums) ? min(static_cast<u64>(want), sums - 1) : sums - 1;
+  if (!(ahead <= at_sum && at_sum < ahead + here)) return;   // one thread stays
+  u64 upto = ahead;
 #pragma unroll 1
-  for (int i = i0; i < i1; ++i) {
-    double w;
-    if (!kept(logit(logits, i), i, w)) continue;
-    token = i;
-    won = w;
-    sums += w;
-    if (sums > want) break;
+  for (int j = t * run; j < min(t * run + run, y.n); ++j) {
+    const float v = logit(y.x, j);
+    upto += share(v, first + j);
+    if (at_sum < upto) {
+      leave(p, row, first + j, weight(v, top, f.c), total);
+      return;
+    }
   }
-  leave(p, row, token, won, total);
 }
 
 // Parts of a row of `vocab` tokens: as many as its bins' entries need, and more where there are few rows.
