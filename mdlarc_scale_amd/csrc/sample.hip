@@ -63,9 +63,24 @@ __device__ __forceinline__ double octaves(float x, float top, double c) {
 }
 
 // x > -inf fails for NaN too: neither has a weight.  An infinite x is the largest value.
+// 2^d for d <= 0, zero below 2^-64: e^y of the nearest whole number's rest, |y| <= ln(2) / 2, to
+// y^11 (y^12 / 12! is below 2^-47), times 2^n.
 __device__ __forceinline__ double weight(float x, float top, double c) {
-  if (!(x > -INFINITY)) return 0.0;
-  return x == top ? 1.0 : exp2(octaves(x, top, c));
+  const double d = x == top ? 0.0 : octaves(x, top, c);   // inf - inf is NaN
+  if (!(x > -INFINITY && d > -64.0)) return 0.0;
+  const double n = rint(d), y = (d - n) * 0.69314718055994530942;
+  double w = 1.0 / 39916800;
+  w = fma(w, y, 1.0 / 3628800);
+  w = fma(w, y, 1.0 / 362880);
+  w = fma(w, y, 1.0 / 40320);
+  w = fma(w, y, 1.0 / 5040);
+  w = fma(w, y, 1.0 / 720);
+  w = fma(w, y, 1.0 / 120);
+  w = fma(w, y, 1.0 / 24);
+  w = fma(w, y, 1.0 / 6);
+  w = fma(w, y, 0.5);
+  w = fma(w, y, 1.0);
+  return ldexp(fma(w, y, 1.0), static_cast<int>(n));
 }
 
 __device__ __forceinline__ u64 fixed(double w) {   // w in [0, 1], to the nearest 2^-43
@@ -84,14 +99,16 @@ __device__ __forceinline__ float value_at(u64 place) {
   return __uint_as_float((up & 0x80000000u) ? up ^ 0x80000000u : ~up);
 }
 
+// Loops here stay loops: a block runs through most of its code once, so that the time to fetch its
+// instructions counts (a row's second launch took 47 us with 14,800 of them).
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
+#pragma unroll 1
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
   return v;
 }
 
 __device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {   // inclusive
-#pragma unroll
+#pragma unroll 1
   for (int o = 1; o < kWave; o <<= 1) {
     const u64 t = __shfl_up(v, o, kWave);
     if (lane >= o) v += t;
@@ -180,7 +197,6 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs p) {
 
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
 constexpr int kList = 4096;        // tokens that are sorted at once
-constexpr int kEachList = kList / kThreads;
 
 // A stretch of a row: tokens up to a 16-byte boundary, pieces of 16 bytes, the rest.
 template <typename T>
@@ -209,7 +225,7 @@ struct Stretch {
   __device__ __forceinline__ void each_between(float least, float most, F f) const {
     const int t = threadIdx.x;
     const int rest = head + pieces * kEach + t;
-    constexpr int kAhead = 32 / kEach;
+    constexpr int kAhead = 16 / kEach;
     const uint4* from = reinterpret_cast<const uint4*>(x + head);
     auto in = [&](float v) { return v >= least && v <= most; };   // not NaN
     for (int c = t - kAhead * kThreads; c < pieces; c += kAhead * kThreads) {
@@ -243,17 +259,21 @@ struct Stretch {
 // The sum of v over the threads before this one, and over all of them (`all`).
 __device__ __forceinline__ u64 block_scan(u64 v, u64* part, u64& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const u64 sums = wave_scan64(v, lane);
-  __syncthreads();
-  if (lane == 63) part[wave] = sums;
-  __syncthreads();
-  u64 before = sums - v;
-  all = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? part[w] : 0;
-    all += part[w];
+  // twice the same code: over the lanes, then over the waves' sums
+  u64 sums = v, lanes = 0, first = 0;
+#pragma unroll 1
+  for (int step = 0; step < 2; ++step) {
+    sums = wave_scan64(sums, lane);
+    if (step == 1) break;
+    lanes = sums;
+    __syncthreads();
+    if (lane == 63) part[wave] = sums;
+    __syncthreads();
+    sums = lane < kWaves ? part[lane] : 0;
   }
-  return before;
+  all = __shfl(sums, kWave - 1, kWave);
+  first = __shfl(sums, wave == 0 ? 0 : wave - 1, kWave);
+  return lanes - v + (wave == 0 ? 0 : first);
 }
 
 // Ascending bitonic sort of list[0 .. n), n <= kList; the entries up to the next power of two are set.
@@ -330,12 +350,8 @@ __device__ __forceinline__ u64 bin_entry(double f) {
 constexpr u64 kEntrySum = (u64{1} << 48) - 1;
 
 __device__ __forceinline__ void add_to_bins(u64* bins, const Grid& g, float x) {
-  if (!(x > -INFINITY)) return;
-  if (g.huge) {
-    if (x == INFINITY) atomicAdd(&bins[0], bin_entry(0.0));
-    return;
-  }
-  const double q = g.at(x), b = floor(q);
+  const double q = g.huge ? (x == INFINITY ? 0.0 : kBins) : g.at(x), b = floor(q);
+  // NaN compares false, and -inf lies at infinity
   if (b - g.base < kBins) atomicAdd(&bins[static_cast<int>(b - g.base)], bin_entry(q - b));
 }
 
@@ -416,34 +432,22 @@ __device__ __forceinline__ Border border_sorted(ListLds& s, const u64* list, int
                                                 const Filters& f, bool by_count, u64 c, u64 m,
                                                 u64 goal) {
   const int t = threadIdx.x;
-  u64 w[kEachList], mine = 0, all;
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    const int i = kEachList * t + e;
-    w[e] = i < n ? fixed(weight(value_at(list[i]), top, f.c)) : 0;
-    mine += w[e];
-    __builtin_amdgcn_sched_barrier(0);
-  }
   if (t == 0) s.found = 0;
-  const u64 first = m + block_scan(mine, s.part, all);
-  u64 before = first;
-  int found = 0;
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    const int i = kEachList * t + e;
-    if (i < n && (by_count ? c + i : before) < goal) found = i;
-    before += w[e];
-  }
-  if (found > 0) atomicMax(&s.found, found);
-  __syncthreads();
-  before = first;
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    before += w[e];
-    if (kEachList * t + e == s.found) {
-      s.last = list[s.found];
-      s.sum = before;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kThreads) {   // a thousand at a time, with what lies before them
+    const int i = i0 + t;
+    const u64 my = i < n ? list[i] : 0;
+    const u64 w = i < n ? fixed(weight(value_at(my), top, f.c)) : 0;
+    u64 all;
+    const u64 before = m + block_scan(w, s.part, all);   // a barrier for s.found too
+    const bool in = i < n && (by_count ? c + i : before) < goal;
+    if (in) atomicMax(&s.found, i);
+    __syncthreads();
+    if (i == s.found) {
+      s.last = my;
+      s.sum = before + w;
     }
+    m += all;
   }
   __syncthreads();
   return Border{s.last, s.sum};
@@ -454,14 +458,6 @@ __device__ __forceinline__ Border border_sorted(ListLds& s, const u64* list, int
 __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, const Filters& f, int row,
                                             int n, float top, const Grid& g, const Bins& b) {
   const int t = threadIdx.x;
-  u64 mine[kEachList];
-  int bin[kEachList];
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    const int i = t + e * kThreads;
-    mine[e] = i < n ? s.list[i] : ~u64{0};
-    bin[e] = i < n ? g.bin(value_at(mine[e])) : kBins;
-  }
   // the border in bin `at`
   auto border_in = [&](int at, bool by_count, u64 goal) {
     __syncthreads();
@@ -472,23 +468,27 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
     }
     if (t == 0) s.n = 0;
     __syncthreads();
-    const u64 c = s.last, m = s.sum;
-    if (s.upto > kThreads) {   // thousands of tokens in a bin: the whole list in order
-      sort_list(s.list, n);
-      return border_sorted(s, s.list, n, top, f, by_count, 0, 0, goal);
-    }
-#pragma unroll
-    for (int e = 0; e < kEachList; ++e)
-      if (bin[e] == at) {
-        const int i = atomicAdd(&s.n, 1);
-        s.few[i] = mine[e];
-        s.few_sum[i] = fixed(weight(value_at(mine[e]), top, f.c));
+    u64 c = s.last, m = s.sum;
+    int some = s.upto;
+    u64* from = s.few;
+    if (some > kThreads) {   // thousands of tokens in a bin: the whole list in order
+      from = s.list;
+      some = n;
+      c = m = 0;
+    } else {
+#pragma unroll 1
+      for (int i = t; i < n; i += kThreads) {
+        const u64 my = s.list[i];
+        if (g.bin(value_at(my)) != at) continue;
+        const int k = atomicAdd(&s.n, 1);
+        s.few[k] = my;
+        s.few_sum[k] = fixed(weight(value_at(my), top, f.c));
       }
+    }
     __syncthreads();
-    const int some = s.n;
     if (some > kCompared) {
-      sort_list(s.few, some);
-      return border_sorted(s, s.few, some, top, f, by_count, c, m, goal);
+      sort_list(from, some);
+      return border_sorted(s, from, some, top, f, by_count, c, m, goal);
     }
     if (t == 0) s.found = 0;
     u64 rank = 0, before = 0, my = 0;
@@ -511,16 +511,17 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
     __syncthreads();
     return Border{s.last, s.sum};
   };
-  // (a border past the last bin of the list is past what min-p keeps)
+  // top-k, then top-p, in one copy of the code (a border past the last bin of the list is past what
+  // min-p keeps)
   Border border{~u64{0}, b.total};
-  if (b.cut && b.bin_k <= b.last) border = border_in(b.bin_k, true, f.top_k);
-  if (b.by_p) {
-    const u64 goal = share_of(f.top_p, border.sum);
-    const int at = b.cut ? b.by_sum(s, goal) : b.bin_p;
-    if (at <= b.last) {
-      const Border other = border_in(at, false, goal);
-      if (other.last < border.last) border = other;
-    }
+#pragma unroll 1
+  for (int step = b.cut ? 0 : 1; step < (b.by_p ? 2 : 1); ++step) {
+    const bool by_count = step == 0;
+    const u64 goal = by_count ? static_cast<u64>(f.top_k) : share_of(f.top_p, border.sum);
+    const int at = by_count ? b.bin_k : b.cut ? b.by_sum(s, goal) : b.bin_p;
+    if (at > b.last) continue;
+    const Border other = border_in(at, by_count, goal);
+    if (other.last < border.last) border = other;
   }
   // sums of the kept tokens by stretches of indexes, a thread each; then the tokens of one stretch
   const int stretch = (p.vocab + kThreads - 1) / kThreads;
@@ -528,14 +529,15 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
   s.few_sum[t] = 0;
   if (t == 0) s.n = 0;
   __syncthreads();
-  u64 w[kEachList];
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    const bool there = bin[e] <= b.last && mine[e] <= border.last;
-    const double x = there ? weight(value_at(mine[e]), top, f.c) : 0.0;
-    w[e] = x >= f.min_p ? fixed(x) : 0;
-    if (w[e] != 0) atomicAdd(&s.few_sum[static_cast<uint32_t>(mine[e]) / stretch], w[e]);
-    __builtin_amdgcn_sched_barrier(0);
+  auto kept = [&](u64 my) -> u64 {   // the token's weight, 0 where it is not kept
+    if (my > border.last || g.bin(value_at(my)) > b.last) return 0;
+    const double w = weight(value_at(my), top, f.c);
+    return w >= f.min_p ? fixed(w) : 0;
+  };
+#pragma unroll 1
+  for (int i = t; i < n; i += kThreads) {
+    const u64 my = s.list[i], w = kept(my);
+    if (w != 0) atomicAdd(&s.few_sum[static_cast<uint32_t>(my) / stretch], w);
   }
   __syncthreads();
   const u64 here = s.few_sum[t];
@@ -547,29 +549,33 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
     s.sum = ahead;
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e)
-    if (w[e] != 0 && static_cast<int>(static_cast<uint32_t>(mine[e]) / stretch) == s.found)
-      s.list[atomicAdd(&s.n, 1)] = mine[e];
+  // its tokens, with their sums, in place of the ones of a bin
+  const uint32_t first = static_cast<uint32_t>(s.found) * stretch;
+  const u64 before_it = s.sum;
   __syncthreads();
-  n = s.n;
+#pragma unroll 1
   for (int i = t; i < n; i += kThreads) {
     const u64 my = s.list[i];
-    u64 before = s.sum;
-    for (int j = 0; j < n; ++j) {
-      const u64 o = s.list[j];
-      if (static_cast<uint32_t>(o) < static_cast<uint32_t>(my))
-        before += fixed(weight(value_at(o), top, f.c));
-    }
-    const double x = weight(value_at(my), top, f.c);
-    if (before <= goal && goal < before + fixed(x))
-      leave(p, row, static_cast<int>(static_cast<uint32_t>(my)), x, total);
+    if (static_cast<uint32_t>(my) - first >= static_cast<uint32_t>(stretch)) continue;
+    const u64 w = kept(my);
+    if (w == 0) continue;
+    const int k = atomicAdd(&s.n, 1);   // at most the stretch's tokens, one a thread or less
+    s.few[k] = my;
+    s.few_sum[k] = w;
   }
+  __syncthreads();
+  if (t >= s.n) return;
+  const u64 my = s.few[t], w = s.few_sum[t];
+  u64 before = before_it;
+#pragma unroll 1
+  for (int j = 0; j < s.n; ++j)
+    if (static_cast<uint32_t>(s.few[j]) < static_cast<uint32_t>(my)) before += s.few_sum[j];
+  if (before <= goal && goal < before + w)
+    leave(p, row, static_cast<int>(static_cast<uint32_t>(my)), weight(value_at(my), top, f.c), total);
 }
 
-// The row's largest value and its first index (0x7fffffff: there is none above -inf).
-__device__ __forceinline__ void block_top(float& top, int& at, float* part_top, int* part_at) {
-#pragma unroll
+__device__ __forceinline__ void wave_top(float& top, int& at) {
+#pragma unroll 1
   for (int o = 32; o > 0; o >>= 1) {
     const float x = __shfl_xor(top, o, kWave);
     const int i = __shfl_xor(at, o, kWave);
@@ -578,19 +584,19 @@ __device__ __forceinline__ void block_top(float& top, int& at, float* part_top, 
       at = i;
     }
   }
+}
+
+// The row's largest value and its first index (0x7fffffff: there is none above -inf).
+__device__ __forceinline__ void block_top(float& top, int& at, float* part_top, int* part_at) {
+  wave_top(top, at);
   if ((threadIdx.x & 63) == 0) {
     part_top[threadIdx.x >> 6] = top;
     part_at[threadIdx.x >> 6] = at;
   }
   __syncthreads();
-  for (int w = 0; w < kWaves; ++w) {
-    const float x = part_top[w];
-    const int i = part_at[w];
-    if (x > top || (x == top && i < at)) {
-      top = x;
-      at = i;
-    }
-  }
+  top = part_top[threadIdx.x & (kWaves - 1)];
+  at = part_at[threadIdx.x & (kWaves - 1)];
+  wave_top(top, at);
 }
 
 __device__ __forceinline__ bool leave_first(const SampleArgs& p, const Filters& f, int row, float top,
@@ -610,16 +616,15 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(const SampleArgs 
   const int row = blockIdx.x, t = threadIdx.x;
   const Filters f = filters_of(p, row);
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-  float v[kEachList], top = -INFINITY;
+  float top = -INFINITY;
   int at = 0x7fffffff;
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    const int i = t + e * kThreads;
-    v[e] = i < p.vocab ? logit(x, i) : -INFINITY;
-    v[e] = v[e] > -INFINITY ? v[e] : -INFINITY;   // no NaN
-    if (i < p.vocab) s.list[i] = place(v[e], i);
-    if (v[e] > top) {
-      top = v[e];
+#pragma unroll 1
+  for (int i = t; i < p.vocab; i += kThreads) {
+    float v = logit(x, i);
+    v = v > -INFINITY ? v : -INFINITY;   // no NaN
+    s.list[i] = place(v, i);
+    if (v > top) {
+      top = v;
       at = i;
     }
   }
@@ -627,11 +632,8 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(const SampleArgs 
   block_top(top, at, part_top, part_at);
   if (leave_first(p, f, row, top, at)) return;
   const Grid g(top, f.c);
-#pragma unroll
-  for (int e = 0; e < kEachList; ++e) {
-    add_to_bins(s.few, g, v[e]);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+#pragma unroll 1
+  for (int i = t; i < p.vocab; i += kThreads) add_to_bins(s.few, g, value_at(s.list[i]));
   __syncthreads();
   const u64 entries = s.few[t];
   const Bins b(s, f, g, entries >> 48, bin_sum(entries, bin_scale(g, t)));
@@ -763,20 +765,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     sum += bin_sum(e, scale);
   }
   const Bins b(s.l, f, g, count, sum);
-  // the tokens of bins `first` .. `last` to the list, which holds them; a call of all threads
-  auto gather = [&](int first, int last) {
-    __syncthreads();
+  if ((b.cut || b.by_p || b.by_m) && s.l.upto <= kList) {
+    const int n = s.l.upto;
     if (t == 0) s.l.n = 0;
     __syncthreads();
-    x.each_between(g.least(last), g.most(first), [&](float v, int i) {
-      const int bin = g.bin(v);
-      if (bin >= first && bin <= last) s.l.list[atomicAdd(&s.l.n, 1)] = place(v, i);
+    x.each_between(g.least(b.last), INFINITY, [&](float v, int i) {
+      if (g.bin(v) <= b.last) s.l.list[atomicAdd(&s.l.n, 1)] = place(v, i);
     });
     __syncthreads();
-  };
-  if ((b.cut || b.by_p || b.by_m) && s.l.upto <= kList) {
-    gather(0, b.last);
-    finish_list(s.l, p, f, row, s.l.n, top, g, b);
+    finish_list(s.l, p, f, row, n, top, g, b);
     return;
   }
 
@@ -837,19 +834,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       m = s.l.sum;
       inside = s.l.upto;
     }
-    if (shift == 64) {
-      gather(bin, bin);
-    } else {
-      __syncthreads();
-      if (t == 0) s.l.n = 0;
-      __syncthreads();
-      x.each_between(g.least(bin), g.most(bin), [&](float v, int i) {
-        if (g.bin(v) != bin) return;
-        const u64 a = place(v, i);
-        if (a >> shift == prefix) s.l.list[atomicAdd(&s.l.n, 1)] = a;
-      });
-      __syncthreads();
-    }
+    __syncthreads();
+    if (t == 0) s.l.n = 0;
+    __syncthreads();
+    x.each_between(g.least(bin), g.most(bin), [&](float v, int i) {
+      const u64 a = place(v, i);
+      if (g.bin(v) == bin && (shift == 64 || a >> shift == prefix))
+        s.l.list[atomicAdd(&s.l.n, 1)] = a;
+    });
+    __syncthreads();
     listed = shift == 64 ? bin : -1;
     const int n = s.l.n;
     sort_list(s.l.list, n);
@@ -858,14 +851,12 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
 
   Border border{~u64{0}, b.total};
   int full = b.by_m ? max(b.bin_m - 1, 0) : kBins;   // bins that are kept whole
-  if (b.cut) {
-    border = border_in(b.bin_k, true, f.top_k);
-    full = min(full, b.bin_k);
-  }
-  if (b.by_p) {
-    const u64 goal = share_of(f.top_p, border.sum);
-    const int bin = b.by_sum(s.l, goal);
-    const Border other = border_in(bin, false, goal);
+#pragma unroll 1
+  for (int step = b.cut ? 0 : 1; step < (b.by_p ? 2 : 1); ++step) {   // top-k, then top-p
+    const bool by_count = step == 0;
+    const u64 goal = by_count ? static_cast<u64>(f.top_k) : share_of(f.top_p, border.sum);
+    const int bin = by_count ? b.bin_k : b.by_sum(s.l, goal);
+    const Border other = border_in(bin, by_count, goal);
     if (other.last < border.last) border = other;
     full = min(full, bin);
   }
