@@ -335,24 +335,25 @@ struct Grid {
 // What a token adds to its bin: a count in the upper 16 bits, and the weight over that of the bin's
 // top, 2^(-f / 16) with 0 <= f < 1, to the nearest 2^-33.
 __device__ __forceinline__ u64 bin_entry(double f) {
-  const double y = f * (-0.69314718055994530942 / kBinsOctave);
-  double w = 1.0 / 720;          // e^y for -0.044 < y <= 0: y^7 / 5040 is below 2^-43
-  w = fma(w, y, 1.0 / 120);
-  w = fma(w, y, 1.0 / 24);
-  w = fma(w, y, 1.0 / 6);
-  w = fma(w, y, 0.5);
-  w = fma(w, y, 1.0);
-  w = fma(w, y, 1.0);
-  return (u64{1} << 48) + __builtin_bit_cast(u64, w + 524288.0) -
-         __builtin_bit_cast(u64, 524288.0);
+  constexpr double h = -0.69314718055994530942 / kBinsOctave;
+  double w = h * h * h * h * h / 120;   // e^(h f): the next term is below 2^-36
+  w = fma(w, f, h * h * h * h / 24);
+  w = fma(w, f, h * h * h / 6);
+  w = fma(w, f, h * h / 2);
+  w = fma(w, f, h);
+  w = fma(w, f, 1.0 + 0x1p19);          // from here on the last bit is 2^-33
+  return __builtin_bit_cast(u64, w) + ((u64{1} << 48) - __builtin_bit_cast(u64, 0x1p19));
 }
 
 constexpr u64 kEntrySum = (u64{1} << 48) - 1;
 
+// x: NaN compares false, and -inf lies at infinity
 __device__ __forceinline__ void add_to_bins(u64* bins, const Grid& g, float x) {
-  const double q = g.huge ? (x == INFINITY ? 0.0 : kBins) : g.at(x), b = floor(q);
-  // NaN compares false, and -inf lies at infinity
-  if (b - g.base < kBins) atomicAdd(&bins[static_cast<int>(b - g.base)], bin_entry(q - b));
+  const double q = g.at(x), b = floor(q), d = b - g.base;
+  if (d < kBins) atomicAdd(&bins[static_cast<int>(d)], bin_entry(q - b));
+}
+__device__ __forceinline__ void add_huge(u64* bins, float x) {   // the row's largest value is infinite
+  if (x == INFINITY) atomicAdd(&bins[0], bin_entry(0.0));
 }
 
 // The sum of weights of bin `bin` with the entries' sum `e`, in multiples of 2^-43; scale: the weight of
@@ -633,7 +634,13 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(const SampleArgs 
   if (leave_first(p, f, row, top, at)) return;
   const Grid g(top, f.c);
 #pragma unroll 1
-  for (int i = t; i < p.vocab; i += kThreads) add_to_bins(s.few, g, value_at(s.list[i]));
+  for (int i = t; i < p.vocab; i += kThreads) {
+    const float v = value_at(s.list[i]);
+    if (g.huge)
+      add_huge(s.few, v);
+    else
+      add_to_bins(s.few, g, v);
+  }
   __syncthreads();
   const u64 entries = s.few[t];
   const Bins b(s, f, g, entries >> 48, bin_sum(entries, bin_scale(g, t)));
@@ -659,7 +666,12 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
   __shared__ u64 bins[kBins];
   __shared__ float part_top[kWaves];
   __shared__ int part_at[kWaves];
-  const int row = blockIdx.x / parts.n, part = blockIdx.x - row * parts.n, t = threadIdx.x;
+  // The blocks of a row go to the XCD that its second launch will read it on: blocks go to the eight in
+  // turn, so eight rows take turns, too (the last rows may be fewer).
+  const int t = threadIdx.x, eight = blockIdx.x / (8 * parts.n) * 8;
+  const int rows = min(8, p.rows - eight), at_block = blockIdx.x - eight * parts.n;
+  const int part = at_block / rows, row = eight + at_block - part * rows;
+  const int slot = row * parts.n + part;
   const int first = part * parts.size;
   const Stretch<T> x(static_cast<const T*>(p.logits) + row * p.ld + first,
                      min(parts.size, p.vocab - first));
@@ -701,25 +713,29 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
   }
   block_top(top, at, part_top, part_at);
   if (t == 0) {
-    parts.top[blockIdx.x] = top;
-    parts.at[blockIdx.x] = first + at;
+    parts.top[slot] = top;
+    parts.at[slot] = first + at;
   }
   if (top == -INFINITY || f.greedy) return;
   const Grid g(top, f.c);
+  if (g.huge) {
+    for (int i = t; i < x.n; i += kThreads) add_huge(bins, logit(x.x, i));
+  } else {
 #pragma unroll
-  for (int j = 0; j < kPieces; ++j) {
-    float v[Stretch<T>::kEach];
-    x.values(u[j], v);
+    for (int j = 0; j < kPieces; ++j) {
+      float v[Stretch<T>::kEach];
+      x.values(u[j], v);
 #pragma unroll
-    for (int e = 0; e < Stretch<T>::kEach; ++e) {
-      add_to_bins(bins, g, v[e]);
-      if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // a few tokens' registers at a time
+      for (int e = 0; e < Stretch<T>::kEach; ++e) {
+        add_to_bins(bins, g, v[e]);
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // a few tokens' registers at a time
+      }
     }
+    add_to_bins(bins, g, v0);
+    add_to_bins(bins, g, v1);
   }
-  add_to_bins(bins, g, v0);
-  add_to_bins(bins, g, v1);
   __syncthreads();
-  parts.bins[static_cast<int64_t>(blockIdx.x) * kBins + t] = bins[t];
+  parts.bins[static_cast<int64_t>(slot) * kBins + t] = bins[t];
 }
 
 struct RowLds {
@@ -860,10 +876,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     if (other.last < border.last) border = other;
     full = min(full, bin);
   }
-  auto kept = [&](float v, int i, double& w) {
-    if (!(v > -INFINITY) || place(v, i) > border.last || g.bin(v) == kBins) return false;
-    w = weight(v, top, f.c);
-    return w >= f.min_p;
+  auto kept = [&](float v, int i) {
+    return v > -INFINITY && place(v, i) <= border.last &&
+           (!b.by_m || weight(v, top, f.c) >= f.min_p);
   };
   // the parts' kept sums: whole bins, then tokens of the others
   for (int i = wave; i < parts.n; i += kWaves) {
@@ -881,14 +896,13 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       for (int i = t; i < s.l.n; i += kThreads) {
         const u64 a = s.l.list[i];
         const int at_i = static_cast<int>(static_cast<uint32_t>(a));
-        double w;
-        if (kept(value_at(a), at_i, w)) atomicAdd(&s.part_sum[at_i / parts.size], fixed(w));
+        const float v = value_at(a);
+        if (kept(v, at_i)) atomicAdd(&s.part_sum[at_i / parts.size], fixed(weight(v, top, f.c)));
       }
     } else {
       x.each_between(g.least(min(to, kBins - 1)), g.most(full), [&](float v, int i) {
-        double w;
-        if (g.bin(v) >= full && kept(v, i, w))
-          atomicAdd(&s.part_sum[i / parts.size], fixed(w));
+        if (g.bin(v) >= full && kept(v, i))
+          atomicAdd(&s.part_sum[i / parts.size], fixed(weight(v, top, f.c)));
       });
     }
   }
@@ -903,27 +917,38 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
   const float best = parts.top[row * parts.n + part];
   const double against = weight(best, top, f.c);
   const int first = part * parts.size, run = (parts.size + kThreads - 1) / kThreads;
-  const Stretch<T> y(logits + first, min(parts.size, p.vocab - first));
+  const int n = min(parts.size, p.vocab - first), j0 = min(t * run, n), j1 = min(j0 + run, n);
   auto share = [&](float v, int i) -> u64 {
-    double w;
-    return kept(v, i, w) ? fixed(weight(v, best, f.c)) : 0;
+    return kept(v, i) ? fixed(weight(v, best, f.c)) : 0;
   };
-  s.l.few_sum[t] = 0;
-  __syncthreads();
-  y.each_between(g.least(kBins - 1), INFINITY, [&](float v, int i) {
-    const u64 w = share(v, first + i);
-    if (w != 0) atomicAdd(&s.l.few_sum[i / run], w);
-  });
-  __syncthreads();
+  u64 here = 0;
+  float next[4];   // four tokens ahead
+  auto load = [&](int j) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) next[e] = j + e < j1 ? logit(logits, first + j + e) : -INFINITY;
+  };
+  load(j0);
+#pragma unroll 1
+  for (int j = j0; j < j1; j += 4) {
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = next[e];
+    load(j + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      here += share(v[e], first + j + e);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
   u64 sums;
-  const u64 here = s.l.few_sum[t], ahead = block_scan(here, s.l.part, sums);
+  const u64 ahead = block_scan(here, s.l.part, sums);
   const double want = static_cast<double>(goal) / against;
   const u64 at_sum = want < static_cast<double>(sums) ? min(static_cast<u64>(want), sums - 1) : sums - 1;
   if (!(ahead <= at_sum && at_sum < ahead + here)) return;   // one thread stays
   u64 upto = ahead;
 #pragma unroll 1
-  for (int j = t * run; j < min(t * run + run, y.n); ++j) {
-    const float v = logit(y.x, j);
+  for (int j = j0; j < j1; ++j) {
+    const float v = logit(logits, first + j);
     upto += share(v, first + j);
     if (at_sum < upto) {
       leave(p, row, first + j, weight(v, top, f.c), total);
