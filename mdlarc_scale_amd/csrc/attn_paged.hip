@@ -42,33 +42,44 @@ int launch_source(const PagedArgs& a, bool fp4, bool tall, unsigned blocks, hipS
              : launch_paged<T, D, kPages>(a, tall, blocks, st);
 }
 
-// ---- single tokens over 4-bit pages ------------------------------------------------------------
+// ---- single tokens over 4-bit and fp32 pages ---------------------------------------------------
 
-// One query a sequence and up to 16 of its heads to a key / value head: rows of 16 x 16 x 32 MFMAs
-// (lane c = lane % 16, g = lane / 16), KT keys at a time.
+// One query a sequence and up to 16 of its heads to a key / value head: rows of 16 x 16 MFMAs (lane
+// c = lane % 16, g = lane / 16), KT keys at a time, twice as few rows as the tiles above have and the
+// operands in registers as they come from memory where that can be.
 //   S^T = K Q^T, 16 keys a block: the k index of an MFMA is whatever both operands agree on, so lane
-//     group g takes dims g D / 4 .. of its key, which are neighbouring bytes: a block is one load a
-//     lane, and its codes become the operand in registers.  Lane c, g holds the scores of row c with
-//     keys 4 g .. 4 g + 3 of each block.
-//   O^T = V^T P^T, 32 keys a step: the weights are the operand where they are; V^T comes from the
-//     wave's own tile of bf16 values in LDS by transposing reads.
-// fp32 queries (PARTS 3): codes are exact in bf16, so q and the weights go as sums of three bf16
-// numbers each (24 bits), and the products are fp32's.  Weights below 2^-126 are zero in either form.
+//     group g takes dims g D / 4 .. of its key, which are neighbouring bytes.  Lane c, g holds the
+//     scores of row c with keys 4 g .. 4 g + 3 of each block.
+//   O^T = V^T P^T: the weights are the operand where they are.
+// 4 bits (k = 32): K's codes become the operand in registers; V^T comes from the wave's own tile of bf16
+//   values in LDS by transposing reads, 32 keys a step.  fp32 queries: codes are exact in bf16, so q
+//   and the weights go as sums of three bf16 numbers each (24 bits), and the products are fp32's;
+//   weights below 2^-126 are zero.
+// fp32 pages (k = 4): lane g takes dims 16 i + 4 g .. + 3 of its key, so that a load covers 64 bytes of
+//   each (pieces of 16 bytes, a D / 4 apart, took twice the time).  Step r of V takes the keys 4 g + r,
+//   whose weights lane c, g holds, and dims 64 i + 4 c .. + 3 of such a row are one load: V needs no
+//   LDS either.
 // The waves of a block take the tiles in turn and merge at the end.  A value that is not finite is
 // seen by every row or (keys behind the last) set to zero.
-template <int D>
+// fp32, us, with the tiles above / so: 64 rows of up to 1,500 keys (12 heads of 64) 136 / 86, 64 of
+// 4,000 (32 heads on 8 of 128) 320 / 291, 16 of 1,203 (12 heads on 4 of 64) 18.5 / 15.1.
+enum TokenForm { kTokenFp4, kTokenFp4F32, kTokenF32 };
+
+template <int D, int FORM>
 struct TokenShape {
-  static constexpr int kTile = D == 128 ? 32 : 64;     // keys of a tile
+  static constexpr bool kF32 = FORM == kTokenF32;
+  static constexpr int kTile = (D == 128 ? 32 : 64) / (kF32 ? 2 : 1);   // keys of a tile
   static constexpr int kBlocks = kTile / 16;
-  static constexpr int kBytes = D / 8;                 // of codes in a lane's piece of a row
+  static constexpr int kBytes = kF32 ? D : D / 8;      // of a lane's piece of a row
   static constexpr int kWords = kBytes / 4;
+  static constexpr int kRowBytes = 4 * kBytes;
   static constexpr int kAhead = 2;                     // tiles in flight
   static constexpr int kWaves = 4;
   static constexpr int kTurn = kTile * kWaves;
   static constexpr int kLd = D + 8;                    // bf16 elements of a row of V in LDS
   static constexpr int kStateLd = D + 4;               // floats of a row of a wave's state
-  static constexpr int kWaveBytes =
-      kTile * kLd * 2 > 16 * kStateLd * 4 ? kTile * kLd * 2 : 16 * kStateLd * 4;
+  static constexpr int kWaveBytes = !kF32 && kTile * kLd * 2 > 16 * kStateLd * 4
+                                        ? kTile * kLd * 2 : 16 * kStateLd * 4;
 };
 
 // The bytes at base + off + at: base and off are the same for the wave, so the load takes their sum from
@@ -81,9 +92,11 @@ __device__ __forceinline__ T load_at(const void* base, int64_t off, uint32_t at)
       (const __attribute__((address_space(1))) T*)((const __attribute__((address_space(1))) uint8_t*)a + at));
 }
 
-template <int D, int PARTS>
-__global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel(const PagedArgs p) {
-  using S = TokenShape<D>;
+template <int D, int FORM>
+__global__ __launch_bounds__(256, FORM == kTokenFp4 ? 3 : 2) void attn_token_kernel(const PagedArgs p) {
+  using S = TokenShape<D, FORM>;
+  constexpr bool kF32 = FORM == kTokenF32;
+  constexpr int PARTS = FORM == kTokenFp4F32 ? 3 : 1;
   constexpr int KT = S::kTile, NB = S::kBlocks, W = S::kWords, DB = D / 16, kTurn = S::kTurn;
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::kWaves * S::kWaveBytes];
   __shared__ float states[S::kWaves][2][16];
@@ -100,19 +113,26 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
   if (p.n_split == 1 && p.slots > 0)
     early = p.table[seq * p.table_ld + min(early0 + lane, quotient(p.slots - 1, p.by_page))];
   const int lo = min(max(p.q_offset[seq], 0), p.tokens);
-  if (min(max(p.q_offset[seq + 1], lo), p.tokens) == lo) return;
+  const int n = min(max(p.q_offset[seq + 1], lo), p.tokens) - lo;
+  if (n == 0) return;
   const int G = p.group;
-  const int kend = min(max(p.kv_len[seq], 0), p.slots);
+  // the keys that the first query of n sees: the others are past max_q and not computed
+  const int kend = max(min(max(p.kv_len[seq], 0), p.slots) - (p.causal ? n - 1 : 0), 0);
   const int per = ((kend + p.n_split - 1) / p.n_split + kTurn - 1) / kTurn * kTurn;
   const int k0 = min(split * per, kend), k1 = min(k0 + per, kend);
   const int64_t qrow = static_cast<int64_t>(lo) * p.heads + kvh * G;
 
-  // q of row c (rows past G: the last one's), dims g D / 4 + 8 s .. + 7 of step s
+  // q of row c (rows past G: the last one's), dims g D / 4 + 8 s .. + 7
   bf16x8_t qf[PARTS][D / 32];
+  float qv[D / 32][8];   // fp32 pages
 #pragma unroll
   for (int s = 0; s < D / 32; ++s) {
     const int64_t at = (qrow + min(c, G - 1)) * D + g * (D / 4) + 8 * s;
-    if constexpr (PARTS == 1) {
+    if constexpr (kF32) {
+      const float* from = static_cast<const float*>(p.q) + at - g * (D / 4) - 8 * s + 32 * s + 4 * g;
+      *reinterpret_cast<float4*>(qv[s]) = *reinterpret_cast<const float4*>(from);
+      *reinterpret_cast<float4*>(qv[s] + 4) = *reinterpret_cast<const float4*>(from + 16);
+    } else if constexpr (PARTS == 1) {
       qf[0][s] = as_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at));
     } else {
       float f[8];
@@ -154,13 +174,18 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
   };
   Tile tiles[S::kAhead];
   // lane's places in a block: K, key c and piece g; V, key lane / 4 and piece lane % 4
-  const uint32_t k_at = c * (D / 2) + g * S::kBytes, v_at = lane * S::kBytes;
+  // (fp32: K, key c and piece g of each 64 bytes; V, key 4 g and piece c of each 256)
+  const uint32_t k_at = c * S::kRowBytes + g * (kF32 ? 16 : S::kBytes);
+  const uint32_t v_at = kF32 ? 4 * g * S::kRowBytes + 16 * c : lane * S::kBytes;
   const uint32_t kp_at = c * (D / 32) + g * (D / 4) / 32;
   const uint32_t vp_at = (lane >> 2) * (D / 32) + (lane & 3) * (D / 4) / 32;
   auto piece = [&](const void* base, int64_t off, uint32_t at, uint32_t (&t)[W]) {
-    if constexpr (W == 4) {
-      const u32x4_t u = load_at<u32x4_t>(base, off, at);
-      t[0] = u.x; t[1] = u.y; t[2] = u.z; t[3] = u.w;
+    if constexpr (W % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const u32x4_t u = load_at<u32x4_t>(base, off + 16 * i, at);   // fp32: i > 0 in 64-byte steps
+        t[i] = u.x; t[i + 1] = u.y; t[i + 2] = u.z; t[i + 3] = u.w;
+      }
     } else {
       const u32x2_t u = load_at<u32x2_t>(base, off, at);
       t[0] = u.x; t[1] = u.y;
@@ -182,10 +207,22 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
       const uint32_t hi32 = __builtin_amdgcn_readlane(row_hi, page - page0);
       const int64_t row = static_cast<int64_t>(static_cast<uint64_t>(hi32) << 32 | lo32) + key -
                           page * p.page_slots;
-      piece(p.k, row * (D / 2), ka, t.k[b]);
-      piece(p.v, row * (D / 2), va, t.v[b]);
-      t.kp[b] = load_at<uint8_t>(p.k_scale, row * (D / 32), kpa);
-      t.vp[b] = load_at<uint8_t>(p.v_scale, row * (D / 32), vpa);
+      piece(p.k, row * S::kRowBytes, ka, t.k[b]);
+      if constexpr (kF32) {
+        // row 4 g + r in words DB r ..
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < DB; i += 4) {
+            const u32x4_t u = load_at<u32x4_t>(p.v, (row + r) * S::kRowBytes + 64 * i, va);
+            t.v[b][DB * r + i] = u.x; t.v[b][DB * r + i + 1] = u.y;
+            t.v[b][DB * r + i + 2] = u.z; t.v[b][DB * r + i + 3] = u.w;
+          }
+      } else {
+        piece(p.v, row * S::kRowBytes, va, t.v[b]);
+        t.kp[b] = load_at<uint8_t>(p.k_scale, row * (D / 32), kpa);
+        t.vp[b] = load_at<uint8_t>(p.v_scale, row * (D / 32), vpa);
+      }
     }
   };
 
@@ -201,6 +238,13 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
     f32x4_t sc[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      if constexpr (kF32) {
+#pragma unroll
+        for (int s = 0; s < W; ++s)
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.k[b][s]), qv[s / 8][s % 8],
+                                                       s == 0 ? start : sc[b], 0, 0, 0);
+        continue;
+      }
       const float power = __uint_as_float(t.kp[b] << 23);
 #pragma unroll
       for (int s = 0; s < W; ++s) {
@@ -215,10 +259,17 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
       __builtin_amdgcn_sched_barrier(0);   // one block's values in registers at a time
     }
     if (!whole) {   // no values behind the keys
-      int x = k1 - kt - (lane >> 2);
+      int x = k1 - kt - (kF32 ? 4 * g : lane >> 2);
       asm volatile("" : "+v"(x));   // keeps this a branch
+      if constexpr (kF32) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+            if (16 * b + i / DB >= x) t.v[b][i] = 0;
+      }
+#pragma unroll
+      for (int b = 0; !kF32 && b < NB; ++b)
         if (16 * b >= x) {
           t.vp[b] = 127;
 #pragma unroll
@@ -226,7 +277,7 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
         }
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
+    for (int b = 0; !kF32 && b < NB; ++b) {
       const float power = __uint_as_float(t.vp[b] << 23);
 #pragma unroll
       for (int s = 0; s < W; ++s) {
@@ -255,7 +306,7 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
       const float tmax = max_over_groups(lmax);
       if (tmax > thr) {   // the same in the four lanes of a row
         const bool fresh = thr == -INFINITY;
-        const float alpha = fresh ? 0.f : __builtin_amdgcn_exp2f(-tmax);
+        const float alpha = fresh ? 0.f : weight_exp2<kF32>(-tmax);
         negm = fresh ? -tmax : negm - tmax;
         start = f32x4_t{negm, negm, negm, negm};
         thr = kGap;
@@ -269,7 +320,20 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sc[b][r] = __builtin_amdgcn_exp2f(sc[b][r]);
+      for (int r = 0; r < 4; ++r) sc[b][r] = weight_exp2<kF32>(sc[b][r]);
+    if constexpr (kF32) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          l += sc[b][r];
+#pragma unroll
+          for (int i = 0; i < DB; ++i)
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.v[b][DB * r + i]),
+                                                        sc[b][r], o[i], 0, 0, 0);
+        }
+      return;
+    }
 #pragma unroll
     for (int kk = 0; kk < NB / 2; ++kk) {
       bf16x8_t pb[PARTS];
@@ -338,8 +402,14 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
   }
 #pragma unroll
   for (int db = 0; db < DB; ++db)
-    *reinterpret_cast<float4*>(st + c * S::kStateLd + 16 * db + 4 * g) =
-        make_float4(o[db][0], o[db][1], o[db][2], o[db][3]);
+    if constexpr (kF32) {   // element e of block 4 i + x: dim 64 i + 4 (4 g + e) + x
+      const int e = db % 4, i = db / 4;
+      *reinterpret_cast<float4*>(st + c * S::kStateLd + 64 * i + 16 * g + 4 * e) =
+          make_float4(o[4 * i][e], o[4 * i + 1][e], o[4 * i + 2][e], o[4 * i + 3][e]);
+    } else {
+      *reinterpret_cast<float4*>(st + c * S::kStateLd + 16 * db + 4 * g) =
+          make_float4(o[db][0], o[db][1], o[db][2], o[db][3]);
+    }
   __syncthreads();
   const bool part = p.ws_o != nullptr;
   const int64_t base = split * static_cast<int64_t>(p.tokens) * p.heads + qrow;
@@ -354,7 +424,7 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
     for (int w = 0; w < S::kWaves; ++w) {
       const float m = states[w][0][row];
       if (m == -INFINITY) continue;
-      const float a = __builtin_amdgcn_exp2f(m - ref);
+      const float a = weight_exp2<kF32>(m - ref);
       sum = fmaf(states[w][1][row], a, sum);
       const float4 v = *reinterpret_cast<const float4*>(
           reinterpret_cast<const float*>(lds + w * S::kWaveBytes) + row * S::kStateLd + dim);
@@ -375,7 +445,7 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
     if (p.out_form != kOutPlain)
       store_split4(static_cast<uint16_t*>(p.out), p.out_form, lo, (kvh * G + row) * D + dim,
                    p.heads * D, t);
-    else if constexpr (PARTS == 1)
+    else if constexpr (FORM == kTokenFp4)
       *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (qrow + row) * D + dim) =
           make_uint2(pack_bf2(t[0], t[1]), pack_bf2(t[2], t[3]));
     else
@@ -384,14 +454,10 @@ __global__ __launch_bounds__(256, PARTS == 3 ? 2 : 3) void attn_token_fp4_kernel
   }
 }
 
-int launch_token_fp4(const PagedArgs& a, int dtype, int head_dim, unsigned blocks, hipStream_t st) {
-  if (dtype == MDL_DTYPE_F32) {
-    if (head_dim == 64) attn_token_fp4_kernel<64, 3><<<blocks, 256, 0, st>>>(a);
-    else attn_token_fp4_kernel<128, 3><<<blocks, 256, 0, st>>>(a);
-  } else {
-    if (head_dim == 64) attn_token_fp4_kernel<64, 1><<<blocks, 256, 0, st>>>(a);
-    else attn_token_fp4_kernel<128, 1><<<blocks, 256, 0, st>>>(a);
-  }
+template <int FORM>
+int launch_token(const PagedArgs& a, int head_dim, unsigned blocks, hipStream_t st) {
+  if (head_dim == 64) attn_token_kernel<64, FORM><<<blocks, 256, 0, st>>>(a);
+  else attn_token_kernel<128, FORM><<<blocks, 256, 0, st>>>(a);
   return launch_status();
 }
 
@@ -405,9 +471,10 @@ int check_paged(int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, i
                      table_width * page_slots);
 }
 
-// Single tokens over 4-bit pages with no more heads to a key / value head than rows of their kernel.
+// Single tokens over 4-bit and fp32 pages with no more heads to a key / value head than rows of their
+// kernel.  bf16 pages stay with the flat tiles, which read them at 6 TB/s and more.
 bool takes_tokens(int page_dtype, int max_q, int n_heads, int n_kv_heads) {
-  return page_dtype == MDL_DTYPE_FP4 && max_q == 1 && n_heads / n_kv_heads <= 16;
+  return page_dtype != MDL_DTYPE_BF16 && max_q == 1 && n_heads / n_kv_heads <= 16;
 }
 
 Plan plan_paged(int n_seq, int max_q, int n_heads, int n_kv_heads, int head_dim, int dtype,
@@ -420,7 +487,10 @@ Plan plan_paged(int n_seq, int max_q, int n_heads, int n_kv_heads, int head_dim,
     // of 811 (12 heads on 4 of 64) uncut 7.7 / in 3 8.6; 16 of 20,000 (12 heads of 64) in 9 58 / in 6
     // 63 / in 32 65.
     const int64_t pairs = static_cast<int64_t>(n_seq) * n_kv_heads;
-    const int turn = head_dim == 128 ? TokenShape<128>::kTurn : TokenShape<64>::kTurn;
+    const bool f32 = page_dtype == MDL_DTYPE_F32;
+    const int turn = head_dim == 128
+        ? (f32 ? TokenShape<128, kTokenF32>::kTurn : TokenShape<128, kTokenFp4>::kTurn)
+        : (f32 ? TokenShape<64, kTokenF32>::kTurn : TokenShape<64, kTokenFp4>::kTurn);
     const int64_t few = slots / (2 * turn), many = slots / 2048;
     int64_t ns = few < 3 ? 1 : std::min<int64_t>((512 + pairs - 1) / pairs, few);
     ns = std::max(ns, std::min<int64_t>((2048 + pairs - 1) / pairs, many));
@@ -504,7 +574,9 @@ extern "C" int mdl_attn_paged(const void* q, int dtype, const void* k_pages, con
   const unsigned n = static_cast<unsigned>(blocks);
   int rc;
   if (takes_tokens(page_dtype, max_q, n_heads, n_kv_heads))
-    rc = launch_token_fp4(a, dtype, head_dim, n, st);
+    rc = !fp4 ? launch_token<kTokenF32>(a, head_dim, n, st)
+              : dtype == MDL_DTYPE_F32 ? launch_token<kTokenFp4F32>(a, head_dim, n, st)
+                                       : launch_token<kTokenFp4>(a, head_dim, n, st);
   else if (dtype == MDL_DTYPE_F32)
     rc = head_dim == 64 ? launch_source<float, 64>(a, fp4, pl.tall, n, st)
                         : launch_source<float, 128>(a, fp4, pl.tall, n, st);

@@ -119,6 +119,37 @@ def test_paged_single_tokens(dtype, D, heads, kv, fp4):
     assert torch.equal(c.run(), c.run())
 
 
+@pytest.mark.parametrize("dtype,D,fp4", [(BF, 64, False), (F32, 64, False), (F32, 128, False),
+                                         (BF, 64, True), (BF, 128, True), (F32, 128, True)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_paged_first_queries_alone(dtype, D, fp4, causal):
+    """max_q 1 where sequences have more queries: the first of each sees what it would see among
+    them, the others stay as they were."""
+    c = Paged(15, dtype, D, 8, 2, [3, 1, 40, 0, 2], [500, 1700, 3, 0, 0], fp4=fp4)
+    ref, bound = c.reference(causal)
+    for workspace in (True, False):
+        out = c.run(max_q=1, causal=causal, workspace=workspace)
+        first = [0, 3, 4, 44]
+        _check(out[first], ref[first], bound[first], "first queries")
+        rest = [i for i in range(c.tokens) if i not in first]
+        assert bool((out[rest] == 7.0).all())
+    # fewer keys than queries: the first sees none
+    keys = [2, 0, 12, 0, 1]
+    out = c.run(max_q=1, keys=keys)
+    assert bool((out[[0, 3, 4, 44]] == 0).all())
+
+
+@pytest.mark.parametrize("dtype,D,fp4", [(F32, 64, False), (F32, 128, False), (BF, 64, True),
+                                         (BF, 128, True), (F32, 64, True), (F32, 128, True)])
+@pytest.mark.parametrize("heads,kv", [(16, 1), (17, 1), (7, 7), (15, 5)])
+def test_paged_single_tokens_of_many_heads(dtype, D, fp4, heads, kv):
+    """16 heads to a key / value head fill the rows of a block, 17 take the other tiles; large scores
+    move the reference often."""
+    c = Paged(17, dtype, D, heads, kv, [1] * 5, [700, 0, 63, 64, 1500], fp4=fp4, std=4.0)
+    c.check("many heads")
+    c.check("whole", workspace=False)
+
+
 @pytest.mark.parametrize("dtype,fp4", [(BF, False), (F32, False), (BF, True), (F32, True)])
 @pytest.mark.parametrize("workspace", [True, False])
 def test_paged_rows_that_see_nothing(dtype, fp4, workspace):
