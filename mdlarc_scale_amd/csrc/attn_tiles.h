@@ -306,52 +306,78 @@ __device__ __forceinline__ void grouped_block(const Args& p, int block, uint8_t*
         dma16_sbase(from, off, dst);
     }
   };
-  // The numbers of 64 pages from page `page0` of the sequence on, one a lane.  One outside the pool
-  // is read as 0, so no address leaves it, and makes the block's results NaN.
-  int page0 = 0, page_no = 0;
+  // The pool's rows at which 64 pages of the sequence begin, from page `page0` on, one a lane.  A page
+  // number outside the pool is read as 0, so no address leaves it, and makes the block's results NaN.
+  int page0 = 0;
+  uint32_t row_lo = 0, row_hi = 0;
   bool astray = false;
   auto load_pages = [&](int page) {
     if constexpr (SRC != kSlots) {
       page0 = page;
       const int last = quotient(kend - 1, p.by_page);
-      page_no = p.table[seq * p.table_ld + min(page + lane, last)];
-      const bool bad = page_no < 0 || page_no >= p.n_pages;
+      const int no = p.table[seq * p.table_ld + min(page + lane, last)];
+      const bool bad = no < 0 || no >= p.n_pages;
       astray = astray || __ballot(bad) != 0;
-      page_no = bad ? 0 : page_no;
+      const uint64_t row = (static_cast<uint64_t>(bad ? 0 : no) * p.kv_heads + kvh) * p.page_slots;
+      row_lo = static_cast<uint32_t>(row);
+      row_hi = static_cast<uint32_t>(row >> 32);
+    }
+  };
+  // The pages of a tile's keys are among the 64.
+  auto hold_pages = [&](int kt) {
+    if constexpr (SRC != kSlots) {
+      const int a = quotient(min(kt, kend - 1), p.by_page);
+      const int b = quotient(min(kt + KT, kend) - 1, p.by_page);
+      if (a < page0 || b >= page0 + kWave) load_pages(a);
     }
   };
   // The row of the pool with key `key` (the same for the wave).  Pages are multiples of 16 slots: the
   // keys up to the next multiple of 16 are the next rows.
   auto pool_row = [&](int key) -> int64_t {
-    int64_t row = 0;
-    if constexpr (SRC != kSlots) {
+    if constexpr (SRC == kSlots) return 0;
+    else {
       const int page = quotient(key, p.by_page);
-      if (static_cast<uint32_t>(page - page0) >= kWave) load_pages(page);
-      const int no = __builtin_amdgcn_readlane(page_no, page - page0);
-      row = (static_cast<int64_t>(no) * p.kv_heads + kvh) * p.page_slots + key - page * p.page_slots;
+      const uint32_t lo32 = __builtin_amdgcn_readlane(row_lo, page - page0);
+      const uint32_t hi32 = __builtin_amdgcn_readlane(row_hi, page - page0);
+      return static_cast<int64_t>(static_cast<uint64_t>(hi32) << 32 | lo32) + key -
+             page * p.page_slots;
     }
-    return row;
   };
-  auto issue_pages = [&](const T* src, int kt, uint32_t at, auto plain) {
-    const T* from = src;
-    int left = 0;   // rows of the sixteen that hold keys, less one
+  // Tile kt of K (of V, of both from one look at the pages) to its slot of the ring.  Where the tile is
+  // whole a lane's offset in its sixteen rows does not depend on it.
+  auto issue_pages = [&](auto do_k, auto do_v, int kt, uint32_t k_to, uint32_t v_to) {
+    hold_pages(kt);
+    auto copies = [&](auto whole) {
+      int64_t row = 0;
+      int left = 15;   // rows of the sixteen that hold keys, less one
 #pragma unroll
-    for (int jj = 0; jj < S::kCopies; ++jj) {
-      const int j = wr + WR * jj;
-      const int r = S::kRowsPerCopy * j + lane / kChunks;
-      if (WR > 1 || (S::kRowsPerCopy * jj) % 16 == 0) {
-        const int key = min(kt + ((S::kRowsPerCopy * j) & ~15), kend - 1);
-        from = scalar_ptr(src + pool_row(key) * D);
-        left = kend - 1 - key;
+      for (int jj = 0; jj < S::kCopies; ++jj) {
+        const int j = wr + WR * jj;
+        if (WR > 1 || (S::kRowsPerCopy * jj) % 16 == 0) {
+          const int first = kt + ((S::kRowsPerCopy * j) & ~15);
+          const int key = decltype(whole)::value ? first : min(first, kend - 1);
+          row = pool_row(key);
+          left = kend - 1 - key;
+        }
+        const int r = (S::kRowsPerCopy * j + lane / kChunks) & 15;
+        const uint32_t at = (decltype(whole)::value ? r : min(r, left)) * S::kRowBytes;
+        auto copy = [&](const void* pool, uint32_t to, bool plain) {
+          const T* from = scalar_ptr(static_cast<const T*>(pool) + row * D);
+          const uint32_t off = at + 16 * ((lane % kChunks) ^ (plain ? 0 : swz<T, D>(r)));
+          const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + to + 1024 * j);
+          if constexpr (WR == 1)
+            dma16_stream(from, off, dst);
+          else
+            dma16_sbase(from, off, dst);
+        };
+        if (decltype(do_k)::value) copy(p.k, k_to, false);
+        if (decltype(do_v)::value) copy(p.v, v_to, kF32);
       }
-      const uint32_t off = min(r & 15, left) * S::kRowBytes +
-                           16 * ((lane % kChunks) ^ (decltype(plain)::value ? 0 : swz<T, D>(r & 15)));
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + at + 1024 * j);
-      if constexpr (WR == 1)
-        dma16_stream(from, off, dst);
-      else
-        dma16_sbase(from, off, dst);
-    }
+    };
+    if (kt + KT <= kend)
+      copies(std::true_type{});
+    else
+      copies(std::false_type{});
   };
   // 4 bits: the wave's part of a tile goes through registers, kCode bytes (of one row) to a lane, kSets
   // times; fetch_codes loads it, store_codes writes its values to the ring as the copies would.
@@ -367,6 +393,7 @@ __device__ __forceinline__ void grouped_block(const Args& p, int block, uint8_t*
       Codes& t = decltype(is_v)::value ? v_codes : k_codes;
       const uint8_t* codes = static_cast<const uint8_t*>(decltype(is_v)::value ? p.v : p.k);
       const uint8_t* powers = decltype(is_v)::value ? p.v_scale : p.k_scale;
+      hold_pages(kt);
 #pragma unroll
       for (int n = 0; n < kSets; ++n) {
         const int r0 = kSetRows * (wr + WR * n);   // tile rows r0 .. r0 + kSetRows - 1
@@ -432,10 +459,18 @@ __device__ __forceinline__ void grouped_block(const Args& p, int block, uint8_t*
     if constexpr (SRC == kSlots) {
       issue(V ? Vg : Kg, kt, at, plain);
     } else if constexpr (SRC == kPages) {
-      issue_pages(static_cast<const T*>(V ? p.v : p.k), kt, at, plain);
+      issue_pages(std::bool_constant<!V>{}, is_v, kt, at, at);
     } else {
       store_codes(is_v, at);
       if (kt + KT * WK < k1) fetch_codes(is_v, kt + KT * WK);
+    }
+  };
+  auto put_both = [&](int kt, uint32_t k_to, uint32_t v_to) {
+    if constexpr (SRC == kPages) {
+      issue_pages(std::true_type{}, std::true_type{}, kt, k_to, v_to);
+    } else {
+      put(kIsK, kt, k_to);
+      put(kIsV, kt, v_to);
     }
   };
   // slots of a ring: K of each stage, then V
@@ -704,10 +739,7 @@ __device__ __forceinline__ void grouped_block(const Args& p, int block, uint8_t*
     }
   }
   if constexpr (WR > 1) {
-    if (first < k1) {
-      put(kIsK, first, k_slot(0));
-      put(kIsV, first, v_slot(0));
-    }
+    if (first < k1) put_both(first, k_slot(0), v_slot(0));
     // q of the wave's 32 rows through the second stage (the first turn's barrier frees it), whole
     // rows to a copy: read into registers directly, an instruction takes 16 bytes of 64 places.
     if constexpr (kCopyQ) {
@@ -737,10 +769,7 @@ __device__ __forceinline__ void grouped_block(const Args& p, int block, uint8_t*
       // after the next stay in flight).
       __builtin_amdgcn_s_waitcnt(SRC == kPagesFp4 ? kWaitLds : kWaitAll);
       asm volatile("s_barrier" ::: "memory");
-      if (kt + kTurn < k1) {
-        put(kIsK, kt + kTurn, k_slot(ST ^ 1));
-        put(kIsV, kt + kTurn, v_slot(ST ^ 1));
-      }
+      if (kt + kTurn < k1) put_both(kt + kTurn, k_slot(ST ^ 1), v_slot(ST ^ 1));
       // past the part, or no row of the wave sees a key
       if (!decltype(fullc)::value && (kt >= k1 || kt > lim_hi)) return;
       compute(ring + k_slot(ST), ring + v_slot(ST), kt, fullc, [] {});

@@ -1327,30 +1327,35 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor |
            dtype: torch.dtype) -> tuple[tuple, int, list, tuple]:
     """Checks of a paged cache for rows of ``dtype``: its (pages, kv_heads, page slots, head dim),
     the pages' type code, the specs of its tensors, and the table's (sequences, width, row stride)."""
-    shape = k_pages.shape
+    shape, held, wide = k_pages.shape, k_pages.dtype, page_table.shape
     if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must both be [pages, kv_heads, page_slots, head_dim] "
                          f"(got {tuple(shape)} and {tuple(v_pages.shape)})")
     n, kv, slots, d = shape
-    fp4 = k_pages.dtype is U8
-    if fp4:
-        d *= 2
+    if held is U8:
+        d, code, dtype = 2 * d, PAGE_FP4, U8
+    else:
+        code = cache_dtype_code(k_pages)
     if d not in GROUPED_HEAD_DIMS:
         raise ValueError(f"pages must have a head_dim of 64 or 128, 4-bit ones half as many bytes "
-                         f"(got {tuple(shape)} of {k_pages.dtype})")
+                         f"(got {tuple(shape)} of {held})")
     if not n or not kv or slots < 16 or slots > 4096 or slots % 16:
         raise ValueError("a pool needs pages, key / value heads, and 16 to 4096 slots a page, in "
                          f"multiples of 16 (got {tuple(shape)})")
-    if len(page_table.shape) != 2:
-        raise ValueError(f"page_table must be [sequences, pages] (got {tuple(page_table.shape)})")
-    n_seq, width = page_table.shape
-    ld, step = page_table.stride()
-    if page_table.dtype is not I32 or (width > 1 and step != 1) or (n_seq > 1 and ld < width):
-        raise ValueError("page_table must be int32 with contiguous rows that do not overlap")
-    code = PAGE_FP4 if fp4 else cache_dtype_code(k_pages)
-    specs = [(k_pages, "k_pages", U8 if fp4 else dtype, 0),
-             (v_pages, "v_pages", U8 if fp4 else dtype, 0)]
-    if fp4:
+    if len(wide) != 2:
+        raise ValueError(f"page_table must be [sequences, pages] (got {tuple(wide)})")
+    n_seq, width = wide
+    ld = width if width else 1
+    if n_seq > 1 or not page_table.is_contiguous():
+        ld, step = page_table.stride()
+        if (width > 1 and step != 1) or (n_seq > 1 and ld < width):
+            raise ValueError("page_table must have contiguous rows that do not overlap")
+        if n_seq <= 1:
+            ld = width if width else 1
+    if page_table.dtype is not I32:
+        raise ValueError(f"page_table must be int32 (got {page_table.dtype})")
+    specs = [(k_pages, "k_pages", dtype, 0), (v_pages, "v_pages", dtype, 0)]
+    if code == PAGE_FP4:
         scales = (n, kv, slots, d // FP4_GROUP)
         for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
             if t is None or t.shape != scales:
@@ -1359,7 +1364,7 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor |
             specs.append((t, name, U8, 0))
     elif k_scale is not None or v_scale is not None:
         raise ValueError("only 4-bit (uint8) pages have scales")
-    return (n, kv, slots, d), code, specs, (n_seq, width, ld if n_seq > 1 else max(width, 1))
+    return (n, kv, slots, d), code, specs, (n_seq, width, ld)
 
 
 def _on(dev: int, t: torch.Tensor, name: str) -> None:
@@ -1403,7 +1408,9 @@ def rope_cache_paged(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.Te
         raise ValueError("the rows of qkv must be contiguous")
     if rows <= 1:
         row_ld = columns
-    mx, my, mz, px, py, pz = (_at_most(n, C_INT_MAX) for n in rope_geom)   # larger: refused
+    mx, my, mz, px, py, pz = rope_geom
+    if min(rope_geom) < 0 or max(rope_geom) > C_INT_MAX:
+        raise ValueError(f"rope_geom {rope_geom} is out of range")
     in_dt, out_dt = cache_dtype_code(qkv), cache_dtype_code(q_out)
     specs += [(pos, "pos", I64, rows * 3),
               (rope_tab, "rope_tab", F32, 2 * (mx * px + my * py + mz * pz)),

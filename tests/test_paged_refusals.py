@@ -155,13 +155,15 @@ def test_wrappers_refuse():
             call()
     geom, ones = (8, 8, 8, 10, 10, 12), torch.ones(64)
 
-    def append(qkv=torch.zeros(3, 640), **kw):
+    def append(qkv=torch.zeros(3, 640), geom=geom, **kw):
         K.rope_cache_paged(qkv, None, off, ones, geom, off, off, table, 1.0, torch.zeros(3, 6, 64), k,
                            k, **kw)
     for what, call in [("GPU tensor", lambda: append()),
                        ("do not hold", lambda: append(torch.zeros(3, 448))),
                        ("must be contiguous", lambda: append(torch.zeros(3, 1280)[:, ::2])),
-                       ("together", lambda: append(q_gamma=ones))]:
+                       ("together", lambda: append(q_gamma=ones)),
+                       ("out of range", lambda: append(geom=(2 ** 31, 8, 8, 10, 10, 12))),
+                       ("out of range", lambda: append(geom=(8, 8, 8, -1, 21, 12)))]:
         with pytest.raises(ValueError, match=what):
             call()
 
