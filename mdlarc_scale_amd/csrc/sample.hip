@@ -28,6 +28,12 @@
 // row's second launch looks for the borders in their bins alone, cut by the digits of value and index
 // where thousands are equal, and takes the parts' kept sums from their bins.
 //
+//
+// What bounds it: one block's chain of steps, most of them waits.  64 rows of 131,072 logits, 52 us:
+// the bins 12 (64-bit arithmetic, 20 instructions a token), a row's second launch some 30 at the
+// median (3 for the parts' largest values, 2 for their bins, 4 for the scans, 8 for the pass over the
+// row, 2 to 6 for a border, 4 for the result) and 40 for the row with the most tokens kept; 256 rows of
+// 4,000 22 us; 256 of 14 5.0 us.
 #include <cfloat>
 
 #include "common.h"
@@ -219,61 +225,102 @@ struct Stretch {
     }
   }
   // f(value, index) for every token of the block's with least <= value <= most.  The loop over the row
-  // compares and no more: few tokens pass, and f works on them (read again) in a loop of its own, of
-  // which there is one copy.
+  // compares and no more: few tokens pass, and f works on them in a loop of its own, of which there is
+  // one copy.  (Read again there instead of picked from the registers, each step waited for memory: 11
+  // us a pass over 131,072 tokens, 7 so.)
   template <typename F>
   __device__ __forceinline__ void each_between(float least, float most, F f) const {
     const int t = threadIdx.x;
     const int rest = head + pieces * kEach + t;
-    constexpr int kAhead = 16 / kEach;
+    constexpr int kAhead = 16 / kEach, kStep = kAhead * kThreads;
     const uint4* from = reinterpret_cast<const uint4*>(x + head);
-    auto in = [&](float v) { return v >= least && v <= most; };   // not NaN
-    for (int c = t - kAhead * kThreads; c < pieces; c += kAhead * kThreads) {
-      uint32_t hits = 0;
+#pragma unroll 1
+    for (int c = t - kStep; c < pieces; c += kStep) {
+      float v[16];
       if (c < 0) {   // once, before the pieces: the first and last few tokens
-        hits = (t < head && in(logit(x, t)) ? 1u : 0u) | (rest < n && in(logit(x, rest)) ? 2u : 0u);
+        v[0] = t < head ? logit(x, t) : NAN;
+        v[1] = rest < n ? logit(x, rest) : NAN;
+#pragma unroll
+        for (int i = 2; i < 16; ++i) v[i] = NAN;
       } else {
         uint4 u[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) u[j] = from[min(c + j * kThreads, pieces - 1)];
+        for (int j = 0; j < kAhead; ++j) {
+          const uint32_t none = 0xffffffffu;   // NaN in either type
+          u[j] = c + j * kThreads < pieces ? from[c + j * kThreads]
+                                           : make_uint4(none, none, none, none);
+        }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-          float v[kEach];
-          values(u[j], v);
+          float w[kEach];
+          values(u[j], w);
 #pragma unroll
-          for (int i = 0; i < kEach; ++i)
-            hits |= in(v[i]) && c + j * kThreads < pieces ? 1u << (j * kEach + i) : 0u;
+          for (int i = 0; i < kEach; ++i) v[j * kEach + i] = w[i];
         }
       }
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) hits |= v[i] >= least && v[i] <= most ? 1u << i : 0u;
 #pragma unroll 1
       for (; hits != 0; hits &= hits - 1) {
         const int b = __ffs(hits) - 1;
+        float w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = v[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)   // halves the choice, bit by bit
+#pragma unroll
+          for (int i = 0; i < (8 >> k); ++i) w[i] = (b >> k & 1) ? w[2 * i + 1] : w[2 * i];
         const int i = c < 0 ? (b == 0 ? t : rest)
                             : head + (c + b / kEach * kThreads) * kEach + b % kEach;
-        f(logit(x, i), i);
+        f(w[0], i);
       }
     }
   }
 };
 
-// The sum of v over the threads before this one, and over all of them (`all`).
-__device__ __forceinline__ u64 block_scan(u64 v, u64* part, u64& all) {
+// The sums of a (and b) over the threads before this one, and over all of them.
+struct Scanned {
+  u64 a, b, all_a, all_b;
+};
+
+template <bool TWO>
+__device__ __forceinline__ Scanned block_scan(u64 a, u64 b, u64 (*part)[2]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u64 sa = a, sb = b, lanes_a = 0, lanes_b = 0;
   // twice the same code: over the lanes, then over the waves' sums
-  u64 sums = v, lanes = 0, first = 0;
 #pragma unroll 1
   for (int step = 0; step < 2; ++step) {
-    sums = wave_scan64(sums, lane);
+#pragma unroll 1
+    for (int o = 1; o < kWave; o <<= 1) {
+      const u64 ta = __shfl_up(sa, o, kWave), tb = TWO ? __shfl_up(sb, o, kWave) : 0;
+      if (lane >= o) {
+        sa += ta;
+        if (TWO) sb += tb;
+      }
+    }
     if (step == 1) break;
-    lanes = sums;
+    lanes_a = sa;
+    lanes_b = sb;
     __syncthreads();
-    if (lane == 63) part[wave] = sums;
+    if (lane == 63) {
+      part[wave][0] = sa;
+      if (TWO) part[wave][1] = sb;
+    }
     __syncthreads();
-    sums = lane < kWaves ? part[lane] : 0;
+    sa = lane < kWaves ? part[lane][0] : 0;
+    if (TWO) sb = lane < kWaves ? part[lane][1] : 0;
   }
-  all = __shfl(sums, kWave - 1, kWave);
-  first = __shfl(sums, wave == 0 ? 0 : wave - 1, kWave);
-  return lanes - v + (wave == 0 ? 0 : first);
+  Scanned r{};
+  r.all_a = __shfl(sa, kWave - 1, kWave);
+  const u64 fa = __shfl(sa, max(wave - 1, 0), kWave);
+  r.a = lanes_a - a + (wave == 0 ? 0 : fa);
+  if (TWO) {
+    r.all_b = __shfl(sb, kWave - 1, kWave);
+    const u64 fb = __shfl(sb, max(wave - 1, 0), kWave);
+    r.b = lanes_b - b + (wave == 0 ? 0 : fb);
+  }
+  return r;
 }
 
 // Ascending bitonic sort of list[0 .. n), n <= kList; the entries up to the next power of two are set.
@@ -374,7 +421,7 @@ struct Border {
 struct ListLds {
   u64 list[kList];
   u64 few[kThreads], few_sum[kThreads];
-  u64 part[kWaves];
+  u64 part[kWaves][2];
   u64 last, sum;
   int n, found, bin_k, bin_p, upto;
 };
@@ -400,9 +447,11 @@ struct Bins {
 
   __device__ __forceinline__ Bins(ListLds& s, const Filters& f, const Grid& g, u64 n, u64 m)
       : count(n), sum(m) {
-    u64 tokens;
-    count_before = block_scan(count, s.part, tokens);
-    sum_before = block_scan(sum, s.part, total);
+    const Scanned r = block_scan<true>(count, sum, s.part);
+    const u64 tokens = r.all_a;
+    count_before = r.a;
+    sum_before = r.b;
+    total = r.all_b;
     cut = f.top_k > 0 && tokens > static_cast<u64>(f.top_k);
     by_p = f.top_p < 1.0;
     by_m = f.min_p > 0.0;
@@ -439,8 +488,8 @@ __device__ __forceinline__ Border border_sorted(ListLds& s, const u64* list, int
     const int i = i0 + t;
     const u64 my = i < n ? list[i] : 0;
     const u64 w = i < n ? fixed(weight(value_at(my), top, f.c)) : 0;
-    u64 all;
-    const u64 before = m + block_scan(w, s.part, all);   // a barrier for s.found too
+    const Scanned r = block_scan<false>(w, 0, s.part);   // a barrier for s.found too
+    const u64 before = m + r.a;
     const bool in = i < n && (by_count ? c + i : before) < goal;
     if (in) atomicMax(&s.found, i);
     __syncthreads();
@@ -448,7 +497,39 @@ __device__ __forceinline__ Border border_sorted(ListLds& s, const u64* list, int
       s.last = my;
       s.sum = before + w;
     }
-    m += all;
+    m += r.all_a;
+  }
+  __syncthreads();
+  return Border{s.last, s.sum};
+}
+
+// The same of a list in any order; a call of all threads, the list is set.
+__device__ __forceinline__ Border border_of(ListLds& s, u64* list, int n, float top, const Filters& f,
+                                            bool by_count, u64 c, u64 m, u64 goal) {
+  const int t = threadIdx.x;
+  if (n > kCompared) {
+    sort_list(list, n);
+    return border_sorted(s, list, n, top, f, by_count, c, m, goal);
+  }
+  u64 rank = 0, before = 0, my = 0;
+  if (t < n) {
+    my = list[t];
+    s.few_sum[t] = fixed(weight(value_at(my), top, f.c));
+  }
+  if (t == 0) s.found = 0;
+  __syncthreads();
+  if (t < n) {
+    for (int j = 0; j < n; ++j) {
+      const bool ahead = list[j] < my;
+      rank += ahead;
+      before += ahead ? s.few_sum[j] : 0;
+    }
+    if ((by_count ? c + rank : m + before) < goal) atomicMax(&s.found, static_cast<int>(rank));
+  }
+  __syncthreads();
+  if (t < n && static_cast<int>(rank) == s.found) {
+    s.last = my;
+    s.sum = m + before + s.few_sum[t];
   }
   __syncthreads();
   return Border{s.last, s.sum};
@@ -481,36 +562,11 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
       for (int i = t; i < n; i += kThreads) {
         const u64 my = s.list[i];
         if (g.bin(value_at(my)) != at) continue;
-        const int k = atomicAdd(&s.n, 1);
-        s.few[k] = my;
-        s.few_sum[k] = fixed(weight(value_at(my), top, f.c));
+        s.few[atomicAdd(&s.n, 1)] = my;
       }
     }
     __syncthreads();
-    if (some > kCompared) {
-      sort_list(from, some);
-      return border_sorted(s, from, some, top, f, by_count, c, m, goal);
-    }
-    if (t == 0) s.found = 0;
-    u64 rank = 0, before = 0, my = 0;
-    if (t < some) {
-      my = s.few[t];
-      for (int j = 0; j < some; ++j) {
-        const bool ahead = s.few[j] < my;
-        rank += ahead;
-        before += ahead ? s.few_sum[j] : 0;
-      }
-    }
-    __syncthreads();
-    if (t < some && (by_count ? c + rank : m + before) < goal)
-      atomicMax(&s.found, static_cast<int>(rank));
-    __syncthreads();
-    if (t < some && static_cast<int>(rank) == s.found) {
-      s.last = my;
-      s.sum = m + before + s.few_sum[t];
-    }
-    __syncthreads();
-    return Border{s.last, s.sum};
+    return border_of(s, from, some, top, f, by_count, c, m, goal);
   };
   // top-k, then top-p, in one copy of the code (a border past the last bin of the list is past what
   // min-p keeps)
@@ -542,8 +598,8 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
   }
   __syncthreads();
   const u64 here = s.few_sum[t];
-  u64 total;
-  const u64 ahead = block_scan(here, s.part, total);
+  const Scanned r = block_scan<false>(here, 0, s.part);
+  const u64 ahead = r.a, total = r.all_a;
   const u64 goal = target_of(p.uniform[row], total);
   if (ahead <= goal && goal < ahead + here) {   // one thread
     s.found = t;
@@ -826,9 +882,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       });
       if (t == 0) s.digit = -1;
       __syncthreads();
-      u64 all;
       const u64 dc = counts[t], dm = sums[t];
-      const u64 cb = c + block_scan(dc, s.l.part, all), mb = m + block_scan(dm, s.l.part, all);
+      const Scanned r = block_scan<true>(dc, dm, s.l.part);
+      const u64 cb = c + r.a, mb = m + r.b;
       const u64 have = by_count ? cb : mb, more = by_count ? dc : dm;
       if (have < goal && have + more >= goal) s.digit = t;
       __syncthreads();
@@ -860,9 +916,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     });
     __syncthreads();
     listed = shift == 64 ? bin : -1;
-    const int n = s.l.n;
-    sort_list(s.l.list, n);
-    return border_sorted(s.l, s.l.list, n, top, f, by_count, c, m, goal);
+    return border_of(s.l, s.l.list, s.l.n, top, f, by_count, c, m, goal);
   };
 
   Border border{~u64{0}, b.total};
@@ -940,8 +994,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  u64 sums;
-  const u64 ahead = block_scan(here, s.l.part, sums);
+  const Scanned r = block_scan<false>(here, 0, s.l.part);
+  const u64 ahead = r.a, sums = r.all_a;
   const double want = static_cast<double>(goal) / against;
   const u64 at_sum = want < static_cast<double>(sums) ? min(static_cast<u64>(want), sums - 1) : sums - 1;
   if (!(ahead <= at_sum && at_sum < ahead + here)) return;   // one thread stays
