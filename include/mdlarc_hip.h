@@ -751,7 +751,8 @@ int64_t mdl_attn_decode_shared_workspace_bytes(int batch, int n_prefix, int max_
  * many slots as the longest.
  *
  * K9, append: mdl_qk_norm_rope_cache with the pages of token m's sequence token_row[m] in place of a
- * cache row, and norms only where q_gamma and k_gamma are not NULL (both or neither).  A slot outside
+ * cache row, and norms only where q_gamma and k_gamma are not NULL (both or neither).  No two tokens may
+ * name the same slot (what remains there is not defined, in 4 bits not even one of them).  A slot outside
  * the table, a sequence outside it and a page number outside the pool are not written.  q_out is of
  * q_dtype, the pages' type unless those are MDL_DTYPE_FP4.  4 bits: the 32 channels' power is the
  * smallest 2^k, -100 <= k <= 125, by which all their magnitudes are below 7, and each value times
@@ -783,7 +784,8 @@ int mdl_paged_rows(const void* k_pages, const void* v_pages, int page_dtype,
 /*
  * K10: mdl_attn_grouped with the pages of a sequence in place of its cache row; cache_slots is
  * table_width * page_slots.  q (and out) are of dtype, the pages' type unless those are
- * MDL_DTYPE_FP4, whose values enter the products as they are.  A sequence that has a page number
+ * MDL_DTYPE_FP4, whose values enter the products as they are (fp32 q of single tokens, max_q 1, over
+ * 4-bit pages: weights below 2^-126 of the largest are zero).  A sequence that has a page number
  * outside the pool among the pages of its keys reads no memory outside the pool and gives NaN in every
  * row that sees such a page (and may in its other rows).
  */
@@ -809,7 +811,8 @@ int64_t mdl_attn_paged_workspace_bytes(int n_seq, int tokens, int max_q, int n_h
  *   logprob_out[r]  (may be NULL) ln of the token's share of the kept weights.
  * temperature, top_k, top_p and min_p are device arrays of a number a row; NULL is 1 and no filter.  A
  * temperature of 0 or below (or NaN), a top_k of 1, a top_p of 0 or below and a min_p above 1 give the
- * first of the order, with logprob 0.  NaN logits count as -inf, which is never taken; a row of nothing
+ * first of the order, with logprob 0; a NaN top_p or min_p is no filter.  uniform outside [0, 1) is taken
+ * as the nearest inside.  NaN logits count as -inf, which is never taken; a row of nothing
  * else gives token 0 and logprob -inf.  Weights are of 64 bits and their sums do not depend on an order,
  * so equal calls give equal tokens; tokens below 2^-43 of the largest may count as nothing.
  * workspace (8-byte aligned): mdl_sample_workspace_bytes of the same sizes, 0 up to 4,096 tokens; calls

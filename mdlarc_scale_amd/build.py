@@ -72,7 +72,8 @@ def _run(cmd: list[str]) -> str:
                            f"{res.stdout}\n{res.stderr}")
     noisy = [ln for ln in res.stderr.splitlines()
              if ln.strip() and "packed-fp32-ops" not in ln and "remark:" not in ln
-             and "'--hip-link'" not in ln]   # hipcc adds it to the device-only assembly pass
+             and "'--hip-link'" not in ln   # hipcc adds it to the device-only assembly pass
+             and not ln.startswith("In file included from")]   # before remarks on a header's kernels
     if noisy:
         print("\n".join(noisy), file=sys.stderr)
     return res.stderr

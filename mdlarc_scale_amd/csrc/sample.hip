@@ -28,7 +28,6 @@
 // row's second launch looks for the borders in their bins alone, cut by the digits of value and index
 // where thousands are equal, and takes the parts' kept sums from their bins.
 //
-//
 // What bounds it: one block's chain of steps, most of them waits.  64 rows of 131,072 logits, 52 us:
 // the bins 12 (64-bit arithmetic, 20 instructions a token), a row's second launch some 30 at the
 // median (3 for the parts' largest values, 2 for their bins, 4 for the scans, 8 for the pass over the
@@ -146,7 +145,8 @@ __device__ __forceinline__ Filters filters_of(const SampleArgs& p, int row) {
   const float t = p.temperature ? p.temperature[row] : 1.f;
   f.top_k = p.top_k ? max(p.top_k[row], 0) : 0;
   f.top_p = p.top_p ? static_cast<double>(p.top_p[row]) : 1.0;
-  f.min_p = p.min_p ? static_cast<double>(p.min_p[row]) : 0.0;
+  const float m = p.min_p ? p.min_p[row] : 0.f;
+  f.min_p = m > 0.f ? static_cast<double>(m) : 0.0;   // NaN: none
   // a share of nothing, and a bound that no weight reaches, leave the first token
   f.greedy = !(t > 0.f) || f.top_k == 1 || f.top_p <= 0.0 || f.min_p > 1.0;
   f.c = kLog2e / static_cast<double>(fminf(t, FLT_MAX));

@@ -1345,13 +1345,13 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor |
     if len(wide) != 2:
         raise ValueError(f"page_table must be [sequences, pages] (got {tuple(wide)})")
     n_seq, width = wide
-    ld = width if width else 1
-    if n_seq > 1 or not page_table.is_contiguous():
-        ld, step = page_table.stride()
-        if (width > 1 and step != 1) or (n_seq > 1 and ld < width):
-            raise ValueError("page_table must have contiguous rows that do not overlap")
-        if n_seq <= 1:
-            ld = width if width else 1
+    if n_seq and not width:
+        raise ValueError("page_table has no columns")
+    ld, step = page_table.stride()
+    if (width > 1 and step != 1) or (n_seq > 1 and ld < width):
+        raise ValueError("page_table must have contiguous rows that do not overlap")
+    if n_seq <= 1:
+        ld = width
     if page_table.dtype is not I32:
         raise ValueError(f"page_table must be int32 (got {page_table.dtype})")
     specs = [(k_pages, "k_pages", dtype, 0), (v_pages, "v_pages", dtype, 0)]
@@ -1424,6 +1424,8 @@ def rope_cache_paged(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.Te
     _on(dev, page_table, "page_table")
     if rows == 0:
         return
+    if not n_seq:
+        raise ValueError("a page_table without rows has no sequence for the tokens of qkv")
     _launch(dev, "mdl_rope_cache_paged", qkv.data_ptr(), in_dt, row_ld, _ptr(rstd), pos.data_ptr(),
             rope_tab.data_ptr(), rows, token_row.data_ptr(), token_slot.data_ptr(),
             page_table.data_ptr(), ld, n_seq, width, n_pages, slots, heads, kv, d, mx, my, mz, px,

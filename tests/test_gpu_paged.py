@@ -493,6 +493,42 @@ def test_append_gives_the_bits_of_the_contiguous_form():
         assert torch.equal(rows_out[0], cache[0]) and torch.equal(rows_out[1], cache[1])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D,heads,kv", [(64, 12, 4), (128, 10, 5)])
+def test_append_fp4_with_norms(dtype, D, heads, kv):
+    """Normed heads in 4 bits: within half a step of the formula's values, by a power that is the
+    formula's but where its largest value lies at a border of two."""
+    g = _gen(D + kv)
+    rows, page, n_seq = 150, 32, 3
+    qkv = _rand(g, rows, (heads + 2 * kv) * D, std=3.0)
+    rstd = torch.rand(rows, generator=g) + 0.3
+    pos = torch.randint(0, 30, (rows, 3), generator=g)
+    tab, geom = _rope(D)
+    gains = 1 + 0.2 * _rand(g, D), 1 + 0.2 * _rand(g, D)
+    row, slot = _tokens(g, rows, n_seq, 64)
+    table = page_table([2] * n_seq, 2, 6, g)
+    dev = lambda t: t.to(DEV)  # noqa: E731
+    pools = [torch.zeros(6, kv, page, D // 2, dtype=U8, device=DEV) for _ in range(2)]
+    scales = [torch.zeros(6, kv, page, D // 32, dtype=U8, device=DEV) for _ in range(2)]
+    q = torch.zeros(rows, heads, D, dtype=dtype, device=DEV)
+    K().rope_cache_paged(dev(qkv), dev(rstd), dev(pos), dev(tab), geom, dev(row), dev(slot),
+                         dev(table), 0.5, q, *pools, k_scale=scales[0], v_scale=scales[1],
+                         q_gamma=dev(gains[0]), k_gamma=dev(gains[1]))
+    refs = _qk_norm_reference(qkv, rstd, pos, tab, geom, *gains, 1e-5, heads, kv, D, 0.5)
+    half = HALF_STEP[dtype]
+    _check(q, refs[0][0], refs[0][1] * (1 + half) + half * refs[0][0].abs() + 1e-30, "q")
+    number, at = table[row.long(), slot.long() // page].long(), slot.long() % page
+    for pool, scale, (ref, err) in zip(pools, scales, refs[1:]):
+        codes, power = pool.cpu()[number, :, at], scale.cpu()[number, :, at]
+        step = torch.pow(2.0, power.double() - 127).repeat_interleave(32, -1)
+        size = ref.abs() / step
+        _check(from_fp4(codes, power), ref,
+               err + step * torch.where(size < 2, 0.25, torch.where(size < 4, 0.5, 1.0)) *
+               (1 + 2.0 ** -20), "pages")
+        top = ref.unflatten(-1, (-1, 32)).abs().amax(-1) / torch.pow(2.0, power.double() - 127)
+        assert bool(((top < 7 * (1 + 2.0 ** -18)) & (top > 3.5 * (1 - 2.0 ** -18))).all())
+
+
 @pytest.mark.parametrize("source", [F32, BF])
 def test_append_fp4_edges(source):
     """Borders between numbers, groups of zeros, the smallest and largest powers, and values that are

@@ -139,6 +139,25 @@ def test_masked_rows_and_values_that_are_not_finite(vocab):
         assert bool((lp[2:] == 0).all())
 
 
+@pytest.mark.parametrize("vocab", [14, 900, 30011])
+def test_filters_that_are_none(vocab):
+    """Numbers that switch a filter off, NaN among them, and a workspace of the caller's."""
+    nan, inf = float("nan"), float("inf")
+    x, u, _ = rows_of(vocab, 4, vocab, F32)
+    plain, lp = draw(x, u)
+    for f in (dict(top_k=[0, -1, -2 ** 31, vocab]), dict(top_p=[1.0, 7.0, inf, nan]),
+              dict(min_p=[0.0, -1.0, -inf, nan]), dict(top_k=[2 ** 31 - 1] * 4)):
+        token, lp2 = draw(x, u, **f)
+        assert torch.equal(token, plain) and torch.equal(lp, lp2), f
+    token = torch.zeros(4, dtype=torch.int64, device=DEV)
+    ws = torch.empty(K().sample_workspace_bytes(4, vocab), dtype=torch.uint8, device=DEV)
+    K().sample_tokens(x.to(DEV), u.to(DEV), token, workspace=ws)
+    assert torch.equal(token.cpu(), plain)
+    if vocab > 4096:
+        with pytest.raises(RuntimeError, match="workspace"):
+            K().sample_tokens(x.to(DEV), u.to(DEV), token, workspace=ws[:-8])
+
+
 @pytest.mark.parametrize("vocab", [14, 900])
 def test_random_numbers_at_the_ends(vocab):
     x, _, _ = rows_of(8, 6, vocab, F32)
@@ -176,8 +195,11 @@ def test_frequencies_follow_the_shares():
     assert bool(((count - n * share).abs() <= 1 + 1e-6).all())
 
 
-def test_graph_streams_and_no_logprob():
-    x, u, _ = rows_of(9, 40, 2000, F32)
+@pytest.mark.parametrize("vocab", [14, 2000, 9000])
+def test_graph_streams_and_no_logprob(vocab):
+    """Captured calls (a long row's takes its workspace from the capture's pool) replayed with other
+    data between eager calls, two of them side by side."""
+    x, u, _ = rows_of(9, 40, vocab, F32)
     xd, ud = x.to(DEV), u.to(DEV)
     token, p = torch.zeros(40, dtype=torch.int64, device=DEV), torch.full((40,), 0.7, device=DEV)
     call = lambda: K().sample_tokens(xd, ud, token, top_p=p)  # noqa: E731
@@ -189,13 +211,23 @@ def test_graph_streams_and_no_logprob():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         call()
+    other, u3, _ = rows_of(10, 40, vocab, F32)
+    other, u3, token3 = other.to(DEV), u3.to(DEV), torch.zeros_like(token)
+    graph3 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph3):
+        K().sample_tokens(other, u3, token3, top_p=p)
+    want3, _ = draw(other, u3, logprob=False, top_p=p)
     for step in range(3):
-        x2, u2, _ = rows_of(50 + step, 40, 2000, F32)
+        x2, u2, _ = rows_of(50 + step, 40, vocab, F32)
         xd.copy_(x2)
         ud.copy_(u2)
         token.fill_(-1)
+        token3.fill_(-1)
+        torch.cuda.synchronize()
         graph.replay()
+        with torch.cuda.stream(side):
+            graph3.replay()
         torch.cuda.synchronize()
         want, _ = draw(x2, u2, logprob=False, top_p=p)
-        assert torch.equal(token.cpu(), want)
+        assert torch.equal(token.cpu(), want) and torch.equal(token3.cpu(), want3)
     K().sample_tokens(xd[:0], ud[:0], token[:0])

@@ -136,6 +136,7 @@ def test_wrappers_refuse():
             ("int32", lambda: attend(table=table.long())),
             ("contiguous rows", lambda: attend(table=table[:, ::2])),
             ("do not overlap", lambda: attend(table=table[:1].expand(2, -1))),
+            ("no columns", lambda: attend(table=table[:, :0])),
             ("only 4-bit", lambda: attend(k_scale=s, v_scale=s)),
             ("k_scale must", lambda: attend(k=k4, v=k4)),
             ("v_scale must", lambda: attend(k=k4, v=k4, k_scale=s, v_scale=s[:2])),
