@@ -180,9 +180,13 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs p) {
   const u64 mine = fixed(w), at = place(x, lane);
   int rank = 0;
   u64 before = 0;
+  auto lane64 = [](u64 v, int j) {
+    return static_cast<u64>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), j)) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), j));
+  };
   for (int j = 0; j < p.vocab; ++j) {
-    const bool ahead = __shfl(at, j, kWave) < at;
-    const u64 other = __shfl(mine, j, kWave);
+    const bool ahead = lane64(at, j) < at;
+    const u64 other = lane64(mine, j);
     rank += ahead;
     before += ahead ? other : 0;
   }
