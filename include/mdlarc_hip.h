@@ -14,7 +14,7 @@
  *   - Return 0 on success, a negative MDL_ERR_* for arguments rejected on the host before any
  *     launch, or a positive hipError_t reported by the launch.
  *   - Head dimension is 64 (all reference model sizes, src/transformer.py:728-745); the entries for
- *     grouped key / value heads (K7, K8) take 64 and 128.
+ *     grouped key / value heads and for caches in pages (K7 to K10) take 64 and 128.
  *   - GEMM inputs ("split activations") are written as hi|lo bf16 pairs: a row of K values is 2K
  *     bf16, hi = bf16(v) in columns [0, K), lo = bf16(v - hi) in [K, 2K).  Multiplied with a
  *     weight packed as [W | W] ([N, 2K] bf16) a bf16 GEMM with fp32 accumulation returns

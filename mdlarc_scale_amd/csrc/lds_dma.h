@@ -1,5 +1,5 @@
 // Direct global -> LDS copies (gfx950 global_load_lds_dwordx4), shared by the kernels that stage
-// their operands in LDS rings (K6, K4a, K4f, K8).
+// their operands in LDS rings (K6, K4a, K4f, K8, K10).
 #pragma once
 
 #include "common.h"
