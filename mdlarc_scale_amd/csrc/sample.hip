@@ -106,20 +106,36 @@ __device__ __forceinline__ float value_at(u64 place) {
 
 // Loops here stay loops: a block runs through most of its code once, so that the time to fetch its
 // instructions counts (a row's second launch took 47 us with 14,800 of them).
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll 1
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+
+// v of another lane by DPP: CTRL 0x110 + n takes it from n lanes before in the row of 16, 0x142 gives
+// lane 15 of a row to the next one, 0x143 lane 31 to the upper half; `none` where there is no such lane.
+// (Shuffles through LDS take some 100 cycles a step, these some 20.)
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t none, uint32_t v) {
+  return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
 }
 
-__device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {   // inclusive
-#pragma unroll 1
-  for (int o = 1; o < kWave; o <<= 1) {
-    const u64 t = __shfl_up(v, o, kWave);
-    if (lane >= o) v += t;
-  }
-  return v;
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ u64 plus_dpp(u64 v) {
+  return v + (static_cast<u64>(dpp<CTRL, ROWS>(0, static_cast<uint32_t>(v >> 32))) << 32 |
+              dpp<CTRL, ROWS>(0, static_cast<uint32_t>(v)));
 }
+
+// the sums over 16 neighbouring lanes up to the lane's own
+__device__ __forceinline__ u64 row_scan64(u64 v) {
+  return plus_dpp<0x118>(plus_dpp<0x114>(plus_dpp<0x112>(plus_dpp<0x111>(v))));
+}
+
+__device__ __forceinline__ u64 wave_scan64(u64 v) {   // inclusive
+  return plus_dpp<0x143, 0xc>(plus_dpp<0x142, 0xa>(row_scan64(v)));
+}
+
+__device__ __forceinline__ u64 of_lane(u64 v, int lane) {   // the same lane for the whole wave
+  return static_cast<u64>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane)) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane));
+}
+
+__device__ __forceinline__ u64 wave_sum64(u64 v) { return of_lane(wave_scan64(v), 63); }
 
 // The sum that the token's own has to pass.  u outside [0, 1) is taken as the nearest inside.
 __device__ __forceinline__ u64 target_of(float u, u64 total) {
@@ -180,13 +196,9 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs p) {
   const u64 mine = fixed(w), at = place(x, lane);
   int rank = 0;
   u64 before = 0;
-  auto lane64 = [](u64 v, int j) {
-    return static_cast<u64>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), j)) << 32 |
-           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), j));
-  };
   for (int j = 0; j < p.vocab; ++j) {
-    const bool ahead = lane64(at, j) < at;
-    const u64 other = lane64(mine, j);
+    const bool ahead = of_lane(at, j) < at;
+    const u64 other = of_lane(mine, j);
     rank += ahead;
     before += ahead ? other : 0;
   }
@@ -196,8 +208,8 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs p) {
     kept = kept && before < share_of(f.top_p, sum);
   }
   kept = kept && w >= f.min_p;
-  const u64 sums = wave_scan64(kept ? mine : 0, lane);
-  const u64 total = __shfl(sums, 63, kWave);
+  const u64 sums = wave_scan64(kept ? mine : 0);
+  const u64 total = of_lane(sums, 63);
   const u64 goal = target_of(p.uniform[row], total);
   const u64 past = __ballot(sums > goal);
   if (lane == __ffsll(past) - 1) leave(p, row, lane, w, total);
@@ -290,39 +302,23 @@ struct Scanned {
 
 template <bool TWO>
 __device__ __forceinline__ Scanned block_scan(u64 a, u64 b, u64 (*part)[2]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 sa = a, sb = b, lanes_a = 0, lanes_b = 0;
-  // twice the same code: over the lanes, then over the waves' sums
-#pragma unroll 1
-  for (int step = 0; step < 2; ++step) {
-#pragma unroll 1
-    for (int o = 1; o < kWave; o <<= 1) {
-      const u64 ta = __shfl_up(sa, o, kWave), tb = TWO ? __shfl_up(sb, o, kWave) : 0;
-      if (lane >= o) {
-        sa += ta;
-        if (TWO) sb += tb;
-      }
-    }
-    if (step == 1) break;
-    lanes_a = sa;
-    lanes_b = sb;
-    __syncthreads();
-    if (lane == 63) {
-      part[wave][0] = sa;
-      if (TWO) part[wave][1] = sb;
-    }
-    __syncthreads();
-    sa = lane < kWaves ? part[lane][0] : 0;
-    if (TWO) sb = lane < kWaves ? part[lane][1] : 0;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u64 sa = wave_scan64(a), sb = TWO ? wave_scan64(b) : 0;
+  __syncthreads();
+  if (lane == 63) {
+    part[wave][0] = sa;
+    if (TWO) part[wave][1] = sb;
   }
+  __syncthreads();
+  static_assert(kWaves == 16, "the waves' sums in a row of lanes");
+  const u64 wa = row_scan64(part[lane & 15][0]), wb = TWO ? row_scan64(part[lane & 15][1]) : 0;
+  const int before = max(wave - 1, 0);
   Scanned r{};
-  r.all_a = __shfl(sa, kWave - 1, kWave);
-  const u64 fa = __shfl(sa, max(wave - 1, 0), kWave);
-  r.a = lanes_a - a + (wave == 0 ? 0 : fa);
+  r.all_a = of_lane(wa, kWaves - 1);
+  r.a = sa - a + (wave == 0 ? 0 : of_lane(wa, before));
   if (TWO) {
-    r.all_b = __shfl(sb, kWave - 1, kWave);
-    const u64 fb = __shfl(sb, max(wave - 1, 0), kWave);
-    r.b = lanes_b - b + (wave == 0 ? 0 : fb);
+    r.all_b = of_lane(wb, kWaves - 1);
+    r.b = sb - b + (wave == 0 ? 0 : of_lane(wb, before));
   }
   return r;
 }
@@ -635,29 +631,38 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
     leave(p, row, static_cast<int>(static_cast<uint32_t>(my)), weight(value_at(my), top, f.c), total);
 }
 
-__device__ __forceinline__ void wave_top(float& top, int& at) {
-#pragma unroll 1
-  for (int o = 32; o > 0; o >>= 1) {
-    const float x = __shfl_xor(top, o, kWave);
-    const int i = __shfl_xor(at, o, kWave);
-    if (x > top || (x == top && i < at)) {
-      top = x;
-      at = i;
-    }
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ void top_dpp(float& top, int& at) {
+  const float x = __uint_as_float(dpp<CTRL, ROWS>(__float_as_uint(top), __float_as_uint(top)));
+  const int i = static_cast<int>(dpp<CTRL, ROWS>(at, at));
+  if (x > top || (x == top && i < at)) {
+    top = x;
+    at = i;
   }
+}
+
+__device__ __forceinline__ void row_top(float& top, int& at) {   // in lane 15 of 16
+  top_dpp<0x111>(top, at);
+  top_dpp<0x112>(top, at);
+  top_dpp<0x114>(top, at);
+  top_dpp<0x118>(top, at);
 }
 
 // The row's largest value and its first index (0x7fffffff: there is none above -inf).
 __device__ __forceinline__ void block_top(float& top, int& at, float* part_top, int* part_at) {
-  wave_top(top, at);
-  if ((threadIdx.x & 63) == 0) {
+  row_top(top, at);
+  top_dpp<0x142, 0xa>(top, at);
+  top_dpp<0x143, 0xc>(top, at);
+  if ((threadIdx.x & 63) == 63) {
     part_top[threadIdx.x >> 6] = top;
     part_at[threadIdx.x >> 6] = at;
   }
   __syncthreads();
   top = part_top[threadIdx.x & (kWaves - 1)];
   at = part_at[threadIdx.x & (kWaves - 1)];
-  wave_top(top, at);
+  row_top(top, at);
+  top = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), kWaves - 1));
+  at = __builtin_amdgcn_readlane(at, kWaves - 1);
 }
 
 __device__ __forceinline__ bool leave_first(const SampleArgs& p, const Filters& f, int row, float top,
