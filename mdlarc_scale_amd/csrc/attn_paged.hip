@@ -68,7 +68,7 @@ int launch_source(const PagedArgs& a, bool fp4, bool tall, unsigned blocks, hipS
 // The waves of a block take the tiles in turn and merge at the end.  A value that is not finite is
 // seen by every row or (keys behind the last) set to zero.
 // fp32, us, with the tiles above / so: 64 rows of up to 1,500 keys (12 heads of 64) 136 / 86, 64 of
-// 4,000 (32 heads on 8 of 128) 320 / 291, 16 of 1,203 (12 heads on 4 of 64) 18.5 / 15.1.
+// 4,000 (32 heads on 8 of 128) 320 / 291, 16 of 1,203 (12 heads on 4 of 64) 18.5 / 14.9.
 enum TokenForm { kTokenFp4, kTokenFp4F32, kTokenF32 };
 
 template <int D, int FORM>
@@ -486,19 +486,26 @@ bool takes_tokens(int page_dtype, int max_q, int n_heads, int n_kv_heads) {
 Plan plan_paged(int n_seq, int max_q, int n_heads, int n_kv_heads, int head_dim, int dtype,
                 int page_dtype, int slots, int max_parts) {
   if (takes_tokens(page_dtype, max_q, n_heads, n_kv_heads)) {
-    // Parts of the keys, which a second launch joins (some 3 us): to two blocks a CU, if the keys are
-    // worth three parts of two turns of the block's waves at least; to eight a CU in parts of 2,048
-    // keys or more.  us, so / in more or fewer parts: 64 rows of 32,750 keys (32 heads on 8 of 128) in
-    // 4 286 / in 2 335 / in 6 285; 64 of 2,000 uncut 26 / in 3 33; 4 of 2,000 in 7 8.5 / uncut 16; 16
-    // of 811 (12 heads on 4 of 64) uncut 7.7 / in 3 8.6; 16 of 20,000 (12 heads of 64) in 9 58 / in 6
-    // 63 / in 32 65.
+    // Parts of the keys, which a second launch joins (some 3 us), three at least.
+    // fp32: parts of 128 keys or more and up to two blocks a CU, the number that takes the fewest rounds
+    // of 256 blocks for its work.  us, so / to two blocks a CU in parts of 256 keys (12 heads on 4 of 64
+    // and 32 on 8 of 128 where no others are named): 16 rows of 811 keys (12 heads) 20.2 / 23.0, 8 of
+    // 1,203 (12 heads) 15.6 / 22.2, 4 of 1,203 11.0 / 13.2, 32 of 600 (8 heads of 128) 25.5 / 32.1.
+    // 4 bits: parts of 256 keys or more, 16 at most (all numbers of parts are read by the second launch),
+    // to two blocks a CU.  us, so / in 32 parts: 2 rows of 8,000 keys 11.4 / 13.8; in parts of 256 keys /
+    // of 512: 4 of 2,203 (64 dims) 8.4 / 9.6; cut / uncut: 4 of 2,000 8.5 / 16; 64 of 2,000 33 / 26.
+    // Both: to eight blocks a CU in parts of 2,048 keys or more: 64 rows of 32,750 4-bit keys in 4 parts
+    // 286, in 2 335, in 6 285; 16 of 20,000 (12 heads of 64) in 9 58, in 6 63, in 32 65.
     const int64_t pairs = static_cast<int64_t>(n_seq) * n_kv_heads;
     const bool f32 = page_dtype == MDL_DTYPE_F32;
-    const int turn = head_dim == 128
-        ? (f32 ? TokenShape<128, kTokenF32>::kTurn : TokenShape<128, kTokenFp4>::kTurn)
-        : (f32 ? TokenShape<64, kTokenF32>::kTurn : TokenShape<64, kTokenFp4>::kTurn);
-    const int64_t few = slots / (2 * turn), many = slots / 2048;
-    int64_t ns = few < 3 ? 1 : std::min<int64_t>((512 + pairs - 1) / pairs, few);
+    const int64_t few = f32 ? slots / 128 : std::min(slots / 256, 16), many = slots / 2048;
+    int64_t ns = 1;
+    if (few >= 3 && !f32) ns = std::min<int64_t>((512 + pairs - 1) / pairs, few);
+    if (few >= 3 && f32) {
+      auto rounds = [&](int64_t n) { return (pairs * n + 255) / 256; };
+      for (int64_t n = 2; n <= few && n <= kMaxParts && pairs * n <= 512; ++n)
+        if (rounds(n) * ns < rounds(ns) * n) ns = n;
+    }
     ns = std::max(ns, std::min<int64_t>((2048 + pairs - 1) / pairs, many));
     return Plan{false, 1, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ns, max_parts)))};
   }
