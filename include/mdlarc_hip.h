@@ -827,6 +827,16 @@ int mdl_sample_tokens(const void* logits, int dtype, int64_t ld, int rows, int v
 int64_t mdl_sample_workspace_bytes(int rows, int vocab);
 
 /*
+ * mdl_rope_cache_paged, mdl_paged_rows, mdl_attn_paged and mdl_sample_tokens with their arguments, all but
+ * the stream, in a block of host memory: in their order, each as a member of a C struct of them would lie.
+ * The block is read before the call returns.
+ */
+int mdl_rope_cache_paged_block(const void* args, void* stream);
+int mdl_paged_rows_block(const void* args, void* stream);
+int mdl_attn_paged_block(const void* args, void* stream);
+int mdl_sample_tokens_block(const void* args, void* stream);
+
+/*
  * Every layer of a prompt or decode step from one call (host code over the entries above, which
  * check their arguments as always; the first error ends the call).  Activations are in the tile
  * layouts; f32: the fp32 form (fp32 q and caches, every *_lo given).

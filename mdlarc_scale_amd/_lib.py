@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import re
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 
@@ -159,6 +160,10 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mdl_sample_tokens": (c_int, [P, c_int, c_int64, c_int, c_int, P, P, P, P, P, P, P, P, c_int64,
                                   P]),
     "mdl_sample_workspace_bytes": (c_int64, [c_int, c_int]),
+    "mdl_rope_cache_paged_block": (c_int, [ctypes.c_char_p, P]),
+    "mdl_paged_rows_block": (c_int, [ctypes.c_char_p, P]),
+    "mdl_attn_paged_block": (c_int, [ctypes.c_char_p, P]),
+    "mdl_sample_tokens_block": (c_int, [ctypes.c_char_p, P]),
     "mdl_lm_head": (c_int, [P, P, c_int, c_int, P, c_float, P, c_int, P, P, CONS, c_int, P]),
     "mdl_decode_head": (c_int, [P, c_int, c_int, P, c_float, P, c_int, P, P, P, c_int64, c_int,
                                 P, P, c_int, c_int, CONS, c_int, P]),
@@ -168,6 +173,13 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mdl_grid_step": (c_int, [P, c_int, c_int, c_int, P, P, P, P, P, P]),
     "mdl_decode_commit": (c_int, [P, c_int, P, c_int64, c_int, P, P, c_int, c_int, P]),
 }
+
+# The entries that also take their arguments in a block: the name of that form, and the packer (ctypes
+# converts each argument of a call by itself, four times as slow).  It takes no None for a pointer and
+# raises struct.error for a number out of range.
+BLOCKS = {name: (name + "_block", struct.Struct("".join(
+    {P: "P", c_int: "i", c_int64: "q", c_float: "f"}[a] for a in args[:-1])).pack)
+    for name, (_, args) in SIGNATURES.items() if name + "_block" in SIGNATURES}
 
 _LIB: ctypes.CDLL | None = None
 

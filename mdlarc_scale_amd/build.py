@@ -36,6 +36,7 @@ SOURCES = [
     "qk_norm.hip",
     "paged_cache.hip",
     "sample.hip",
+    "arg_blocks.hip",
     "head_state.hip",
     "prompt_build.hip",
     "split_gemm.hip",

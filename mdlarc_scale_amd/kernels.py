@@ -9,6 +9,7 @@ non-zero library status raises ``RuntimeError`` / ``ValueError``.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -1133,6 +1134,16 @@ def _launch(dev: int, name: str, *args) -> None:
         _lib.check(code, name)
 
 
+def _launch_block(dev: int, name: str, *args) -> None:
+    """``_launch`` of an entry that takes its arguments in a block (0 for an absent pointer)."""
+    entry, pack = _lib.BLOCKS[name]
+    try:
+        block = pack(*args)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"{name}: a number is out of range ({e})") from None
+    _launch(dev, entry, block)
+
+
 def _same_shapes(k: torch.Tensor, v: torch.Tensor, name: str, shape: tuple, want: tuple) -> None:
     """K (of ``shape``) and V caches [rows, kv_heads, slots, head_dim] of one shape; ``want`` without
     the slots."""
@@ -1373,8 +1384,8 @@ def _on(dev: int, t: torch.Tensor, name: str) -> None:
                          "one device")
 
 
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def rope_cache_paged(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.Tensor,
@@ -1426,11 +1437,12 @@ def rope_cache_paged(qkv: torch.Tensor, rstd: torch.Tensor | None, pos: torch.Te
         return
     if not n_seq:
         raise ValueError("a page_table without rows has no sequence for the tokens of qkv")
-    _launch(dev, "mdl_rope_cache_paged", qkv.data_ptr(), in_dt, row_ld, _ptr(rstd), pos.data_ptr(),
-            rope_tab.data_ptr(), rows, token_row.data_ptr(), token_slot.data_ptr(),
-            page_table.data_ptr(), ld, n_seq, width, n_pages, slots, heads, kv, d, mx, my, mz, px,
-            py, pz, _ptr(q_gamma), _ptr(k_gamma), eps, q_scale, q_out.data_ptr(), out_dt,
-            k_pages.data_ptr(), v_pages.data_ptr(), code, _ptr(k_scale), _ptr(v_scale))
+    _launch_block(dev, "mdl_rope_cache_paged", qkv.data_ptr(), in_dt, row_ld, _ptr(rstd),
+                  pos.data_ptr(), rope_tab.data_ptr(), rows, token_row.data_ptr(),
+                  token_slot.data_ptr(), page_table.data_ptr(), ld, n_seq, width, n_pages, slots,
+                  heads, kv, d, mx, my, mz, px, py, pz, _ptr(q_gamma), _ptr(k_gamma), eps, q_scale,
+                  q_out.data_ptr(), out_dt, k_pages.data_ptr(), v_pages.data_ptr(), code,
+                  _ptr(k_scale), _ptr(v_scale))
 
 
 def paged_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -1456,10 +1468,10 @@ def paged_rows(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     _on(dev, page_table, "page_table")
     if n_seq == 0 or shape[2] == 0:
         return
-    _launch(dev, "mdl_paged_rows", k_pages.data_ptr(), v_pages.data_ptr(), code, _ptr(k_scale),
-            _ptr(v_scale), page_table.data_ptr(), ld, n_seq, width, n_pages, slots, kv, d,
-            start.data_ptr(), count.data_ptr(), shape[2], k_out.data_ptr(), v_out.data_ptr(),
-            cache_dtype_code(k_out))
+    _launch_block(dev, "mdl_paged_rows", k_pages.data_ptr(), v_pages.data_ptr(), code,
+                  _ptr(k_scale), _ptr(v_scale), page_table.data_ptr(), ld, n_seq, width, n_pages,
+                  slots, kv, d, start.data_ptr(), count.data_ptr(), shape[2], k_out.data_ptr(),
+                  v_out.data_ptr(), cache_dtype_code(k_out))
 
 
 def _paged_q(q: torch.Tensor, kv: int, d: int) -> tuple[int, int]:
@@ -1502,7 +1514,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     dev, code = q.get_device(), cache_dtype_code(q)
     specs += [(q, "q", dt, 0), (q_offset, "q_offset", I32, 0), (kv_len, "kv_len", I32, 0),
               _out_spec(out, q, tokens, heads * d, split, tiled)]
-    ws, ws_bytes = None, 0
+    ws, ws_bytes = 0, 0
     if workspace is not None:
         specs.append((workspace, "workspace", F32, 0))
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * 4
@@ -1510,10 +1522,11 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     _on(dev, page_table, "page_table")
     if tokens == 0 or n_seq == 0:
         return
-    _launch(dev, "mdl_attn_paged", q.data_ptr(), code, k_pages.data_ptr(), v_pages.data_ptr(),
-            page_code, _ptr(k_scale), _ptr(v_scale), n_pages, slots, page_table.data_ptr(), ld,
-            width, n_seq, tokens, _at_most(max_q, tokens), heads, kv, d, q_offset.data_ptr(),
-            kv_len.data_ptr(), int(causal), out.data_ptr(), split + tiled, ws, ws_bytes)
+    _launch_block(dev, "mdl_attn_paged", q.data_ptr(), code, k_pages.data_ptr(),
+                  v_pages.data_ptr(), page_code, _ptr(k_scale), _ptr(v_scale), n_pages, slots,
+                  page_table.data_ptr(), ld, width, n_seq, tokens, _at_most(max_q, tokens), heads,
+                  kv, d, q_offset.data_ptr(), kv_len.data_ptr(), int(causal), out.data_ptr(),
+                  split + tiled, ws, ws_bytes)
 
 
 # --- sampling (K11) ------------------------------------------------------------------------------
@@ -1558,9 +1571,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, token_out: torch.
         return
     if workspace is None and vocab > SAMPLE_LIST:
         workspace = torch.empty(sample_workspace_bytes(rows, vocab), dtype=U8, device=logits.device)
-    _launch(dev, "mdl_sample_tokens", logits.data_ptr(), code, ld, rows, vocab, uniform.data_ptr(),
-            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), token_out.data_ptr(),
-            _ptr(logprob_out), _ptr(workspace), 0 if workspace is None else workspace.numel())
+    _launch_block(dev, "mdl_sample_tokens", logits.data_ptr(), code, ld, rows, vocab,
+                  uniform.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+                  token_out.data_ptr(), _ptr(logprob_out), _ptr(workspace),
+                  0 if workspace is None else workspace.numel())
 
 
 class HeadConstraints:

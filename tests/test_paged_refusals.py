@@ -200,3 +200,15 @@ def test_plain_order():
     assert kept_tokens(x, top_p=0.3)[0].tolist() == [1]
     assert sampled(x, 0.0)[0] == 0 and sampled(x, 1 - 2.0 ** -24)[0] == 5
     assert sampled(x, 0.5, temperature=0.0)[:2] == (1, 0.0)
+
+
+@pytest.mark.parametrize("name,plain,refusals", [
+    ("mdl_rope_cache_paged", AP, test_append_refusals), ("mdl_paged_rows", RO, test_rows_refusals),
+    ("mdl_attn_paged", AT, test_attention_refusals), ("mdl_sample_tokens", SA, test_sample_refusals)])
+def test_blocks_hold_the_arguments(L, name, plain, refusals):
+    """The forms with their arguments in a block refuse what the plain ones do."""
+    entry, pack = _lib.BLOCKS[name]
+    for change, code in refusals.pytestmark[0].args[1]:
+        values = list({**plain, **change}.values())[:-1]
+        assert getattr(L, entry)(pack(*(0 if v is None else v for v in values)), None) == code, change
+    assert getattr(L, entry)(None, None) == NULL
