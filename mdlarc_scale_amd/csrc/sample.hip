@@ -137,6 +137,15 @@ __device__ __forceinline__ u64 of_lane(u64 v, int lane) {   // the same lane for
 
 __device__ __forceinline__ u64 wave_sum64(u64 v) { return of_lane(wave_scan64(v), 63); }
 
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {   // in lane 63
+  v = max(v, dpp<0x111>(v, v));
+  v = max(v, dpp<0x112>(v, v));
+  v = max(v, dpp<0x114>(v, v));
+  v = max(v, dpp<0x118>(v, v));
+  v = max(v, dpp<0x142, 0xa>(v, v));
+  return max(v, dpp<0x143, 0xc>(v, v));
+}
+
 // The sum that the token's own has to pass.  u outside [0, 1) is taken as the nearest inside.
 __device__ __forceinline__ u64 target_of(float u, u64 total) {
   const double t = static_cast<double>(u) * static_cast<double>(total);
@@ -323,28 +332,6 @@ __device__ __forceinline__ Scanned block_scan(u64 a, u64 b, u64 (*part)[2]) {
   return r;
 }
 
-// Ascending bitonic sort of list[0 .. n), n <= kList; the entries up to the next power of two are set.
-__device__ __forceinline__ void sort_list(u64* list, int n) {
-  const int t = threadIdx.x;
-  int size = 2;
-  while (size < n) size *= 2;
-  __syncthreads();
-  for (int i = n + t; i < size; i += kThreads) list[i] = ~u64{0};
-  for (int k = 2; k <= size; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      __syncthreads();
-      for (int i = t; i < size / 2; i += kThreads) {
-        const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const u64 u = list[a], v = list[b];
-        if ((u > v) == ((a & k) == 0)) {
-          list[a] = v;
-          list[b] = u;
-        }
-      }
-    }
-  __syncthreads();
-}
-
 constexpr int kBins = 1024;            // one a thread
 constexpr double kBinsOctave = 16.0;
 static_assert(kBins == kThreads, "a bin a thread");
@@ -423,10 +410,13 @@ struct ListLds {
   u64 few[kThreads], few_sum[kThreads];
   u64 part[kWaves][2];
   u64 last, sum;
-  int n, found, bin_k, bin_p, upto;
+  uint32_t range[2];
+  int n, found, picked, bin_k, bin_p, upto;
 };
 
-constexpr int kCompared = 192;   // tokens of a bin that are compared pair by pair, more are sorted
+constexpr int kCompared = 64;    // tokens that are compared pair by pair
+constexpr int kDigit = 10;       // bits of a digit, kBins values
+static_assert(kBins == 1 << kDigit, "a digit a thread");
 
 // What each filter makes of the bins: those that the filters reach into (kBins: none), and the thread's
 // bin.
@@ -435,7 +425,7 @@ struct Bins {
   u64 count_before, sum_before;    // of the bins before it
   u64 total;
   bool cut, by_p, by_m;            // top-k keeps fewer than there are; top-p; min-p
-  int bin_k, bin_p, bin_m, last;
+  int bin_k, bin_p, bin_m, bin_m_to, last;
 
   // the bin in which the sum reaches `goal`, at most the sum of all; a call of all threads
   __device__ __forceinline__ int by_sum(ListLds& s, u64 goal) const {
@@ -455,9 +445,12 @@ struct Bins {
     cut = f.top_k > 0 && tokens > static_cast<u64>(f.top_k);
     by_p = f.top_p < 1.0;
     by_m = f.min_p > 0.0;
-    // the first bin with weights below min_p, but for roundings: a bin more is looked at either side
-    const double low = by_m ? g.at_top - g.base - kBinsOctave * log2(f.min_p) : kBins;
-    bin_m = low < kBins ? static_cast<int>(low) : kBins;
+    // The bins that may hold weights on both sides of min_p: one, or two where it lies at a border but for
+    // roundings.  (A value's place in bins is off by 2^-52 of |x| scale; values lie 2^-24 of that apart,
+    // so where other values than the largest are in the bins at all, by less than 2^-16.)
+    const double low = by_m ? g.at_top - g.base - kBinsOctave * log2(f.min_p) : 2.0 * kBins;
+    bin_m = low - 0x1p-12 < kBins ? max(static_cast<int>(floor(low - 0x1p-12)), 0) : kBins;
+    bin_m_to = low + 0x1p-12 < kBins ? static_cast<int>(low + 0x1p-12) : kBins;
     bin_k = bin_p = kBins;
     if (cut) {
       if (count_before < static_cast<u64>(f.top_k) &&
@@ -470,56 +463,117 @@ struct Bins {
     }
     // everything that is kept is in bins up to `last`, and so is what top-p's share is of: all that
     // top-k keeps, or the total
-    last = cut && by_p ? bin_k : min(min(bin_k, bin_p), min(bin_m + 1, kBins - 1));
+    last = cut && by_p ? bin_k : min(min(bin_k, bin_p), min(bin_m_to, kBins - 1));
     if (threadIdx.x == last) s.upto = static_cast<int>(count_before + count);
     __syncthreads();
   }
 };
 
-// The last token of a sorted list of n before which there is less than `goal`, tokens (by_count) or
-// sums; c and m lie before the list.
-__device__ __forceinline__ Border border_sorted(ListLds& s, const u64* list, int n, float top,
-                                                const Filters& f, bool by_count, u64 c, u64 m,
-                                                u64 goal) {
+// The last token of a list of n (places in any order) before which there is less than `goal`, tokens
+// (by_count) or sums; c and m lie before the list.  A call of all threads; s.few and s.few_sum are used,
+// and the list may be s.few.
+__device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, float top,
+                                            const Filters& f, bool by_count, u64 c, u64 m, u64 goal) {
   const int t = threadIdx.x;
-  if (t == 0) s.found = 0;
+  u64 base = 0, span = ~u64{0};   // the places that the border is among, `inside` of them
+  int inside = n;
+  if (n > kCompared) {   // from the least value to the largest
+    uint32_t least = ~0u, most = 0;
+    if (t < 2) s.range[t] = t == 0 ? ~0u : 0u;
 #pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += kThreads) {   // a thousand at a time, with what lies before them
-    const int i = i0 + t;
-    const u64 my = i < n ? list[i] : 0;
-    const u64 w = i < n ? fixed(weight(value_at(my), top, f.c)) : 0;
-    const Scanned r = block_scan<false>(w, 0, s.part);   // a barrier for s.found too
-    const u64 before = m + r.a;
-    const bool in = i < n && (by_count ? c + i : before) < goal;
-    if (in) atomicMax(&s.found, i);
-    __syncthreads();
-    if (i == s.found) {
-      s.last = my;
-      s.sum = before + w;
+    for (int i = t; i < n; i += kThreads) {
+      const uint32_t v = static_cast<uint32_t>(list[i] >> 32);
+      least = min(least, v);
+      most = max(most, v);
     }
-    m += r.all_a;
+    least = ~wave_most(~least);
+    most = wave_most(most);
+    __syncthreads();
+    if ((t & 63) == 63) {
+      atomicMin(&s.range[0], least);
+      atomicMax(&s.range[1], most);
+    }
+    __syncthreads();
+    base = static_cast<u64>(s.range[0]) << 32;
+    span = (static_cast<u64>(s.range[1] - s.range[0]) << 32) | 0xffffffffu;
   }
-  __syncthreads();
-  return Border{s.last, s.sum};
-}
-
-// The same of a list in any order; a call of all threads, the list is set.
-__device__ __forceinline__ Border border_of(ListLds& s, u64* list, int n, float top, const Filters& f,
-                                            bool by_count, u64 c, u64 m, u64 goal) {
-  const int t = threadIdx.x;
+#pragma unroll 1
+  while (inside > kCompared) {   // a digit, of 1,024 values, of the places
+    const int shift = max(64 - kDigit - __clzll(static_cast<long long>(span)), 0);
+    s.few_sum[t] = 0;
+    if (t == 0) s.found = -1;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = t; i < n; i += kThreads) {
+      const u64 d = list[i] - base;
+      if (d <= span)
+        atomicAdd(&s.few_sum[d >> shift],
+                  by_count ? u64{1} : fixed(weight(value_at(list[i]), top, f.c)));
+    }
+    __syncthreads();
+    const u64 mine = s.few_sum[t];
+    const Scanned r = block_scan<false>(mine, 0, s.part);
+    const u64 have = (by_count ? c : m) + r.a;
+    if (have < goal && have + mine >= goal) {
+      s.found = t;
+      s.sum = r.a;
+    }
+    __syncthreads();
+    // sums of single weights and of bins differ in their last bits: a goal past the last digit is in the
+    // last one that has tokens
+    const bool none = s.found < 0;
+    __syncthreads();
+    if (none) {
+#pragma unroll 1
+      for (int i = t; i < n; i += kThreads) {
+        const u64 d = list[i] - base;
+        if (d <= span) atomicMax(&s.found, static_cast<int>(d >> shift));
+      }
+      __syncthreads();
+      if (t == s.found) s.sum = r.a;
+      __syncthreads();
+    }
+    const int digit = s.found;
+    if (by_count) c += s.sum;
+    u64 some = 0, before = 0;
+#pragma unroll 1
+    for (int i = t; i < n; i += kThreads) {
+      const u64 d = list[i] - base;
+      if (d > span) continue;
+      const int at = static_cast<int>(d >> shift);
+      some += at == digit;
+      if (at < digit) before += fixed(weight(value_at(list[i]), top, f.c));
+    }
+    const Scanned q = block_scan<true>(some, before, s.part);
+    inside = static_cast<int>(q.all_a);
+    m += q.all_b;
+    base += static_cast<u64>(digit) << shift;
+    span = (u64{1} << shift) - 1;
+  }
+  // those left are compared pair by pair
+  u64 my = 0;
   if (n > kCompared) {
-    sort_list(list, n);
-    return border_sorted(s, list, n, top, f, by_count, c, m, goal);
+    if (t == 0) s.picked = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += kThreads) {
+      const u64 a = i0 + t < n ? list[i0 + t] : ~u64{0};
+      const bool in = i0 + t < n && a - base <= span;
+      __syncthreads();   // a list in s.few has one round
+      if (in) s.few[atomicAdd(&s.picked, 1)] = a;
+    }
+    __syncthreads();
+    list = s.few;
   }
-  u64 rank = 0, before = 0, my = 0;
-  if (t < n) {
+  u64 rank = 0, before = 0;
+  if (t < inside) {
     my = list[t];
     s.few_sum[t] = fixed(weight(value_at(my), top, f.c));
   }
   if (t == 0) s.found = 0;
   __syncthreads();
-  if (t < n) {
-    for (int j = 0; j < n; ++j) {
+  if (t < inside) {
+    for (int j = 0; j < inside; ++j) {
       const bool ahead = list[j] < my;
       rank += ahead;
       before += ahead ? s.few_sum[j] : 0;
@@ -527,7 +581,7 @@ __device__ __forceinline__ Border border_of(ListLds& s, u64* list, int n, float 
     if ((by_count ? c + rank : m + before) < goal) atomicMax(&s.found, static_cast<int>(rank));
   }
   __syncthreads();
-  if (t < n && static_cast<int>(rank) == s.found) {
+  if (t < inside && static_cast<int>(rank) == s.found) {
     s.last = my;
     s.sum = m + before + s.few_sum[t];
   }
@@ -714,10 +768,8 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(const SampleArgs 
 
 // ---- a row in parts ----------------------------------------------------------------------------
 
-constexpr int kDigit = 10;             // bits of a digit, kBins values
 constexpr int kPart = 16384;           // tokens of a part: their sum stays below 2^48 (bin_entry)
 constexpr int kMaxParts = 64;
-static_assert(kBins == 1 << kDigit, "a digit a thread");
 
 struct Parts {
   u64* bins;      // [rows][parts][kBins]
@@ -929,19 +981,23 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
   };
 
   Border border{~u64{0}, b.total};
-  int full = b.by_m ? max(b.bin_m - 1, 0) : kBins;   // bins that are kept whole
+  int full = b.bin_m;   // bins that are kept whole
 #pragma unroll 1
   for (int step = b.cut ? 0 : 1; step < (b.by_p ? 2 : 1); ++step) {   // top-k, then top-p
     const bool by_count = step == 0;
     const u64 goal = by_count ? static_cast<u64>(f.top_k) : share_of(f.top_p, border.sum);
     const int bin = by_count ? b.bin_k : b.by_sum(s.l, goal);
+    if (bin > b.bin_m_to && !(by_count && b.by_p)) continue;   // past what min-p keeps
     const Border other = border_in(bin, by_count, goal);
     if (other.last < border.last) border = other;
     full = min(full, bin);
   }
+  // min-p: weights are needed in the bins about its own only
+  const float below_m = b.by_m ? g.least(b.bin_m_to) : -INFINITY;
+  const float above_m = b.by_m ? g.most(b.bin_m) : -INFINITY;
   auto kept = [&](float v, int i) {
-    return v > -INFINITY && place(v, i) <= border.last &&
-           (!b.by_m || weight(v, top, f.c) >= f.min_p);
+    return v > -INFINITY && place(v, i) <= border.last && v >= below_m &&
+           (v > above_m || !b.by_m || weight(v, top, f.c) >= f.min_p);
   };
   // the parts' kept sums: whole bins, then tokens of the others
   for (int i = wave; i < parts.n; i += kWaves) {
@@ -954,20 +1010,29 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
   __syncthreads();
   if (full < kBins) {
     int to = border.last == ~u64{0} ? kBins - 1 : g.bin(value_at(border.last));   // the last bin kept
-    if (b.by_m) to = min(to, b.bin_m + 1);
+    if (b.by_m) to = min(to, b.bin_m_to);
+    // by sixteen lanes of their own, of which there are fewer at one sum
+    auto add = [&](int i, float v) {
+      atomicAdd(&s.l.few[i / parts.size * 16 + (t & 15)], fixed(weight(v, top, f.c)));
+    };
+    s.l.few[t] = 0;
+    __syncthreads();
     if (to == full && listed == full) {
       for (int i = t; i < s.l.n; i += kThreads) {
         const u64 a = s.l.list[i];
         const int at_i = static_cast<int>(static_cast<uint32_t>(a));
         const float v = value_at(a);
-        if (kept(v, at_i)) atomicAdd(&s.part_sum[at_i / parts.size], fixed(weight(v, top, f.c)));
+        if (kept(v, at_i)) add(at_i, v);
       }
     } else {
       x.each_between(g.least(min(to, kBins - 1)), g.most(full), [&](float v, int i) {
-        if (g.bin(v) >= full && kept(v, i))
-          atomicAdd(&s.part_sum[i / parts.size], fixed(weight(v, top, f.c)));
+        if (g.bin(v) >= full && kept(v, i)) add(i, v);
       });
     }
+    __syncthreads();
+    static_assert(kMaxParts * 16 <= kThreads, "a sum a thread");
+    const u64 sum16 = row_scan64(s.l.few[t]);
+    if ((t & 15) == 15 && t / 16 < parts.n) s.part_sum[t / 16] += sum16;
   }
   __syncthreads();
   u64 total = 0;
