@@ -22,17 +22,17 @@
 //   is kept, up to 4,096 of them, to LDS.
 // Counts and sums of weights in 1,024 bins of 1/16 octave say which bins the filters reach into.  (The
 // bins lie on a grid that does not depend on the part, so those of parts add up; in a bin a weight is
-// its top times 2^(-f / 16), a short polynomial.)  Inside such a bin tokens are compared pair by pair, or
-// sorted where they are many.  The kept weights are then summed by stretches of indexes, and the tokens
+// its top times 2^(-f / 16), a short polynomial.)  Inside such a bin the border is found by
+// digits of the tokens' places in the order, 1,024 values each, and the last 64 by comparing every pair.
+// The kept weights are then summed by stretches of indexes, and the tokens
 // of the stretch that holds the result compared by index.  Where more than 4,096 tokens are kept the
 // row's second launch looks for the borders in their bins alone, cut by the digits of value and index
 // where thousands are equal, and takes the parts' kept sums from their bins.
 //
-// What bounds it: one block's chain of steps, most of them waits.  64 rows of 131,072 logits, 52 us:
-// the bins 12 (64-bit arithmetic, 20 instructions a token), a row's second launch some 30 at the
-// median (3 for the parts' largest values, 2 for their bins, 4 for the scans, 8 for the pass over the
-// row, 2 to 6 for a border, 4 for the result) and 40 for the row with the most tokens kept; 256 rows of
-// 4,000 22 us; 256 of 14 5.0 us.
+// What bounds it: one block's chain of steps, most of them waits (VALU busy 8% in the second launch).  64
+// rows of 131,072 logits, 43 to 54 us by their filters: the bins 12 (64-bit arithmetic, 20 instructions
+// a token), a row's second launch 25 at the median, the most for its pass over the row (8), and up to 40
+// where more than 4,096 tokens are kept; 256 rows of 4,000 20 us, of 14 4.2 to 4.9 us.
 #include <cfloat>
 
 #include "common.h"
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs p) {
 // ---- a block a row -----------------------------------------------------------------------------
 
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
-constexpr int kList = 4096;        // tokens that are sorted at once
+constexpr int kList = 4096;        // tokens of a row in LDS
 
 // A stretch of a row: tokens up to a 16-byte boundary, pieces of 16 bytes, the rest.
 template <typename T>

@@ -106,6 +106,36 @@ def test_many_equal_logits(dtype, vocab, values):
     check(x, u, top_k=k, top_p=p)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("vocab", [300, 1025, 2500, 4096, 4097, 30011])
+@pytest.mark.parametrize("std", [0.0, 1e-4, 0.01, 0.3])
+def test_borders_among_close_logits(dtype, vocab, std):
+    """Thousands of tokens within a hundredth of an octave, or equal, in rows of every kind."""
+    rows = 10
+    x, u, g = rows_of(vocab + int(1e4 * std), rows, vocab, dtype, std=std)
+    k = torch.randint(2, vocab + 1, (rows,), generator=g).int()
+    p, m = 0.05 + 0.9 * torch.rand(rows, generator=g), 0.5 + 0.5 * torch.rand(rows, generator=g)
+    check(x, u, top_k=k)
+    check(x, u, top_p=p)
+    check(x, u, min_p=m)
+    check(x, u, top_k=k, top_p=p)
+    check(x - 50, u, top_k=k, top_p=p, min_p=m)
+
+
+@pytest.mark.parametrize("vocab", [500, 4096, 30011])
+def test_shares_next_to_one_and_weights_below_the_sums(vocab):
+    """Low temperatures leave most weights below 2^-43; top-p and min-p among them."""
+    rows = 16
+    x, u, g = rows_of(vocab + 3, rows, vocab, F32)
+    heat = 0.02 + 0.2 * torch.rand(rows, generator=g)
+    p = 1 - 2.0 ** -torch.randint(10, 25, (rows,), generator=g).float()
+    m = 2.0 ** -(60 * torch.rand(rows, generator=g))
+    check(x, u, temperature=heat, top_p=p)
+    check(x, u, temperature=heat, min_p=m)
+    check(x, u, temperature=heat, top_p=p, min_p=m)
+    check(x, u, temperature=heat, top_p=p, top_k=torch.full((rows,), vocab - 1, dtype=torch.int32))
+
+
 @pytest.mark.parametrize("vocab", [14, 64, 65, 3001])
 def test_masked_rows_and_values_that_are_not_finite(vocab):
     inf, nan = float("inf"), float("nan")
