@@ -169,6 +169,29 @@ def test_masked_rows_and_values_that_are_not_finite(vocab):
         assert bool((lp[2:] == 0).all())
 
 
+def test_the_longest_rows():
+    vocab, rows = 2 ** 20, 3
+    x, u, g = rows_of(77, rows, vocab, BF)
+    p, m = 0.3 + 0.6 * torch.rand(rows, generator=g), 0.01 * torch.rand(rows, generator=g)
+    k = torch.randint(2000, 9000, (rows,), generator=g).int()
+    check(x, u)
+    check(x, u, top_p=p)
+    check(x, u, top_k=k, top_p=p)
+    check(x, u, top_p=p, min_p=m)
+
+
+@pytest.mark.parametrize("rows,vocab", [(70001, 14), (70001, 65), (5003, 4100)])
+def test_many_rows(rows, vocab):
+    """Copies of four rows, whose tokens are checked."""
+    x, u, g = rows_of(5, 4, vocab, F32)
+    p, m = 0.3 + 0.6 * torch.rand(4, generator=g), 0.05 * torch.rand(4, generator=g)
+    check(x, u, top_p=p, min_p=m)
+    few, few_lp = draw(x, u, top_p=p, min_p=m)
+    i = torch.arange(rows) % 4
+    token, lp = draw(x.to(DEV)[i.to(DEV)], u[i], top_p=p[i], min_p=m[i])
+    assert torch.equal(token, few[i]) and torch.equal(lp, few_lp[i])
+
+
 @pytest.mark.parametrize("vocab", [14, 900, 30011])
 def test_filters_that_are_none(vocab):
     """Numbers that switch a filter off, NaN among them, and a workspace of the caller's."""
