@@ -119,6 +119,19 @@ def test_paged_single_tokens(dtype, D, heads, kv, fp4):
     assert torch.equal(c.run(), c.run())
 
 
+@pytest.mark.parametrize("dtype,D,heads,kv,fp4", FORMS)
+@pytest.mark.parametrize("keys", [[9001], [5, 130, 0], [2600, 1, 900, 4000, 77, 31]])
+@pytest.mark.parametrize("extra", [0, 600])
+def test_paged_single_tokens_in_many_parts(dtype, D, heads, kv, fp4, keys, extra):
+    """Few rows behind keys that are cut into as many parts as there are; a wide table leaves most of
+    them empty."""
+    c = Paged(19, dtype, D, heads, kv, [1] * len(keys), [max(k - 1, 0) for k in keys], fp4=fp4,
+              extra=extra)
+    c.keys = keys
+    c.check("many parts")
+    assert torch.equal(c.run(), c.run())
+
+
 @pytest.mark.parametrize("dtype,D,fp4", [(BF, 64, False), (F32, 64, False), (F32, 128, False),
                                          (BF, 64, True), (BF, 128, True), (F32, 128, True)])
 @pytest.mark.parametrize("causal", [True, False])
