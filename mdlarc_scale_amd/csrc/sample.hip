@@ -11,8 +11,9 @@
 // Each filter keeps a run of the order from its first token on.
 //
 // Exactness: a token flips where a sum of weights passes a border, so weights are computed in 64
-// bits and summed as whole multiples of 2^-43: such sums do not depend on their order (atomics among
-// them), and 2^20 weights fit 64 bits.  (CDNA's 64-bit multiply-adds run at the rate of 32-bit ones.)
+// bits and summed as whole numbers: such sums do not depend on their order (atomics among them).  The draw's
+// are multiples of 2^-43, of which 2^20 fit 64 bits.  (CDNA's 64-bit multiply-adds run at the rate of
+// 32-bit ones.)  The filters' are those of "weights in sums" below, to 2^-34 of a weight, in 128 bits.
 //
 // Three sizes of rows:
 //   up to 64 tokens: a wave a row, a token a lane; the order comes from comparing every pair;
@@ -55,6 +56,7 @@ struct SampleArgs {
 };
 
 typedef unsigned long long u64;
+typedef unsigned __int128 u128;
 
 constexpr u64 kOne = u64{1} << 43;          // the fixed-point 1
 constexpr double kLog2e = 1.4426950408889634074;
@@ -121,13 +123,24 @@ __device__ __forceinline__ u64 plus_dpp(u64 v) {
               dpp<CTRL, ROWS>(0, static_cast<uint32_t>(v)));
 }
 
-// the sums over 16 neighbouring lanes up to the lane's own
-__device__ __forceinline__ u64 row_scan64(u64 v) {
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ u128 plus_dpp(u128 v) {
+  u128 other = 0;
+#pragma unroll
+  for (int i = 96; i >= 0; i -= 32)
+    other = other << 32 | dpp<CTRL, ROWS>(0, static_cast<uint32_t>(v >> i));
+  return v + other;
+}
+
+// the sums over 16 neighbouring lanes up to the lane's own (T: u64 or u128)
+template <typename T>
+__device__ __forceinline__ T row_scan(T v) {
   return plus_dpp<0x118>(plus_dpp<0x114>(plus_dpp<0x112>(plus_dpp<0x111>(v))));
 }
 
-__device__ __forceinline__ u64 wave_scan64(u64 v) {   // inclusive
-  return plus_dpp<0x143, 0xc>(plus_dpp<0x142, 0xa>(row_scan64(v)));
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {   // inclusive
+  return plus_dpp<0x143, 0xc>(plus_dpp<0x142, 0xa>(row_scan(v)));
 }
 
 __device__ __forceinline__ u64 of_lane(u64 v, int lane) {   // the same lane for the whole wave
@@ -135,7 +148,13 @@ __device__ __forceinline__ u64 of_lane(u64 v, int lane) {   // the same lane for
          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane));
 }
 
-__device__ __forceinline__ u64 wave_sum64(u64 v) { return of_lane(wave_scan64(v), 63); }
+__device__ __forceinline__ u128 of_lane(u128 v, int lane) {
+  return static_cast<u128>(of_lane(static_cast<u64>(v >> 64), lane)) << 64 |
+         of_lane(static_cast<u64>(v), lane);
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_total(T v) { return of_lane(wave_scan(v), 63); }
 
 __device__ __forceinline__ uint32_t wave_most(uint32_t v) {   // in lane 63
   v = max(v, dpp<0x111>(v, v));
@@ -154,13 +173,31 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
   return at < total ? at : total - 1;
 }
 
-// Tokens before which there is less than p of `total` are kept: less than this whole number.
-__device__ __forceinline__ u64 share_of(double p, u64 total) {
-  return static_cast<u64>(ceil(p * static_cast<double>(total)));
+// f times `total` (0 < f < 1, total below 2^116), rounded up.  Tokens before which there is less than
+// this whole number are those before which there is less than the share f.
+__device__ __forceinline__ u128 share_of(float f, u128 total) {
+  const uint32_t b = __float_as_uint(f);
+  const uint32_t m = (b & 0x7fffffu) | (b >= 0x800000u ? 0x800000u : 0u);
+  const int k = 150 - max(static_cast<int>(b >> 23), 1);   // f = m 2^-k, 24 <= k <= 149
+  // m total = 2^64 high + low
+  const u128 first = static_cast<u128>(m) * static_cast<u64>(total);
+  const u128 high = static_cast<u128>(m) * static_cast<u64>(total >> 64) + (first >> 64);
+  const u64 low = static_cast<u64>(first);
+  u128 whole;
+  bool rest;
+  if (k < 64) {
+    whole = high << (64 - k) | low >> k;
+    rest = low << (64 - k) != 0;
+  } else {
+    whole = high >> (k - 64);
+    rest = low != 0 || whole << (k - 64) != high;
+  }
+  return whole + (rest ? 1 : 0);
 }
 
 struct Filters {
-  double c, top_p, min_p;
+  double c, min_p;
+  float top_p;
   int top_k;      // 0: none
   bool greedy;
 };
@@ -169,11 +206,11 @@ __device__ __forceinline__ Filters filters_of(const SampleArgs& p, int row) {
   Filters f;
   const float t = p.temperature ? p.temperature[row] : 1.f;
   f.top_k = p.top_k ? max(p.top_k[row], 0) : 0;
-  f.top_p = p.top_p ? static_cast<double>(p.top_p[row]) : 1.0;
+  f.top_p = p.top_p ? p.top_p[row] : 1.f;
   const float m = p.min_p ? p.min_p[row] : 0.f;
   f.min_p = m > 0.f ? static_cast<double>(m) : 0.0;   // NaN: none
   // a share of nothing, and a bound that no weight reaches, leave the first token
-  f.greedy = !(t > 0.f) || f.top_k == 1 || f.top_p <= 0.0 || f.min_p > 1.0;
+  f.greedy = !(t > 0.f) || f.top_k == 1 || f.top_p <= 0.f || f.min_p > 1.0;
   f.c = kLog2e / static_cast<double>(fminf(t, FLT_MAX));
   return f;
 }
@@ -182,6 +219,102 @@ __device__ __forceinline__ void leave(const SampleArgs& p, int row, int token, d
   p.token[row] = token;
   if (p.logprob)
     p.logprob[row] = static_cast<float>(log(w / (static_cast<double>(total) / kOne)));
+}
+
+// ---- weights in sums -------------------------------------------------------------------------------
+
+// Weights as whole numbers that add up: the borders of the filters compare sums of tokens with shares of
+// others, and equal sums have to be equal whatever they are made of.  A token's weight is its entry (its
+// weight over that of its bin's top, to the nearest 2^-33) times bin_top of its bin, both of which depend
+// on the token and the row's largest alone, so that a bin's sum is bin_top times the sum of its entries.
+// 2^20 tokens make less than 2^116.
+
+constexpr int kBins = 1024;
+constexpr double kBinsOctave = 16.0;
+
+// What a token adds to its bin: a count in the upper 16 bits, and the weight over that of the bin's
+// top, 2^(-f / 16) with 0 <= f < 1, to the nearest 2^-33 (and 2^-36 that the polynomial is off by).
+__device__ __forceinline__ u64 bin_entry(double f) {
+  constexpr double h = -0.69314718055994530942 / kBinsOctave;
+  double w = h * h * h * h * h / 120;   // e^(h f): the next term is below 2^-36
+  w = fma(w, f, h * h * h * h / 24);
+  w = fma(w, f, h * h * h / 6);
+  w = fma(w, f, h * h / 2);
+  w = fma(w, f, h);
+  w = fma(w, f, 1.0 + 0x1p19);          // from here on the last bit is 2^-33
+  return __builtin_bit_cast(u64, w) + ((u64{1} << 48) - __builtin_bit_cast(u64, 0x1p19));
+}
+
+constexpr u64 kEntrySum = (u64{1} << 48) - 1;
+
+// 2^62 times 2^(-bin / 16), the weight of a bin's top, to the nearest whole number (but for 2^-60 of it)
+__device__ __forceinline__ u64 bin_top(int bin) {
+  u64 t = u64{1} << 63;
+  t = bin & 1 ? __umul64hi(t, 0xf5257d152486cc2cull) : t;   // 2^64 times 2^(-1 / 16)
+  t = bin & 2 ? __umul64hi(t, 0xeac0c6e7dd24392full) : t;   // 2^(-2 / 16)
+  t = bin & 4 ? __umul64hi(t, 0xd744fccad69d6af4ull) : t;   // 2^(-4 / 16)
+  t = bin & 8 ? __umul64hi(t, 0xb504f333f9de6484ull) : t;   // 2^(-8 / 16)
+  return ((t >> (bin >> 4)) + 1) >> 1;                      // bins below 1,024
+}
+
+// The row's bins: 1/16 octave each, bin 0 with the largest value; kBins for values below all of them.
+// A logit lies at -x times the scale, in bins; `base` is where bin 0 begins.
+struct Grid {
+  double scale, at_top, base;
+  bool huge;      // the largest value is infinite: it alone has a weight, in bin 0
+
+  __device__ __forceinline__ Grid(float top, double c) : scale(c * kBinsOctave) {
+    huge = top == INFINITY;
+    at_top = huge ? 0.0 : at(top);
+    base = floor(at_top);
+  }
+  // Nothing here is contracted: a token's bin and entry are the same wherever they are computed.
+  __device__ __forceinline__ double at(float x) const {
+#pragma clang fp contract(off)
+    return -static_cast<double>(x) * scale;
+  }
+  __device__ __forceinline__ int bin(float x) const {
+    if (huge) return x == INFINITY ? 0 : kBins;
+    const double d = floor(at(x)) - base;
+    return d < kBins ? static_cast<int>(d) : kBins;
+  }
+  // the token's entry in its bin (bin_entry's weight), 0 below all bins
+  __device__ __forceinline__ u64 entry(float x) const {
+#pragma clang fp contract(off)
+    if (huge) return x == INFINITY ? bin_entry(0.0) & kEntrySum : 0;
+    const double q = at(x), b = floor(q);   // of NaN and -inf: no bin
+    return b - base < kBins ? bin_entry(q - b) & kEntrySum : 0;
+  }
+  // bounds of the values in bins `first` .. `last` (a few roundings of fp32 wider)
+  __device__ __forceinline__ float least(int last) const {
+    if (huge) return INFINITY;
+    const double x = -(base + last + 1) / scale;
+    return static_cast<float>(x - fabs(x) * 0x1p-20);
+  }
+  __device__ __forceinline__ float most(int first) const {
+    if (huge || first == 0) return INFINITY;
+    const double x = -(base + first) / scale;
+    return static_cast<float>(x + fabs(x) * 0x1p-20);
+  }
+};
+
+// A token's weight in the sums
+__device__ __forceinline__ u128 sum_weight(const Grid& g, float x) {
+  const u64 e = g.entry(x);
+  return e == 0 ? 0 : static_cast<u128>(e) * bin_top(g.bin(x));
+}
+
+// The least whole number that times `top` reaches `need`.  It is at most the entries of 2^20 tokens, 2^53, of
+// which four roundings of the estimate make 4.
+__device__ __forceinline__ u64 entries_for(u128 need, u64 top) {
+  const double high = static_cast<double>(static_cast<u64>(need >> 64));
+  u64 n = static_cast<u64>((high * 0x1p64 + static_cast<double>(static_cast<u64>(need))) /
+                           static_cast<double>(top));
+#pragma unroll 1
+  for (int i = 0; i < 8 && static_cast<u128>(n) * top < need; ++i) ++n;
+#pragma unroll 1
+  for (int i = 0; i < 8 && n > 0 && static_cast<u128>(n - 1) * top >= need; ++i) --n;
+  return n;
 }
 
 // ---- a wave a row ------------------------------------------------------------------------------
@@ -203,21 +336,22 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs p) {
   }
   const double w = weight(x, top, f.c);
   const u64 mine = fixed(w), at = place(x, lane);
+  const u128 held = sum_weight(Grid(top, f.c), x);
   int rank = 0;
-  u64 before = 0;
+  u128 before = 0;
   for (int j = 0; j < p.vocab; ++j) {
     const bool ahead = of_lane(at, j) < at;
-    const u64 other = of_lane(mine, j);
+    const u128 other = of_lane(held, j);
     rank += ahead;
     before += ahead ? other : 0;
   }
-  bool kept = mine != 0 && (f.top_k == 0 || rank < f.top_k);
-  if (f.top_p < 1.0) {
-    const u64 sum = wave_sum64(kept ? mine : 0);
+  bool kept = held != 0 && (f.top_k == 0 || rank < f.top_k);
+  if (f.top_p < 1.f) {
+    const u128 sum = wave_total(kept ? held : 0);
     kept = kept && before < share_of(f.top_p, sum);
   }
   kept = kept && w >= f.min_p;
-  const u64 sums = wave_scan64(kept ? mine : 0);
+  const u64 sums = wave_scan(kept ? mine : 0);
   const u64 total = of_lane(sums, 63);
   const u64 goal = target_of(p.uniform[row], total);
   const u64 past = __ballot(sums > goal);
@@ -304,85 +438,49 @@ struct Stretch {
   }
 };
 
-// The sums of a (and b) over the threads before this one, and over all of them.
+// The sum over the threads before this one, and over all of them.
+template <typename T>
 struct Scanned {
-  u64 a, b, all_a, all_b;
+  T before, all;
 };
 
-template <bool TWO>
-__device__ __forceinline__ Scanned block_scan(u64 a, u64 b, u64 (*part)[2]) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const u64 sa = wave_scan64(a), sb = TWO ? wave_scan64(b) : 0;
-  __syncthreads();
-  if (lane == 63) {
-    part[wave][0] = sa;
-    if (TWO) part[wave][1] = sb;
-  }
-  __syncthreads();
+template <typename T>
+__device__ __forceinline__ Scanned<T> with_waves(T v, T scan, const T* part) {
   static_assert(kWaves == 16, "the waves' sums in a row of lanes");
-  const u64 wa = row_scan64(part[lane & 15][0]), wb = TWO ? row_scan64(part[lane & 15][1]) : 0;
-  const int before = max(wave - 1, 0);
-  Scanned r{};
-  r.all_a = of_lane(wa, kWaves - 1);
-  r.a = sa - a + (wave == 0 ? 0 : of_lane(wa, before));
-  if (TWO) {
-    r.all_b = of_lane(wb, kWaves - 1);
-    r.b = sb - b + (wave == 0 ? 0 : of_lane(wb, before));
-  }
-  return r;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T waves = row_scan(part[threadIdx.x & 15]);
+  return {scan - v + (wave == 0 ? 0 : of_lane(waves, max(wave - 1, 0))), of_lane(waves, kWaves - 1)};
 }
 
-constexpr int kBins = 1024;            // one a thread
-constexpr double kBinsOctave = 16.0;
+template <typename T>
+__device__ __forceinline__ Scanned<T> block_scan(T v, T* part) {
+  const T scan = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = scan;
+  __syncthreads();
+  return with_waves(v, scan, part);
+}
+
+template <typename A, typename B>
+__device__ __forceinline__ void block_scan(A a, A* part_a, Scanned<A>& sums_a, B b, B* part_b,
+                                           Scanned<B>& sums_b) {
+  const A scan_a = wave_scan(a);
+  const B scan_b = wave_scan(b);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) {
+    part_a[threadIdx.x >> 6] = scan_a;
+    part_b[threadIdx.x >> 6] = scan_b;
+  }
+  __syncthreads();
+  sums_a = with_waves(a, scan_a, part_a);
+  sums_b = with_waves(b, scan_b, part_b);
+}
+
 static_assert(kBins == kThreads, "a bin a thread");
-
-// The row's bins: 1/16 octave each, bin 0 with the largest value; kBins for values below all of them.
-// A logit lies at -x times the scale, in bins; `base` is where bin 0 begins.
-struct Grid {
-  double scale, at_top, base;
-  bool huge;      // the largest value is infinite: it alone has a weight, in bin 0
-
-  __device__ __forceinline__ Grid(float top, double c) : scale(c * kBinsOctave) {
-    huge = top == INFINITY;
-    at_top = huge ? 0.0 : at(top);
-    base = floor(at_top);
-  }
-  __device__ __forceinline__ double at(float x) const { return -static_cast<double>(x) * scale; }
-  __device__ __forceinline__ int bin(float x) const {
-    if (huge) return x == INFINITY ? 0 : kBins;
-    const double d = floor(at(x)) - base;
-    return d < kBins ? static_cast<int>(d) : kBins;
-  }
-  // bounds of the values in bins `first` .. `last` (a few roundings of fp32 wider)
-  __device__ __forceinline__ float least(int last) const {
-    if (huge) return INFINITY;
-    const double x = -(base + last + 1) / scale;
-    return static_cast<float>(x - fabs(x) * 0x1p-20);
-  }
-  __device__ __forceinline__ float most(int first) const {
-    if (huge || first == 0) return INFINITY;
-    const double x = -(base + first) / scale;
-    return static_cast<float>(x + fabs(x) * 0x1p-20);
-  }
-};
-
-// What a token adds to its bin: a count in the upper 16 bits, and the weight over that of the bin's
-// top, 2^(-f / 16) with 0 <= f < 1, to the nearest 2^-33.
-__device__ __forceinline__ u64 bin_entry(double f) {
-  constexpr double h = -0.69314718055994530942 / kBinsOctave;
-  double w = h * h * h * h * h / 120;   // e^(h f): the next term is below 2^-36
-  w = fma(w, f, h * h * h * h / 24);
-  w = fma(w, f, h * h * h / 6);
-  w = fma(w, f, h * h / 2);
-  w = fma(w, f, h);
-  w = fma(w, f, 1.0 + 0x1p19);          // from here on the last bit is 2^-33
-  return __builtin_bit_cast(u64, w) + ((u64{1} << 48) - __builtin_bit_cast(u64, 0x1p19));
-}
-
-constexpr u64 kEntrySum = (u64{1} << 48) - 1;
 
 // x: NaN compares false, and -inf lies at infinity
 __device__ __forceinline__ void add_to_bins(u64* bins, const Grid& g, float x) {
+#pragma clang fp contract(off)
   const double q = g.at(x), b = floor(q), d = b - g.base;
   if (d < kBins) atomicAdd(&bins[static_cast<int>(d)], bin_entry(q - b));
 }
@@ -402,14 +500,16 @@ __device__ __forceinline__ double bin_scale(const Grid& g, int bin) {
 
 struct Border {
   u64 last;    // the place of the last token that is kept
-  u64 sum;     // of the weights up to it
+  u128 sum;    // of the weights up to it
 };
 
 struct ListLds {
   u64 list[kList];
   u64 few[kThreads], few_sum[kThreads];
-  u64 part[kWaves][2];
+  u64 part[2][kWaves];
+  u128 part_sum[kWaves];
   u64 last, sum;
+  u128 before;
   uint32_t range[2];
   int n, found, picked, bin_k, bin_p, upto;
 };
@@ -421,29 +521,31 @@ static_assert(kBins == 1 << kDigit, "a digit a thread");
 // What each filter makes of the bins: those that the filters reach into (kBins: none), and the thread's
 // bin.
 struct Bins {
-  u64 count, sum;                  // of the thread's bin
-  u64 count_before, sum_before;    // of the bins before it
-  u64 total;
+  u64 count, count_before;         // tokens of the thread's bin, and of the bins before it
+  u128 sum, sum_before, total;     // and weights
   bool cut, by_p, by_m;            // top-k keeps fewer than there are; top-p; min-p
   int bin_k, bin_p, bin_m, bin_m_to, last;
 
   // the bin in which the sum reaches `goal`, at most the sum of all; a call of all threads
-  __device__ __forceinline__ int by_sum(ListLds& s, u64 goal) const {
+  __device__ __forceinline__ int by_sum(ListLds& s, u128 goal) const {
     __syncthreads();
     if (sum_before < goal && sum_before + sum >= goal) s.bin_p = threadIdx.x;
     __syncthreads();
     return s.bin_p;
   }
 
+  // n, m: the tokens of the thread's bin and the sum of their entries
   __device__ __forceinline__ Bins(ListLds& s, const Filters& f, const Grid& g, u64 n, u64 m)
-      : count(n), sum(m) {
-    const Scanned r = block_scan<true>(count, sum, s.part);
-    const u64 tokens = r.all_a;
-    count_before = r.a;
-    sum_before = r.b;
-    total = r.all_b;
+      : count(n), sum(static_cast<u128>(m) * bin_top(threadIdx.x)) {
+    Scanned<u64> counts;
+    Scanned<u128> sums;
+    block_scan(count, s.part[0], counts, sum, s.part_sum, sums);
+    const u64 tokens = counts.all;
+    count_before = counts.before;
+    sum_before = sums.before;
+    total = sums.all;
     cut = f.top_k > 0 && tokens > static_cast<u64>(f.top_k);
-    by_p = f.top_p < 1.0;
+    by_p = f.top_p < 1.f;
     by_m = f.min_p > 0.0;
     // The bins that may hold weights on both sides of min_p: one, or two where it lies at a border but for
     // roundings.  (A value's place in bins is off by 2^-52 of |x| scale; values lie 2^-24 of that apart,
@@ -469,19 +571,21 @@ struct Bins {
   }
 };
 
-// The last token of a list of n (places in any order) before which there is less than `goal`, tokens
-// (by_count) or sums; c and m lie before the list.  A call of all threads; s.few and s.few_sum are used,
-// and the list may be s.few.
-__device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, float top,
-                                            const Filters& f, bool by_count, u64 c, u64 m, u64 goal) {
+// The border in a bin: the last of its tokens before which there are less than `goal` tokens (by_count) or
+// entries.  Of a list of n places in any order `inside` are the bin's (all, where 64 or fewer are); c and m
+// lie before those.  Returns the entries up to the border in s.sum, its place in s.last.  A call of all
+// threads; s.few and s.few_sum are used, and the list may be s.few.
+__device__ __forceinline__ void border_of(ListLds& s, const u64* list, int n, int inside, const Grid& g,
+                                          int bin, bool by_count, u64 c, u64 m, u64 goal) {
   const int t = threadIdx.x;
   u64 base = 0, span = ~u64{0};   // the places that the border is among, `inside` of them
-  int inside = n;
-  if (n > kCompared) {   // from the least value to the largest
+  const bool many = inside > kCompared;
+  if (many) {   // from the bin's least value to the largest
     uint32_t least = ~0u, most = 0;
     if (t < 2) s.range[t] = t == 0 ? ~0u : 0u;
 #pragma unroll 1
     for (int i = t; i < n; i += kThreads) {
+      if (g.bin(value_at(list[i])) != bin) continue;
       const uint32_t v = static_cast<uint32_t>(list[i] >> 32);
       least = min(least, v);
       most = max(most, v);
@@ -498,41 +602,25 @@ __device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, 
     span = (static_cast<u64>(s.range[1] - s.range[0]) << 32) | 0xffffffffu;
   }
 #pragma unroll 1
-  while (inside > kCompared) {   // a digit, of 1,024 values, of the places
+  while (inside > kCompared && span != 0) {   // a digit, of 1,024 values, of the places
     const int shift = max(64 - kDigit - __clzll(static_cast<long long>(span)), 0);
     s.few_sum[t] = 0;
-    if (t == 0) s.found = -1;
     __syncthreads();
 #pragma unroll 1
     for (int i = t; i < n; i += kThreads) {
       const u64 d = list[i] - base;
       if (d <= span)
-        atomicAdd(&s.few_sum[d >> shift],
-                  by_count ? u64{1} : fixed(weight(value_at(list[i]), top, f.c)));
+        atomicAdd(&s.few_sum[d >> shift], by_count ? u64{1} : g.entry(value_at(list[i])));
     }
     __syncthreads();
     const u64 mine = s.few_sum[t];
-    const Scanned r = block_scan<false>(mine, 0, s.part);
-    const u64 have = (by_count ? c : m) + r.a;
-    if (have < goal && have + mine >= goal) {
+    const Scanned<u64> r = block_scan(mine, s.part[0]);
+    const u64 have = (by_count ? c : m) + r.before;
+    if (have < goal && have + mine >= goal) {   // one thread
       s.found = t;
-      s.sum = r.a;
+      s.sum = r.before;
     }
     __syncthreads();
-    // sums of single weights and of bins differ in their last bits: a goal past the last digit is in the
-    // last one that has tokens
-    const bool none = s.found < 0;
-    __syncthreads();
-    if (none) {
-#pragma unroll 1
-      for (int i = t; i < n; i += kThreads) {
-        const u64 d = list[i] - base;
-        if (d <= span) atomicMax(&s.found, static_cast<int>(d >> shift));
-      }
-      __syncthreads();
-      if (t == s.found) s.sum = r.a;
-      __syncthreads();
-    }
     const int digit = s.found;
     if (by_count) c += s.sum;
     u64 some = 0, before = 0;
@@ -542,17 +630,18 @@ __device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, 
       if (d > span) continue;
       const int at = static_cast<int>(d >> shift);
       some += at == digit;
-      if (at < digit) before += fixed(weight(value_at(list[i]), top, f.c));
+      if (at < digit) before += g.entry(value_at(list[i]));
     }
-    const Scanned q = block_scan<true>(some, before, s.part);
-    inside = static_cast<int>(q.all_a);
-    m += q.all_b;
+    Scanned<u64> left, entries;
+    block_scan(some, s.part[0], left, before, s.part[1], entries);
+    inside = static_cast<int>(left.all);
+    m += entries.all;
     base += static_cast<u64>(digit) << shift;
     span = (u64{1} << shift) - 1;
   }
   // those left are compared pair by pair
   u64 my = 0;
-  if (n > kCompared) {
+  if (many) {
     if (t == 0) s.picked = 0;
     __syncthreads();
 #pragma unroll 1
@@ -568,7 +657,7 @@ __device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, 
   u64 rank = 0, before = 0;
   if (t < inside) {
     my = list[t];
-    s.few_sum[t] = fixed(weight(value_at(my), top, f.c));
+    s.few_sum[t] = g.entry(value_at(my));
   }
   if (t == 0) s.found = 0;
   __syncthreads();
@@ -586,7 +675,6 @@ __device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, 
     s.sum = m + before + s.few_sum[t];
   }
   __syncthreads();
-  return Border{s.last, s.sum};
 }
 
 // The token of a row whose tokens in bins up to b.last, n <= kList of them, are in s.list as places in
@@ -594,23 +682,24 @@ __device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, 
 __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, const Filters& f, int row,
                                             int n, float top, const Grid& g, const Bins& b) {
   const int t = threadIdx.x;
-  // the border in bin `at`
-  auto border_in = [&](int at, bool by_count, u64 goal) {
+  // the border in bin `at`, before which there is less than `goal` (tokens or weights) of the row
+  auto border_in = [&](int at, bool by_count, u128 goal) {
     __syncthreads();
     if (t == at) {
-      s.sum = b.sum_before;
+      s.before = b.sum_before;
       s.last = b.count_before;
       s.upto = static_cast<int>(b.count);
     }
     if (t == 0) s.n = 0;
     __syncthreads();
-    u64 c = s.last, m = s.sum;
-    int some = s.upto;
+    const u64 c = s.last, top_at = bin_top(at);
+    const u128 ahead = s.before;
+    const int inside = s.upto;
+    int some = inside;
     u64* from = s.few;
-    if (some > kThreads) {   // thousands of tokens in a bin: the whole list in order
+    if (inside > kThreads) {   // thousands of tokens in a bin: among the whole list
       from = s.list;
       some = n;
-      c = m = 0;
     } else {
 #pragma unroll 1
       for (int i = t; i < n; i += kThreads) {
@@ -620,7 +709,9 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
       }
     }
     __syncthreads();
-    return border_of(s, from, some, top, f, by_count, c, m, goal);
+    border_of(s, from, some, inside, g, at, by_count, c, 0,
+              by_count ? static_cast<u64>(goal) : entries_for(goal - ahead, top_at));
+    return Border{s.last, ahead + static_cast<u128>(s.sum) * top_at};
   };
   // top-k, then top-p, in one copy of the code (a border past the last bin of the list is past what
   // min-p keeps)
@@ -628,7 +719,7 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
 #pragma unroll 1
   for (int step = b.cut ? 0 : 1; step < (b.by_p ? 2 : 1); ++step) {
     const bool by_count = step == 0;
-    const u64 goal = by_count ? static_cast<u64>(f.top_k) : share_of(f.top_p, border.sum);
+    const u128 goal = by_count ? static_cast<u128>(f.top_k) : share_of(f.top_p, border.sum);
     const int at = by_count ? b.bin_k : b.cut ? b.by_sum(s, goal) : b.bin_p;
     if (at > b.last) continue;
     const Border other = border_in(at, by_count, goal);
@@ -652,8 +743,8 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
   }
   __syncthreads();
   const u64 here = s.few_sum[t];
-  const Scanned r = block_scan<false>(here, 0, s.part);
-  const u64 ahead = r.a, total = r.all_a;
+  const Scanned<u64> r = block_scan(here, s.part[0]);
+  const u64 ahead = r.before, total = r.all;
   const u64 goal = target_of(p.uniform[row], total);
   if (ahead <= goal && goal < ahead + here) {   // one thread
     s.found = t;
@@ -762,7 +853,7 @@ __global__ __launch_bounds__(kThreads) void sample_list_kernel(const SampleArgs 
   }
   __syncthreads();
   const u64 entries = s.few[t];
-  const Bins b(s, f, g, entries >> 48, bin_sum(entries, bin_scale(g, t)));
+  const Bins b(s, f, g, entries >> 48, entries & kEntrySum);
   finish_list(s, p, f, row, p.vocab, top, g, b);
 }
 
@@ -886,8 +977,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     s.shift[t] = d < kBins ? static_cast<int>(d) : kBins;
   }
   const u64* bins = parts.bins + static_cast<int64_t>(row) * parts.n * kBins;
-  const double scale = bin_scale(g, t);
-  s.scale[t] = scale;
+  s.scale[t] = bin_scale(g, t);
   __syncthreads();
   u64 count = 0, sum = 0;
 #pragma unroll 4
@@ -895,7 +985,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     const int from = t - s.shift[i];
     const u64 e = from >= 0 ? bins[i * kBins + from] : 0;
     count += e >> 48;
-    sum += bin_sum(e, scale);
+    sum += e & kEntrySum;
   }
   const Bins b(s.l, f, g, count, sum);
   if ((b.cut || b.by_p || b.by_m) && s.l.upto <= kList) {
@@ -910,24 +1000,27 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     return;
   }
 
-  // The border in bin `bin`: the last token of the order before which there is less than `goal`, which
-  // the bin reaches.
+  // The border in bin `bin`: the last token of the order before which there is less than `share` (tokens
+  // or weights), which the bin reaches.
   int listed = -1;   // the bin whose tokens the list holds
-  auto border_in = [&](int bin, bool by_count, u64 goal) {
+  auto border_in = [&](int bin, bool by_count, u128 share) {
     __syncthreads();
     if (t == bin) {
-      s.l.sum = b.sum_before;
+      s.l.before = b.sum_before;
       s.l.last = b.count_before;
       s.l.upto = static_cast<int>(b.count);
     }
     __syncthreads();
-    u64 c = s.l.last, m = s.l.sum;
+    const u128 ahead = s.l.before;
+    const u64 top_at = bin_top(bin);
+    const u64 goal = by_count ? static_cast<u64>(share) : entries_for(share - ahead, top_at);
+    u64 c = s.l.last, m = 0;   // tokens before those looked at, and entries of the bin
     int inside = s.l.upto;
     u64 prefix = 0;      // the places' upper bits from `shift` on, once digits are taken
     int shift = 64;
     u64* sums = s.l.few_sum;
     u64* counts = s.l.few;
-    while (inside > kList) {
+    while (inside > kList && shift > 0) {
       const int next = max(shift - kDigit, 0);
       __syncthreads();
       sums[t] = 0;
@@ -939,23 +1032,16 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
         if (shift < 64 && a >> shift != prefix) return;
         const int digit = static_cast<int>((a >> next) & ((u64{1} << (shift - next)) - 1));
         atomicAdd(&counts[digit], u64{1});
-        atomicAdd(&sums[digit], fixed(weight(v, top, f.c)));
+        atomicAdd(&sums[digit], g.entry(v));
       });
-      if (t == 0) s.digit = -1;
       __syncthreads();
       const u64 dc = counts[t], dm = sums[t];
-      const Scanned r = block_scan<true>(dc, dm, s.l.part);
-      const u64 cb = c + r.a, mb = m + r.b;
+      Scanned<u64> rc, rm;
+      block_scan(dc, s.l.part[0], rc, dm, s.l.part[1], rm);
+      const u64 cb = c + rc.before, mb = m + rm.before;
       const u64 have = by_count ? cb : mb, more = by_count ? dc : dm;
-      if (have < goal && have + more >= goal) s.digit = t;
-      __syncthreads();
-      // sums of single weights and of bins differ in their last bits: a goal past the last digit is in
-      // the last one that has tokens
-      const bool none = s.digit < 0;
-      __syncthreads();
-      if (none && dc > 0) atomicMax(&s.digit, t);
-      __syncthreads();
-      if (t == s.digit) {
+      if (have < goal && have + more >= goal) {   // one thread
+        s.digit = t;
         s.l.sum = mb;
         s.l.last = cb;
         s.l.upto = static_cast<int>(dc);
@@ -977,7 +1063,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     });
     __syncthreads();
     listed = shift == 64 ? bin : -1;
-    return border_of(s.l, s.l.list, s.l.n, top, f, by_count, c, m, goal);
+    border_of(s.l, s.l.list, s.l.n, s.l.n, g, bin, by_count, c, m, goal);
+    return Border{s.l.last, ahead + static_cast<u128>(s.l.sum) * top_at};
   };
 
   Border border{~u64{0}, b.total};
@@ -985,7 +1072,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
 #pragma unroll 1
   for (int step = b.cut ? 0 : 1; step < (b.by_p ? 2 : 1); ++step) {   // top-k, then top-p
     const bool by_count = step == 0;
-    const u64 goal = by_count ? static_cast<u64>(f.top_k) : share_of(f.top_p, border.sum);
+    const u128 goal = by_count ? static_cast<u128>(f.top_k) : share_of(f.top_p, border.sum);
     const int bin = by_count ? b.bin_k : b.by_sum(s.l, goal);
     if (bin > b.bin_m_to && !(by_count && b.by_p)) continue;   // past what min-p keeps
     const Border other = border_in(bin, by_count, goal);
@@ -1004,7 +1091,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     u64 m = 0;
     for (int bin = lane; bin < full; bin += kWave)
       if (bin >= s.shift[i]) m += bin_sum(bins[i * kBins + bin - s.shift[i]], s.scale[bin]);
-    m = wave_sum64(m);
+    m = wave_total(m);
     if (lane == 0) s.part_sum[i] = m;
   }
   __syncthreads();
@@ -1031,7 +1118,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     }
     __syncthreads();
     static_assert(kMaxParts * 16 <= kThreads, "a sum a thread");
-    const u64 sum16 = row_scan64(s.l.few[t]);
+    const u64 sum16 = row_scan(s.l.few[t]);
     if ((t & 15) == 15 && t / 16 < parts.n) s.part_sum[t / 16] += sum16;
   }
   __syncthreads();
@@ -1068,8 +1155,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  const Scanned r = block_scan<false>(here, 0, s.l.part);
-  const u64 ahead = r.a, sums = r.all_a;
+  const Scanned<u64> r = block_scan(here, s.l.part[0]);
+  const u64 ahead = r.before, sums = r.all;
   const double want = static_cast<double>(goal) / against;
   const u64 at_sum = want < static_cast<double>(sums) ? min(static_cast<u64>(want), sums - 1) : sums - 1;
   if (!(ahead <= at_sum && at_sum < ahead + here)) return;   // one thread stays
