@@ -813,8 +813,10 @@ int64_t mdl_attn_paged_workspace_bytes(int n_seq, int tokens, int max_q, int n_h
  * temperature of 0 or below (or NaN), a top_k of 1, a top_p of 0 or below and a min_p above 1 give the
  * first of the order, with logprob 0; a NaN top_p or min_p is no filter.  uniform outside [0, 1) is taken
  * as the nearest inside.  NaN logits count as -inf, which is never taken; a row of nothing
- * else gives token 0 and logprob -inf.  Weights are of 64 bits and their sums do not depend on an order,
- * so equal calls give equal tokens; tokens below 2^-43 of the largest may count as nothing.
+ * else gives token 0 and logprob -inf.  In sums, weights are whole numbers (to 2^-33 of their own size, and
+ * 2^-59 of the largest) that are added without rounding, so a row's token and logprob are the same in
+ * every call, whatever rows are beside it, and equal logits make equal steps: a share or a random number that
+ * meets their sum exactly is taken as above.  Tokens below 2^-58 of the largest may count as nothing.
  * workspace (8-byte aligned): mdl_sample_workspace_bytes of the same sizes, 0 up to 4,096 tokens; calls
  * that may overlap in time need workspaces of their own.
  * Replaces: the temperature / top-k branch of generate_output (src/inference.py:573-583) with the

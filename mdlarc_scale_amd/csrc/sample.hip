@@ -10,10 +10,10 @@
 //           u times the sum of all.
 // Each filter keeps a run of the order from its first token on.
 //
-// Exactness: a token flips where a sum of weights passes a border, so weights are computed in 64
-// bits and summed as whole numbers: such sums do not depend on their order (atomics among them).  The draw's
-// are multiples of 2^-43, of which 2^20 fit 64 bits.  (CDNA's 64-bit multiply-adds run at the rate of
-// 32-bit ones.)  The filters' are those of "weights in sums" below, to 2^-34 of a weight, in 128 bits.
+// Exactness: a token flips where a sum of weights passes a border, so weights are computed in 64 bits, held
+// as whole numbers to 2^-33 of themselves, and summed in 128 bits without rounding ("weights in sums"
+// below): sums depend neither on their order (atomics among them) nor on how a row is cut, and equal
+// logits make equal steps.  (CDNA's 64-bit multiply-adds run at the rate of 32-bit ones.)
 //
 // Three sizes of rows:
 //   up to 64 tokens: a wave a row, a token a lane; the order comes from comparing every pair;
@@ -23,17 +23,17 @@
 //   is kept, up to 4,096 of them, to LDS.
 // Counts and sums of weights in 1,024 bins of 1/16 octave say which bins the filters reach into.  (The
 // bins lie on a grid that does not depend on the part, so those of parts add up; in a bin a weight is
-// its top times 2^(-f / 16), a short polynomial.)  Inside such a bin the border is found by
-// digits of the tokens' places in the order, 1,024 values each, and the last 64 by comparing every pair.
-// The kept weights are then summed by stretches of indexes, and the tokens
-// of the stretch that holds the result compared by index.  Where more than 4,096 tokens are kept the
+// its top times 2^(-f / 16), a short polynomial.)  Inside such a bin the border is found by digits of the
+// tokens' places in the order, 1,024 values each, and the last 64 by comparing every pair.  The kept
+// weights are then summed by stretches of indexes, and the tokens of the stretch that holds the result
+// compared by index.  Where more than 4,096 tokens are kept the
 // row's second launch looks for the borders in their bins alone, cut by the digits of value and index
 // where thousands are equal, and takes the parts' kept sums from their bins.
 //
 // What bounds it: one block's chain of steps, most of them waits (VALU busy 8% in the second launch).  64
-// rows of 131,072 logits, 43 to 54 us by their filters: the bins 12 (64-bit arithmetic, 20 instructions
-// a token), a row's second launch 25 at the median, the most for its pass over the row (8), and up to 40
-// where more than 4,096 tokens are kept; 256 rows of 4,000 20 us, of 14 4.2 to 4.9 us.
+// rows of 131,072 logits, 45 to 56 us by their filters: the bins 11.5 (64-bit arithmetic, 20 instructions
+// a token), the second launch 33 to 43, as long as its longest row, one with more than 4,096 tokens kept;
+// 256 rows of 4,000 21 us, of 14 5.6 us.
 #include <cfloat>
 
 #include "common.h"
@@ -58,7 +58,6 @@ struct SampleArgs {
 typedef unsigned long long u64;
 typedef unsigned __int128 u128;
 
-constexpr u64 kOne = u64{1} << 43;          // the fixed-point 1
 constexpr double kLog2e = 1.4426950408889634074;
 
 __device__ __forceinline__ float logit(const float* p, int64_t i) { return p[i]; }
@@ -90,10 +89,6 @@ __device__ __forceinline__ double weight(float x, float top, double c) {
   return ldexp(fma(w, y, 1.0), static_cast<int>(n));
 }
 
-__device__ __forceinline__ u64 fixed(double w) {   // w in [0, 1], to the nearest 2^-43
-  return __builtin_bit_cast(u64, w + 512.0) - __builtin_bit_cast(u64, 512.0);
-}
-
 // Ascending in the order of tokens: larger values first (-0 is 0), then lower indexes.
 __device__ __forceinline__ u64 place(float x, int i) {
   const uint32_t b = __float_as_uint(x + 0.f);
@@ -117,22 +112,57 @@ __device__ __forceinline__ uint32_t dpp(uint32_t none, uint32_t v) {
   return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
 }
 
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ u64 plus_dpp(u64 v) {
-  return v + (static_cast<u64>(dpp<CTRL, ROWS>(0, static_cast<uint32_t>(v >> 32))) << 32 |
-              dpp<CTRL, ROWS>(0, static_cast<uint32_t>(v)));
+__device__ __forceinline__ u64 of_words(uint32_t low, uint32_t high) {
+  return __builtin_bit_cast(u64, make_uint2(low, high));
+}
+
+// dpp with none = 0 (without a mask of rows the instruction makes the zeros itself)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, ROWS == 0xf);
 }
 
 template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ u128 plus_dpp(u128 v) {
-  u128 other = 0;
-#pragma unroll
-  for (int i = 96; i >= 0; i -= 32)
-    other = other << 32 | dpp<CTRL, ROWS>(0, static_cast<uint32_t>(v >> i));
+__device__ __forceinline__ u64 plus_dpp(u64 v) {
+  u64 other = of_words(dpp0<CTRL, ROWS>(static_cast<uint32_t>(v)),
+                       dpp0<CTRL, ROWS>(static_cast<uint32_t>(v >> 32)));
+  asm("" : "+v"(other));   // one addition of 64 bits: the compiler makes one of each half otherwise
   return v + other;
 }
 
-// the sums over 16 neighbouring lanes up to the lane's own (T: u64 or u128)
+__device__ __forceinline__ u64 of_lane(u64 v, int lane) {   // the same lane for the whole wave
+  return of_words(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane),
+                  __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane));
+}
+
+__device__ __forceinline__ u128 of_lane(u128 v, int lane) {
+  return static_cast<u128>(of_lane(static_cast<u64>(v >> 64), lane)) << 64 |
+         of_lane(static_cast<u64>(v), lane);
+}
+
+// A sum below 2^112 in two words, 2^48 high + low.  Split so, 2^15 sums add up to it without a carry.
+// (Sums of 128 bits take a carry, and its two wait cycles, for every 32 bits of a step.)
+struct Words {
+  u64 low, high;
+};
+
+__device__ __forceinline__ Words split(u128 v) {
+  return {static_cast<u64>(v) & ((u64{1} << 48) - 1), static_cast<u64>(v >> 48)};
+}
+__device__ __forceinline__ u128 joined(Words v) { return (static_cast<u128>(v.high) << 48) + v.low; }
+
+__device__ __forceinline__ Words operator+(Words a, Words b) { return {a.low + b.low, a.high + b.high}; }
+__device__ __forceinline__ Words operator-(Words a, Words b) { return {a.low - b.low, a.high - b.high}; }
+
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ Words plus_dpp(Words v) {
+  return {plus_dpp<CTRL, ROWS>(v.low), plus_dpp<CTRL, ROWS>(v.high)};
+}
+__device__ __forceinline__ Words of_lane(Words v, int lane) {
+  return {of_lane(v.low, lane), of_lane(v.high, lane)};
+}
+
+// the sums over 16 neighbouring lanes up to the lane's own (T: u64 or Words)
 template <typename T>
 __device__ __forceinline__ T row_scan(T v) {
   return plus_dpp<0x118>(plus_dpp<0x114>(plus_dpp<0x112>(plus_dpp<0x111>(v))));
@@ -143,19 +173,6 @@ __device__ __forceinline__ T wave_scan(T v) {   // inclusive
   return plus_dpp<0x143, 0xc>(plus_dpp<0x142, 0xa>(row_scan(v)));
 }
 
-__device__ __forceinline__ u64 of_lane(u64 v, int lane) {   // the same lane for the whole wave
-  return static_cast<u64>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane)) << 32 |
-         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane));
-}
-
-__device__ __forceinline__ u128 of_lane(u128 v, int lane) {
-  return static_cast<u128>(of_lane(static_cast<u64>(v >> 64), lane)) << 64 |
-         of_lane(static_cast<u64>(v), lane);
-}
-
-template <typename T>
-__device__ __forceinline__ T wave_total(T v) { return of_lane(wave_scan(v), 63); }
-
 __device__ __forceinline__ uint32_t wave_most(uint32_t v) {   // in lane 63
   v = max(v, dpp<0x111>(v, v));
   v = max(v, dpp<0x112>(v, v));
@@ -165,39 +182,38 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {   // in lane 63
   return max(v, dpp<0x143, 0xc>(v, v));
 }
 
-// The sum that the token's own has to pass.  u outside [0, 1) is taken as the nearest inside.
-__device__ __forceinline__ u64 target_of(float u, u64 total) {
-  const double t = static_cast<double>(u) * static_cast<double>(total);
-  if (!(t > 0.0)) return 0;
-  const u64 at = t < 0x1p63 ? static_cast<u64>(t) : total;
-  return at < total ? at : total - 1;
-}
-
-// f times `total` (0 < f < 1, total below 2^116), rounded up.  Tokens before which there is less than
-// this whole number are those before which there is less than the share f.
-__device__ __forceinline__ u128 share_of(float f, u128 total) {
+// f times `total` (0 < f < 1, total below 2^112), rounded down or up.  The sums below a share are those below
+// the number rounded up, the ones above it those above the number rounded down.
+__device__ __forceinline__ u128 share_of(float f, u128 total, bool up) {
   const uint32_t b = __float_as_uint(f);
   const uint32_t m = (b & 0x7fffffu) | (b >= 0x800000u ? 0x800000u : 0u);
   const int k = 150 - max(static_cast<int>(b >> 23), 1);   // f = m 2^-k, 24 <= k <= 149
-  // m total = 2^64 high + low
   const u128 first = static_cast<u128>(m) * static_cast<u64>(total);
   const u128 high = static_cast<u128>(m) * static_cast<u64>(total >> 64) + (first >> 64);
-  const u64 low = static_cast<u64>(first);
-  u128 whole;
-  bool rest;
-  if (k < 64) {
-    whole = high << (64 - k) | low >> k;
-    rest = low << (64 - k) != 0;
-  } else {
-    whole = high >> (k - 64);
-    rest = low != 0 || whole << (k - 64) != high;
-  }
-  return whole + (rest ? 1 : 0);
+  // m total in words of 64 bits, shifted by k: whole words, then bits
+  u64 w[3] = {static_cast<u64>(first), static_cast<u64>(high), static_cast<u64>(high >> 64)};
+  u64 rest = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (k >= 64 * (i + 1)) {
+      rest |= w[0];
+      w[0] = w[1]; w[1] = w[2]; w[2] = 0;
+    }
+  const int n = k & 63;
+  rest |= w[0] & ((u64{1} << n) - 1);
+  const u64 low = w[0] >> n | w[1] << 1 << (63 - n), top = w[1] >> n | w[2] << 1 << (63 - n);
+  return (static_cast<u128>(top) << 64 | low) + (up && rest != 0 ? 1 : 0);
+}
+
+// The sum that the token's own has to pass.  u outside [0, 1) is taken as the nearest inside.
+__device__ __forceinline__ u128 target_of(float u, u128 total) {
+  if (!(u > 0.f)) return 0;
+  return u < 1.f ? share_of(u, total, false) : total - 1;
 }
 
 struct Filters {
   double c, min_p;
-  float top_p;
+  float top_p, u;
   int top_k;      // 0: none
   bool greedy;
 };
@@ -207,6 +223,7 @@ __device__ __forceinline__ Filters filters_of(const SampleArgs& p, int row) {
   const float t = p.temperature ? p.temperature[row] : 1.f;
   f.top_k = p.top_k ? max(p.top_k[row], 0) : 0;
   f.top_p = p.top_p ? p.top_p[row] : 1.f;
+  f.u = p.uniform[row];   // needed last, and read with the others
   const float m = p.min_p ? p.min_p[row] : 0.f;
   f.min_p = m > 0.f ? static_cast<double>(m) : 0.0;   // NaN: none
   // a share of nothing, and a bound that no weight reaches, leave the first token
@@ -215,46 +232,62 @@ __device__ __forceinline__ Filters filters_of(const SampleArgs& p, int row) {
   return f;
 }
 
-__device__ __forceinline__ void leave(const SampleArgs& p, int row, int token, double w, u64 total) {
+__device__ __forceinline__ double to_double(u128 v) {
+  return static_cast<double>(static_cast<u64>(v >> 64)) * 0x1p64 +
+         static_cast<double>(static_cast<u64>(v));
+}
+
+// w of `total` is the token's share
+__device__ __forceinline__ void leave(const SampleArgs& p, int row, int token, u128 w, u128 total) {
   p.token[row] = token;
-  if (p.logprob)
-    p.logprob[row] = static_cast<float>(log(w / (static_cast<double>(total) / kOne)));
+  if (p.logprob) p.logprob[row] = static_cast<float>(log(to_double(w) / to_double(total)));
+}
+
+// the first of the order alone, or (top -inf) token 0 of a row of nothing
+__device__ __forceinline__ void leave_alone(const SampleArgs& p, int row, int token, float top) {
+  p.token[row] = top == -INFINITY ? 0 : token;
+  if (p.logprob) p.logprob[row] = top == -INFINITY ? -INFINITY : 0.f;
 }
 
 // ---- weights in sums -------------------------------------------------------------------------------
 
-// Weights as whole numbers that add up: the borders of the filters compare sums of tokens with shares of
-// others, and equal sums have to be equal whatever they are made of.  A token's weight is its entry (its
-// weight over that of its bin's top, to the nearest 2^-33) times bin_top of its bin, both of which depend
-// on the token and the row's largest alone, so that a bin's sum is bin_top times the sum of its entries.
-// 2^20 tokens make less than 2^116.
+// Weights as whole numbers that add up: the borders of the filters and the draw compare sums of tokens with
+// shares of others, and equal sums have to be equal whatever they are made of.  A token's weight is its
+// entry (its weight over that of its bin's top, to the nearest 2^-33) times bin_top of its bin, both of
+// which depend on the token and the row's largest alone, so that a bin's sum is bin_top times the sum of
+// its entries.  2^20 tokens make less than 2^112.  min-p alone, which sums nothing, compares weight().
 
 constexpr int kBins = 1024;
 constexpr double kBinsOctave = 16.0;
 
-// What a token adds to its bin: a count in the upper 16 bits, and the weight over that of the bin's
-// top, 2^(-f / 16) with 0 <= f < 1, to the nearest 2^-33 (and 2^-36 that the polynomial is off by).
-__device__ __forceinline__ u64 bin_entry(double f) {
+// The weight over that of the bin's top, 2^(-f / 16) with 0 <= f < 1, to the nearest 2^-33 (and 2^-36 that
+// the polynomial is off by), as a double: 2^19 more, whose last bit is 2^-33.
+__device__ __forceinline__ u64 entry_bits(double f) {
   constexpr double h = -0.69314718055994530942 / kBinsOctave;
   double w = h * h * h * h * h / 120;   // e^(h f): the next term is below 2^-36
   w = fma(w, f, h * h * h * h / 24);
   w = fma(w, f, h * h * h / 6);
   w = fma(w, f, h * h / 2);
   w = fma(w, f, h);
-  w = fma(w, f, 1.0 + 0x1p19);          // from here on the last bit is 2^-33
-  return __builtin_bit_cast(u64, w) + ((u64{1} << 48) - __builtin_bit_cast(u64, 0x1p19));
+  return __builtin_bit_cast(u64, fma(w, f, 1.0 + 0x1p19));
+}
+
+// What a token adds to its bin: a count in the upper 16 bits, and its entry.
+__device__ __forceinline__ u64 bin_entry(double f) {
+  return entry_bits(f) + ((u64{1} << 48) - __builtin_bit_cast(u64, 0x1p19));
 }
 
 constexpr u64 kEntrySum = (u64{1} << 48) - 1;
 
-// 2^62 times 2^(-bin / 16), the weight of a bin's top, to the nearest whole number (but for 2^-60 of it)
+// 2^58 times 2^(-bin / 16), the weight of a bin's top, to the nearest whole number (but for 2^-50 of it)
 __device__ __forceinline__ u64 bin_top(int bin) {
-  u64 t = u64{1} << 63;
-  t = bin & 1 ? __umul64hi(t, 0xf5257d152486cc2cull) : t;   // 2^64 times 2^(-1 / 16)
-  t = bin & 2 ? __umul64hi(t, 0xeac0c6e7dd24392full) : t;   // 2^(-2 / 16)
-  t = bin & 4 ? __umul64hi(t, 0xd744fccad69d6af4ull) : t;   // 2^(-4 / 16)
-  t = bin & 8 ? __umul64hi(t, 0xb504f333f9de6484ull) : t;   // 2^(-8 / 16)
-  return ((t >> (bin >> 4)) + 1) >> 1;                      // bins below 1,024
+#pragma clang fp contract(off)
+  double t = 0x1p58;
+  t *= bin & 1 ? 0.95760328069857364694 : 1.0;   // 2^(-1 / 16)
+  t *= bin & 2 ? 0.91700404320467123174 : 1.0;
+  t *= bin & 4 ? 0.84089641525371454303 : 1.0;
+  t *= bin & 8 ? 0.70710678118654752440 : 1.0;   // 2^(-8 / 16)
+  return static_cast<u64>(ldexp(t, -(bin >> 4)) + 0.5);
 }
 
 // The row's bins: 1/16 octave each, bin 0 with the largest value; kBins for values below all of them.
@@ -278,13 +311,18 @@ struct Grid {
     const double d = floor(at(x)) - base;
     return d < kBins ? static_cast<int>(d) : kBins;
   }
-  // the token's entry in its bin (bin_entry's weight), 0 below all bins
-  __device__ __forceinline__ u64 entry(float x) const {
+  // a token's bin, and its entry there; none below all bins
+  struct Token {
+    u64 entry;
+    int bin;
+  };
+  __device__ __forceinline__ Token token(float x) const {
 #pragma clang fp contract(off)
-    if (huge) return x == INFINITY ? bin_entry(0.0) & kEntrySum : 0;
-    const double q = at(x), b = floor(q);   // of NaN and -inf: no bin
-    return b - base < kBins ? bin_entry(q - b) & kEntrySum : 0;
+    const double q = huge ? (x == INFINITY ? 0.0 : INFINITY) : at(x), b = floor(q);
+    if (!(b - base < kBins)) return {0, kBins};   // NaN and -inf too
+    return {entry_bits(q - b) & ((u64{1} << 52) - 1), static_cast<int>(b - base)};
   }
+  __device__ __forceinline__ u64 entry(float x) const { return token(x).entry; }
   // bounds of the values in bins `first` .. `last` (a few roundings of fp32 wider)
   __device__ __forceinline__ float least(int last) const {
     if (huge) return INFINITY;
@@ -297,25 +335,6 @@ struct Grid {
     return static_cast<float>(x + fabs(x) * 0x1p-20);
   }
 };
-
-// A token's weight in the sums
-__device__ __forceinline__ u128 sum_weight(const Grid& g, float x) {
-  const u64 e = g.entry(x);
-  return e == 0 ? 0 : static_cast<u128>(e) * bin_top(g.bin(x));
-}
-
-// The least whole number that times `top` reaches `need`.  It is at most the entries of 2^20 tokens, 2^53, of
-// which four roundings of the estimate make 4.
-__device__ __forceinline__ u64 entries_for(u128 need, u64 top) {
-  const double high = static_cast<double>(static_cast<u64>(need >> 64));
-  u64 n = static_cast<u64>((high * 0x1p64 + static_cast<double>(static_cast<u64>(need))) /
-                           static_cast<double>(top));
-#pragma unroll 1
-  for (int i = 0; i < 8 && static_cast<u128>(n) * top < need; ++i) ++n;
-#pragma unroll 1
-  for (int i = 0; i < 8 && n > 0 && static_cast<u128>(n - 1) * top >= need; ++i) --n;
-  return n;
-}
 
 // ---- a wave a row ------------------------------------------------------------------------------
 
@@ -331,31 +350,35 @@ __global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs p) {
   const float top = wave_max(x);
   if (top == -INFINITY || f.greedy) {
     const u64 best = __ballot(x == top);
-    if (lane == 0) leave(p, row, __ffsll(best) - 1, top == -INFINITY ? 0.0 : 1.0, kOne);
+    if (lane == 0) leave_alone(p, row, __ffsll(best) - 1, top);
     return;
   }
-  const double w = weight(x, top, f.c);
-  const u64 mine = fixed(w), at = place(x, lane);
-  const u128 held = sum_weight(Grid(top, f.c), x);
+  const u64 at = place(x, lane);
+  const Grid::Token my = Grid(top, f.c).token(x);
+  const u128 mine = static_cast<u128>(my.entry) * bin_top(my.bin);
+  const Words words = split(mine);
   int rank = 0;
-  u128 before = 0;
-  for (int j = 0; j < p.vocab; ++j) {
+  Words ahead_of_it{0, 0};
+  for (int j = 0; j < p.vocab && (f.top_k > 0 || f.top_p < 1.f); ++j) {
     const bool ahead = of_lane(at, j) < at;
-    const u128 other = of_lane(held, j);
+    const Words other = of_lane(words, j);
     rank += ahead;
-    before += ahead ? other : 0;
+    ahead_of_it = ahead_of_it + (ahead ? other : Words{0, 0});
   }
-  bool kept = held != 0 && (f.top_k == 0 || rank < f.top_k);
+  const u128 before = joined(ahead_of_it);
+  bool kept = mine != 0 && (f.top_k == 0 || rank < f.top_k);
   if (f.top_p < 1.f) {
-    const u128 sum = wave_total(kept ? held : 0);
-    kept = kept && before < share_of(f.top_p, sum);
+    // the sum of what top-k keeps: up to its last token
+    const int last = (f.top_k == 0 ? p.vocab : min(f.top_k, p.vocab)) - 1;
+    const u128 sum = of_lane(before + mine, __ffsll(__ballot(rank == last)) - 1);
+    kept = kept && before < share_of(f.top_p, sum, true);
   }
-  kept = kept && w >= f.min_p;
-  const u64 sums = wave_scan(kept ? mine : 0);
-  const u64 total = of_lane(sums, 63);
-  const u64 goal = target_of(p.uniform[row], total);
+  if (f.min_p > 0.0) kept = kept && weight(x, top, f.c) >= f.min_p;
+  const u128 sums = joined(wave_scan(split(kept ? mine : 0)));
+  const u128 total = of_lane(sums, 63);
+  const u128 goal = target_of(f.u, total);
   const u64 past = __ballot(sums > goal);
-  if (lane == __ffsll(past) - 1) leave(p, row, lane, w, total);
+  if (lane == __ffsll(past) - 1) leave(p, row, lane, mine, total);
 }
 
 // ---- a block a row -----------------------------------------------------------------------------
@@ -449,7 +472,7 @@ __device__ __forceinline__ Scanned<T> with_waves(T v, T scan, const T* part) {
   static_assert(kWaves == 16, "the waves' sums in a row of lanes");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T waves = row_scan(part[threadIdx.x & 15]);
-  return {scan - v + (wave == 0 ? 0 : of_lane(waves, max(wave - 1, 0))), of_lane(waves, kWaves - 1)};
+  return {scan - v + (wave == 0 ? T{} : of_lane(waves, max(wave - 1, 0))), of_lane(waves, kWaves - 1)};
 }
 
 template <typename T>
@@ -461,11 +484,16 @@ __device__ __forceinline__ Scanned<T> block_scan(T v, T* part) {
   return with_waves(v, scan, part);
 }
 
-template <typename A, typename B>
-__device__ __forceinline__ void block_scan(A a, A* part_a, Scanned<A>& sums_a, B b, B* part_b,
-                                           Scanned<B>& sums_b) {
-  const A scan_a = wave_scan(a);
-  const B scan_b = wave_scan(b);
+__device__ __forceinline__ Scanned<u128> block_scan(u128 v, Words* part) {
+  const Scanned<Words> r = block_scan(split(v), part);
+  return {joined(r.before), joined(r.all)};
+}
+
+template <typename T>
+__device__ __forceinline__ void block_scan(u64 a, u64* part_a, Scanned<u64>& sums_a, T b, T* part_b,
+                                           Scanned<T>& sums_b) {
+  const u64 scan_a = wave_scan(a);
+  const T scan_b = wave_scan(b);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) {
     part_a[threadIdx.x >> 6] = scan_a;
@@ -488,14 +516,11 @@ __device__ __forceinline__ void add_huge(u64* bins, float x) {   // the row's la
   if (x == INFINITY) atomicAdd(&bins[0], bin_entry(0.0));
 }
 
-// The sum of weights of bin `bin` with the entries' sum `e`, in multiples of 2^-43; scale: the weight of
-// the bin's top.
-__device__ __forceinline__ u64 bin_sum(u64 e, double scale) {
-  return static_cast<u64>(static_cast<double>(e & kEntrySum) * scale * 0x1p10 + 0.5);
-}
-
-__device__ __forceinline__ double bin_scale(const Grid& g, int bin) {
-  return exp2((g.at_top - g.base - bin) * (1.0 / kBinsOctave));
+// Sums of up to 2^15 weights by atomics, in Words.
+__device__ __forceinline__ void add_weight(u64* low, u64* high, u128 w) {
+  const Words v = split(w);
+  atomicAdd(low, v.low);
+  atomicAdd(high, v.high);
 }
 
 struct Border {
@@ -505,11 +530,12 @@ struct Border {
 
 struct ListLds {
   u64 list[kList];
-  u64 few[kThreads], few_sum[kThreads];
+  u64 few[kThreads], few_sum[kThreads], few_high[kThreads];
+  u64 tops[kBins];   // bin_top
   u64 part[2][kWaves];
-  u128 part_sum[kWaves];
+  Words part_sum[kWaves];
   u64 last, sum;
-  u128 before;
+  u128 before;   // weights before what is looked at
   uint32_t range[2];
   int n, found, picked, bin_k, bin_p, upto;
 };
@@ -523,6 +549,7 @@ static_assert(kBins == 1 << kDigit, "a digit a thread");
 struct Bins {
   u64 count, count_before;         // tokens of the thread's bin, and of the bins before it
   u128 sum, sum_before, total;     // and weights
+  u128 goal_p;                     // top-p's, where top-k does not change its sum
   bool cut, by_p, by_m;            // top-k keeps fewer than there are; top-p; min-p
   int bin_k, bin_p, bin_m, bin_m_to, last;
 
@@ -536,14 +563,17 @@ struct Bins {
 
   // n, m: the tokens of the thread's bin and the sum of their entries
   __device__ __forceinline__ Bins(ListLds& s, const Filters& f, const Grid& g, u64 n, u64 m)
-      : count(n), sum(static_cast<u128>(m) * bin_top(threadIdx.x)) {
+      : count(n) {
+    const u64 top = bin_top(threadIdx.x);
+    s.tops[threadIdx.x] = top;   // for all from here on
+    sum = static_cast<u128>(m) * top;
     Scanned<u64> counts;
-    Scanned<u128> sums;
-    block_scan(count, s.part[0], counts, sum, s.part_sum, sums);
+    Scanned<Words> sums;
+    block_scan(count, s.part[0], counts, split(sum), s.part_sum, sums);
     const u64 tokens = counts.all;
     count_before = counts.before;
-    sum_before = sums.before;
-    total = sums.all;
+    sum_before = joined(sums.before);
+    total = joined(sums.all);
     cut = f.top_k > 0 && tokens > static_cast<u64>(f.top_k);
     by_p = f.top_p < 1.f;
     by_m = f.min_p > 0.0;
@@ -561,7 +591,8 @@ struct Bins {
       __syncthreads();
       bin_k = s.bin_k;
     } else if (by_p) {
-      bin_p = by_sum(s, share_of(f.top_p, total));
+      goal_p = share_of(f.top_p, total, true);
+      bin_p = by_sum(s, goal_p);
     }
     // everything that is kept is in bins up to `last`, and so is what top-p's share is of: all that
     // top-k keeps, or the total
@@ -571,12 +602,26 @@ struct Bins {
   }
 };
 
-// The border in a bin: the last of its tokens before which there are less than `goal` tokens (by_count) or
-// entries.  Of a list of n places in any order `inside` are the bin's (all, where 64 or fewer are); c and m
-// lie before those.  Returns the entries up to the border in s.sum, its place in s.last.  A call of all
-// threads; s.few and s.few_sum are used, and the list may be s.few.
-__device__ __forceinline__ void border_of(ListLds& s, const u64* list, int n, int inside, const Grid& g,
-                                          int bin, bool by_count, u64 c, u64 m, u64 goal) {
+// What a border is looked for by: a number of tokens of the row, or a weight.
+struct Goal {
+  bool by_count;
+  u128 goal;
+  u128 ahead;   // the weights before the border's bin
+  u64 top;      // bin_top of that bin
+
+  // c tokens, or m entries of the bin, are less than it
+  __device__ __forceinline__ bool above(u64 c, u64 m) const {
+    return by_count ? c < static_cast<u64>(goal) : ahead + static_cast<u128>(m) * top < goal;
+  }
+};
+
+// The border in a bin: the last of its tokens before which there is less than the goal.  Of a list of n
+// places in any order `inside` are the bin's (all, where 64 or fewer are); c tokens and m entries of the
+// bin lie before those.  Returns the place of the border, and the weights up to it.  A call of all threads;
+// s.few and s.few_sum are used, and the list may be s.few.
+__device__ __forceinline__ Border border_of(ListLds& s, const u64* list, int n, int inside, const Grid& g,
+                                            int bin, const Goal& goal, u64 c, u64 m) {
+  const bool by_count = goal.by_count;
   const int t = threadIdx.x;
   u64 base = 0, span = ~u64{0};   // the places that the border is among, `inside` of them
   const bool many = inside > kCompared;
@@ -616,7 +661,7 @@ __device__ __forceinline__ void border_of(ListLds& s, const u64* list, int n, in
     const u64 mine = s.few_sum[t];
     const Scanned<u64> r = block_scan(mine, s.part[0]);
     const u64 have = (by_count ? c : m) + r.before;
-    if (have < goal && have + mine >= goal) {   // one thread
+    if (goal.above(have, have) && !goal.above(have + mine, have + mine)) {   // one thread
       s.found = t;
       s.sum = r.before;
     }
@@ -667,7 +712,7 @@ __device__ __forceinline__ void border_of(ListLds& s, const u64* list, int n, in
       rank += ahead;
       before += ahead ? s.few_sum[j] : 0;
     }
-    if ((by_count ? c + rank : m + before) < goal) atomicMax(&s.found, static_cast<int>(rank));
+    if (goal.above(c + rank, m + before)) atomicMax(&s.found, static_cast<int>(rank));
   }
   __syncthreads();
   if (t < inside && static_cast<int>(rank) == s.found) {
@@ -675,6 +720,7 @@ __device__ __forceinline__ void border_of(ListLds& s, const u64* list, int n, in
     s.sum = m + before + s.few_sum[t];
   }
   __syncthreads();
+  return Border{s.last, goal.ahead + static_cast<u128>(s.sum) * goal.top};
 }
 
 // The token of a row whose tokens in bins up to b.last, n <= kList of them, are in s.list as places in
@@ -692,8 +738,8 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
     }
     if (t == 0) s.n = 0;
     __syncthreads();
-    const u64 c = s.last, top_at = bin_top(at);
-    const u128 ahead = s.before;
+    const u64 c = s.last;
+    const Goal border{by_count, goal, s.before, s.tops[at]};
     const int inside = s.upto;
     int some = inside;
     u64* from = s.few;
@@ -709,9 +755,7 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
       }
     }
     __syncthreads();
-    border_of(s, from, some, inside, g, at, by_count, c, 0,
-              by_count ? static_cast<u64>(goal) : entries_for(goal - ahead, top_at));
-    return Border{s.last, ahead + static_cast<u128>(s.sum) * top_at};
+    return border_of(s, from, some, inside, g, at, border, c, 0);
   };
   // top-k, then top-p, in one copy of the code (a border past the last bin of the list is past what
   // min-p keeps)
@@ -719,7 +763,8 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
 #pragma unroll 1
   for (int step = b.cut ? 0 : 1; step < (b.by_p ? 2 : 1); ++step) {
     const bool by_count = step == 0;
-    const u128 goal = by_count ? static_cast<u128>(f.top_k) : share_of(f.top_p, border.sum);
+    const u128 goal = by_count ? static_cast<u128>(f.top_k)
+                               : b.cut ? share_of(f.top_p, border.sum, true) : b.goal_p;
     const int at = by_count ? b.bin_k : b.cut ? b.by_sum(s, goal) : b.bin_p;
     if (at > b.last) continue;
     const Border other = border_in(at, by_count, goal);
@@ -728,52 +773,56 @@ __device__ __forceinline__ void finish_list(ListLds& s, const SampleArgs& p, con
   // sums of the kept tokens by stretches of indexes, a thread each; then the tokens of one stretch
   const int stretch = (p.vocab + kThreads - 1) / kThreads;
   __syncthreads();
-  s.few_sum[t] = 0;
+  s.few_sum[t] = s.few_high[t] = 0;
   if (t == 0) s.n = 0;
   __syncthreads();
-  auto kept = [&](u64 my) -> u64 {   // the token's weight, 0 where it is not kept
-    if (my > border.last || g.bin(value_at(my)) > b.last) return 0;
-    const double w = weight(value_at(my), top, f.c);
-    return w >= f.min_p ? fixed(w) : 0;
+  auto kept = [&](u64 my) -> u128 {   // the token's weight, 0 where it is not kept
+    const float v = value_at(my);
+    const Grid::Token i = g.token(v);
+    if (my > border.last || i.bin > b.last) return 0;
+    return !b.by_m || weight(v, top, f.c) >= f.min_p ? static_cast<u128>(i.entry) * s.tops[i.bin] : 0;
   };
 #pragma unroll 1
   for (int i = t; i < n; i += kThreads) {
-    const u64 my = s.list[i], w = kept(my);
-    if (w != 0) atomicAdd(&s.few_sum[static_cast<uint32_t>(my) / stretch], w);
+    const u64 my = s.list[i];
+    const u128 w = kept(my);
+    const int at = static_cast<uint32_t>(my) / stretch;
+    if (w != 0) add_weight(&s.few_sum[at], &s.few_high[at], w);
   }
   __syncthreads();
-  const u64 here = s.few_sum[t];
-  const Scanned<u64> r = block_scan(here, s.part[0]);
-  const u64 ahead = r.before, total = r.all;
-  const u64 goal = target_of(p.uniform[row], total);
-  if (ahead <= goal && goal < ahead + here) {   // one thread
+  const Words here{s.few_sum[t], s.few_high[t]};
+  const Scanned<Words> r = block_scan(here, s.part_sum);   // of no more than kList weights
+  const u128 ahead = joined(r.before), total = joined(r.all);
+  const u128 goal = target_of(f.u, total);
+  if (ahead <= goal && goal < joined(r.before + here)) {   // one thread
     s.found = t;
-    s.sum = ahead;
+    s.before = ahead;
   }
   __syncthreads();
   // its tokens, with their sums, in place of the ones of a bin
   const uint32_t first = static_cast<uint32_t>(s.found) * stretch;
-  const u64 before_it = s.sum;
-  __syncthreads();
+  u128 before = s.before;
 #pragma unroll 1
   for (int i = t; i < n; i += kThreads) {
     const u64 my = s.list[i];
     if (static_cast<uint32_t>(my) - first >= static_cast<uint32_t>(stretch)) continue;
-    const u64 w = kept(my);
+    const u128 w = kept(my);
     if (w == 0) continue;
     const int k = atomicAdd(&s.n, 1);   // at most the stretch's tokens, one a thread or less
     s.few[k] = my;
-    s.few_sum[k] = w;
+    s.few_sum[k] = static_cast<u64>(w);
+    s.few_high[k] = static_cast<u64>(w >> 64);
   }
   __syncthreads();
   if (t >= s.n) return;
-  const u64 my = s.few[t], w = s.few_sum[t];
-  u64 before = before_it;
+  auto weight_at = [&](int k) { return static_cast<u128>(s.few_high[k]) << 64 | s.few_sum[k]; };
+  const u64 my = s.few[t];
+  const u128 w = weight_at(t);
 #pragma unroll 1
   for (int j = 0; j < s.n; ++j)
-    if (static_cast<uint32_t>(s.few[j]) < static_cast<uint32_t>(my)) before += s.few_sum[j];
+    if (static_cast<uint32_t>(s.few[j]) < static_cast<uint32_t>(my)) before += weight_at(j);
   if (before <= goal && goal < before + w)
-    leave(p, row, static_cast<int>(static_cast<uint32_t>(my)), weight(value_at(my), top, f.c), total);
+    leave(p, row, static_cast<int>(static_cast<uint32_t>(my)), w, total);
 }
 
 template <int CTRL, int ROWS = 0xf>
@@ -813,8 +862,7 @@ __device__ __forceinline__ void block_top(float& top, int& at, float* part_top, 
 __device__ __forceinline__ bool leave_first(const SampleArgs& p, const Filters& f, int row, float top,
                                             int at) {
   if (top != -INFINITY && !f.greedy) return false;
-  if (threadIdx.x == 0)
-    leave(p, row, top == -INFINITY ? 0 : at, top == -INFINITY ? 0.0 : 1.0, kOne);
+  if (threadIdx.x == 0) leave_alone(p, row, at, top);
   return true;
 }
 
@@ -948,8 +996,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
 
 struct RowLds {
   ListLds l;
-  double scale[kBins];       // weight of a bin's top
-  u64 part_sum[kMaxParts];
+  u128 part_sum[kMaxParts];
   int shift[kMaxParts];      // of a part's bins against the row's
   float part_top[kWaves];
   int part_at[kWaves];
@@ -977,7 +1024,6 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     s.shift[t] = d < kBins ? static_cast<int>(d) : kBins;
   }
   const u64* bins = parts.bins + static_cast<int64_t>(row) * parts.n * kBins;
-  s.scale[t] = bin_scale(g, t);
   __syncthreads();
   u64 count = 0, sum = 0;
 #pragma unroll 4
@@ -1011,9 +1057,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       s.l.upto = static_cast<int>(b.count);
     }
     __syncthreads();
-    const u128 ahead = s.l.before;
-    const u64 top_at = bin_top(bin);
-    const u64 goal = by_count ? static_cast<u64>(share) : entries_for(share - ahead, top_at);
+    const Goal goal{by_count, share, s.l.before, s.l.tops[bin]};
     u64 c = s.l.last, m = 0;   // tokens before those looked at, and entries of the bin
     int inside = s.l.upto;
     u64 prefix = 0;      // the places' upper bits from `shift` on, once digits are taken
@@ -1039,8 +1083,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       Scanned<u64> rc, rm;
       block_scan(dc, s.l.part[0], rc, dm, s.l.part[1], rm);
       const u64 cb = c + rc.before, mb = m + rm.before;
-      const u64 have = by_count ? cb : mb, more = by_count ? dc : dm;
-      if (have < goal && have + more >= goal) {   // one thread
+      if (goal.above(cb, mb) && !goal.above(cb + dc, mb + dm)) {   // one thread
         s.digit = t;
         s.l.sum = mb;
         s.l.last = cb;
@@ -1063,8 +1106,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     });
     __syncthreads();
     listed = shift == 64 ? bin : -1;
-    border_of(s.l, s.l.list, s.l.n, s.l.n, g, bin, by_count, c, m, goal);
-    return Border{s.l.last, ahead + static_cast<u128>(s.l.sum) * top_at};
+    return border_of(s.l, s.l.list, s.l.n, s.l.n, g, bin, goal, c, m);
   };
 
   Border border{~u64{0}, b.total};
@@ -1072,7 +1114,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
 #pragma unroll 1
   for (int step = b.cut ? 0 : 1; step < (b.by_p ? 2 : 1); ++step) {   // top-k, then top-p
     const bool by_count = step == 0;
-    const u128 goal = by_count ? static_cast<u128>(f.top_k) : share_of(f.top_p, border.sum);
+    const u128 goal = by_count ? static_cast<u128>(f.top_k)
+                               : b.cut ? share_of(f.top_p, border.sum, true) : b.goal_p;
     const int bin = by_count ? b.bin_k : b.by_sum(s.l, goal);
     if (bin > b.bin_m_to && !(by_count && b.by_p)) continue;   // past what min-p keeps
     const Border other = border_in(bin, by_count, goal);
@@ -1086,13 +1129,18 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     return v > -INFINITY && place(v, i) <= border.last && v >= below_m &&
            (v > above_m || !b.by_m || weight(v, top, f.c) >= f.min_p);
   };
+  auto weight_of = [&](float v) {
+    const Grid::Token i = g.token(v);
+    return static_cast<u128>(i.entry) * s.l.tops[min(i.bin, kBins - 1)];   // no bin: entry 0
+  };
   // the parts' kept sums: whole bins, then tokens of the others
   for (int i = wave; i < parts.n; i += kWaves) {
-    u64 m = 0;
+    u128 m = 0;
     for (int bin = lane; bin < full; bin += kWave)
-      if (bin >= s.shift[i]) m += bin_sum(bins[i * kBins + bin - s.shift[i]], s.scale[bin]);
-    m = wave_total(m);
-    if (lane == 0) s.part_sum[i] = m;
+      if (bin >= s.shift[i])
+        m += static_cast<u128>(bins[i * kBins + bin - s.shift[i]] & kEntrySum) * s.l.tops[bin];
+    const Words sums = wave_scan(split(m));
+    if (lane == kWave - 1) s.part_sum[i] = joined(sums);
   }
   __syncthreads();
   if (full < kBins) {
@@ -1100,9 +1148,10 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     if (b.by_m) to = min(to, b.bin_m_to);
     // by sixteen lanes of their own, of which there are fewer at one sum
     auto add = [&](int i, float v) {
-      atomicAdd(&s.l.few[i / parts.size * 16 + (t & 15)], fixed(weight(v, top, f.c)));
+      const int at = i / parts.size * 16 + (t & 15);
+      add_weight(&s.l.few_sum[at], &s.l.few_high[at], weight_of(v));
     };
-    s.l.few[t] = 0;
+    s.l.few_sum[t] = s.l.few_high[t] = 0;
     __syncthreads();
     if (to == full && listed == full) {
       for (int i = t; i < s.l.n; i += kThreads) {
@@ -1118,25 +1167,24 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
     }
     __syncthreads();
     static_assert(kMaxParts * 16 <= kThreads, "a sum a thread");
-    const u64 sum16 = row_scan(s.l.few[t]);
+    const u128 sum16 = joined(row_scan(Words{s.l.few_sum[t], s.l.few_high[t]}));
     if ((t & 15) == 15 && t / 16 < parts.n) s.part_sum[t / 16] += sum16;
   }
   __syncthreads();
-  u64 total = 0;
-  for (int i = 0; i < parts.n; ++i) total += s.part_sum[i];
-  u64 goal = target_of(p.uniform[row], total);
-  int part = 0;
-  while (part < parts.n - 1 && goal >= s.part_sum[part]) goal -= s.part_sum[part++];
+  // the part with the result: the first whose sum, with those before it, is above the goal
+  static_assert(kMaxParts <= kWave, "a part a lane");
+  const u128 mine = lane < parts.n ? s.part_sum[lane] : 0;
+  const u128 sums = joined(wave_scan(split(mine)));
+  const u128 total = of_lane(sums, kWave - 1);
+  u128 goal = target_of(f.u, total);
+  const int part = __ffsll(__ballot(sums > goal)) - 1;
+  goal -= of_lane(sums - mine, part);
   // The part's tokens: sums by runs of neighbours, a thread each, then the run that holds the result in
-  // order.  Weights are those against the part's own largest, which is kept where any of its tokens is.
-  const float best = parts.top[row * parts.n + part];
-  const double against = weight(best, top, f.c);
+  // order.
   const int first = part * parts.size, run = (parts.size + kThreads - 1) / kThreads;
   const int n = min(parts.size, p.vocab - first), j0 = min(t * run, n), j1 = min(j0 + run, n);
-  auto share = [&](float v, int i) -> u64 {
-    return kept(v, i) ? fixed(weight(v, best, f.c)) : 0;
-  };
-  u64 here = 0;
+  auto share = [&](float v, int i) -> u128 { return kept(v, i) ? weight_of(v) : 0; };
+  u128 here = 0;
   float next[4];   // four tokens ahead
   auto load = [&](int j) {
 #pragma unroll
@@ -1155,18 +1203,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs p
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  const Scanned<u64> r = block_scan(here, s.l.part[0]);
-  const u64 ahead = r.before, sums = r.all;
-  const double want = static_cast<double>(goal) / against;
-  const u64 at_sum = want < static_cast<double>(sums) ? min(static_cast<u64>(want), sums - 1) : sums - 1;
-  if (!(ahead <= at_sum && at_sum < ahead + here)) return;   // one thread stays
-  u64 upto = ahead;
+  u128 upto = block_scan(here, s.l.part_sum).before;
+  if (!(upto <= goal && goal < upto + here)) return;   // one thread stays
 #pragma unroll 1
   for (int j = j0; j < j1; ++j) {
     const float v = logit(logits, first + j);
-    upto += share(v, first + j);
-    if (at_sum < upto) {
-      leave(p, row, first + j, weight(v, top, f.c), total);
+    const u128 w = share(v, first + j);
+    upto += w;
+    if (goal < upto) {
+      leave(p, row, first + j, w, total);
       return;
     }
   }
