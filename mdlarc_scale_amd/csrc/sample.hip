@@ -970,7 +970,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
   block_top(top, at, part_top, part_at);
   if (t == 0) {
     parts.top[slot] = top;
-    parts.at[slot] = first + at;
+    parts.at[slot] = at == 0x7fffffff ? at : first + at;   // none: no index is asked for, or there is none
   }
   if (top == -INFINITY || f.greedy) return;
   const Grid g(top, f.c);
