@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from .test_gpu_sample import BF, DEV, F32, K, draw
+from .test_gpu_sample import BF, DEV, F32, check, draw
 
 pytestmark = pytest.mark.gpu
 
@@ -160,8 +160,6 @@ def test_long_rows_with_values_that_are_not_finite(dtype, vocab):
     assert bool((lp[[2, 6, 7, 10]] == 0).all())
     assert token[5] == last and token[8] == last and token[11] == 1
     assert float(lp[11]) == pytest.approx(-math.log(3), abs=2.0 ** -23)
-    from .test_gpu_sample import check
-
     keep = [3, 4, 9]
     check(x[keep], u[keep])
     check(x[keep], u[keep], top_k=torch.full((3,), 50).int(), top_p=torch.full((3,), 0.9))
@@ -181,9 +179,3 @@ def test_long_rows_at_the_ends_of_the_random_numbers(vocab):
     u = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, -1.0, float("nan"), 2.0])
     token, _ = draw(x, u)
     assert token.tolist() == [0, vocab - 1, vocab - 1, 0, 0, vocab - 1]
-
-
-def test_rows_that_need_no_workspace():
-    """The bound that the wrapper goes by is the library's."""
-    assert K().sample_workspace_bytes(7, K().SAMPLE_LIST) == 0
-    assert K().sample_workspace_bytes(7, K().SAMPLE_LIST + 1) > 0
