@@ -1230,27 +1230,49 @@ int64_t parts_bytes(int rows, int vocab) {
          (kBins * sizeof(u64) + sizeof(float) + sizeof(int));
 }
 
+// A grid counts its threads in 32 bits, and a larger one is cut without an error: so many go to a launch,
+// and the rows of a call that has more in several.
+constexpr int64_t kLaunchThreads = int64_t{1} << 31;
+
 template <typename T>
-int launch_sample(const SampleArgs& a, void* workspace, hipStream_t st) {
-  if (a.vocab <= kWave) {
-    sample_short_kernel<T><<<(a.rows + 3) / 4, 256, 0, st>>>(a);
-  } else if (a.vocab <= kList) {
-    sample_list_kernel<T><<<a.rows, kThreads, 0, st>>>(a);
-  } else {
-    Parts parts;
-    parts.n = parts_of(a.rows, a.vocab);
+int launch_sample(const SampleArgs& all, void* workspace, hipStream_t st) {
+  Parts parts{};
+  if (all.vocab > kList) {
+    parts.n = parts_of(all.rows, all.vocab);
     // whole 16-byte pieces, so that the parts of an aligned row are aligned
-    parts.size = ((a.vocab + parts.n - 1) / parts.n + 7) / 8 * 8;
-    const int64_t all = static_cast<int64_t>(a.rows) * parts.n;
-    parts.bins = static_cast<u64*>(workspace);
-    parts.top = reinterpret_cast<float*>(parts.bins + all * kBins);
-    parts.at = reinterpret_cast<int*>(parts.top + all);
-    sample_bins_kernel<T><<<static_cast<unsigned>(all), kThreads, 0, st>>>(a, parts);
+    parts.size = ((all.vocab + parts.n - 1) / parts.n + 7) / 8 * 8;
+  }
+  const int64_t threads = all.vocab <= kWave ? kWave : static_cast<int64_t>(kThreads) * (parts.n > 0 ? parts.n : 1);
+  const int64_t most = kLaunchThreads / threads;
+  for (int64_t r0 = 0; r0 < all.rows; r0 += most) {
+    SampleArgs a = all;
+    a.rows = static_cast<int>(all.rows - r0 < most ? all.rows - r0 : most);
+    a.logits = static_cast<const T*>(all.logits) + r0 * all.ld;
+    a.uniform += r0;
+    a.token += r0;
+    if (a.temperature) a.temperature += r0;
+    if (a.top_k) a.top_k += r0;
+    if (a.top_p) a.top_p += r0;
+    if (a.min_p) a.min_p += r0;
+    if (a.logprob) a.logprob += r0;
+    if (a.vocab <= kWave) {
+      sample_short_kernel<T><<<(a.rows + 3) / 4, 256, 0, st>>>(a);
+    } else if (a.vocab <= kList) {
+      sample_list_kernel<T><<<a.rows, kThreads, 0, st>>>(a);
+    } else {
+      const int64_t n = static_cast<int64_t>(a.rows) * parts.n;
+      parts.bins = static_cast<u64*>(workspace);
+      parts.top = reinterpret_cast<float*>(parts.bins + n * kBins);
+      parts.at = reinterpret_cast<int*>(parts.top + n);
+      sample_bins_kernel<T><<<static_cast<unsigned>(n), kThreads, 0, st>>>(a, parts);
+      const int rc = launch_status();
+      if (rc != MDL_OK) return rc;
+      sample_row_kernel<T><<<a.rows, kThreads, 0, st>>>(a, parts);
+    }
     const int rc = launch_status();
     if (rc != MDL_OK) return rc;
-    sample_row_kernel<T><<<a.rows, kThreads, 0, st>>>(a, parts);
   }
-  return launch_status();
+  return MDL_OK;
 }
 
 }  // namespace

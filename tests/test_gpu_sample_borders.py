@@ -1,5 +1,5 @@
-"""K11 on the GPU where a filter's border or the random number meets a sum of weights exactly, and where
-the tokens must not depend on the rows beside them.
+"""K11 on the GPU where a filter's border or the random number meets a sum of weights exactly, where the
+tokens must not depend on the rows beside them, and with more rows than a launch takes.
 
 Equal logits have equal weights, so n of them (the rest -inf) have the sums j / n of all, whatever their
 value: the expected tokens follow in whole numbers, and no tolerance is needed for them.  logprob is
@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from .test_gpu_sample import BF, DEV, F32, check, draw
+from .test_gpu_sample import BF, DEV, F32, K, check, draw
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +179,29 @@ def test_long_rows_at_the_ends_of_the_random_numbers(vocab):
     u = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, -1.0, float("nan"), 2.0])
     token, _ = draw(x, u)
     assert token.tolist() == [0, vocab - 1, vocab - 1, 0, 0, vocab - 1]
+
+
+@pytest.mark.parametrize("rows,vocab", [(2 ** 22 + 5, 65), (2 ** 26 + 9, 2)])
+def test_more_rows_than_a_launch_takes(rows, vocab):
+    """2^32 threads and more, a grid's limit: a block of 1,024 a row, a wave of 64 a row."""
+    x = torch.zeros(rows, vocab, dtype=BF, device=DEV)
+    want = torch.arange(rows, device=DEV) * 40503 % vocab
+    x.scatter_(1, want[:, None], 50.0)
+    token = torch.full((rows,), -5, dtype=torch.int64, device=DEV)
+    u = torch.full((rows,), 0.5, device=DEV)
+    K().sample_tokens(x, u, token, top_p=u)
+    assert torch.equal(token, want)
+
+
+def test_more_parts_than_a_launch_takes():
+    """Rows above 4,096 tokens, a block of 1,024 threads for each part of them."""
+    rows, vocab = 2 ** 22 + 3, 4104
+    if torch.cuda.mem_get_info()[0] < 100 * 2 ** 30:
+        pytest.skip("needs 100 GB of free memory")
+    row = torch.zeros(1, vocab, dtype=BF, device=DEV)
+    row[0, 4100] = 50.0
+    x = row.expand(rows, vocab).contiguous()
+    x[-2:, 4100], x[-2:, 7] = 0.0, 50.0
+    token = torch.full((rows,), -5, dtype=torch.int64, device=DEV)
+    K().sample_tokens(x, torch.full((rows,), 0.5, device=DEV), token)
+    assert bool((token[:-2] == 4100).all()) and bool((token[-2:] == 7).all())
