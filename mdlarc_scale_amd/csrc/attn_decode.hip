@@ -343,6 +343,7 @@ static int decode_impl(bool fused, const RopeIn& rin, const uint16_t* q, uint16_
   if ((!fused && !aligned16(q)) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned4(out))
     return MDL_ERR_ALIGN;
   if (batch == 0) return MDL_OK;
+  if (!fits_launch(static_cast<int64_t>(batch) * n_heads, 256)) return MDL_ERR_SHAPE;
   const int ns = n_splits(cache_slots, split_len);
   const int64_t need = mdl_attn_decode_workspace_bytes(batch, n_heads, cache_slots, split_len);
   if (need > 0 && (!workspace || workspace_bytes < need)) return MDL_ERR_WORKSPACE;

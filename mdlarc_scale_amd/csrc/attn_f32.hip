@@ -515,7 +515,7 @@ template <int QW, int KG, int CH>
 int launch_prefill_f32(F32Args p, hipStream_t st) {
   p.q_tiles = (p.seq + kQT * QW - 1) / (kQT * QW);
   const int64_t blocks = (p.items + 7) / 8 * 8 * p.q_tiles;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 64 * QW * KG)) return MDL_ERR_SHAPE;
   hipLaunchKernelGGL((attn_f32_prefill_kernel<QW, KG, CH>), dim3(static_cast<unsigned>(blocks)),
                      dim3(64 * QW * KG), 0, st, p);
   return launch_status();
@@ -609,12 +609,11 @@ extern "C" int mdl_attn_decode_f32(const float* q, const float* k_cache, const f
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (p.items == 0) return MDL_OK;
   const int64_t blocks = (p.items + kWavesF - 1) / kWavesF;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 64 * kWavesF) || !fits_launch((n_bh + 3) / 4, 256)) return MDL_ERR_SHAPE;
   hipLaunchKernelGGL(attn_f32_decode_kernel, dim3(static_cast<unsigned>(blocks)),
                      dim3(64 * kWavesF), 0, st, p);
   const int rc2 = launch_status();
   if (rc2 != MDL_OK || n_split == 1) return rc2;
-  if ((n_bh + 3) / 4 > 0x7fffffff) return MDL_ERR_SHAPE;
   hipLaunchKernelGGL(attn_f32_combine_kernel, dim3(static_cast<unsigned>((n_bh + 3) / 4)),
                      dim3(256), 0, st, workspace, static_cast<int>(n_bh), n_heads, n_split, out,
                      out_layout);

@@ -33,12 +33,19 @@ int launch_tiles(const GroupedArgs* a, const bool* tall, int lists, hipStream_t 
   constexpr bool f32 = sizeof(T) == 4;
   // waves of a flat block.  Four (half as many blocks on a CU, one with 128 dims) were 1-40% slower.
   constexpr int kFlatGroups = 2;
+  auto blocks_of = [](const GroupedArgs& t) {
+    return static_cast<int64_t>(t.n_seq) * t.kv_heads * t.n_tiles * t.n_split;
+  };
+  int64_t all_flat = 0;
+  for (int i = 0; i < lists; ++i) {
+    if (tall[i] && !fits_launch(blocks_of(a[i]), 256)) return MDL_ERR_SHAPE;
+    if (!tall[i]) all_flat += blocks_of(a[i]);
+  }
+  if (!fits_launch(all_flat, 64 * kFlatGroups)) return MDL_ERR_SHAPE;
   GroupedPair flat{};
   int64_t n_flat = 0;
   for (int i = 0; i < lists; ++i) {
-    const int64_t blocks =
-        static_cast<int64_t>(a[i].n_seq) * a[i].kv_heads * a[i].n_tiles * a[i].n_split;
-    if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+    const int64_t blocks = blocks_of(a[i]);
     GroupedArgs t = a[i];
     t.by_pairs = divisor(static_cast<uint32_t>(t.n_seq) * t.kv_heads);
     t.by_split = divisor(t.n_split);
@@ -56,7 +63,6 @@ int launch_tiles(const GroupedArgs* a, const bool* tall, int lists, hipStream_t 
       n_flat += blocks;
     }
   }
-  if (n_flat > 0x7fffffff) return MDL_ERR_SHAPE;
   if (n_flat == 0) return MDL_OK;
   attn_flat_kernel<T, D, kFlatGroups>
       <<<static_cast<unsigned>(n_flat), 64 * kFlatGroups, 0, st>>>(flat);
@@ -113,6 +119,7 @@ extern "C" int mdl_attn_grouped(const void* q, const void* k_cache, const void* 
   const int64_t rows = static_cast<int64_t>(tokens) * n_heads;
   if (pl.n_split > 1 && workspace_bytes < state_bytes(pl.n_split, rows, head_dim))
     return MDL_ERR_WORKSPACE;
+  if (pl.n_split > 1 && !merge_fits(rows)) return MDL_ERR_SHAPE;
   GroupedArgs a{};
   a.q = q; a.k = k_cache; a.v = v_cache; a.q_offset = q_offset; a.kv_len = kv_len; a.out = out;
   a.n_seq = n_seq; a.tokens = tokens; a.heads = n_heads; a.kv_heads = n_kv_heads;
@@ -209,6 +216,7 @@ extern "C" int mdl_attn_decode_shared(const void* q, const void* prefix_k, const
   const int64_t rows = static_cast<int64_t>(batch) * n_heads;
   const int parts = pl.prefix.n_split + pl.own.n_split;
   if (workspace_bytes < state_bytes(parts, rows, head_dim)) return MDL_ERR_WORKSPACE;
+  if (!merge_fits(rows)) return MDL_ERR_SHAPE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   GroupedArgs a[2]{};
   a[0].q = q; a[0].k = prefix_k; a[0].v = prefix_v; a[0].q_offset = row_offset;

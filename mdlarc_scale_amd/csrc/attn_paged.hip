@@ -565,7 +565,9 @@ extern "C" int mdl_attn_paged(const void* q, int dtype, const void* k_pages, con
   if (pl.n_split > 1 && workspace_bytes < state_bytes(pl.n_split, rows, head_dim))
     return MDL_ERR_WORKSPACE;
   const int64_t blocks = static_cast<int64_t>(n_seq) * n_kv_heads * pl.n_tiles * pl.n_split;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  const bool single = takes_tokens(page_dtype, max_q, n_heads, n_kv_heads);
+  if (!fits_launch(blocks, single || pl.tall ? 256 : 128) || (pl.n_split > 1 && !merge_fits(rows)))
+    return MDL_ERR_SHAPE;
   PagedArgs a{};
   a.q = q; a.k = k_pages; a.v = v_pages; a.q_offset = q_offset; a.kv_len = kv_len; a.out = out;
   a.n_seq = n_seq; a.tokens = tokens; a.heads = n_heads; a.kv_heads = n_kv_heads;
@@ -586,7 +588,7 @@ extern "C" int mdl_attn_paged(const void* q, int dtype, const void* k_pages, con
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned n = static_cast<unsigned>(blocks);
   int rc;
-  if (takes_tokens(page_dtype, max_q, n_heads, n_kv_heads))
+  if (single)
     rc = !fp4 ? launch_token<kTokenF32>(a, head_dim, n, st)
               : dtype == MDL_DTYPE_F32 ? launch_token<kTokenFp4F32>(a, head_dim, n, st)
                                        : launch_token<kTokenFp4>(a, head_dim, n, st);

@@ -626,7 +626,7 @@ int launch_prefill(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v
   const bool small = heads * ((seq + 127) / 128) <= kOneGroupBlocks;
   const int64_t nqt = small ? (seq + 63) / 64 : (seq + 127) / 128;
   const int64_t blocks = (heads + kXcds - 1) / kXcds * kXcds * nqt;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 256)) return MDL_ERR_SHAPE;
   auto* kernel = small ? attn_prefill_kernel<1> : attn_prefill_kernel<2>;
   kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(
       q, k_cache, v_cache, seq, n_heads, cache_slots, key_mask, row_holes, kv_start, q_offset,
@@ -678,7 +678,7 @@ extern "C" int mdl_attn_prefill_lead(const float* qkv, int64_t qkv_ld, const flo
     return MDL_ERR_ALIGN;
   const int64_t blocks = static_cast<int64_t>(batch) * n_heads;
   if (blocks == 0 || seq == 0) return MDL_OK;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 512)) return MDL_ERR_SHAPE;
   const RopeArgs ra{max_x, max_y, max_z, px, py, pz};
   attn_lead_kernel<<<static_cast<unsigned>(blocks), 512, 0, static_cast<hipStream_t>(stream)>>>(
       qkv, qkv_ld, rstd, pos, rope_tab, ra, q_scale, seq, n_heads, key_mask, kv_start, q_offset,

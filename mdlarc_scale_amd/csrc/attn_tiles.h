@@ -1087,10 +1087,11 @@ Plan plan_tiles(int64_t pairs, int64_t max_rows, int slots, int max_parts, int m
   return r;
 }
 
+// of a row (token, head) a wave; asked before the parts are launched
+bool merge_fits(int64_t rows) { return fits_launch((rows + 3) / 4, 256); }
+
 int run_merge(const MergeArgs& m, int dtype, int head_dim, hipStream_t st) {
-  const int64_t blocks = (static_cast<int64_t>(m.tokens) * m.heads + 3) / 4;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
-  const unsigned n = static_cast<unsigned>(blocks);
+  const unsigned n = static_cast<unsigned>((static_cast<int64_t>(m.tokens) * m.heads + 3) / 4);
   if (dtype == MDL_DTYPE_F32) {
     if (head_dim == 64) attn_merge_kernel<float, 64><<<n, 256, 0, st>>>(m);
     else attn_merge_kernel<float, 128><<<n, 256, 0, st>>>(m);

@@ -194,6 +194,10 @@ inline int launch_status() {
   return e == hipSuccess ? MDL_OK : static_cast<int>(e);
 }
 
+// Whether a launch takes so many blocks of `threads` threads: a grid counts its threads in 32 bits, and one
+// with more is cut without an error.
+inline bool fits_launch(int64_t blocks, int threads) { return blocks <= 0xffffffffll / threads; }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }

@@ -273,6 +273,7 @@ int launch_head(const float* x, const int32_t* row_index, int rows, int d, const
     cons = HeadCons{c->disallow_mask, c->palette_mask, c->palette_penalty, c->target_shape,
                     c->grid_x, c->grid_y, c->shape_penalty};
   }
+  if (!fits_launch(rows, 256)) return MDL_ERR_SHAPE;
   const dim3 grid(rows);
   const int nv = vocab <= 16 ? 16 : 32;
 #define MDL_HEAD(N)                                                                            \
@@ -350,6 +351,7 @@ extern "C" int mdl_grid_init(const int64_t* ids, const int64_t* pos, const uint8
       static_cast<int64_t>(batch) * seq > INT32_MAX)
     return MDL_ERR_SHAPE;
   if (batch == 0) return MDL_OK;
+  if (!fits_launch((int64_t{batch} + 3) / 4, 256)) return MDL_ERR_SHAPE;
   grid_init_kernel<<<dim3((batch + 3) / 4), 256, 0, static_cast<hipStream_t>(stream)>>>(
       ids, pos, mask, row_shift, batch, seq, max_x, max_y, gx, gy, in_out, kv_start, last_row,
       row_holes);

@@ -507,7 +507,7 @@ int launch_embed_tiles(const int64_t* ids, const int64_t* ex_ids, const void* to
                         float* x, const PackArgs* pk, hipStream_t s) {
   const int parts = (d / 32 + kEmbCols - 1) / kEmbCols;
   const int64_t blocks = (static_cast<int64_t>(rows) + 15) / 16 * parts;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 256)) return MDL_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(blocks));
   const PackArgs none{};
   const bool wide = aligned16(tok) && (!ex_ids || aligned16(ex));
@@ -568,6 +568,7 @@ extern "C" int mdl_embed_rmsnorm(const int64_t* ids, const int64_t* example_ids,
   if (!aligned16(x_out) || !aligned16(gamma) || (xs_out && !aligned8(xs_out)))
     return MDL_ERR_ALIGN;
   if (rows == 0) return MDL_OK;
+  if (!fits_launch((int64_t{rows} + 3) / 4, 256)) return MDL_ERR_SHAPE;
   const dim3 grid((rows + 3) / 4);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (layout == MDL_LAYOUT_TILES && !xs_out && !rstd_out &&   // x alone
@@ -606,6 +607,7 @@ extern "C" int mdl_embed_rmsnorm_bf16(const int64_t* ids, const int64_t* example
       !aligned16(xn_out) || !aligned16(gamma))
     return MDL_ERR_ALIGN;
   if (rows == 0) return MDL_OK;
+  if (!fits_launch((int64_t{rows} + 7) / 8, 256)) return MDL_ERR_SHAPE;
   dispatch_nc<LaunchEmbedBf16>(d, dim3((rows + 7) / 8), static_cast<hipStream_t>(stream), use_ex,
                                ids, example_ids, tok_table, ex_table, vocab, n_examples, rows,
                                row_len, d, gamma, eps, x_out, xn_out);
@@ -627,6 +629,7 @@ extern "C" int mdl_decode_embed(const int64_t* token, const int64_t* example_ids
   if (!aligned16(x_out) || !aligned16(gamma) || (xs_out && !aligned8(xs_out)))
     return MDL_ERR_ALIGN;
   if (batch == 0) return MDL_OK;
+  if (!fits_launch((int64_t{batch} + 3) / 4, 256)) return MDL_ERR_SHAPE;
   const dim3 grid((batch + 3) / 4);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (table_dtype == MDL_DTYPE_F32)
@@ -654,6 +657,7 @@ extern "C" int mdl_add_rmsnorm(float* x, const float* delta, const float* bias, 
       (bias && !aligned16(bias)) || (xs_out && !aligned8(xs_out)))
     return MDL_ERR_ALIGN;
   if (rows == 0) return MDL_OK;
+  if (!fits_launch((int64_t{rows} + 3) / 4, 256)) return MDL_ERR_SHAPE;
   const bool nt = static_cast<int64_t>(rows) * d * (8 + (delta ? 4 : 0) + (xs_out ? 4 : 0)) >=
                   kStreamBytes;
   dispatch_nc<LaunchAdd>(d, dim3((rows + 3) / 4), static_cast<hipStream_t>(stream), nt,

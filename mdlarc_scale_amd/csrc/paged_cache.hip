@@ -195,7 +195,7 @@ int launch_append(AppendArgs& a, hipStream_t st) {
   const int ni = few ? 1 : (passes + 3) / 4 * 4 <= (passes + 2) / 3 * 3 ? 4 : 3;
   a.n_items = (passes + ni - 1) / ni;
   const int64_t blocks = (a.rows * a.n_items + 3) / 4;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 256)) return MDL_ERR_SHAPE;
   const unsigned n = static_cast<unsigned>(blocks);
   // prompts stream: their rows are read once and the pages are larger than the caches in between
   const bool nt = a.rows * a.ld * static_cast<int64_t>(sizeof(TI)) >= kStreamBytes;
@@ -307,7 +307,7 @@ int launch_rows_of(RowsArgs& a, hipStream_t st) {
   const int each = pairs * ((a.run + 4 * rows - 1) / (4 * rows)) < kFewBlocks ? 1 : 4;
   a.tiles = (a.run + each * rows - 1) / (each * rows);
   const int64_t blocks = pairs * a.tiles;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 256)) return MDL_ERR_SHAPE;
   const unsigned n = static_cast<unsigned>(blocks);
   if (each == 1)
     paged_rows_kernel<TO, FP4, D, 1><<<n, 256, 0, st>>>(a);

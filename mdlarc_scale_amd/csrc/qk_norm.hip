@@ -121,7 +121,7 @@ int launch_qk_norm(QkNormArgs& a, hipStream_t st) {
   const int ni = few ? 1 : (passes + 3) / 4 * 4 <= (passes + 2) / 3 * 3 ? 4 : 3;
   a.n_items = (passes + ni - 1) / ni;
   const int64_t blocks = (a.rows * a.n_items + 3) / 4;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 256)) return MDL_ERR_SHAPE;
   const unsigned n = static_cast<unsigned>(blocks);
   // prompts stream: their rows are read once and the caches are larger than the caches in between
   const bool nt = a.rows * a.ld * static_cast<int64_t>(sizeof(TI)) >= kStreamBytes;

@@ -185,7 +185,7 @@ int launch_k2(const float* qkv, int64_t qkv_ld, const float* rstd, const int64_t
               int cache_slots, int slot0, const int32_t* slot_dev, const int32_t* tok_row,
               const int32_t* tok_slot, int64_t batch, hipStream_t st) {
   if (rows == 0) return MDL_OK;
-  if ((rows + 3) / 4 > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch((rows + 3) / 4, 256)) return MDL_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
   if (out_dtype == MDL_DTYPE_F32) {
     qkv_rope_cache_kernel<float><<<grid, 256, 0, st>>>(
@@ -274,7 +274,7 @@ extern "C" int mdl_qkv_rope_cache_bf16(const uint16_t* qkv, int64_t qkv_ld, cons
     return MDL_ERR_ALIGN;
   const int64_t rows = static_cast<int64_t>(batch) * seq;
   if (rows == 0) return MDL_OK;
-  if ((rows + 3) / 4 > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch((rows + 3) / 4, 256)) return MDL_ERR_SHAPE;
   const RopeArgs ra{max_x, max_y, max_z, px, py, pz};
   const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
   hipStream_t st = static_cast<hipStream_t>(stream);

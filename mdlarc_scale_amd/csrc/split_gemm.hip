@@ -471,7 +471,7 @@ int launch_tile(GemmArgs p, hipStream_t st) {
   p.m_tiles = (p.M + TM - 1) / TM;
   const int64_t tiles = static_cast<int64_t>(p.n_tiles) * p.m_tiles;
   const int64_t per_xcd = (tiles + 7) / 8;
-  if (8 * per_xcd > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(8 * per_xcd, 64 * kGemmWaves)) return MDL_ERR_SHAPE;
   p.per_xcd = static_cast<int>(per_xcd);
   hipLaunchKernelGGL((split_gemm_kernel<TN, TM, WT, AMODE, EPI, WL>),
                      dim3(static_cast<unsigned>(8 * per_xcd)), dim3(64 * kGemmWaves), 0, st, p);
@@ -755,7 +755,7 @@ extern "C" int mdl_tile_matrix(const uint16_t* src, int64_t ld, int rows, int co
   if (rows == 0) return MDL_OK;
   const int64_t chunks = static_cast<int64_t>((rows + 15) / 16) * 16 * (cols / 8);
   const int64_t blocks = (chunks + 255) / 256;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 256)) return MDL_ERR_SHAPE;
   hipLaunchKernelGGL(tile_matrix_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), src, ld, rows, cols, chunks, dst);
   return launch_status();
@@ -768,7 +768,7 @@ extern "C" int mdl_zero_tiled_rows(uint16_t* buf, int r0, int r1, int cols, void
   if (r0 == r1) return MDL_OK;
   const int64_t chunks = static_cast<int64_t>(r1 - r0) * (cols / 8);
   const int64_t blocks = (chunks + 255) / 256;
-  if (blocks > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch(blocks, 256)) return MDL_ERR_SHAPE;
   hipLaunchKernelGGL(zero_tiled_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), buf, r0, chunks, cols);
   return launch_status();

@@ -136,6 +136,7 @@ extern "C" int mdl_swiglu_bf16(const uint16_t* gate_up, int64_t ld, const float*
       (bias_gate && !aligned16(bias_gate)) || (bias_up && !aligned16(bias_up)))
     return MDL_ERR_ALIGN;
   if (rows == 0) return MDL_OK;
+  if (!fits_launch((int64_t{rows} + kBf16Rows - 1) / kBf16Rows, 256)) return MDL_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>((rows + kBf16Rows - 1) / kBf16Rows),
                   static_cast<unsigned>((d_ff + 2047) / 2048));
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -163,7 +164,7 @@ extern "C" int mdl_swiglu(const float* gate_up, int64_t ld, const float* rstd,
     return MDL_ERR_ALIGN;
   if (rows == 0) return MDL_OK;
   const int64_t items = static_cast<int64_t>(rows) * (d_ff / 8);
-  if ((items + 255) / 256 > 0x7fffffff) return MDL_ERR_SHAPE;
+  if (!fits_launch((items + 255) / 256, 256)) return MDL_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>((items + 255) / 256));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (static_cast<int64_t>(rows) * d_ff * 12 >= kStreamBytes)
