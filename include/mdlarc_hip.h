@@ -13,6 +13,8 @@
  *   - Nothing allocates, frees or synchronises; all work is ordered on `stream`.
  *   - Return 0 on success, a negative MDL_ERR_* for arguments rejected on the host before any
  *     launch, or a positive hipError_t reported by the launch.
+ *   - A launch takes fewer than 2^32 threads (a larger grid would be cut without an error): calls that need
+ *     more return MDL_ERR_SHAPE; mdl_sample_tokens makes several launches of them.
  *   - Head dimension is 64 (all reference model sizes, src/transformer.py:728-745); the entries for
  *     grouped key / value heads and for caches in pages (K7 to K10) take 64 and 128.
  *   - GEMM inputs ("split activations") are written as hi|lo bf16 pairs: a row of K values is 2K
@@ -784,8 +786,9 @@ int mdl_paged_rows(const void* k_pages, const void* v_pages, int page_dtype,
 /*
  * K10: mdl_attn_grouped with the pages of a sequence in place of its cache row; cache_slots is
  * table_width * page_slots.  q (and out) are of dtype, the pages' type unless those are
- * MDL_DTYPE_FP4, whose values enter the products as they are (fp32 q of single tokens, max_q 1, over
- * 4-bit pages: weights below 2^-126 of the largest are zero).  A sequence that has a page number
+ * MDL_DTYPE_FP4, whose values enter the products as they are (bf16 q: the weights are rounded to bf16 for
+ * the product with V, as there; fp32 q of single tokens, max_q 1, over 4-bit pages: weights below 2^-126
+ * of the largest are zero).  A sequence that has a page number
  * outside the pool among the pages of its keys reads no memory outside the pool and gives NaN in every
  * row that sees such a page (and may in its other rows).
  */
@@ -817,10 +820,12 @@ int64_t mdl_attn_paged_workspace_bytes(int n_seq, int tokens, int max_q, int n_h
  * 2^-59 of the largest) that are added without rounding, so a row's token and logprob are the same in
  * every call, whatever rows are beside it, and equal logits make equal steps: a share or a random number that
  * meets their sum exactly is taken as above.  Tokens below 2^-58 of the largest may count as nothing.
- * workspace (8-byte aligned): mdl_sample_workspace_bytes of the same sizes, 0 up to 4,096 tokens; calls
- * that may overlap in time need workspaces of their own.
- * Replaces: the temperature / top-k branch of generate_output (src/inference.py:573-583) with the
- *           random number as an input, so a sampled step can be captured and repeated.
+ * workspace (8-byte aligned): mdl_sample_workspace_bytes of the same sizes, 0 up to 4,096 tokens (a call of
+ * fewer rows cuts them in more parts and may need more); calls that may overlap in time need workspaces
+ * of their own.
+ * Counterpart: the temperature / top-k branch of generate_output (src/inference.py:573-583), with the
+ *           random number as an input, so a sampled step can be captured and repeated; for a caller's
+ *           own loop (generate draws with torch.multinomial between launches, as the reference does).
  */
 int mdl_sample_tokens(const void* logits, int dtype, int64_t ld, int rows, int vocab,
                       const float* uniform, const float* temperature, const int32_t* top_k,
@@ -831,7 +836,7 @@ int64_t mdl_sample_workspace_bytes(int rows, int vocab);
 /*
  * mdl_rope_cache_paged, mdl_paged_rows, mdl_attn_paged and mdl_sample_tokens with their arguments, all but
  * the stream, in a block of host memory: in their order, each as a member of a C struct of them would lie.
- * The block is read before the call returns.
+ * The block is read before the call returns; it has to hold all of them, for its length is not passed.
  */
 int mdl_rope_cache_paged_block(const void* args, void* stream);
 int mdl_paged_rows_block(const void* args, void* stream);

@@ -12,10 +12,11 @@
 // power is a bf16 number.
 //
 // What bounds it.  Prompts: as K8 (attn_tiles.h), with a look at a page number for each sixteen keys: 4
-// prompts of up to 4,096 tokens, 32 heads on 8 of 128, bf16: 472 us, 980 TFLOP/s (over contiguous
-// caches 446).  Single tokens, 4 bits: HBM; 256 rows of up to 2,664 keys, 16 heads of 64: 112 us, 5.4
-// TB/s, 64 of up to 32,750, 32 heads on 8 of 128: 285 us, 5.9 TB/s.  Few rows: two launches and a block's
-// chain of loads, the page number before the first; 3 continuations behind 4,099 keys: 16 + 4 us.
+// prompts of up to 4,096 tokens, 32 heads on 8 of 128, bf16: 472 to 496 us with the card and its clock, 933
+// to 980 TFLOP/s (over contiguous caches 446).  Single tokens, 4 bits: HBM; 256 rows of up to 2,664 keys, 16
+// heads of 64: 112 us, 5.4 TB/s, 64 of up to 32,750, 32 heads on 8 of 128: 286 to 292 us, 5.9 TB/s.  Few
+// rows: two launches and a block's chain of loads, the page number before the first; 3 continuations behind
+// 4,099 keys: 16 + 4 us.
 #include <algorithm>
 
 #include "attn_tiles.h"
@@ -478,7 +479,8 @@ int check_paged(int n_seq, int tokens, int max_q, int n_heads, int n_kv_heads, i
 }
 
 // Single tokens over 4-bit and fp32 pages with no more heads to a key / value head than rows of their
-// kernel.  bf16 pages stay with the flat tiles, which read them at 6 TB/s and more.
+// kernel.  bf16 pages stay with the flat tiles: 64 rows of up to 4,000 keys (32 heads on 8 of 128) 131 us,
+// 6.0 TB/s, 256 of up to 2,664 (16 heads of 64) 345 us, 6.5 TB/s.
 bool takes_tokens(int page_dtype, int max_q, int n_heads, int n_kv_heads) {
   return page_dtype != MDL_DTYPE_BF16 && max_q == 1 && n_heads / n_kv_heads <= 16;
 }

@@ -30,7 +30,7 @@
 // row's second launch looks for the borders in their bins alone, cut by the digits of value and index
 // where thousands are equal, and takes the parts' kept sums from their bins.
 //
-// What bounds it: one block's chain of steps, most of them waits (VALU busy 8% in the second launch).  64
+// What bounds it: one block's chain of steps, most of them waits (VALU busy 7% in the second launch).  64
 // rows of 131,072 logits, 45 to 56 us by their filters: the bins 11.5 (64-bit arithmetic, 20 instructions
 // a token), the second launch 33 to 43, as long as its longest row, one with more than 4,096 tokens kept;
 // 256 rows of 4,000 21 us, of 14 5.6 us.
