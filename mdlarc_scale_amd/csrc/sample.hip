@@ -291,7 +291,9 @@ __device__ __forceinline__ u64 bin_top(int bin) {
 }
 
 // The row's bins: 1/16 octave each, bin 0 with the largest value; kBins for values below all of them.
-// A logit lies at -x times the scale, in bins; `base` is where bin 0 begins.
+// A logit lies at 1/2 - x times the scale, in bins; `base` is where bin 0 begins.  Weights on two sides of a
+// border of bins are off against each other by 2^-33, so the half keeps the borders away from 0, where high
+// temperatures bring all logits: their weights are then equal.
 struct Grid {
   double scale, at_top, base;
   bool huge;      // the largest value is infinite: it alone has a weight, in bin 0
@@ -301,11 +303,9 @@ struct Grid {
     at_top = huge ? 0.0 : at(top);
     base = floor(at_top);
   }
-  // Nothing here is contracted: a token's bin and entry are the same wherever they are computed.
-  __device__ __forceinline__ double at(float x) const {
-#pragma clang fp contract(off)
-    return -static_cast<double>(x) * scale;
-  }
+  // Here and below nothing is left to be contracted: a token's bin and entry are the same wherever they are
+  // computed.
+  __device__ __forceinline__ double at(float x) const { return fma(-static_cast<double>(x), scale, 0.5); }
   __device__ __forceinline__ int bin(float x) const {
     if (huge) return x == INFINITY ? 0 : kBins;
     const double d = floor(at(x)) - base;
@@ -326,12 +326,12 @@ struct Grid {
   // bounds of the values in bins `first` .. `last` (a few roundings of fp32 wider)
   __device__ __forceinline__ float least(int last) const {
     if (huge) return INFINITY;
-    const double x = -(base + last + 1) / scale;
+    const double x = (0.5 - (base + last + 1)) / scale;
     return static_cast<float>(x - fabs(x) * 0x1p-20);
   }
   __device__ __forceinline__ float most(int first) const {
     if (huge || first == 0) return INFINITY;
-    const double x = -(base + first) / scale;
+    const double x = (0.5 - (base + first)) / scale;
     return static_cast<float>(x + fabs(x) * 0x1p-20);
   }
 };

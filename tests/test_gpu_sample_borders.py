@@ -66,6 +66,31 @@ def test_shares_that_meet_a_sum(dtype, vocab, n):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("vocab", VOCABS)
+@pytest.mark.parametrize("heat", [1e20, 1e30, float("inf")])
+def test_temperatures_that_make_all_weights_equal(dtype, vocab, heat):
+    """Weights differ by less than 2^-60, and the ones that are kept are the largest: a share of a quarter,
+    a half or three quarters keeps as many of them."""
+    g = torch.Generator().manual_seed(vocab)
+    rows = 12
+    x = (torch.randn(rows, vocab, generator=g) * 4).to(dtype)
+    x[:, ::5] = -x[:, ::5].abs()
+    u = torch.rand(rows, generator=g)
+    n = vocab // 4 * 4
+    x[:, n:] = float("-inf")
+    order = x.float().sort(dim=1, descending=True, stable=True).indices
+    for q in (1, 2, 3, 4):
+        m = n * q // 4
+        at = order[:, :m].sort(1).values
+        p = torch.full((rows,), q / 4)
+        token, lp = draw(x, u, top_p=p, temperature=torch.full((rows,), heat))
+        for r in range(rows):
+            # u m is exact in 64 bits (24 and 17 of them)
+            assert int(token[r]) == int(at[r, int(float(u[r]) * m)]), (q, r)
+            assert abs(float(lp[r]) + math.log(m)) <= (2.0 ** -24 + 2.0 ** -50) * math.log(m), (q, r)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("vocab,n", [(v, n) for v in VOCABS for n in (2, 4, 64, 8192) if n <= v])
 def test_random_numbers_that_meet_a_sum(dtype, vocab, n):
     """u = j / n: the sum up to token j - 1 is not above it, that up to token j is."""
